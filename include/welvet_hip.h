@@ -393,6 +393,91 @@ int wv_decoder_prefill(uint64_t decoder, const int32_t *tokens, int32_t n_tokens
 /* Releases the decoder (not the blobs it references). */
 int wv_decoder_free(uint64_t decoder);
 
+/* ---- paged KV cache: the rows of many sequences in one pool of pages ---- */
+
+/* The reference keeps one cache per layer and sequence, MaxSeqLen x kvDim f64
+ * (layers/mha/cpu.go:11-21, 178-193). Here a cache handle owns, for every
+ * layer, a pool of n_pages pages of page_size token positions that any number
+ * of sequences share: the caller's page table says which pages a sequence
+ * holds, and slot = page * page_size + offset names a position of the pool.
+ *
+ * Rows are held as codes with one f32 scale per position and KV head, for K
+ * and V each. For a row x of head_dim values with amax = max |x|:
+ *   WV_KV_F16  scale = 2^(floor(log2 amax) - 14), code = fp16(x / scale)
+ *              (nearest, ties to even): 2 bytes per value, no overflow
+ *   WV_KV_Q8   scale = f32(amax / 127), code = x / scale rounded half away
+ *              from zero (the exact quotient; Q8_0's rule): 1 byte per value
+ * and a row reads back as code * scale. A row with amax < 2^-100 is held as
+ * zeros. A row that holds a NaN or an infinity reads back as NaN in every
+ * value (and what attends to it is NaN). Positions never written read back 0. */
+#define WV_KV_F16 0
+#define WV_KV_Q8 1
+typedef struct wv_kv_config {
+    int32_t n_layers, n_kv_heads;
+    int32_t head_dim;  /* 64 or 128 */
+    int32_t page_size; /* 32, 64, 128 or 256 positions */
+    int32_t n_pages;
+    int32_t type;      /* WV_KV_* */
+} wv_kv_config;
+
+/* Allocates the pools on the current device, all positions unwritten. */
+int wv_kv_create(const wv_kv_config *cfg, uint64_t *cache);
+/* Configuration and device bytes of a cache; either pointer may be NULL. */
+int wv_kv_info(uint64_t cache, wv_kv_config *cfg, size_t *device_bytes);
+/* Releases a cache once its work is done (waits for the device). */
+int wv_kv_free(uint64_t cache);
+
+/* Writes n token rows of `layer`: K and V of row t are n_kv_heads * head_dim
+ * floats at d_k + t * k_stride and d_v + t * v_stride (strides in floats; 0:
+ * rows back to back), their position d_slots[t]. A slot outside the pool (-1
+ * for the padding rows of a batch) is skipped. The slots of one call have to
+ * differ: of two rows for one slot, which codes and scale end there is not
+ * defined. Device pointers, enqueued on `stream`; allocates nothing. */
+int wv_kv_write_dev(uint64_t cache, int32_t layer, const float *d_k, const float *d_v, int64_t k_stride,
+                    int64_t v_stride, const int64_t *d_slots, int32_t n, void *stream);
+/* Reads n positions back into f32 rows (laid out as in wv_kv_write_dev); rows
+ * of slots outside the pool come back as zeros. */
+int wv_kv_read_dev(uint64_t cache, int32_t layer, const int64_t *d_slots, int32_t n, float *d_k, float *d_v,
+                   int64_t k_stride, int64_t v_stride, void *stream);
+
+/* New tokens of n_seqs sequences in one batch. Sequence b owns the query rows
+ * d_cu_q[b] .. d_cu_q[b+1]-1 of n_tokens rows (ascending from 0; rows behind
+ * the last sequence are padding) and the keys 0 .. d_kv_len[b]-1, its new
+ * tokens' own among them (write them first); key j lies in page
+ * d_pages[b * max_pages + j / page_size]. A page outside the pool holds no
+ * keys, nor do positions past the table. Device arrays, read when the work
+ * runs, so a captured call takes new lengths and tables on replay. */
+typedef struct wv_kv_batch {
+    int32_t n_seqs, n_tokens, max_pages;
+    int32_t max_q; /* most new tokens of one sequence, 0: unknown. Steers the launch only. */
+    const int32_t *d_cu_q;   /* [n_seqs + 1] */
+    const int32_t *d_kv_len; /* [n_seqs] */
+    const int32_t *d_pages;  /* [n_seqs][max_pages] */
+} wv_kv_batch;
+
+/* Causal grouped-query attention of a batch's new tokens over the cache
+ * (layers/mha/attn.go:40-118 with its causal and sliding-window masks). Token
+ * i of a sequence with n new tokens stands at position p = kv_len - n + i and
+ * attends the keys j <= p, of those only j > p - window where window > 0:
+ *   out[t][h] = sum_j exp(scale q[t][h].K_j - max) V_j / sum_j exp(...)
+ * with KV head h / (n_heads / n_kv_heads). A row without keys comes out as
+ * zeros; padding rows are left as they are. q and out are f32, row t at
+ * t * stride floats (0: n_heads * head_dim), n_heads a multiple of n_kv_heads;
+ * out may be q. The codes enter the matrix products exactly, queries and
+ * probabilities in two fp16 terms each (22 bits), sums are f32: within a few
+ * 1e-7 normwise of the same sums in f64.
+ * Long key ranges are split over blocks and joined in order; the partial rows
+ * lie in d_scratch (wv_kv_attention_scratch bytes, 16-byte aligned, held by
+ * the call until its work is done), or, with NULL, in the library's own
+ * scratch. A call with NULL on a stream under capture does not split. */
+int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch *batch, const float *d_q, int64_t q_stride,
+                        int32_t n_heads, float scale, int32_t window, float *d_out, int64_t out_stride,
+                        void *d_scratch, size_t scratch_bytes, void *stream);
+/* Scratch bytes of such a call (0: it splits nothing). Only the batch's
+ * n_seqs, n_tokens, max_pages and max_q are read. */
+int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch *batch, int32_t n_heads, int32_t window,
+                            size_t *bytes);
+
 /* ---- streams ---- */
 
 /* Blocks until all work the library enqueued on `stream` (NULL = its own) is done. */

@@ -45,6 +45,8 @@ EXPORTS = (
     "wv_store_matvec_t", "wv_matmul", "wv_matmul_dev", "wv_sync",
     "wv_decoder_create", "wv_decoder_set_layer", "wv_decoder_set_output", "wv_decoder_set_kv",
     "wv_decoder_use_graph", "wv_decoder_generate", "wv_decoder_prefill", "wv_decoder_free",
+    "wv_kv_create", "wv_kv_info", "wv_kv_free", "wv_kv_write_dev", "wv_kv_read_dev", "wv_kv_attention_dev",
+    "wv_kv_attention_scratch",
 )
 
 
@@ -110,6 +112,14 @@ def lib():
                                       _P, _P]
     L.wv_decoder_prefill.argtypes = [ctypes.c_uint64, _P, ctypes.c_int32, ctypes.c_int32, _P, _P]
     L.wv_decoder_free.argtypes = [ctypes.c_uint64]
+    L.wv_kv_create.argtypes = [_P, _P]
+    L.wv_kv_info.argtypes = [ctypes.c_uint64, _P, _P]
+    L.wv_kv_free.argtypes = [ctypes.c_uint64]
+    L.wv_kv_write_dev.argtypes = [ctypes.c_uint64, ctypes.c_int32, _P, _P, _I64, _I64, _P, ctypes.c_int32, _P]
+    L.wv_kv_read_dev.argtypes = [ctypes.c_uint64, ctypes.c_int32, _P, ctypes.c_int32, _P, _P, _I64, _I64, _P]
+    L.wv_kv_attention_dev.argtypes = [ctypes.c_uint64, ctypes.c_int32, _P, _P, _I64, ctypes.c_int32, ctypes.c_float,
+                                      ctypes.c_int32, _P, _I64, _P, _SZ, _P]
+    L.wv_kv_attention_scratch.argtypes = [ctypes.c_uint64, _P, ctypes.c_int32, ctypes.c_int32, _P]
     _lib = L
     return L
 

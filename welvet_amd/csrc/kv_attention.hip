@@ -1,0 +1,558 @@
+// kv_attention.hip — causal attention of a batch's new tokens over the paged
+// KV cache.
+//
+// With t = scale log2(e) q.K the row's output is sum_j 2^(t_j - m) V_j over
+// sum_j 2^(t_j - m), m the running maximum: one pass over the keys, the sums
+// so far scaled by 2^(m_old - m_new) when m grows. K and V are codes c with a
+// scale s per key, exact in fp16, so with the query row split in two fp16
+// terms q = 2^e (qh + ql) (22 bits)
+//   t_j = (c_j.qh + c_j.ql) s_j * (2^e scale log2 e)
+// on the fp16 matrix cores with f32 sums. For the second product the
+// probabilities take the V scales, P_j = 2^14 p_j s_j 2^-E, with E the running
+// exponent of the largest scale met (P_j then fills fp16's range whatever the
+// values' magnitude), and are split as ph + pl the same way.
+#include <algorithm>
+#include <cmath>
+
+#include "kv.h"
+#include "rt_internal.h"
+#include "wave_ops.h"
+
+namespace wv {
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -3.402823466e38f;  // the running maximum of a row that has met no key
+constexpr int kMaxSplits = 64;
+
+// 8 biased int8 codes (two words) as fp16: 0x6400 | b is 1024 + b, less 1152
+// the code; one byte permute and half a packed subtraction per code pair.
+__device__ __forceinline__ h8 q8_half(uint32_t x, uint32_t y) {
+    union {
+        uint32_t u[4];
+        h2 h[4];
+        h8 v;
+    } r;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, y, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, y, 0x04030402u);
+    const h2 b = {_Float16(1152.0f), _Float16(1152.0f)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.h[i] -= b;
+    return r.v;
+}
+__device__ __forceinline__ h8 as_half(uint4 x) {
+    union {
+        uint4 u;
+        h8 v;
+    } r;
+    r.u = x;
+    return r.v;
+}
+
+// hi + lo of 8 floats: hi truncated to fp16, lo the rounded rest.
+__device__ __forceinline__ void split8(const float* x, h8& hi, h8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
+        hi[i] = _Float16(h[0]);
+        hi[i + 1] = _Float16(h[1]);
+        lo[i] = _Float16(x[i] - float(h[0]));
+        lo[i + 1] = _Float16(x[i + 1] - float(h[1]));
+    }
+}
+
+// Maximum / sum over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float max_over_quads(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_over_quads(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// A tile of query rows: row = token * G + head of the group, in one sequence.
+struct Tile {
+    int seq = -1, r0 = 0, rows = 0;  // first row of the tile, rows of the sequence
+    int q0 = 0, n = 0, kv_len = 0;   // the sequence's first token row, new tokens, keys
+};
+
+// Tile `idx` of the batch's tiles of RT rows, over the sequences with at
+// least min_rows and at most max_rows rows, in order of the sequences: every
+// wave scans 64 sequences at a time. False: past the last tile.
+template <int RT>
+__device__ __forceinline__ bool find_tile(const KvAttn& a, int G, int idx, int min_rows, int max_rows, Tile& t) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const int s = base + lane;
+        int c0 = 0, n = 0, tiles = 0;
+        if (s < a.n_seqs) {
+            c0 = min(max(a.cu[s], 0), a.n_tokens);
+            n = min(max(a.cu[s + 1], c0), a.n_tokens) - c0;
+            const int rows = n * G;
+            if (rows >= min_rows && rows <= max_rows) tiles = (rows + RT - 1) / RT;
+        }
+        int incl = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += o;
+        }
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        if (idx < total) {
+            const int w = __ffsll((unsigned long long)__ballot(incl > idx)) - 1;
+            t.seq = base + w;
+            t.q0 = __builtin_amdgcn_readlane(c0, w);
+            t.n = __builtin_amdgcn_readlane(n, w);
+            t.rows = t.n * G;
+            t.r0 = (idx - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(tiles, w))) * RT;
+            t.kv_len = max(a.kv_len[t.seq], 0);
+            return true;
+        }
+        idx -= total;
+    }
+    return false;
+}
+
+// The 32-key blocks [begin, end) that split `sp` of a tile's rows
+// r0 .. r0 + RT - 1 walks, and the positions of its first and last row.
+struct Range {
+    int begin, end, p_first, p_last, limit;
+};
+template <int RT>
+__device__ __forceinline__ Range tile_range(const KvAttn& a, const Tile& t, int G, int sp, int least) {
+    Range r;
+    r.limit = min(t.kv_len, a.max_pages << a.c.page_shift);
+    r.p_first = t.kv_len - t.n + t.r0 / G;
+    r.p_last = t.kv_len - t.n + min(t.r0 + RT - 1, t.rows - 1) / G;
+    const int lo = a.window > 0 ? max(0, r.p_first - a.window + 1) : 0;
+    const int hi = min(r.limit - 1, r.p_last);
+    r.begin = lo >> 5;
+    r.end = hi >= lo ? (hi >> 5) + 1 : r.begin;
+    const int nb = r.end - r.begin;
+    const int chunk = max(least, (nb + a.splits - 1) / a.splits);
+    r.begin = min(r.begin + sp * chunk, r.end);
+    r.end = min(r.begin + chunk, r.end);
+    return r;
+}
+
+// The power of two that brings a row of magnitude amax into fp16's range
+// ([2^14, 2^15)), and its inverse.
+__device__ __forceinline__ float row_unit(float amax, float& inv) {
+    const int e = min(max(int(__float_as_uint(amax) >> 23) - 127, -100), 127);
+    inv = __uint_as_float(uint32_t(14 - e + 127) << 23);
+    return __uint_as_float(uint32_t(e - 14 + 127) << 23);
+}
+
+// Few rows: 16 query rows of one sequence and KV head per block, each of its
+// 4 waves over its own 32-key blocks (every fourth of the block's range), in
+// registers from the cache to the sums: a lane's 16-byte loads are operands
+// of the 16x16x32 products as they lie in the cache. S^T = K Q^T leaves a
+// lane (row l & 15, octet l >> 4) with the 8 keys of its octet, which are its
+// operand of O^T += V^T P^T. The waves' sums meet in LDS.
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int max_rows) {
+    constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
+    constexpr int S = HD / 32;                   // k steps of a score product
+    constexpr int NK = S / (TYPE == WV_KV_F16 ? 1 : 2);   // 16-byte K loads of a 16-key tile
+    constexpr int T = HD / 16;                   // dim tiles of the output
+    constexpr int NV = T / (TYPE == WV_KV_F16 ? 1 : 2);   // 16-byte V loads
+    constexpr int BB = 32 * HD * E;              // bytes of a block
+    constexpr int LD = HD + 4;
+    __shared__ float red[4][16][LD];
+    __shared__ float rm[4][16], rl[4][16];
+
+    const int kvh = blockIdx.y, sp = blockIdx.z;
+    Tile t;
+    if (!find_tile<16>(a, G, blockIdx.x, 1, max_rows, t)) return;
+    const Range rg = tile_range<16>(a, t, G, sp, 4);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = lane & 15, g = lane >> 4;
+
+    const int row = t.r0 + n;
+    const bool live = row < t.rows;
+    const int pos = t.kv_len - t.n + (live ? row : t.r0) / G;
+    const int first = a.window > 0 ? pos - a.window + 1 : 0;
+
+    // the query row: dims of lane group g in the order of the K codes
+    h8 qh[S], ql[S];
+    float qs;
+    {
+        const int tok = (live ? row : t.r0) / G, h = kvh * G + (live ? row : t.r0) % G;
+        const float* qp = a.q + int64_t(t.q0 + tok) * a.qs + h * HD;
+        float x[S][8], m = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int d = TYPE == WV_KV_F16 ? 8 * (4 * s + g) + j : 16 * (4 * (s / 2) + g) + 8 * (s % 2) + j;
+                x[s][j] = qp[d];
+                m = fmaxf(m, fabsf(x[s][j]));
+            }
+        float inv;
+        qs = row_unit(max_over_quads(m), inv) * a.scale * kLog2e;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[s][j] *= inv;
+            split8(x[s], qh[s], ql[s]);
+        }
+    }
+
+    f4 o[T];
+#pragma unroll
+    for (int i = 0; i < T; ++i) o[i] = f4{0, 0, 0, 0};
+    float mx = kNoMax, l = 0.0f;
+    int eo = -200;  // E: the outputs are in units of 2^eo
+
+    const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
+    const int pb = a.c.page_shift - 5;  // log2 blocks per page
+    auto block_at = [&](int kb, bool& ok) {
+        const int pg = __builtin_amdgcn_readfirstlane(pages[kb >> pb]);
+        ok = unsigned(pg) < unsigned(a.c.n_pages);
+        return kv_block(a.c, ok ? pg : 0, kvh, (kb & ((1 << pb) - 1)) << 5);
+    };
+    // key of A row n in tile x: index x * 4 + (n & 3) of octet n >> 2
+    const int key0 = kv_octet_key(n >> 2, n & 3);
+    uint4 kr[2][NK], vr[NV];
+    float4 sk[2], sv[2];
+    auto load_k = [&](int64_t b) {
+        const uint8_t* p = a.c.k + b * BB;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+                kr[x][i] = ld_nt16(reinterpret_cast<const uint4*>(p + ((4 * i + g) * 32 + key0 + 8 * x) * 16));
+    };
+    auto load_v = [&](int64_t b) {
+        const uint8_t* p = a.c.v + b * BB + g * HD * 8 * E;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) vr[i] = ld_nt16(reinterpret_cast<const uint4*>(p + (16 * i + n) * 16));
+    };
+    auto load_s = [&](int64_t b) {
+        const float4* p = reinterpret_cast<const float4*>(a.c.s + b * kKvScales + g * 16);
+        sk[0] = p[0], sk[1] = p[1], sv[0] = p[2], sv[1] = p[3];
+    };
+
+    int kb = rg.begin + wave;
+    bool ok = false;
+    int64_t blk = 0;
+    if (kb < rg.end) {
+        blk = block_at(kb, ok);
+        load_s(blk);
+        load_k(blk);
+        load_v(blk);
+    }
+    while (kb < rg.end) {
+        const int next = kb + 4;
+        bool nok = false;
+        int64_t nblk = 0;
+        if (next < rg.end) nblk = block_at(next, nok);
+        f4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            h8 f0, f1;
+            if (TYPE == WV_KV_F16) {
+                f0 = as_half(kr[0][s]), f1 = as_half(kr[1][s]);
+            } else {
+                const uint4 u0 = kr[0][s / 2], u1 = kr[1][s / 2];
+                f0 = s % 2 ? q8_half(u0.z, u0.w) : q8_half(u0.x, u0.y);
+                f1 = s % 2 ? q8_half(u1.z, u1.w) : q8_half(u1.x, u1.y);
+            }
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, ql[s], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, ql[s], s1, 0, 0, 0);
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qh[s], s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, qh[s], s1, 0, 0, 0);
+        }
+        const float ks[8] = {sk[0].x, sk[0].y, sk[0].z, sk[0].w, sk[1].x, sk[1].y, sk[1].z, sk[1].w};
+        float vs[8] = {sv[0].x, sv[0].y, sv[0].z, sv[0].w, sv[1].x, sv[1].y, sv[1].z, sv[1].w};
+        if (next < rg.end) {
+            load_s(nblk);
+            load_k(nblk);
+        }
+        if (ok) {
+            float p[8], top = 0.0f, m = mx;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = (j < 4 ? s0[j & 3] : s1[j & 3]) * ks[j];
+            // whole: every row of the tile attends every key of the block
+            const int k0 = kb << 5;
+            const bool whole = k0 + 31 <= rg.p_first && k0 + 31 < rg.limit &&
+                               (a.window <= 0 || k0 > rg.p_last - a.window);
+            if (!whole) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = k0 + kv_octet_key(g, j);
+                    if (key > pos || key < first || key >= rg.limit) p[j] = -INFINITY;
+                    if (key >= rg.limit) vs[j] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                m = fmaxf(m, p[j]);
+                top = fmaxf(top, vs[j]);
+            }
+            m = max_over_quads(m);
+            top = max_over_quads(top);
+            const int et = __builtin_amdgcn_readfirstlane(int(__float_as_uint(top) >> 23) - 126);  // top < 2^et
+            float f = __builtin_amdgcn_exp2f((mx - m) * qs);
+            l *= f;
+            if (et > eo) {
+                f *= ldexpf(1.0f, max(eo - et, -250));
+                eo = et;
+            }
+            mx = m;
+            const float unit = ldexpf(1.0f, -eo);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(p[j] - m, qs, 14.0f));
+                l += e;
+                p[j] = whole || e != 0.0f ? e * (vs[j] * unit) : 0.0f;
+            }
+            h8 ph, pl;
+            split8(p, ph, pl);
+            if (__ballot(f != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < T; ++i) o[i] *= f;
+            }
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                h8 fv;
+                if (TYPE == WV_KV_F16) {
+                    fv = as_half(vr[i]);
+                } else {
+                    const uint4 u = vr[i / 2];
+                    fv = i % 2 ? q8_half(u.z, u.w) : q8_half(u.x, u.y);
+                }
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fv, pl, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fv, ph, o[i], 0, 0, 0);
+            }
+        }
+        if (next < rg.end) load_v(nblk);
+        kb = next;
+        ok = nok;
+    }
+
+    // the waves' sums: out = sum_w 2^(m_w - M) O_w / sum_w 2^(m_w - M) l_w
+    l = sum_over_quads(l);
+    const float back = ldexpf(1.0f, max(eo, -126));
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int md = 4 * g + k;
+            const int d = TYPE == WV_KV_F16 ? 16 * i + md : 32 * (i / 2) + 2 * md + i % 2;
+            red[wave][n][d] = o[i][k] * back;
+        }
+    if (g == 0) {
+        rm[wave][n] = mx * qs;
+        rl[wave][n] = l;
+    }
+    __syncthreads();
+    const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
+    const int orow = t.r0 + r;
+    if (orow >= t.rows) return;
+    float M = -INFINITY, w[4], L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (rl[i][r] != 0.0f) M = fmaxf(M, rm[i][r]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = rl[i][r] != 0.0f ? __builtin_amdgcn_exp2f(rm[i][r] - M) : 0.0f;
+        L += w[i] * rl[i][r];
+    }
+    const int tok = t.q0 + orow / G, head = kvh * G + orow % G;
+    const float inv = a.part ? 1.0f : L != 0.0f ? 1.0f / L : 0.0f;
+    float* dst = a.part ? a.part + ((int64_t(tok) * a.n_heads + head) * a.splits + sp) * LD
+                        : a.out + int64_t(tok) * a.os + head * HD;
+#pragma unroll
+    for (int d = c; d < HD; d += 16) {
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (w[i] != 0.0f) x += w[i] * red[i][r][d];
+        dst[d] = x * inv;
+    }
+    if (a.part && c == 0) {
+        dst[HD] = M;
+        dst[HD + 1] = L;
+    }
+}
+
+// The key ranges of one (token, head) row joined: the ranges' maxima and sums
+// weigh their partial rows, added in the order of the ranges by four waves.
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
+    constexpr int LD = HD + 4, W = HD / 64;
+    __shared__ float red[4][HD];
+    const int tok = blockIdx.x, head = blockIdx.y;
+    if (tok >= min(a.cu[a.n_seqs], a.n_tokens)) return;
+    const float* p = a.part + (int64_t(tok) * a.n_heads + head) * a.splits * LD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float m = -INFINITY, l = 0.0f;
+    if (lane < a.splits) {
+        m = p[lane * LD + HD];
+        l = p[lane * LD + HD + 1];
+    }
+    const float M = wave_maximum(l != 0.0f ? m : -INFINITY);
+    const float w = l != 0.0f ? __builtin_amdgcn_exp2f(m - M) : 0.0f;
+    const float L = wave_total(w * l);
+    float x[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) x[i] = 0.0f;
+    for (int s0 = wave; s0 < a.splits; s0 += 16) {  // four ranges' rows in flight
+        float y[4][W];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < W; ++i) y[k][i] = s0 + 4 * k < a.splits ? p[(s0 + 4 * k) * LD + W * lane + i] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (s0 + 4 * k) & 63));
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (s0 + 4 * k < a.splits) x[i] += ws * y[k][i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) red[wave][W * lane + i] = x[i];
+    __syncthreads();
+    if (threadIdx.x < HD) {
+        const int d = threadIdx.x;
+        const float y = red[0][d] + red[1][d] + red[2][d] + red[3][d];
+        a.out[int64_t(tok) * a.os + head * HD + d] = L != 0.0f ? y / L : 0.0f;
+    }
+}
+
+}  // namespace
+
+int kv_attn_splits(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
+    if (!n_seqs || !n_tokens) return 1;
+    const int64_t G = n_heads / c.n_kv;
+    const int64_t tiles = std::max<int64_t>((n_tokens * G + 15) / 16, std::min(n_seqs, n_tokens));
+    const int64_t width = int64_t(max_pages) << c.page_shift;
+    const int64_t keys = window > 0 ? std::min<int64_t>(width, int64_t(window) + 16 / G) : width;
+    const int64_t blocks = (keys + 31) / 32;
+    const int64_t most = std::min<int64_t>(kMaxSplits, (blocks + 3) / 4);
+    return int(std::max<int64_t>(1, std::min<int64_t>(512 / (tiles * c.n_kv), most)));
+}
+
+size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits) {
+    return splits > 1 ? size_t(n_tokens) * size_t(n_heads) * size_t(splits) * size_t(c.hd + 4) : 0;
+}
+
+int launch_kv_attn(const KvAttn& a, hipStream_t s) {
+    const int G = a.n_heads / a.c.n_kv;
+    const int64_t tiles = (int64_t(a.n_tokens) * G + 15) / 16 + a.n_seqs;
+    const dim3 grid{unsigned(tiles), unsigned(a.c.n_kv), unsigned(a.splits)};
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, G, 1 << 30); };
+    if (a.c.hd == 128)
+        a.c.type == WV_KV_F16 ? go(k_kv_attn_rows<128, WV_KV_F16>) : go(k_kv_attn_rows<128, WV_KV_Q8>);
+    else
+        a.c.type == WV_KV_F16 ? go(k_kv_attn_rows<64, WV_KV_F16>) : go(k_kv_attn_rows<64, WV_KV_Q8>);
+    if (a.splits > 1) {
+        const dim3 jg{unsigned(a.n_tokens), unsigned(a.n_heads)};
+        if (a.c.hd == 128)
+            hipLaunchKernelGGL(k_kv_attn_join<128>, jg, dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL(k_kv_attn_join<64>, jg, dim3(256), 0, s, a);
+    }
+    return int(hipGetLastError());
+}
+
+}  // namespace wv
+
+using namespace wv;
+
+namespace {
+
+// The checks of a batch's sizes.
+int check_batch(const char* what, uint64_t cache, const wv_kv_batch* b, int32_t n_heads, int32_t window, KvCache& c) {
+    if (!kv_lookup(cache, c)) return rt_fail(WV_E_HANDLE, "%s: unknown cache %llu", what, (unsigned long long)cache);
+    if (!b) return rt_fail(WV_E_ARG, "%s: nil batch", what);
+    if (n_heads <= 0 || n_heads % c.c.n_kv_heads || n_heads > 65535)
+        return rt_fail(WV_E_SHAPE, "%s: %d heads over %d KV heads", what, n_heads, c.c.n_kv_heads);
+    if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_pages < 0 || b->max_q < 0 || window < 0)
+        return rt_fail(WV_E_SHAPE, "%s: negative size (seqs %d, tokens %d, pages %d, max_q %d, window %d)", what,
+                       b->n_seqs, b->n_tokens, b->max_pages, b->max_q, window);
+    if (int64_t(b->max_pages) * c.c.page_size >= int64_t(1) << 31)
+        return rt_fail(WV_E_SHAPE, "%s: a table of %d pages of %d positions (2^31 and more)", what, b->max_pages,
+                       c.c.page_size);
+    if (int64_t(b->n_tokens) * n_heads >= int64_t(1) << 31 || b->n_tokens > 1 << 28 || b->n_seqs > 1 << 24)
+        return rt_fail(WV_E_SHAPE, "%s: %d tokens of %d heads, %d sequences in one call", what, b->n_tokens, n_heads,
+                       b->n_seqs);
+    return WV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch* batch, int32_t n_heads, int32_t window,
+                            size_t* bytes) {
+    KvCache c;
+    const int rc = check_batch("wv_kv_attention_scratch", cache, batch, n_heads, window, c);
+    if (rc) return rc;
+    if (!bytes) return rt_fail(WV_E_ARG, "wv_kv_attention_scratch: nil bytes");
+    const KvView v = c.layer(0);
+    const int sp = kv_attn_splits(v, batch->n_seqs, batch->n_tokens, batch->max_pages, batch->max_q, n_heads, window);
+    *bytes = kv_attn_part_floats(v, batch->n_tokens, n_heads, sp) * sizeof(float);
+    return WV_OK;
+}
+
+int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch* batch, const float* d_q, int64_t q_stride,
+                        int32_t n_heads, float scale, int32_t window, float* d_out, int64_t out_stride,
+                        void* d_scratch, size_t scratch_bytes, void* stream) {
+    KvCache c;
+    int rc = check_batch("wv_kv_attention", cache, batch, n_heads, window, c);
+    if (rc) return rc;
+    if (layer < 0 || layer >= c.c.n_layers)
+        return rt_fail(WV_E_ARG, "wv_kv_attention: layer %d of %d", layer, c.c.n_layers);
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return rt_fail(WV_E_ARG, "wv_kv_attention: scale %g", double(scale));
+    const int64_t w = int64_t(n_heads) * c.c.head_dim;
+    if (!q_stride) q_stride = w;
+    if (!out_stride) out_stride = w;
+    if (q_stride < w || out_stride < w)
+        return rt_fail(WV_E_SHAPE, "wv_kv_attention: row strides %lld and %lld under the row's %lld floats",
+                       (long long)q_stride, (long long)out_stride, (long long)w);
+    if (!batch->n_seqs || !batch->n_tokens) return WV_OK;
+    if (!d_q || !d_out || !batch->d_cu_q || !batch->d_kv_len || (batch->max_pages && !batch->d_pages))
+        return rt_fail(WV_E_ARG, "wv_kv_attention: nil q/out/cu_q/kv_len/pages");
+    (void)hipSetDevice(c.device);
+    hipStream_t s = rt_stream(stream, c.device);
+    KvAttn a{};
+    a.c = c.layer(layer);
+    a.q = d_q, a.out = d_out, a.qs = q_stride, a.os = out_stride;
+    a.cu = batch->d_cu_q, a.kv_len = batch->d_kv_len, a.pages = batch->d_pages;
+    a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages, a.max_q = batch->max_q;
+    a.n_heads = n_heads, a.window = std::min(window, 1 << 30), a.scale = scale;
+    a.splits = kv_attn_splits(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, n_heads, window);
+    const size_t floats = kv_attn_part_floats(a.c, a.n_tokens, n_heads, a.splits);
+    RtScratch sc;
+    if (d_scratch) {
+        if (reinterpret_cast<uintptr_t>(d_scratch) & 15)
+            return rt_fail(WV_E_ARG, "wv_kv_attention: scratch not 16-byte aligned");
+        if (scratch_bytes < floats * sizeof(float))
+            return rt_fail(WV_E_SHAPE, "wv_kv_attention: %zu bytes of scratch, needs %zu", scratch_bytes,
+                           floats * sizeof(float));
+        if (floats) a.part = static_cast<float*>(d_scratch);
+    } else if (floats && rt_capturing(s)) {
+        a.splits = 1;  // what a replay writes must not lie in a slot that other calls take
+    } else if (floats) {
+        if ((rc = sc.get(floats, s, "wv_kv_attention: scratch"))) return rc;
+        a.part = sc.f();
+    }
+    const int e = launch_kv_attn(a, s);
+    return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_kv_attention: kernel launch");
+}
+
+}  // extern "C"

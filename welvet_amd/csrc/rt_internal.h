@@ -20,5 +20,25 @@ int rt_ensure_init();
 bool rt_lookup(uint64_t h, DevBlob& out);
 // The device wv_init selected (-1 before any init).
 int rt_current_device();
+// `stream`, or the library's own stream of `device` for NULL.
+hipStream_t rt_stream(void* stream, int device);
+// Whether `s` is being captured into a HIP graph.
+bool rt_capturing(hipStream_t s);
+
+// A slot of the current device's per-call scratch (CallScratch, runtime.hip):
+// held from get() until this object goes, which has to be after the call's
+// last launch. Not for a stream under capture.
+class RtScratch {
+public:
+    RtScratch() = default;
+    RtScratch(const RtScratch&) = delete;
+    RtScratch& operator=(const RtScratch&) = delete;
+    ~RtScratch();
+    int get(size_t floats, hipStream_t s, const char* what);
+    float* f() const;
+
+private:
+    void* impl_ = nullptr;
+};
 
 }  // namespace wv

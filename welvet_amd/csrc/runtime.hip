@@ -10,12 +10,14 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <unordered_map>
 #include <vector>
 
 #include "../../include/welvet_hip.h"
+#include "rt_internal.h"
 #include "wv_internal.h"
 
 // Scratch of wv_matvec_dev_noalloc: a fixed device array, one copy per GPU
@@ -826,6 +828,19 @@ int rt_current_device() {
     std::lock_guard<std::mutex> lk(g_mu);
     return g_current;
 }
+hipStream_t rt_stream(void* stream, int device) { return stream_or_default(stream, device); }
+bool rt_capturing(hipStream_t s) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(s, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone;
+}
+RtScratch::~RtScratch() { delete static_cast<CallScratch*>(impl_); }
+int RtScratch::get(size_t floats, hipStream_t s, const char* what) {
+    CallScratch* c = new (std::nothrow) CallScratch();
+    if (!c) return fail(WV_E_OOM, "%s: host memory exhausted", what);
+    impl_ = c;
+    return c->get(floats, s, what);
+}
+float* RtScratch::f() const { return impl_ ? static_cast<CallScratch*>(impl_)->f() : nullptr; }
 }  // namespace wv
 
 using namespace wv;
