@@ -478,6 +478,35 @@ int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch *batch,
 int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch *batch, int32_t n_heads, int32_t window,
                             size_t *bytes);
 
+/* ---- sampling: the next token of each row of logits ---- */
+
+/* How each row's token is drawn: device arrays of one value per row; NULL
+ * leaves that step out (d_uniform is always needed). The reference draws on the
+ * host (model/sampling/topk.go, model/transformer/generate.go:53-183); here
+ * the random numbers are the caller's, so a draw can be repeated. */
+typedef struct wv_sampling {
+    const float *d_temperature; /* T; NaN or T <= 0: the largest logit's first index */
+    const int32_t *d_top_k;     /* <= 0 or >= vocab: all */
+    const float *d_top_p;       /* >= 1 or NaN: all; <= 0: one token */
+    const float *d_min_p;       /* <= 0 or NaN: all; > 1 is 1 */
+    const float *d_uniform;     /* u in [0, 1); others are clamped into it, NaN is 0 */
+} wv_sampling;
+
+/* Draws d_tokens[r] from row r of d_logits (rows of vocab floats, `stride`
+ * floats apart, 0: vocab): with w_i = exp((l_i - max) / T), tokens in order of
+ * falling logit, equal logits by index,
+ *   the first top_k tokens; of those the shortest prefix that holds at least
+ *   top_p of their weight; of those the ones with w_i >= min_p;
+ *   the token: the first by index at which the running sum of the kept
+ *   weights exceeds u times their total.
+ * NaN logits count as -inf; a +inf logit takes all. A row of nothing but -inf
+ * gives token -1. Weights are f32 (relative error about 2^-23) and summed
+ * exactly in units of 2^-44 of the largest. d_probs (may be NULL): the drawn
+ * token's share of the kept weights (1 where T <= 0, 0 for token -1). vocab is
+ * at most 2^19. Device pointers, enqueued on `stream`; allocates nothing. */
+int wv_sample_dev(const float *d_logits, int64_t stride, int32_t rows, int32_t vocab, const wv_sampling *sampling,
+                  int32_t *d_tokens, float *d_probs, void *stream);
+
 /* ---- streams ---- */
 
 /* Blocks until all work the library enqueued on `stream` (NULL = its own) is done. */

@@ -46,7 +46,7 @@ EXPORTS = (
     "wv_decoder_create", "wv_decoder_set_layer", "wv_decoder_set_output", "wv_decoder_set_kv",
     "wv_decoder_use_graph", "wv_decoder_generate", "wv_decoder_prefill", "wv_decoder_free",
     "wv_kv_create", "wv_kv_info", "wv_kv_free", "wv_kv_write_dev", "wv_kv_read_dev", "wv_kv_attention_dev",
-    "wv_kv_attention_scratch",
+    "wv_kv_attention_scratch", "wv_sample_dev",
 )
 
 
@@ -120,6 +120,7 @@ def lib():
     L.wv_kv_attention_dev.argtypes = [ctypes.c_uint64, ctypes.c_int32, _P, _P, _I64, ctypes.c_int32, ctypes.c_float,
                                       ctypes.c_int32, _P, _I64, _P, _SZ, _P]
     L.wv_kv_attention_scratch.argtypes = [ctypes.c_uint64, _P, ctypes.c_int32, ctypes.c_int32, _P]
+    L.wv_sample_dev.argtypes = [_P, _I64, ctypes.c_int32, ctypes.c_int32, _P, _P, _P, _P]
     _lib = L
     return L
 
