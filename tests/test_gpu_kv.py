@@ -185,7 +185,7 @@ LAYOUTS = [(8, 8, 64), (8, 2, 128), (5, 1, 64), (32, 8, 128), (6, 2, 64), (24, 1
 
 @pytest.mark.parametrize("typ", ["f16", "q8"])
 @pytest.mark.parametrize("heads,kv_heads,hd", LAYOUTS)
-@pytest.mark.parametrize("kv,new", [(1, 1), (31, 1), (33, 3), (200, 7), (65, 65), (700, 130)])
+@pytest.mark.parametrize("kv,new", [(1, 1), (31, 1), (33, 3), (200, 7), (65, 65), (700, 130), (2500, 301)])
 def test_attention_one_sequence(typ, heads, kv_heads, hd, kv, new):
     rng = np.random.default_rng(kv * 7 + heads)
     p = Pool(rng, [kv], kv_heads, hd, 32, typ).fill()

@@ -24,10 +24,13 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.402823466e38f;  // the running maximum of a row that has met no key
 constexpr int kMaxSplits = 64;
+constexpr int kFewRows = 16;  // query rows of a sequence and KV head up to which the row kernel takes it
 
 // 8 biased int8 codes (two words) as fp16: 0x6400 | b is 1024 + b, less 1152
 // the code; one byte permute and half a packed subtraction per code pair.
@@ -46,14 +49,8 @@ __device__ __forceinline__ h8 q8_half(uint32_t x, uint32_t y) {
     for (int i = 0; i < 4; ++i) r.h[i] -= b;
     return r.v;
 }
-__device__ __forceinline__ h8 as_half(uint4 x) {
-    union {
-        uint4 u;
-        h8 v;
-    } r;
-    r.u = x;
-    return r.v;
-}
+__device__ __forceinline__ h8 as_half(uint4 x) { return __builtin_bit_cast(h8, x); }
+__device__ __forceinline__ h8 as_half(u4 x) { return __builtin_bit_cast(h8, x); }
 
 // hi + lo of 8 floats: hi truncated to fp16, lo the rounded rest.
 __device__ __forceinline__ void split8(const float* x, h8& hi, h8& lo) {
@@ -172,9 +169,9 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     __shared__ float red[4][16][LD];
     __shared__ float rm[4][16], rl[4][16];
 
-    const int kvh = blockIdx.y, sp = blockIdx.z;
+    const int kvh = blockIdx.x, sp = blockIdx.z;
     Tile t;
-    if (!find_tile<16>(a, G, blockIdx.x, 1, max_rows, t)) return;
+    if (!find_tile<16>(a, G, blockIdx.y, 1, max_rows, t)) return;
     const Range rg = tile_range<16>(a, t, G, sp, 4);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = lane & 15, g = lane >> 4;
@@ -388,6 +385,277 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     }
 }
 
+// Many rows: 128 query rows of one sequence and KV head per block, 32 to a
+// wave, over tiles of 64 keys that the block stages through LDS once, as fp16
+// codes in operand order (a 16-byte unit per lane, so staging and reading are
+// linear and free of bank conflicts). While a tile is multiplied the next
+// one's codes are on their way into registers; they are converted into the
+// other buffer after it. S^T = K Q^T on 32x32x16 products leaves a lane with
+// one row (l & 31) and the 8 keys of octets h and 2 + h of each block
+// (h = l >> 5), which are its operand of O^T += V^T P^T. The V scales are
+// staged as s_j 2^-E already, with the factor by which E moved.
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows) {
+    constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
+    constexpr int BB = 32 * HD * E;       // bytes of a block's codes
+    constexpr int S = HD / 16;            // k steps of a score product
+    constexpr int T = HD / 32;            // dim tiles of the output
+    constexpr int UN = 32 * HD / 8;       // 16-byte fp16 units of a staged block
+    constexpr int NU = 2 * BB / 16 / 256; // 16-byte loads of a thread for two blocks of codes
+    constexpr int LD = HD + 4;
+    __shared__ u4 lk[2][2 * UN], lv[2][2 * UN];
+    __shared__ float ls[2][2][kKvScales];  // [buffer][block]: K scales, V scales / 2^E, by octet
+    __shared__ float lf[2];                // [buffer]: 2^(E before - E)
+    __shared__ int le;
+
+    const int kvh = blockIdx.x, sp = blockIdx.z;
+    // a sequence's later tiles walk more keys and start first; where all blocks
+    // run at once, two to a CU, the second half goes up again, so that the two
+    // of a CU walk about as many keys as those of any other
+    const int half = (gridDim.y + 1) / 2, y = int(blockIdx.y);
+    const bool once = gridDim.x * gridDim.y * gridDim.z <= 512;
+    const int idx = once && y >= half ? y - half : int(gridDim.y) - 1 - y;
+    Tile t;
+    if (!find_tile<128>(a, G, idx, min_rows, 1 << 30, t)) return;
+    const Range rg = tile_range<128>(a, t, G, sp, 8);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n = lane & 31, h = lane >> 5;
+
+    const int wr0 = t.r0 + 32 * wave;  // the wave's first row
+    const bool busy = wr0 < t.rows;
+    const int row = min(wr0 + n, t.rows - 1);
+    const int pos = t.kv_len - t.n + row / G;
+    const int first = a.window > 0 ? pos - a.window + 1 : 0;
+    const int w_first = t.kv_len - t.n + min(wr0, t.rows - 1) / G;       // positions of the wave's first
+    const int w_last = t.kv_len - t.n + min(wr0 + 31, t.rows - 1) / G;   // and last row
+    const int64_t orow = int64_t(t.q0 + row / G);
+    const int head = kvh * G + row % G;
+
+    h8 qh[S], ql[S];
+    float qs;
+    {
+        const float* qp = a.q + orow * a.qs + head * HD + 8 * h;
+        float x[S][8], m = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[s][j] = qp[16 * s + j];
+                m = fmaxf(m, fabsf(x[s][j]));
+            }
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+        float inv;
+        qs = row_unit(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), inv) * a.scale * kLog2e;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[s][j] *= inv;
+            split8(x[s], qh[s], ql[s]);
+        }
+    }
+    f16v o[T];
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
+    float mx = kNoMax, l = 0.0f;
+    int eo = -200;  // of wave 0, which stages the scales
+
+    const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
+    const int pb = a.c.page_shift - 5;
+    // block kb of the sequence; one past the range is read as its last and masked
+    auto block_at = [&](int kb, bool& ok) {
+        kb = min(kb, rg.end - 1);
+        const int pg = __builtin_amdgcn_readfirstlane(pages[kb >> pb]);
+        ok = unsigned(pg) < unsigned(a.c.n_pages);
+        return kv_block(a.c, ok ? pg : 0, kvh, (kb & ((1 << pb) - 1)) << 5);
+    };
+    u4 kr[NU], vr[NU];
+    float sk = 0.0f, sv = 0.0f;
+    int64_t b0 = 0, b1 = 0;
+    bool ok0 = false, ok1 = false;  // of the tile whose codes are in registers
+    auto load = [&](int kb) {
+        b0 = block_at(kb, ok0);
+        b1 = block_at(kb + 1, ok1);
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int64_t off = ((i * 256 + tid) / (BB / 16) ? b1 : b0) * BB + (i * 256 + tid) % (BB / 16) * 16;
+            kr[i] = *reinterpret_cast<const u4*>(a.c.k + off);
+            vr[i] = *reinterpret_cast<const u4*>(a.c.v + off);
+        }
+        if (wave == 0) {  // lane: scale (lane & 7) of octet (lane >> 3) & 3 of block lane >> 5
+            const float* p = a.c.s + (h ? b1 : b0) * kKvScales + (n >> 3) * 16 + (n & 7);
+            sk = p[0];
+            sv = p[8];
+        }
+    };
+    auto stage = [&](int kb, int buf) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int blk = (i * 256 + tid) / (BB / 16), u = (i * 256 + tid) % (BB / 16);
+            if (TYPE == WV_KV_F16) {
+                lk[buf][blk * UN + u] = kr[i];
+                lv[buf][blk * UN + u] = vr[i];
+            } else {
+                const u4 k0 = __builtin_bit_cast(u4, q8_half(kr[i].x, kr[i].y));
+                const u4 k1 = __builtin_bit_cast(u4, q8_half(kr[i].z, kr[i].w));
+                u4* dk = &lk[buf][blk * UN + (u >> 5) * 64 + (u & 31)];  // units 2c and 2c + 1 of a key
+                dk[0] = k0;
+                dk[32] = k1;
+                const u4 v0 = __builtin_bit_cast(u4, q8_half(vr[i].x, vr[i].y));
+                const u4 v1 = __builtin_bit_cast(u4, q8_half(vr[i].z, vr[i].w));
+                // two dims of an octet, side by side: every other four lanes store the second one first, so
+                // that eight lanes reach all banks
+                u4* dv = &lv[buf][blk * UN + 2 * u];
+                const int f = (tid >> 2) & 1;
+                dv[f] = f ? v1 : v0;
+                dv[1 - f] = f ? v0 : v1;
+            }
+        }
+        if (wave == 0) {
+            const int key = ((kb + h) << 5) + kv_octet_key(n >> 3, n & 7);
+            const bool in = key < rg.limit && (h ? ok1 : ok0);
+            const float v = in ? sv : 0.0f;
+            const int et = int(__float_as_uint(wave_maximum(fmaxf(v, 0.0f))) >> 23) - 126;
+            const int en = max(eo, et);
+            ls[buf][h][(n >> 3) * 16 + (n & 7)] = sk;
+            ls[buf][h][(n >> 3) * 16 + 8 + (n & 7)] = v * ldexpf(1.0f, -en);
+            if (lane == 0) lf[buf] = ldexpf(1.0f, max(eo - en, -250));
+            eo = en;
+        }
+    };
+
+    int kb = rg.begin;
+    bool c0 = false, c1 = false;  // whether the staged tile's blocks hold keys
+    if (kb < rg.end) {
+        load(kb);
+        stage(kb, 0);
+        c0 = ok0, c1 = ok1 && kb + 1 < rg.end;
+    }
+    __syncthreads();
+    for (int buf = 0; kb < rg.end; kb += 2, buf ^= 1) {
+        const bool more = kb + 2 < rg.end;
+        if (more) load(kb + 2);
+        const int k0 = kb << 5;
+        // nothing for this wave: every row stands before the tile, or past its window
+        const bool idle = !busy || k0 > w_last || (a.window > 0 && k0 + 63 <= w_first - a.window);
+        float f = lf[buf];
+        if (!idle) {
+            f16v s[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) s[b][k] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < S; ++c) {
+                    const h8 fk = as_half(lk[buf][b * UN + (2 * c + h) * 32 + n]);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, ql[c], s[b], 0, 0, 0);
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, qh[c], s[b], 0, 0, 0);
+                }
+            }
+            const bool whole = c0 && c1 && k0 + 63 <= w_first && k0 + 63 < rg.limit &&
+                               (a.window <= 0 || k0 > w_last - a.window);
+            float m = mx;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f4 ks = *reinterpret_cast<const f4*>(&ls[buf][b][(2 * (q >> 1) + h) * 16 + 4 * (q & 1)]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[b][4 * q + k] *= ks[k];
+                }
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
+                        if (key > pos || key < first || key >= rg.limit || !(b ? c1 : c0)) s[b][i] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][i]);
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+            m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            const float al = __builtin_amdgcn_exp2f((mx - m) * qs);
+            l *= al;
+            f *= al;
+            mx = m;
+            h8 ph[4], pl[4];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    const float* vp = &ls[buf][b][(2 * kk + h) * 16 + 8];
+                    const f4 v0 = *reinterpret_cast<const f4*>(vp), v1 = *reinterpret_cast<const f4*>(vp + 4);
+                    float p[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[b][8 * kk + j] - m, qs, 14.0f));
+                        l += e;
+                        p[j] = e * (j < 4 ? v0[j & 3] : v1[j & 3]);
+                        if (!whole) p[j] = e != 0.0f ? p[j] : 0.0f;
+                    }
+                    split8(p, ph[2 * b + kk], pl[2 * b + kk]);
+                }
+            if (__ballot(f != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < T; ++i)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[i][k] *= f;
+            }
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const h8 fv = as_half(lv[buf][(q >> 1) * UN + (2 * (q & 1) + h) * HD + 32 * i + n]);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv, pl[q], o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv, ph[q], o[i], 0, 0, 0);
+                }
+        } else if (busy && f != 1.0f) {
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[i][k] *= f;
+        }
+        if (more) {
+            stage(kb + 2, buf ^ 1);
+            c0 = ok0, c1 = ok1 && kb + 3 < rg.end;
+        }
+        __syncthreads();
+    }
+    if (tid == 0) le = eo;
+    __syncthreads();
+    if (!busy || wr0 + n >= t.rows) return;
+    const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
+    const float back = ldexpf(1.0f, max(le, -126));
+    const float inv = a.part ? back : l != 0.0f ? back / l : 0.0f;
+    float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
+    const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            f4 x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = o[i][4 * q + k] * inv;
+            float* d = dst + 32 * i + 8 * q + 4 * h;
+            if (al) {
+                *reinterpret_cast<f4*>(d) = x;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) d[k] = x[k];
+            }
+        }
+    if (a.part && h == 0) {
+        dst[HD] = mx * qs;
+        dst[HD + 1] = l;
+    }
+}
+
 // The key ranges of one (token, head) row joined: the ranges' maxima and sums
 // weigh their partial rows, added in the order of the ranges by four waves.
 template <int HD>
@@ -452,13 +720,32 @@ size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int split
 
 int launch_kv_attn(const KvAttn& a, hipStream_t s) {
     const int G = a.n_heads / a.c.n_kv;
-    const int64_t tiles = (int64_t(a.n_tokens) * G + 15) / 16 + a.n_seqs;
-    const dim3 grid{unsigned(tiles), unsigned(a.c.n_kv), unsigned(a.splits)};
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, G, 1 << 30); };
-    if (a.c.hd == 128)
-        a.c.type == WV_KV_F16 ? go(k_kv_attn_rows<128, WV_KV_F16>) : go(k_kv_attn_rows<128, WV_KV_Q8>);
-    else
-        a.c.type == WV_KV_F16 ? go(k_kv_attn_rows<64, WV_KV_F16>) : go(k_kv_attn_rows<64, WV_KV_Q8>);
+    const int64_t rows = int64_t(a.n_tokens) * G;
+    const bool f16 = a.c.type == WV_KV_F16;
+    auto go = [&](auto kern, int64_t tiles, int bound) {
+        const dim3 grid{unsigned(a.c.n_kv), unsigned(tiles), unsigned(a.splits)};
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, G, bound);
+    };
+    // Sequences with more than kFewRows rows go to the tile kernel, unless none
+    // can have as many; the others to the row kernel, unless there is but one.
+    const bool many = rows > kFewRows && int64_t(a.max_q ? a.max_q : a.n_tokens) * G > kFewRows;
+    const bool few = !many || a.n_seqs > 1;
+    if (few) {
+        const int64_t tiles = (rows + 15) / 16 + a.n_seqs;
+        const int most = many ? kFewRows : 1 << 30;
+        if (a.c.hd == 128)
+            f16 ? go(k_kv_attn_rows<128, WV_KV_F16>, tiles, most) : go(k_kv_attn_rows<128, WV_KV_Q8>, tiles, most);
+        else
+            f16 ? go(k_kv_attn_rows<64, WV_KV_F16>, tiles, most) : go(k_kv_attn_rows<64, WV_KV_Q8>, tiles, most);
+    }
+    if (many) {
+        const int64_t tiles = (rows + 127) / 128 + a.n_seqs;
+        const int least = few ? kFewRows + 1 : 1;
+        if (a.c.hd == 128)
+            f16 ? go(k_kv_attn_tile<128, WV_KV_F16>, tiles, least) : go(k_kv_attn_tile<128, WV_KV_Q8>, tiles, least);
+        else
+            f16 ? go(k_kv_attn_tile<64, WV_KV_F16>, tiles, least) : go(k_kv_attn_tile<64, WV_KV_Q8>, tiles, least);
+    }
     if (a.splits > 1) {
         const dim3 jg{unsigned(a.n_tokens), unsigned(a.n_heads)};
         if (a.c.hd == 128)
