@@ -2,8 +2,9 @@
 // KV cache.
 //
 // With t = scale log2(e) q.K the row's output is sum_j 2^(t_j - m) V_j over
-// sum_j 2^(t_j - m), m the running maximum: one pass over the keys, the sums
-// so far scaled by 2^(m_old - m_new) when m grows. K and V are codes c with a
+// sum_j 2^(t_j - m), m the running maximum rounded up to a whole number: one
+// pass over the keys, the sums so far scaled by 2^(m_old - m_new), exactly,
+// when m grows. K and V are codes c with a
 // scale s per key, exact in fp16, so with the query row split in two fp16
 // terms q = 2^e (qh + ql) (22 bits)
 //   t_j = (c_j.qh + c_j.ql) s_j * (2^e scale log2 e)
@@ -28,7 +29,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoMax = -3.402823466e38f;  // the running maximum of a row that has met no key
+constexpr float kNoMax = -3.0e38f;  // m of a row that has met no key
 constexpr int kMaxSplits = 64;
 constexpr int kFewRows = 16;  // query rows of a sequence and KV head up to which the row kernel takes it
 
@@ -52,15 +53,16 @@ __device__ __forceinline__ h8 q8_half(uint32_t x, uint32_t y) {
 __device__ __forceinline__ h8 as_half(uint4 x) { return __builtin_bit_cast(h8, x); }
 __device__ __forceinline__ h8 as_half(u4 x) { return __builtin_bit_cast(h8, x); }
 
-// hi + lo of 8 floats: hi truncated to fp16, lo the rounded rest.
+// hi + lo of 8 floats: hi truncated to fp16, lo the rounded rest (a mixed fma
+// each: fp16 in, fp16 out).
 __device__ __forceinline__ void split8(const float* x, h8& hi, h8& lo) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const auto h = __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]);
         hi[i] = _Float16(h[0]);
         hi[i + 1] = _Float16(h[1]);
-        lo[i] = _Float16(x[i] - float(h[0]));
-        lo[i + 1] = _Float16(x[i + 1] - float(h[1]));
+        lo[i] = _Float16(fmaf(float(hi[i]), -1.0f, x[i]));
+        lo[i + 1] = _Float16(fmaf(float(hi[i + 1]), -1.0f, x[i + 1]));
     }
 }
 
@@ -77,6 +79,10 @@ __device__ __forceinline__ float sum_over_quads(float v) {
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// A block's barrier for what lies in LDS: unlike __syncthreads it does not wait
+// for loads from memory that are on their way into registers.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // A tile of query rows: row = token * G + head of the group, in one sequence.
 struct Tile {
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     Tile t;
     if (!find_tile<16>(a, G, blockIdx.y, 1, max_rows, t)) return;
     const Range rg = tile_range<16>(a, t, G, sp, 4);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
 
     const int row = t.r0 + n;
@@ -271,14 +277,19 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
             s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qh[s], s0, 0, 0, 0);
             s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, qh[s], s1, 0, 0, 0);
         }
-        const float ks[8] = {sk[0].x, sk[0].y, sk[0].z, sk[0].w, sk[1].x, sk[1].y, sk[1].z, sk[1].w};
+        float ks[8] = {sk[0].x, sk[0].y, sk[0].z, sk[0].w, sk[1].x, sk[1].y, sk[1].z, sk[1].w};
         float vs[8] = {sv[0].x, sv[0].y, sv[0].z, sv[0].w, sv[1].x, sv[1].y, sv[1].z, sv[1].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // a NaN V scale makes the score NaN, where the mask can drop it
+            ks[j] = vs[j] == vs[j] ? ks[j] : vs[j];
+            vs[j] = fmaxf(vs[j], 0.0f);
+        }
         if (next < rg.end) {
             load_s(nblk);
             load_k(nblk);
         }
         if (ok) {
-            float p[8], top = 0.0f, m = mx;
+            float p[8], top = 0.0f, m = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[j] = (j < 4 ? s0[j & 3] : s1[j & 3]) * ks[j];
             // whole: every row of the tile attends every key of the block
@@ -301,20 +312,23 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
             m = max_over_quads(m);
             top = max_over_quads(top);
             const int et = __builtin_amdgcn_readfirstlane(int(__float_as_uint(top) >> 23) - 126);  // top < 2^et
-            float f = __builtin_amdgcn_exp2f((mx - m) * qs);
-            l *= f;
+            m = fmaxf(mx, ceilf(m * qs));
+            float f = __builtin_amdgcn_exp2f(mx - m);
+            float add = 0.0f;
+            const float al = f;
             if (et > eo) {
                 f *= ldexpf(1.0f, max(eo - et, -250));
                 eo = et;
             }
             mx = m;
-            const float unit = ldexpf(1.0f, -eo);
+            const float unit = ldexpf(1.0f, -eo), up = 14.0f - m;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float e = __builtin_amdgcn_exp2f(fmaf(p[j] - m, qs, 14.0f));
-                l += e;
-                p[j] = whole || e != 0.0f ? e * (vs[j] * unit) : 0.0f;
+                const float e = __builtin_amdgcn_exp2f(fmaf(p[j], qs, up));
+                add += e;
+                p[j] = e * (vs[j] * unit);
             }
+            l = fmaf(l, al, add);
             h8 ph, pl;
             split8(p, ph, pl);
             if (__ballot(f != 1.0f)) {
@@ -351,7 +365,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
             red[wave][n][d] = o[i][k] * back;
         }
     if (g == 0) {
-        rm[wave][n] = mx * qs;
+        rm[wave][n] = mx;
         rl[wave][n] = l;
     }
     __syncthreads();
@@ -385,17 +399,24 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     }
 }
 
-// Many rows: 128 query rows of one sequence and KV head per block, 32 to a
-// wave, over tiles of 64 keys that the block stages through LDS once, as fp16
-// codes in operand order (a 16-byte unit per lane, so staging and reading are
-// linear and free of bank conflicts). While a tile is multiplied the next
-// one's codes are on their way into registers; they are converted into the
-// other buffer after it. S^T = K Q^T on 32x32x16 products leaves a lane with
-// one row (l & 31) and the 8 keys of octets h and 2 + h of each block
-// (h = l >> 5), which are its operand of O^T += V^T P^T. The V scales are
-// staged as s_j 2^-E already, with the factor by which E moved.
+// Many rows: 128 query rows of one sequence and KV head per block, in two
+// groups of 4 waves (32 rows to a wave): the groups take every other tile of
+// 64 keys and their sums are added at the end. S^T = K Q^T on 32x32x16
+// products leaves a lane with one row (l & 31) and the 8 keys of octets h and
+// 2 + h of each block (h = l >> 5), which are its operand of O^T += V^T P^T.
+//
+// A SIMD holds one wave of each group. A tile costs a wave about as long on
+// the matrix unit (4 HD / 8 products, 2048 cycles at 128) as on the vector
+// unit, so the groups run half a tile apart: between two barriers one group
+// multiplies (O += V P of its last tile, then S of its next) while the other
+// one turns scores into probabilities and stages. A group's K and V tiles lie
+// in LDS as fp16 codes in operand order (a 16-byte unit per lane, staging and
+// reading are linear and free of bank conflicts), one buffer each: a group
+// writes them only where none of its waves multiplies. The codes of the tile
+// after are on their way into registers meanwhile. The V scales are staged as
+// s_j 2^-E already, with the factor by which E moved.
 template <int HD, int TYPE>
-__global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows) {
+__global__ void __launch_bounds__(512, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
     constexpr int BB = 32 * HD * E;       // bytes of a block's codes
     constexpr int S = HD / 16;            // k steps of a score product
@@ -403,22 +424,19 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     constexpr int UN = 32 * HD / 8;       // 16-byte fp16 units of a staged block
     constexpr int NU = 2 * BB / 16 / 256; // 16-byte loads of a thread for two blocks of codes
     constexpr int LD = HD + 4;
-    __shared__ u4 lk[2][2 * UN], lv[2][2 * UN];
-    __shared__ float ls[2][2][kKvScales];  // [buffer][block]: K scales, V scales / 2^E, by octet
-    __shared__ float lf[2];                // [buffer]: 2^(E before - E)
-    __shared__ int le;
+    __shared__ u4 lkv[2][2][2 * UN];       // [group][K, V]; group 1's sums at the end
+    __shared__ float ls[2][2][2][kKvScales];  // [group][tile parity][block]: K scales, V scales / 2^E, by octet
+    __shared__ float lf[2][2];             // [group][tile parity]: 2^(E before - E)
+    __shared__ int le[2];
+    __shared__ float lm[2][4][32];         // group 1's m and l
 
     const int kvh = blockIdx.x, sp = blockIdx.z;
-    // a sequence's later tiles walk more keys and start first; where all blocks
-    // run at once, two to a CU, the second half goes up again, so that the two
-    // of a CU walk about as many keys as those of any other
-    const int half = (gridDim.y + 1) / 2, y = int(blockIdx.y);
-    const bool once = gridDim.x * gridDim.y * gridDim.z <= 512;
-    const int idx = once && y >= half ? y - half : int(gridDim.y) - 1 - y;
+    // a sequence's later tiles walk more keys and start first
     Tile t;
-    if (!find_tile<128>(a, G, idx, min_rows, 1 << 30, t)) return;
+    if (!find_tile<128>(a, G, int(gridDim.y) - 1 - int(blockIdx.y), min_rows, 1 << 30, t)) return;
     const Range rg = tile_range<128>(a, t, G, sp, 8);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
 
     const int wr0 = t.r0 + 32 * wave;  // the wave's first row
@@ -430,6 +448,92 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const int w_last = t.kv_len - t.n + min(wr0 + 31, t.rows - 1) / G;   // and last row
     const int64_t orow = int64_t(t.q0 + row / G);
     const int head = kvh * G + row % G;
+
+    const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
+    const int pb = a.c.page_shift - 5;
+    // block kb of the sequence; one past the range is read as its last and masked
+    auto block_at = [&](int kb, bool& ok) {
+        ok = kb < rg.end;
+        const int pg = __builtin_amdgcn_readfirstlane(pages[min(kb, rg.end - 1) >> pb]);
+        ok = ok && unsigned(pg) < unsigned(a.c.n_pages);
+        return kv_block(a.c, ok ? pg : 0, kvh, (kb & ((1 << pb) - 1)) << 5);
+    };
+    u4 kr[NU], vr[NU];
+    float sk = 0.0f, sv = 0.0f;
+    int64_t b0 = 0, b1 = 0;        // the blocks of the tile whose K codes are in kr
+    bool ok0 = false, ok1 = false;
+    auto load_k = [&](int kb) {
+        b0 = block_at(kb, ok0);
+        b1 = block_at(kb + 1, ok1);
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+            kr[i] = *reinterpret_cast<const u4*>(a.c.k + ((i * 256 + tid) / (BB / 16) ? b1 : b0) * BB +
+                                                 (i * 256 + tid) % (BB / 16) * 16);
+        if (wave == 0) {  // lane: scale (lane & 7) of octet (lane >> 3) & 3 of block lane >> 5
+            const float* p = a.c.s + (h ? b1 : b0) * kKvScales + (n >> 3) * 16 + (n & 7);
+            sk = p[0];
+            sv = p[8];
+        }
+    };
+    auto load_v = [&]() {  // of the same tile
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+            vr[i] = *reinterpret_cast<const u4*>(a.c.v + ((i * 256 + tid) / (BB / 16) ? b1 : b0) * BB +
+                                                 (i * 256 + tid) % (BB / 16) * 16);
+    };
+    int eo = -200;  // of the group's wave 0, which stages the scales
+    auto stage_k = [&](int kb, int par) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int blk = (i * 256 + tid) / (BB / 16), u = (i * 256 + tid) % (BB / 16);
+            if (TYPE == WV_KV_F16) {
+                lkv[grp][0][blk * UN + u] = kr[i];
+            } else {
+                u4* d = &lkv[grp][0][blk * UN + (u >> 5) * 64 + (u & 31)];  // units 2c and 2c + 1 of a key
+                d[0] = __builtin_bit_cast(u4, q8_half(kr[i].x, kr[i].y));
+                d[32] = __builtin_bit_cast(u4, q8_half(kr[i].z, kr[i].w));
+            }
+        }
+        if (wave == 0) {
+            const int key = ((kb + h) << 5) + kv_octet_key(n >> 3, n & 7);
+            const bool in = key < rg.limit && (h ? ok1 : ok0);
+            const float v = in ? fmaxf(sv, 0.0f) : 0.0f;
+            const int et = int(__float_as_uint(wave_maximum(v)) >> 23) - 126;
+            const int en = max(eo, et);
+            float* d = &ls[grp][par][h][(n >> 3) * 16 + (n & 7)];
+            d[0] = sv == sv ? sk : sv;  // a NaN V scale makes the score NaN, where the mask can drop it
+            d[8] = v * ldexpf(1.0f, -en);
+            if (lane == 0) lf[grp][par] = ldexpf(1.0f, max(eo - en, -250));
+            eo = en;
+        }
+    };
+    auto stage_v = [&]() {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int blk = (i * 256 + tid) / (BB / 16), u = (i * 256 + tid) % (BB / 16);
+            if (TYPE == WV_KV_F16) {
+                lkv[grp][1][blk * UN + u] = vr[i];
+            } else {
+                // two dims of an octet, side by side: every other four lanes store the second one first, so
+                // that eight lanes reach all banks
+                const u4 x = __builtin_bit_cast(u4, q8_half(vr[i].x, vr[i].y));
+                const u4 y = __builtin_bit_cast(u4, q8_half(vr[i].z, vr[i].w));
+                u4* d = &lkv[grp][1][blk * UN + 2 * u];
+                const int f = (tid >> 2) & 1;
+                d[f] = f ? y : x;
+                d[1 - f] = f ? x : y;
+            }
+        }
+    };
+
+    // tile j of the group: blocks first_kb + 4 j and the next one
+    const int kb0 = rg.begin + 2 * grp;
+    const int tiles = (rg.end - rg.begin + 3) / 4;  // of group 0; group 1's last may be empty
+    bool c0 = false, c1 = false;  // whether the staged tile's blocks hold keys
+    if (tiles) {
+        load_k(kb0);
+        load_v();
+    }
 
     h8 qh[S], ql[S];
     float qs;
@@ -459,108 +563,66 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 #pragma unroll
         for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
     float mx = kNoMax, l = 0.0f;
-    int eo = -200;  // of wave 0, which stages the scales
-
-    const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
-    const int pb = a.c.page_shift - 5;
-    // block kb of the sequence; one past the range is read as its last and masked
-    auto block_at = [&](int kb, bool& ok) {
-        kb = min(kb, rg.end - 1);
-        const int pg = __builtin_amdgcn_readfirstlane(pages[kb >> pb]);
-        ok = unsigned(pg) < unsigned(a.c.n_pages);
-        return kv_block(a.c, ok ? pg : 0, kvh, (kb & ((1 << pb) - 1)) << 5);
-    };
-    u4 kr[NU], vr[NU];
-    float sk = 0.0f, sv = 0.0f;
-    int64_t b0 = 0, b1 = 0;
-    bool ok0 = false, ok1 = false;  // of the tile whose codes are in registers
-    auto load = [&](int kb) {
-        b0 = block_at(kb, ok0);
-        b1 = block_at(kb + 1, ok1);
+    f16v s[2];           // the scores of the tile at hand
+    h8 ph[4], pl[4];     // its probabilities
+    auto qk = [&]() {
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const int64_t off = ((i * 256 + tid) / (BB / 16) ? b1 : b0) * BB + (i * 256 + tid) % (BB / 16) * 16;
-            kr[i] = *reinterpret_cast<const u4*>(a.c.k + off);
-            vr[i] = *reinterpret_cast<const u4*>(a.c.v + off);
-        }
-        if (wave == 0) {  // lane: scale (lane & 7) of octet (lane >> 3) & 3 of block lane >> 5
-            const float* p = a.c.s + (h ? b1 : b0) * kKvScales + (n >> 3) * 16 + (n & 7);
-            sk = p[0];
-            sv = p[8];
+        for (int k = 0; k < 16; ++k) s[0][k] = s[1][k] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < S; ++c) {
+            const h8 x = as_half(lkv[grp][0][(2 * c + h) * 32 + n]), y = as_half(lkv[grp][0][UN + (2 * c + h) * 32 + n]);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[c], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[c], s[1], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[c], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[c], s[1], 0, 0, 0);
         }
     };
-    auto stage = [&](int kb, int buf) {
+    auto pv = [&]() {
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const int blk = (i * 256 + tid) / (BB / 16), u = (i * 256 + tid) % (BB / 16);
-            if (TYPE == WV_KV_F16) {
-                lk[buf][blk * UN + u] = kr[i];
-                lv[buf][blk * UN + u] = vr[i];
-            } else {
-                const u4 k0 = __builtin_bit_cast(u4, q8_half(kr[i].x, kr[i].y));
-                const u4 k1 = __builtin_bit_cast(u4, q8_half(kr[i].z, kr[i].w));
-                u4* dk = &lk[buf][blk * UN + (u >> 5) * 64 + (u & 31)];  // units 2c and 2c + 1 of a key
-                dk[0] = k0;
-                dk[32] = k1;
-                const u4 v0 = __builtin_bit_cast(u4, q8_half(vr[i].x, vr[i].y));
-                const u4 v1 = __builtin_bit_cast(u4, q8_half(vr[i].z, vr[i].w));
-                // two dims of an octet, side by side: every other four lanes store the second one first, so
-                // that eight lanes reach all banks
-                u4* dv = &lv[buf][blk * UN + 2 * u];
-                const int f = (tid >> 2) & 1;
-                dv[f] = f ? v1 : v0;
-                dv[1 - f] = f ? v0 : v1;
+        for (int q = 0; q < 4; ++q) {
+            h8 fv[T];
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                fv[i] = as_half(lkv[grp][1][(q >> 1) * UN + (2 * (q & 1) + h) * HD + 32 * i + n]);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv[i], pl[q], o[i], 0, 0, 0);
             }
-        }
-        if (wave == 0) {
-            const int key = ((kb + h) << 5) + kv_octet_key(n >> 3, n & 7);
-            const bool in = key < rg.limit && (h ? ok1 : ok0);
-            const float v = in ? sv : 0.0f;
-            const int et = int(__float_as_uint(wave_maximum(fmaxf(v, 0.0f))) >> 23) - 126;
-            const int en = max(eo, et);
-            ls[buf][h][(n >> 3) * 16 + (n & 7)] = sk;
-            ls[buf][h][(n >> 3) * 16 + 8 + (n & 7)] = v * ldexpf(1.0f, -en);
-            if (lane == 0) lf[buf] = ldexpf(1.0f, max(eo - en, -250));
-            eo = en;
+#pragma unroll
+            for (int i = 0; i < T; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv[i], ph[q], o[i], 0, 0, 0);
         }
     };
 
-    int kb = rg.begin;
-    bool c0 = false, c1 = false;  // whether the staged tile's blocks hold keys
-    if (kb < rg.end) {
-        load(kb);
-        stage(kb, 0);
-        c0 = ok0, c1 = ok1 && kb + 1 < rg.end;
+    if (tiles) {
+        stage_k(kb0, 0);
+        c0 = ok0, c1 = ok1;
+        if (tiles > 1) load_k(kb0 + 4);
     }
-    __syncthreads();
-    for (int buf = 0; kb < rg.end; kb += 2, buf ^= 1) {
-        const bool more = kb + 2 < rg.end;
-        if (more) load(kb + 2);
-        const int k0 = kb << 5;
+    lds_barrier();
+    if (grp) lds_barrier();  // half a tile behind
+    __builtin_amdgcn_s_setprio(1);
+    if (tiles) qk();
+    for (int j = 0; j < tiles; ++j) {
+        const int k0 = (kb0 + 4 * j) << 5, par = j & 1;
         // nothing for this wave: every row stands before the tile, or past its window
-        const bool idle = !busy || k0 > w_last || (a.window > 0 && k0 + 63 <= w_first - a.window);
-        float f = lf[buf];
+        const bool idle = !busy || !(c0 || c1) || k0 > w_last || (a.window > 0 && k0 + 63 <= w_first - a.window);
+        __builtin_amdgcn_s_setprio(0);
+        lds_barrier();
+        // K of the next tile, V of this one; then the codes after those
+        const bool d0 = c0, d1 = c1;
+        stage_v();
+        if (j + 1 < tiles) {
+            stage_k(kb0 + 4 * (j + 1), par ^ 1);
+            c0 = ok0, c1 = ok1;
+        }
+        float f = lf[grp][par];
         if (!idle) {
-            f16v s[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) s[b][k] = 0.0f;
-#pragma unroll
-                for (int c = 0; c < S; ++c) {
-                    const h8 fk = as_half(lk[buf][b * UN + (2 * c + h) * 32 + n]);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, ql[c], s[b], 0, 0, 0);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk, qh[c], s[b], 0, 0, 0);
-                }
-            }
-            const bool whole = c0 && c1 && k0 + 63 <= w_first && k0 + 63 < rg.limit &&
+            const bool whole = d0 && d1 && k0 + 63 <= w_first && k0 + 63 < rg.limit &&
                                (a.window <= 0 || k0 > w_last - a.window);
-            float m = mx;
+            float m = -INFINITY;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const f4 ks = *reinterpret_cast<const f4*>(&ls[buf][b][(2 * (q >> 1) + h) * 16 + 4 * (q & 1)]);
+                    const f4 ks = *reinterpret_cast<const f4*>(&ls[grp][par][b][(2 * (q >> 1) + h) * 16 + 4 * (q & 1)]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) s[b][4 * q + k] *= ks[k];
                 }
@@ -570,7 +632,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                        if (key > pos || key < first || key >= rg.limit || !(b ? c1 : c0)) s[b][i] = -INFINITY;
+                        if (key > pos || key < first || key >= rg.limit || !(b ? d1 : d0)) s[b][i] = -INFINITY;
                     }
             }
 #pragma unroll
@@ -578,60 +640,71 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 #pragma unroll
                 for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][i]);
             const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-            m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-            const float al = __builtin_amdgcn_exp2f((mx - m) * qs);
-            l *= al;
+            m = fmaxf(mx, ceilf(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * qs));
+            const float al = __builtin_amdgcn_exp2f(mx - m), up = 14.0f - m;
             f *= al;
             mx = m;
-            h8 ph[4], pl[4];
+            float add[4];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
-                    const float* vp = &ls[buf][b][(2 * kk + h) * 16 + 8];
+                    const float* vp = &ls[grp][par][b][(2 * kk + h) * 16 + 8];
                     const f4 v0 = *reinterpret_cast<const f4*>(vp), v1 = *reinterpret_cast<const f4*>(vp + 4);
-                    float p[8];
+                    float p[8], sum = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(s[b][8 * kk + j] - m, qs, 14.0f));
-                        l += e;
-                        p[j] = e * (j < 4 ? v0[j & 3] : v1[j & 3]);
-                        if (!whole) p[j] = e != 0.0f ? p[j] : 0.0f;
+                    for (int i = 0; i < 8; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(s[b][8 * kk + i], qs, up));
+                        sum += e;
+                        p[i] = e * (i < 4 ? v0[i & 3] : v1[i & 3]);
                     }
                     split8(p, ph[2 * b + kk], pl[2 * b + kk]);
+                    add[2 * b + kk] = sum;
                 }
-            if (__ballot(f != 1.0f)) {
+            l = fmaf(l, al, (add[0] + add[1]) + (add[2] + add[3]));
+        } else {
 #pragma unroll
-                for (int i = 0; i < T; ++i)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) o[i][k] *= f;
-            }
-#pragma unroll
-            for (int i = 0; i < T; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const h8 fv = as_half(lv[buf][(q >> 1) * UN + (2 * (q & 1) + h) * HD + 32 * i + n]);
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv, pl[q], o[i], 0, 0, 0);
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv, ph[q], o[i], 0, 0, 0);
-                }
-        } else if (busy && f != 1.0f) {
+            for (int q = 0; q < 4; ++q) ph[q] = pl[q] = h8{};
+        }
+        if (__ballot(f != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < T; ++i)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[i][k] *= f;
         }
-        if (more) {
-            stage(kb + 2, buf ^ 1);
-            c0 = ok0, c1 = ok1 && kb + 3 < rg.end;
-        }
-        __syncthreads();
+        // the next codes set out where neither scores nor probabilities in the making take registers
+        if (j + 1 < tiles) load_v();
+        if (j + 2 < tiles) load_k(kb0 + 4 * (j + 2));
+        lds_barrier();
+        __builtin_amdgcn_s_setprio(1);
+        pv();
+        qk();  // after the last tile, of that one again, for nothing
     }
-    if (tid == 0) le = eo;
+    if (!grp) lds_barrier();
+    if (tid == 0) le[grp] = eo;
+    // group 1's sums through LDS; both groups are done with the tiles
     __syncthreads();
-    if (!busy || wr0 + n >= t.rows) return;
+    float* lo = reinterpret_cast<float*>(&lkv[0][0][0]) + wave * 32 * HD;
+    const int ec = max(max(le[0], le[1]), -126);
+    if (grp) {
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) lo[(i * 16 + k) * 64 + lane] = o[i][k];
+        lm[0][wave][n] = mx;
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        lm[1][wave][n] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    __syncthreads();
+    if (grp || wr0 + n >= t.rows) return;
     const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
-    const float back = ldexpf(1.0f, max(le, -126));
+    const float m1 = lm[0][wave][n], l1 = lm[1][wave][n], M = fmaxf(mx, m1);
+    float w0 = __builtin_amdgcn_exp2f(mx - M), w1 = __builtin_amdgcn_exp2f(m1 - M);
+    l = l * w0 + l1 * w1;
+    w0 *= ldexpf(1.0f, max(le[0] - ec, -250));  // the sums are in units of 2^E of their group
+    w1 *= ldexpf(1.0f, max(le[1] - ec, -250));
+    const float back = ldexpf(1.0f, ec);
     const float inv = a.part ? back : l != 0.0f ? back / l : 0.0f;
     float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
     const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
@@ -641,7 +714,8 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
         for (int q = 0; q < 4; ++q) {
             f4 x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = o[i][4 * q + k] * inv;
+            for (int k = 0; k < 4; ++k)
+                x[k] = (o[i][4 * q + k] * w0 + lo[(i * 16 + 4 * q + k) * 64 + lane] * w1) * inv;
             float* d = dst + 32 * i + 8 * q + 4 * h;
             if (al) {
                 *reinterpret_cast<f4*>(d) = x;
@@ -651,7 +725,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
             }
         }
     if (a.part && h == 0) {
-        dst[HD] = mx * qs;
+        dst[HD] = M;
         dst[HD + 1] = l;
     }
 }
@@ -722,9 +796,9 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
     const int G = a.n_heads / a.c.n_kv;
     const int64_t rows = int64_t(a.n_tokens) * G;
     const bool f16 = a.c.type == WV_KV_F16;
-    auto go = [&](auto kern, int64_t tiles, int bound) {
+    auto go = [&](auto kern, int64_t tiles, int bound, int threads = 256) {
         const dim3 grid{unsigned(a.c.n_kv), unsigned(tiles), unsigned(a.splits)};
-        hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, G, bound);
+        hipLaunchKernelGGL(kern, grid, dim3(unsigned(threads)), 0, s, a, G, bound);
     };
     // Sequences with more than kFewRows rows go to the tile kernel, unless none
     // can have as many; the others to the row kernel, unless there is but one.
@@ -742,9 +816,11 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
         const int64_t tiles = (rows + 127) / 128 + a.n_seqs;
         const int least = few ? kFewRows + 1 : 1;
         if (a.c.hd == 128)
-            f16 ? go(k_kv_attn_tile<128, WV_KV_F16>, tiles, least) : go(k_kv_attn_tile<128, WV_KV_Q8>, tiles, least);
+            f16 ? go(k_kv_attn_tile<128, WV_KV_F16>, tiles, least, 512)
+                : go(k_kv_attn_tile<128, WV_KV_Q8>, tiles, least, 512);
         else
-            f16 ? go(k_kv_attn_tile<64, WV_KV_F16>, tiles, least) : go(k_kv_attn_tile<64, WV_KV_Q8>, tiles, least);
+            f16 ? go(k_kv_attn_tile<64, WV_KV_F16>, tiles, least, 512)
+                : go(k_kv_attn_tile<64, WV_KV_Q8>, tiles, least, 512);
     }
     if (a.splits > 1) {
         const dim3 jg{unsigned(a.n_tokens), unsigned(a.n_heads)};
