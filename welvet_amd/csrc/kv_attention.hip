@@ -80,9 +80,29 @@ __device__ __forceinline__ float sum_over_quads(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// Ties a value to this place among the other volatile statements: what makes
+// it comes before, what uses it after.
+template <class V>
+__device__ __forceinline__ void pin(V& v) { asm volatile("" : "+v"(v)); }
+
 // A block's barrier for what lies in LDS: unlike __syncthreads it does not wait
 // for loads from memory that are on their way into registers.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Largest of 32 lanes' bit patterns of floats >= 0 (lanes 32..63 hold the same), in one instruction a step.
+__device__ __forceinline__ uint32_t max_of_32(float v) {
+    uint32_t x = __float_as_uint(v);
+    x = max(x, uint32_t(dpp_i<kDppRowShr1>(0, int(x))));
+    x = max(x, uint32_t(dpp_i<kDppRowShr2>(0, int(x))));
+    x = max(x, uint32_t(dpp_i<kDppRowShr4>(0, int(x))));
+    x = max(x, uint32_t(dpp_i<kDppRowShr8>(0, int(x))));
+    x = max(x, uint32_t(dpp_i<kDppRowBcast15>(0, int(x))));
+    return uint32_t(__builtin_amdgcn_readlane(int(x), 31));
+}
+// 2^e for a uniform e, clamped to what a normal float holds (0 below).
+__device__ __forceinline__ float exp2_int(int e) {
+    return e < -126 ? 0.0f : __uint_as_float(uint32_t(min(e, 127) + 127) << 23);
+}
 
 // A tile of query rows: row = token * G + head of the group, in one sequence.
 struct Tile {
@@ -399,44 +419,45 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     }
 }
 
-// Many rows: 128 query rows of one sequence and KV head per block, in two
-// groups of 4 waves (32 rows to a wave): the groups take every other tile of
-// 64 keys and their sums are added at the end. S^T = K Q^T on 32x32x16
-// products leaves a lane with one row (l & 31) and the 8 keys of octets h and
-// 2 + h of each block (h = l >> 5), which are its operand of O^T += V^T P^T.
+// Many rows: 128 query rows of one sequence and KV head per block, 32 to a
+// wave, over blocks of 32 keys that the four waves stage through LDS, as fp16
+// codes in operand order (a 16-byte unit per lane, so staging and reading are
+// linear and free of bank conflicts). S^T = K Q^T on 32x32x16 products leaves
+// a lane with one row (l & 31) and the 8 keys of octets h and 2 + h (h = l >>
+// 5), which are its operand of O^T += V^T P^T.
 //
-// A SIMD holds one wave of each group. A tile costs a wave about as long on
-// the matrix unit (4 HD / 8 products, 2048 cycles at 128) as on the vector
-// unit, so the groups run half a tile apart: between two barriers one group
-// multiplies (O += V P of its last tile, then S of its next) while the other
-// one turns scores into probabilities and stages. A group's K and V tiles lie
-// in LDS as fp16 codes in operand order (a 16-byte unit per lane, staging and
-// reading are linear and free of bank conflicts), one buffer each: a group
-// writes them only where none of its waves multiplies. The codes of the tile
-// after are on their way into registers meanwhile. The V scales are staged as
-// s_j 2^-E already, with the factor by which E moved.
+// A key block costs a wave 32 products (1024 cycles of the matrix unit) and
+// about as long on the vector unit, so one iteration holds three key blocks:
+// the products O += V P of the last one and S of the next one run under the
+// exponentials of the one between. The codes of the key block after those are
+// on their way into registers. The V scales are staged as s_j 2^-E already,
+// with the factor by which E moved.
 template <int HD, int TYPE>
-__global__ void __launch_bounds__(512, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows) {
+__global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
-    constexpr int BB = 32 * HD * E;       // bytes of a block's codes
-    constexpr int S = HD / 16;            // k steps of a score product
-    constexpr int T = HD / 32;            // dim tiles of the output
-    constexpr int UN = 32 * HD / 8;       // 16-byte fp16 units of a staged block
-    constexpr int NU = 2 * BB / 16 / 256; // 16-byte loads of a thread for two blocks of codes
+    constexpr int BB = 32 * HD * E;   // bytes of a block's codes
+    constexpr int S = HD / 16;        // k steps of a score product
+    constexpr int T = HD / 32;        // dim tiles of the output
+    constexpr int UN = 32 * HD / 8;   // 16-byte fp16 units of a staged block
+    constexpr int CU = BB / 16;       // 16-byte units of a block's codes
+    constexpr int NU = (CU + 255) / 256;  // 16-byte loads of a thread
     constexpr int LD = HD + 4;
-    __shared__ u4 lkv[2][2][2 * UN];       // [group][K, V]; group 1's sums at the end
-    __shared__ float ls[2][2][2][kKvScales];  // [group][tile parity][block]: K scales, V scales / 2^E, by octet
-    __shared__ float lf[2][2];             // [group][tile parity]: 2^(E before - E)
-    __shared__ int le[2];
-    __shared__ float lm[2][4][32];         // group 1's m and l
+    __shared__ u4 lk[2][UN], lv[2][UN];
+    __shared__ float ls[4][kKvScales];  // K scales, V scales / 2^E, by octet
+    __shared__ float lf[4];             // 2^(E before - E)
+    __shared__ int le;
 
     const int kvh = blockIdx.x, sp = blockIdx.z;
-    // a sequence's later tiles walk more keys and start first
+    // a sequence's later tiles walk more keys and start first; where all blocks
+    // run at once, two to a CU, the second half goes up again, so that the two
+    // of a CU walk about as many keys as those of any other
+    const int half = (gridDim.y + 1) / 2, y = int(blockIdx.y);
+    const bool once = gridDim.x * gridDim.y * gridDim.z <= 512;
+    const int idx = once && y >= half ? y - half : int(gridDim.y) - 1 - y;
     Tile t;
-    if (!find_tile<128>(a, G, int(gridDim.y) - 1 - int(blockIdx.y), min_rows, 1 << 30, t)) return;
+    if (!find_tile<128>(a, G, idx, min_rows, 1 << 30, t)) return;
     const Range rg = tile_range<128>(a, t, G, sp, 8);
-    const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
 
     const int wr0 = t.r0 + 32 * wave;  // the wave's first row
@@ -446,99 +467,91 @@ __global__ void __launch_bounds__(512, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const int first = a.window > 0 ? pos - a.window + 1 : 0;
     const int w_first = t.kv_len - t.n + min(wr0, t.rows - 1) / G;       // positions of the wave's first
     const int w_last = t.kv_len - t.n + min(wr0 + 31, t.rows - 1) / G;   // and last row
-    const int64_t orow = int64_t(t.q0 + row / G);
-    const int head = kvh * G + row % G;
 
     const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
     const int pb = a.c.page_shift - 5;
-    // block kb of the sequence; one past the range is read as its last and masked
-    auto block_at = [&](int kb, bool& ok) {
-        ok = kb < rg.end;
-        const int pg = __builtin_amdgcn_readfirstlane(pages[min(kb, rg.end - 1) >> pb]);
-        ok = ok && unsigned(pg) < unsigned(a.c.n_pages);
-        return kv_block(a.c, ok ? pg : 0, kvh, (kb & ((1 << pb) - 1)) << 5);
+    // Key block i of the range; one past it is read as the last and masked. Lane l holds the page of the
+    // i'th with i % 64 = l: asked for in ascending order, the table is read once in 64.
+    const int nb = rg.end - rg.begin;
+    int pg64 = 0;
+    auto block_at = [&](int i, bool& ok) {
+        if ((i & 63) == 0) pg64 = pages[(rg.begin + min(i + lane, nb - 1)) >> pb];
+        const int pg = __builtin_amdgcn_readlane(pg64, i & 63);
+        ok = i < nb && unsigned(pg) < unsigned(a.c.n_pages);
+        return kv_block(a.c, ok ? pg : 0, kvh, ((rg.begin + i) & ((1 << pb) - 1)) << 5);
     };
+    const bool loads = CU >= 256 || tid < CU;
     u4 kr[NU], vr[NU];
     float sk = 0.0f, sv = 0.0f;
-    int64_t b0 = 0, b1 = 0;        // the blocks of the tile whose K codes are in kr
-    bool ok0 = false, ok1 = false;
-    auto load_k = [&](int kb) {
-        b0 = block_at(kb, ok0);
-        b1 = block_at(kb + 1, ok1);
+    int64_t kblk = 0, vblk = 0;  // the blocks of kr and of the V codes to load next
+    auto load_k = [&](int64_t blk) {
+        if (loads)
 #pragma unroll
-        for (int i = 0; i < NU; ++i)
-            kr[i] = *reinterpret_cast<const u4*>(a.c.k + ((i * 256 + tid) / (BB / 16) ? b1 : b0) * BB +
-                                                 (i * 256 + tid) % (BB / 16) * 16);
-        if (wave == 0) {  // lane: scale (lane & 7) of octet (lane >> 3) & 3 of block lane >> 5
-            const float* p = a.c.s + (h ? b1 : b0) * kKvScales + (n >> 3) * 16 + (n & 7);
-            sk = p[0];
-            sv = p[8];
-        }
+            for (int i = 0; i < NU; ++i)
+                kr[i] = *reinterpret_cast<const u4*>(a.c.k + blk * BB + (i * 256 + tid) * 16);
     };
-    auto load_v = [&]() {  // of the same tile
-#pragma unroll
-        for (int i = 0; i < NU; ++i)
-            vr[i] = *reinterpret_cast<const u4*>(a.c.v + ((i * 256 + tid) / (BB / 16) ? b1 : b0) * BB +
-                                                 (i * 256 + tid) % (BB / 16) * 16);
+    auto load_s = [&](int64_t blk) {  // lanes 0..31: in order of octets
+        const float* p = a.c.s + blk * kKvScales + (n >> 3) * 16 + (n & 7);
+        sk = p[0];
+        sv = p[8];
     };
-    int eo = -200;  // of the group's wave 0, which stages the scales
-    auto stage_k = [&](int kb, int par) {
+    auto load_v = [&](int64_t blk) {
+        if (loads)
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const int blk = (i * 256 + tid) / (BB / 16), u = (i * 256 + tid) % (BB / 16);
-            if (TYPE == WV_KV_F16) {
-                lkv[grp][0][blk * UN + u] = kr[i];
-            } else {
-                u4* d = &lkv[grp][0][blk * UN + (u >> 5) * 64 + (u & 31)];  // units 2c and 2c + 1 of a key
-                d[0] = __builtin_bit_cast(u4, q8_half(kr[i].x, kr[i].y));
-                d[32] = __builtin_bit_cast(u4, q8_half(kr[i].z, kr[i].w));
+            for (int i = 0; i < NU; ++i)
+                vr[i] = *reinterpret_cast<const u4*>(a.c.v + blk * BB + (i * 256 + tid) * 16);
+    };
+    int eo = -126;  // of wave 0, which stages the scales
+    auto stage_k = [&](int buf) {
+        if (loads)
+#pragma unroll
+            for (int i = 0; i < NU; ++i) {
+                const int u = i * 256 + tid;
+                if (TYPE == WV_KV_F16) {
+                    lk[buf][u] = kr[i];
+                } else {
+                    u4* d = &lk[buf][(u >> 5) * 64 + (u & 31)];  // units 2c and 2c + 1 of a key
+                    d[0] = __builtin_bit_cast(u4, q8_half(kr[i].x, kr[i].y));
+                    d[32] = __builtin_bit_cast(u4, q8_half(kr[i].z, kr[i].w));
+                }
             }
-        }
-        if (wave == 0) {
-            const int key = ((kb + h) << 5) + kv_octet_key(n >> 3, n & 7);
-            const bool in = key < rg.limit && (h ? ok1 : ok0);
-            const float v = in ? fmaxf(sv, 0.0f) : 0.0f;
-            const int et = int(__float_as_uint(wave_maximum(v)) >> 23) - 126;
-            const int en = max(eo, et);
-            float* d = &ls[grp][par][h][(n >> 3) * 16 + (n & 7)];
+    };
+    auto stage_s = [&](int kb, bool ok, int ring) {
+        const int key = (kb << 5) + kv_octet_key(n >> 3, n & 7);
+        const float v = ok && key < rg.limit ? fmaxf(sv, 0.0f) : 0.0f;
+        const int et = int(max_of_32(v) >> 23) - 126;  // the largest is below 2^et
+        const int en = max(eo, et);
+        if (lane < 32) {
+            float* d = &ls[ring][(n >> 3) * 16 + (n & 7)];
             d[0] = sv == sv ? sk : sv;  // a NaN V scale makes the score NaN, where the mask can drop it
-            d[8] = v * ldexpf(1.0f, -en);
-            if (lane == 0) lf[grp][par] = ldexpf(1.0f, max(eo - en, -250));
-            eo = en;
+            d[8] = v * exp2_int(-en);
         }
+        if (lane == 0) lf[ring] = exp2_int(eo - en);
+        eo = en;
     };
-    auto stage_v = [&]() {
+    auto stage_v = [&](int buf) {
+        if (loads)
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const int blk = (i * 256 + tid) / (BB / 16), u = (i * 256 + tid) % (BB / 16);
-            if (TYPE == WV_KV_F16) {
-                lkv[grp][1][blk * UN + u] = vr[i];
-            } else {
-                // two dims of an octet, side by side: every other four lanes store the second one first, so
-                // that eight lanes reach all banks
-                const u4 x = __builtin_bit_cast(u4, q8_half(vr[i].x, vr[i].y));
-                const u4 y = __builtin_bit_cast(u4, q8_half(vr[i].z, vr[i].w));
-                u4* d = &lkv[grp][1][blk * UN + 2 * u];
-                const int f = (tid >> 2) & 1;
-                d[f] = f ? y : x;
-                d[1 - f] = f ? x : y;
+            for (int i = 0; i < NU; ++i) {
+                const int u = i * 256 + tid;
+                if (TYPE == WV_KV_F16) {
+                    lv[buf][u] = vr[i];
+                } else {
+                    // two dims of an octet, side by side: every other four lanes store the second one
+                    // first, so that eight lanes reach all banks
+                    const u4 v0 = __builtin_bit_cast(u4, q8_half(vr[i].x, vr[i].y));
+                    const u4 v1 = __builtin_bit_cast(u4, q8_half(vr[i].z, vr[i].w));
+                    const int f = (tid >> 2) & 1;
+                    lv[buf][2 * u + f] = f ? v1 : v0;
+                    lv[buf][2 * u + 1 - f] = f ? v0 : v1;
+                }
             }
-        }
     };
-
-    // tile j of the group: blocks first_kb + 4 j and the next one
-    const int kb0 = rg.begin + 2 * grp;
-    const int tiles = (rg.end - rg.begin + 3) / 4;  // of group 0; group 1's last may be empty
-    bool c0 = false, c1 = false;  // whether the staged tile's blocks hold keys
-    if (tiles) {
-        load_k(kb0);
-        load_v();
-    }
 
     h8 qh[S], ql[S];
     float qs;
     {
-        const float* qp = a.q + orow * a.qs + head * HD + 8 * h;
+        const float* qp = a.q + int64_t(t.q0 + row / G) * a.qs + (kvh * G + row % G) * HD + 8 * h;
         float x[S][8], m = 0.0f;
 #pragma unroll
         for (int s = 0; s < S; ++s)
@@ -563,148 +576,183 @@ __global__ void __launch_bounds__(512, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 #pragma unroll
         for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
     float mx = kNoMax, l = 0.0f;
-    f16v s[2];           // the scores of the tile at hand
-    h8 ph[4], pl[4];     // its probabilities
-    auto qk = [&]() {
+    u4 ph[2] = {}, pl[2] = {};  // the probabilities that wait for their product, as fp16
+
+    auto qk = [&](int buf, f16v& s) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) s[0][k] = s[1][k] = 0.0f;
+        for (int k = 0; k < 16; ++k) s[k] = 0.0f;
 #pragma unroll
         for (int c = 0; c < S; ++c) {
-            const h8 x = as_half(lkv[grp][0][(2 * c + h) * 32 + n]), y = as_half(lkv[grp][0][UN + (2 * c + h) * 32 + n]);
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[c], s[0], 0, 0, 0);
-            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[c], s[1], 0, 0, 0);
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[c], s[0], 0, 0, 0);
-            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[c], s[1], 0, 0, 0);
+            const h8 x = as_half(lk[buf][(2 * c + h) * 32 + n]);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[c], s, 0, 0, 0);
         }
     };
-    auto pv = [&]() {
+    auto pv = [&](int buf) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
             h8 fv[T];
 #pragma unroll
             for (int i = 0; i < T; ++i) {
-                fv[i] = as_half(lkv[grp][1][(q >> 1) * UN + (2 * (q & 1) + h) * HD + 32 * i + n]);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv[i], pl[q], o[i], 0, 0, 0);
+                fv[i] = as_half(lv[buf][(2 * q + h) * HD + 32 * i + n]);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv[i], as_half(pl[q]), o[i], 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < T; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv[i], ph[q], o[i], 0, 0, 0);
+            for (int i = 0; i < T; ++i) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv[i], as_half(ph[q]), o[i], 0, 0, 0);
         }
     };
 
-    if (tiles) {
-        stage_k(kb0, 0);
-        c0 = ok0, c1 = ok1;
-        if (tiles > 1) load_k(kb0 + 4);
+    bool ok0 = false, ok1 = false, ok2 = false;  // whether the key blocks b, b + 1, b + 2 exist
+    f16v sa, sb;
+    if (nb) {
+        const int64_t first_blk = block_at(0, ok0);
+        load_k(first_blk);
+        load_v(first_blk);
+        vblk = block_at(1, ok1);
+        kblk = block_at(2, ok2);
+        stage_k(0);
+        load_k(vblk);
+        if (2 * tid < UN) lv[1][2 * tid] = lv[1][2 * tid + 1] = u4{};  // times P = 0 in the first iteration
+        if (wave == 0) {
+            load_s(first_blk);
+            stage_s(rg.begin, ok0, 0);
+            load_s(vblk);
+            stage_s(rg.begin + 1, ok1, 1);
+            load_s(kblk);
+        }
+        stage_k(1);
+        load_k(kblk);
     }
-    lds_barrier();
-    if (grp) lds_barrier();  // half a tile behind
-    __builtin_amdgcn_s_setprio(1);
-    if (tiles) qk();
-    for (int j = 0; j < tiles; ++j) {
-        const int k0 = (kb0 + 4 * j) << 5, par = j & 1;
-        // nothing for this wave: every row stands before the tile, or past its window
-        const bool idle = !busy || !(c0 || c1) || k0 > w_last || (a.window > 0 && k0 + 63 <= w_first - a.window);
-        __builtin_amdgcn_s_setprio(0);
-        lds_barrier();
-        // K of the next tile, V of this one; then the codes after those
-        const bool d0 = c0, d1 = c1;
-        stage_v();
-        if (j + 1 < tiles) {
-            stage_k(kb0 + 4 * (j + 1), par ^ 1);
-            c0 = ok0, c1 = ok1;
-        }
-        float f = lf[grp][par];
-        if (!idle) {
-            const bool whole = d0 && d1 && k0 + 63 <= w_first && k0 + 63 < rg.limit &&
-                               (a.window <= 0 || k0 > w_last - a.window);
-            float m = -INFINITY;
+    __syncthreads();
+    // Key block b, its scores in s0: those of b + 1 into s1.
+    auto step = [&](int b, f16v& s0, f16v& s1) {
+        const int k0 = (rg.begin + b) << 5, cur = b & 1, ring = b & 3;
+        const bool live = busy && ok0 && k0 <= w_last && !(a.window > 0 && k0 + 31 <= w_first - a.window);
+        const bool whole = live && k0 + 31 <= w_first && k0 + 31 < rg.limit && (a.window <= 0 || k0 > w_last - a.window);
+        f4 ks[4];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+        for (int q = 0; q < 4; ++q)
+            ks[q] = *reinterpret_cast<const f4*>(&ls[ring][(2 * (q >> 1) + h) * 16 + 4 * (q & 1)]);
+        const float fe = lf[ring];
+        auto v_at = [&](int f) { return as_half(lv[cur ^ 1][(2 * (f / T) + h) * HD + 32 * (f % T) + n]); };
+        auto k_at = [&](int c) { return as_half(lk[cur ^ 1][(2 * c + h) * 32 + n]); };
+        h8 f0 = v_at(0), f1 = v_at(1);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const f4 ks = *reinterpret_cast<const f4*>(&ls[grp][par][b][(2 * (q >> 1) + h) * 16 + 4 * (q & 1)]);
+        for (int i = 0; i < 16; ++i) s0[i] *= ks[i >> 2][i & 3];
+        if (!whole) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) s[b][4 * q + k] *= ks[k];
-                }
-            if (!whole) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
-                        if (key > pos || key < first || key >= rg.limit || !(b ? d1 : d0)) s[b][i] = -INFINITY;
-                    }
+            for (int i = 0; i < 16; ++i) {
+                const int key = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                if (!live || key > pos || key < first || key >= rg.limit) s0[i] = -INFINITY;
             }
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][i]);
-            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-            m = fmaxf(mx, ceilf(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * qs));
-            const float al = __builtin_amdgcn_exp2f(mx - m), up = 14.0f - m;
-            f *= al;
-            mx = m;
-            float add[4];
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    const float* vp = &ls[grp][par][b][(2 * kk + h) * 16 + 8];
-                    const f4 v0 = *reinterpret_cast<const f4*>(vp), v1 = *reinterpret_cast<const f4*>(vp + 4);
-                    float p[8], sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(s[b][8 * kk + i], qs, up));
-                        sum += e;
-                        p[i] = e * (i < 4 ? v0[i & 3] : v1[i & 3]);
-                    }
-                    split8(p, ph[2 * b + kk], pl[2 * b + kk]);
-                    add[2 * b + kk] = sum;
-                }
-            l = fmaf(l, al, (add[0] + add[1]) + (add[2] + add[3]));
-        } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) ph[q] = pl[q] = h8{};
         }
+        // O += V P of key block b - 1, two dim tiles at a time. Between the products, piece by piece: K of
+        // b + 2 and V of b into the buffers that the last barrier freed, the loads after those, the maximum.
+        // The pins keep products and pieces in turn.
+        float m = -INFINITY, al = 0.0f, up = 0.0f;
+        bool ok3 = false;
+        auto piece = [&](int i) {
+            if (i == 0) stage_k(cur);
+            if (i == T / 2) stage_v(cur);
+            if (i == T) {
+                load_v(vblk);
+                vblk = kblk;
+                kblk = block_at(b + 3, ok3);
+                load_k(kblk);
+            }
+            if (i == 2 * T - 2) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) m = fmaxf(m, s0[e]);
+                pin(m);
+            }
+            if (i == 2 * T - 1) {
+                const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+                m = fmaxf(mx, ceilf(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])) * qs));
+                al = __builtin_amdgcn_exp2f(mx - m);
+                up = 14.0f - m;
+                mx = m;
+                pin(up);
+            }
+        };
+        h8 x = k_at(0);
+        f4 vs[2];
+        vs[0] = *reinterpret_cast<const f4*>(&ls[ring][h * 16 + 8]);
+#pragma unroll
+        for (int f = 0; f < 2 * T; f += 2) {
+            const int q = f / T, i = f % T;
+            h8 g0 = f0, g1 = f1;
+            pin(g0), pin(g1);
+            if (f + 2 < 2 * T) f0 = v_at(f + 2), f1 = v_at(f + 3);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g0, as_half(pl[q]), o[i], 0, 0, 0);
+            o[i + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g1, as_half(pl[q]), o[i + 1], 0, 0, 0);
+            piece(f);
+            pin(g0), pin(g1);
+            o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g0, as_half(ph[q]), o[i], 0, 0, 0);
+            o[i + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g1, as_half(ph[q]), o[i + 1], 0, 0, 0);
+            piece(f + 1);
+        }
+        // The scores of b + 1; between the products the probabilities of b, some keys at a time
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s1[e] = 0.0f;
+        float add[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < S; ++c) {
+            h8 y = x;
+            pin(y);
+            if (c + 1 < S) x = k_at(c + 1);
+            if (c % (S / 4) == 0 && c < S - S / 4)
+                vs[(4 * c / S + 1) & 1] = *reinterpret_cast<const f4*>(
+                    &ls[ring][(2 * ((4 * c / S + 1) >> 1) + h) * 16 + 8 + 4 * ((4 * c / S + 1) & 1)]);
+            s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[c], s1, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[c], s1, 0, 0, 0);
+#pragma unroll
+            for (int e = 16 / S * c; e < 16 / S * (c + 1); e += 2) {
+                const int q = e / 8, i = e % 8 / 2;
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(s0[e], qs, up));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(s0[e + 1], qs, up));
+                add[q] += e0;
+                add[q] += e1;
+                const float p0 = e0 * vs[(e >> 2) & 1][e & 3], p1 = e1 * vs[(e >> 2) & 1][(e + 1) & 3];
+                const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+                const h2 lo = {_Float16(fmaf(float(hi[0]), -1.0f, p0)), _Float16(fmaf(float(hi[1]), -1.0f, p1))};
+                uint32_t wh = __builtin_bit_cast(uint32_t, hi), wl = __builtin_bit_cast(uint32_t, lo);
+                pin(wh), pin(wl), pin(add[q]);
+                ph[q][i] = wh, pl[q][i] = wl;
+            }
+        }
+        l = fmaf(l, al, add[0] + add[1]);
+        const float f = fe * al;
+        if (wave == 0) {
+            stage_s(rg.begin + b + 2, ok2, (b + 2) & 3);
+            load_s(kblk);
+        }
+        ok0 = ok1, ok1 = ok2, ok2 = ok3;
         if (__ballot(f != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < T; ++i)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[i][k] *= f;
         }
-        // the next codes set out where neither scores nor probabilities in the making take registers
-        if (j + 1 < tiles) load_v();
-        if (j + 2 < tiles) load_k(kb0 + 4 * (j + 2));
         lds_barrier();
-        __builtin_amdgcn_s_setprio(1);
-        pv();
-        qk();  // after the last tile, of that one again, for nothing
+    };
+    if (nb) qk(0, sa);
+    // The first step stages into the buffer that qk(0) reads.
+    lds_barrier();
+    int b = 0;
+    for (; b + 1 < nb; b += 2) {
+        step(b, sa, sb);
+        step(b + 1, sb, sa);
     }
-    if (!grp) lds_barrier();
-    if (tid == 0) le[grp] = eo;
-    // group 1's sums through LDS; both groups are done with the tiles
+    if (b < nb) step(b++, sa, sb);
+    if (nb) pv((nb - 1) & 1);
+    if (tid == 0) le = eo;
     __syncthreads();
-    float* lo = reinterpret_cast<float*>(&lkv[0][0][0]) + wave * 32 * HD;
-    const int ec = max(max(le[0], le[1]), -126);
-    if (grp) {
-#pragma unroll
-        for (int i = 0; i < T; ++i)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) lo[(i * 16 + k) * 64 + lane] = o[i][k];
-        lm[0][wave][n] = mx;
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-        lm[1][wave][n] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    __syncthreads();
-    if (grp || wr0 + n >= t.rows) return;
+    if (!busy || wr0 + n >= t.rows) return;
     const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
-    const float m1 = lm[0][wave][n], l1 = lm[1][wave][n], M = fmaxf(mx, m1);
-    float w0 = __builtin_amdgcn_exp2f(mx - M), w1 = __builtin_amdgcn_exp2f(m1 - M);
-    l = l * w0 + l1 * w1;
-    w0 *= ldexpf(1.0f, max(le[0] - ec, -250));  // the sums are in units of 2^E of their group
-    w1 *= ldexpf(1.0f, max(le[1] - ec, -250));
-    const float back = ldexpf(1.0f, ec);
+    const int64_t orow = int64_t(t.q0 + row / G);
+    const int head = kvh * G + row % G;
+    const float back = ldexpf(1.0f, max(le, -126));
     const float inv = a.part ? back : l != 0.0f ? back / l : 0.0f;
     float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
     const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
@@ -714,8 +762,7 @@ __global__ void __launch_bounds__(512, 2) k_kv_attn_tile(KvAttn a, int G, int mi
         for (int q = 0; q < 4; ++q) {
             f4 x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                x[k] = (o[i][4 * q + k] * w0 + lo[(i * 16 + 4 * q + k) * 64 + lane] * w1) * inv;
+            for (int k = 0; k < 4; ++k) x[k] = o[i][4 * q + k] * inv;
             float* d = dst + 32 * i + 8 * q + 4 * h;
             if (al) {
                 *reinterpret_cast<f4*>(d) = x;
@@ -725,7 +772,7 @@ __global__ void __launch_bounds__(512, 2) k_kv_attn_tile(KvAttn a, int G, int mi
             }
         }
     if (a.part && h == 0) {
-        dst[HD] = M;
+        dst[HD] = mx;
         dst[HD + 1] = l;
     }
 }
@@ -816,11 +863,11 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
         const int64_t tiles = (rows + 127) / 128 + a.n_seqs;
         const int least = few ? kFewRows + 1 : 1;
         if (a.c.hd == 128)
-            f16 ? go(k_kv_attn_tile<128, WV_KV_F16>, tiles, least, 512)
-                : go(k_kv_attn_tile<128, WV_KV_Q8>, tiles, least, 512);
+            f16 ? go(k_kv_attn_tile<128, WV_KV_F16>, tiles, least)
+                : go(k_kv_attn_tile<128, WV_KV_Q8>, tiles, least);
         else
-            f16 ? go(k_kv_attn_tile<64, WV_KV_F16>, tiles, least, 512)
-                : go(k_kv_attn_tile<64, WV_KV_Q8>, tiles, least, 512);
+            f16 ? go(k_kv_attn_tile<64, WV_KV_F16>, tiles, least)
+                : go(k_kv_attn_tile<64, WV_KV_Q8>, tiles, least);
     }
     if (a.splits > 1) {
         const dim3 jg{unsigned(a.n_tokens), unsigned(a.n_heads)};
