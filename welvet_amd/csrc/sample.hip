@@ -20,11 +20,13 @@ constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;         // of falling a, kPerUnit to a factor of two; the last holds the rest
 constexpr float kPerUnit = 64.0f;
-constexpr int kList = kThreads;     // tokens ranked one per thread
+constexpr int kList = 512;          // tokens ranked one per thread
 constexpr int kFewK = 128;          // top-k up to which the candidates alone are looked at
+constexpr int kPass = 4 * kThreads; // tokens of a pass of the block, four to a thread
 constexpr int kSegment = 256;       // tokens of a wave's pass, in order of index
 constexpr int kMaxVocab = 1 << 19;  // 2^19 weights of at most 2^44 stay below 2^63
 constexpr int kSegments = kMaxVocab / kSegment;
+constexpr int kResident = 32768;    // logits of a row that stay in LDS
 
 // Order-preserving integer of a float (NaN does not occur).
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -33,73 +35,70 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 // Tokens as integers whose falling order is the tokens' order.
 __device__ __forceinline__ u64 token_key(float l, int i) { return u64(order_key(l)) << 32 | uint32_t(~i); }
+__device__ __forceinline__ float key_logit(u64 key) {
+    const uint32_t o = uint32_t(key >> 32);
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
 
-// The row's scale: log2(e) / T in two floats.
+// The row's scale: log2(e) / T in two floats, and the difference to the
+// maximum from which on weights are 0.
 struct Scale {
-    float max, hi, lo;
+    float max, hi, lo, least;
 };
-// log2 weight and weight of logit l. a is monotone in l; the product's and
-// the scale's rounding, which a drops, come back to first order in w.
+// log2 weight of logit l, monotone in l; the maximum itself (infinite or not) has 0.
 __device__ __forceinline__ float log_weight(const Scale& c, float l) {
-    return l == c.max ? 0.0f : (l - c.max) * c.hi;
+    const float t = fmaxf(fminf(l - c.max, 0.0f), c.least);  // inf - inf: min(NaN, 0) = 0
+    return fmaf(t, c.hi, t * c.lo);
 }
-__device__ __forceinline__ float weight(const Scale& c, float l) {
-    if (l == c.max) return 1.0f;
-    const float t = l - c.max, a = t * c.hi;
-    const float e = fmaf(t, c.lo, fmaf(t, c.hi, -a));
-    const float w = __builtin_amdgcn_exp2f(a);
-    return a > -100.0f ? fminf(fmaf(w, e * 0.6931472f, w), 1.0f) : 0.0f;
-}
+__device__ __forceinline__ float weight(const Scale& c, float l) { return __builtin_amdgcn_exp2f(log_weight(c, l)); }
 __device__ __forceinline__ int bin_of(float a) { return int(fminf(-a * kPerUnit, float(kBins - 1))); }
 // A weight in units of 2^-44: adding 256 leaves them in a double's last bits.
 __device__ __forceinline__ u64 fixed(float w) {
     return u64(__double_as_longlong(256.0 + double(w)) - __double_as_longlong(256.0));
 }
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
-    const uint32_t lo = __shfl_up(uint32_t(v), d, 64), hi = __shfl_up(uint32_t(v >> 32), d, 64);
+template <int Ctrl, int RowMask, int BankMask>
+__device__ __forceinline__ u64 dpp_u64(u64 v) {
+    const uint32_t lo = uint32_t(dpp_i<Ctrl, RowMask, BankMask>(0, int(uint32_t(v))));
+    const uint32_t hi = uint32_t(dpp_i<Ctrl, RowMask, BankMask>(0, int(uint32_t(v >> 32))));
     return u64(hi) << 32 | lo;
 }
+// Inclusive sums over the lanes.
 __device__ __forceinline__ u64 wave_scan(u64 v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = shfl_up64(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        const uint32_t lo = __shfl_xor(uint32_t(v), d, 64), hi = __shfl_xor(uint32_t(v >> 32), d, 64);
-        v += u64(hi) << 32 | lo;
-    }
+    v += dpp_u64<kDppRowShr1, 0xf, 0xf>(v);
+    v += dpp_u64<kDppRowShr2, 0xf, 0xf>(v);
+    v += dpp_u64<kDppRowShr4, 0xf, 0xe>(v);
+    v += dpp_u64<kDppRowShr8, 0xf, 0xc>(v);
+    v += dpp_u64<kDppRowBcast15, 0xa, 0xf>(v);
+    v += dpp_u64<kDppRowBcast31, 0xc, 0xf>(v);
     return v;
 }
 
+template <bool RESIDENT>
 struct Shared {
+    float row[RESIDENT ? kResident : 4];
     u64 hist[kBins];
     u64 list[kList];
     u64 weights[kList];
-    u64 seg[kSegments];
+    u64 seg[RESIDENT ? kResident / kSegment : kSegments];
     u64 part[kWaves];
     u64 key;   // a result of one thread for all
     u64 sum;
     int at, n;
 };
 
-// One row: its logits in registers (N > 0: at most N * 1024) or read again in
-// every pass. f(l, index) of this thread's logits; 256 consecutive ones to a
-// wave's pass. NaN counts as -inf.
-template <int N>
+// One row, read from memory once where it fits LDS, else in every pass.
+// each4(f): f(four logits, index of the first, pass) for this thread's ones,
+// 256 consecutive ones to a wave's pass. NaN and what lies behind the row are
+// -inf, which no step counts.
+template <bool RESIDENT>
 struct Row {
     const float* p;
+    float* lds;
     int vocab;
     bool aligned;
-    float r[N > 0 ? N : 1];
 
-    __device__ __forceinline__ float4 at(int i) const {
+    __device__ __forceinline__ float4 fetch(int i) const {
         float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         if (aligned && i + 3 < vocab) {
             x = *reinterpret_cast<const float4*>(p + i);
@@ -109,35 +108,55 @@ struct Row {
             if (i + 2 < vocab) x.z = p[i + 2];
             if (i + 3 < vocab) x.w = p[i + 3];
         }
-        x.x = x.x == x.x ? x.x : -INFINITY;
-        x.y = x.y == x.y ? x.y : -INFINITY;
-        x.z = x.z == x.z ? x.z : -INFINITY;
-        x.w = x.w == x.w ? x.w : -INFINITY;
         return x;
     }
-    __device__ __forceinline__ void load() {
-        if constexpr (N > 0) {
+    __device__ __forceinline__ static float4 clean(float4 x) {
+        x.x = fmaxf(x.x, -INFINITY);  // NaN: the other operand
+        x.y = fmaxf(x.y, -INFINITY);
+        x.z = fmaxf(x.z, -INFINITY);
+        x.w = fmaxf(x.w, -INFINITY);
+        return x;
+    }
+    __device__ __forceinline__ int passes() const { return (vocab + kPass - 1) / kPass; }
+    // From memory, four passes' loads on their way.
+    template <class F>
+    __device__ __forceinline__ void stream(F f) const {
+        const int n = passes(), i0 = 4 * int(threadIdx.x);
+        float4 x[4];
 #pragma unroll
-            for (int k = 0; k < N / 4; ++k) {
-                const float4 x = at(4 * kThreads * k + 4 * int(threadIdx.x));
-                r[4 * k] = x.x, r[4 * k + 1] = x.y, r[4 * k + 2] = x.z, r[4 * k + 3] = x.w;
-            }
+        for (int k = 0; k < 4; ++k) x[k] = fetch(k * kPass + i0);
+        for (int k = 0; k < n; ++k) {
+            const float4 y = x[0];
+            x[0] = x[1], x[1] = x[2], x[2] = x[3];
+            x[3] = fetch((k + 4) * kPass + i0);
+            f(clean(y), k * kPass + i0, k);
         }
     }
-    // f(four logits, index of the first, pass)
+    // The first pass over the row, which fills LDS.
+    template <class F>
+    __device__ __forceinline__ void first(F f) const {
+        if constexpr (RESIDENT) {
+            const int i0 = 4 * int(threadIdx.x);
+            float4 x[kResident / kPass];
+#pragma unroll
+            for (int k = 0; k < kResident / kPass; ++k) x[k] = fetch(k * kPass + i0);
+#pragma unroll
+            for (int k = 0; k < kResident / kPass; ++k) {
+                x[k] = clean(x[k]);
+                *reinterpret_cast<float4*>(lds + k * kPass + i0) = x[k];
+                f(x[k], k * kPass + i0, k);
+            }
+        } else {
+            stream(f);
+        }
+    }
     template <class F>
     __device__ __forceinline__ void each4(F f) const {
-        if constexpr (N > 0) {
-#pragma unroll
-            for (int k = 0; k < N / 4; ++k)
-                f(make_float4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]),
-                  4 * kThreads * k + 4 * int(threadIdx.x), k);
+        if constexpr (RESIDENT) {
+            const int n = passes(), i0 = 4 * int(threadIdx.x);
+            for (int k = 0; k < n; ++k) f(*reinterpret_cast<const float4*>(lds + k * kPass + i0), k * kPass + i0, k);
         } else {
-            const int passes = (vocab + 4 * kThreads - 1) / (4 * kThreads);
-            for (int k = 0; k < passes; ++k) {
-                const int i = 4 * kThreads * k + 4 * int(threadIdx.x);
-                f(at(i), i, k);
-            }
+            stream(f);
         }
     }
     template <class F>
@@ -149,19 +168,26 @@ struct Row {
             f(x.w, i + 3);
         });
     }
+    // Four logits from index i (a multiple of 4) on.
+    __device__ __forceinline__ float4 at(int i) const {
+        if constexpr (RESIDENT) return *reinterpret_cast<const float4*>(lds + i);
+        return clean(fetch(i));
+    }
 };
 
-__device__ __forceinline__ void clear_hist(Shared& s) {
-    s.hist[threadIdx.x] = 0;
-    s.hist[threadIdx.x + kThreads] = 0;
+template <bool R>
+__device__ __forceinline__ void clear_hist(Shared<R>& s) {
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) s.hist[threadIdx.x + i * kThreads] = 0;
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
 }
 
 // v[0 .. n) (n at most 2 * 1024) added up in order: the index where the sum
 // reaches `target` (> 0) into s.at, the sum in front of it into s.sum, and the
-// whole sum returned. s.at stays -1 where the whole is less.
-__device__ u64 find_in(Shared& s, const u64* v, int n, u64 target) {
+// whole sum returned. s.at is -1 where the whole is less.
+template <bool R>
+__device__ __forceinline__ u64 find_in(Shared<R>& s, const u64* v, int n, u64 target) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (t == 0) s.at = -1;
     const u64 x = 2 * t < n ? v[2 * t] : 0, y = 2 * t + 1 < n ? v[2 * t + 1] : 0;
@@ -169,9 +195,11 @@ __device__ u64 find_in(Shared& s, const u64* v, int n, u64 target) {
     if (lane == 63) s.part[wave] = incl;
     __syncthreads();
     u64 before = 0, whole = 0;
+#pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) before += s.part[w];
-        whole += s.part[w];
+        const u64 p = s.part[w];
+        if (w < wave) before += p;
+        whole += p;
     }
     before += incl - (x + y);
     if (before < target && before + x + y >= target) {
@@ -183,18 +211,15 @@ __device__ u64 find_in(Shared& s, const u64* v, int n, u64 target) {
     return whole;
 }
 
-// The cut's token where tokens of the same logit l share it: the `nth` (from
-// 1) of them by index.
-template <int N>
-__device__ u64 nth_equal(Shared& s, const Row<N>& row, float l, u64 nth) {
+// Where tokens of one logit l share the cut: the `nth` (from 1) of them by index.
+template <bool R>
+__device__ __forceinline__ u64 nth_equal(Shared<R>& s, const Row<R>& row, float l, u64 nth) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int segs = (row.vocab + kSegment - 1) / kSegment;
-    row.each4([&](float4 x, int i, int k) {
-        const int c = (i < row.vocab && x.x == l) + (i + 1 < row.vocab && x.y == l) + (i + 2 < row.vocab && x.z == l) +
-                      (i + 3 < row.vocab && x.w == l);
-        const u64 n = wave_sum(u64(c));
-        const int sg = k * kWaves + wave;
-        if (lane == 0 && sg < segs) s.seg[sg] = n;
+    row.each4([&](float4 x, int, int k) {
+        const int c = (x.x == l) + (x.y == l) + (x.z == l) + (x.w == l);
+        const int n = wave_total_i(c), sg = k * kWaves + wave;
+        if (lane == 0 && sg < segs) s.seg[sg] = u64(n);
     });
     __syncthreads();
     find_in(s, s.seg, segs, nth);
@@ -206,21 +231,23 @@ __device__ u64 nth_equal(Shared& s, const Row<N>& row, float l, u64 nth) {
         const float v[4] = {x.x, x.y, x.z, x.w};
         u64 c = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c += i + j < row.vocab && v[j] == l;
+        for (int j = 0; j < 4; ++j) c += v[j] == l;
         u64 before = wave_scan(c) - c;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (i + j < row.vocab && v[j] == l && ++before == want) s.key = token_key(l, i + j);
+            if (v[j] == l && ++before == want) s.key = token_key(l, i + j);
     }
     __syncthreads();
     return s.key;
 }
 
-// Ranks the s.n tokens of the list, one per thread: how many of them, and how
+// Ranks the n tokens of the list, one per thread: how many of them, and how
 // much weight, come before this thread's in the tokens' order.
-__device__ __forceinline__ void rank_list(const Shared& s, int n, u64 key, int& rank, u64& mass) {
+template <bool R>
+__device__ __forceinline__ void rank_list(const Shared<R>& s, int n, u64 key, int& rank, u64& mass) {
     rank = 0;
     mass = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) {
         const bool b = s.list[j] > key;
         rank += b;
@@ -228,30 +255,25 @@ __device__ __forceinline__ void rank_list(const Shared& s, int n, u64 key, int& 
     }
 }
 
-__device__ __forceinline__ float key_logit(u64 key) {
-    const uint32_t o = uint32_t(key >> 32);
-    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
-}
-
 // The cut that keeps, of the tokens down to `floor` (0: all), the first
-// `target` (MASS: the shortest prefix whose weights reach target). s.hist
-// holds their counts (weights) by bin.
-template <bool MASS, int N>
-__device__ u64 find_cut(Shared& s, const Row<N>& row, const Scale& c, u64 floor, u64 target) {
+// `target` (by_mass: the shortest prefix whose weights reach target); floor
+// where there are not as many. s.hist holds their counts (weights) by bin.
+template <bool R>
+__device__ __forceinline__ u64 find_cut(Shared<R>& s, const Row<R>& row, const Scale& c, u64 floor, u64 target,
+                                     bool by_mass) {
     find_in(s, s.hist, kBins, target);
     const int bin = s.at;
+    if (bin < 0) return floor;
     const u64 left = target - s.sum;  // of this bin
     __syncthreads();
     clear_hist(s);
-    auto in_bin = [&](float l, int i) {
-        return i < row.vocab && bin_of(log_weight(c, l)) == bin && token_key(l, i) >= floor;
-    };
     row.each([&](float l, int i) {
-        if (in_bin(l, i)) {
+        const float a = log_weight(c, l);
+        if (bin_of(a) == bin && l > -INFINITY && token_key(l, i) >= floor) {
             const int at = atomicAdd(&s.n, 1);
             if (at < kList) {
                 s.list[at] = token_key(l, i);
-                if (MASS) s.weights[at] = fixed(weight(c, l));
+                s.weights[at] = fixed(__builtin_amdgcn_exp2f(a));
             }
         }
     });
@@ -263,7 +285,7 @@ __device__ u64 find_cut(Shared& s, const Row<N>& row, const Scale& c, u64 floor,
             int rank;
             u64 mass;
             rank_list(s, n, key, rank, mass);
-            const bool cut = MASS ? mass < left && mass + s.weights[threadIdx.x] >= left : u64(rank) + 1 == left;
+            const bool cut = by_mass ? mass < left && mass + s.weights[threadIdx.x] >= left : u64(rank) + 1 == left;
             if (cut) s.key = key;
         }
         __syncthreads();
@@ -277,8 +299,9 @@ __device__ u64 find_cut(Shared& s, const Row<N>& row, const Scale& c, u64 floor,
         clear_hist(s);
         row.each([&](float l, int i) {
             const uint32_t k = ~order_key(l);  // falls with the logit
-            if (in_bin(l, i) && (k & mask) == prefix)
-                atomicAdd(&s.hist[(k >> shift) & ((1u << bits) - 1)], MASS ? fixed(weight(c, l)) : u64(1));
+            const float a = log_weight(c, l);
+            if (bin_of(a) == bin && l > -INFINITY && token_key(l, i) >= floor && (k & mask) == prefix)
+                atomicAdd(&s.hist[(k >> shift) & ((1u << bits) - 1)], by_mass ? fixed(__builtin_amdgcn_exp2f(a)) : u64(1));
         });
         __syncthreads();
         find_in(s, s.hist, kBins, rest);
@@ -289,7 +312,7 @@ __device__ u64 find_cut(Shared& s, const Row<N>& row, const Scale& c, u64 floor,
     }
     const float l = key_logit(u64(~prefix) << 32);
     u64 nth = rest;
-    if (MASS) {
+    if (by_mass) {
         const u64 w = fixed(weight(c, l));
         nth = (rest + w - 1) / w;
     }
@@ -310,62 +333,72 @@ __device__ __forceinline__ void put(const SampleArgs& a, int row, int token, flo
 }
 
 // One row per block.
-template <int N>
+template <bool R>
 __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned) {
-    __shared__ Shared s;
+    extern __shared__ __align__(16) uint8_t raw[];
+    Shared<R>& s = *reinterpret_cast<Shared<R>*>(raw);
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    Row<N> row;
-    row.p = a.logits + int64_t(r) * a.stride;
-    row.vocab = a.vocab;
-    row.aligned = aligned;
-    row.load();
+    const Row<R> row{a.logits + int64_t(r) * a.stride, s.row, a.vocab, aligned};
 
-    float top = -INFINITY;  // this thread's largest
-    row.each([&](float l, int) { top = fmaxf(top, l); });
-    const float wm = wave_maximum(top);
-    if (lane == 0) s.part[wave] = __float_as_uint(wm);
-    if (t == 0) s.key = 0;
-    __syncthreads();
-    Scale c;
-    c.max = __uint_as_float(uint32_t(s.part[0]));
-    for (int w = 1; w < kWaves; ++w) c.max = fmaxf(c.max, __uint_as_float(uint32_t(s.part[w])));
-    if (c.max == -INFINITY) {  // every token masked
-        if (t == 0) put(a, r, -1, 0.0f);
-        return;
-    }
     const float temp = a.p.d_temperature ? a.p.d_temperature[r] : 1.0f;
     const int top_k = a.p.d_top_k ? a.p.d_top_k[r] : 0;
     const float top_p = a.p.d_top_p ? a.p.d_top_p[r] : 1.0f;
     float min_p = a.p.d_min_p ? a.p.d_min_p[r] : 0.0f;
     min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
+    float u = a.p.d_uniform[a.state ? a.state[3] : r];
+    u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+
+    float top = -INFINITY;  // this thread's largest
+    row.first([&](float4 x, int, int) { top = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), top); });
+    const float wm = wave_maximum(top);
+    if (lane == 0) s.part[wave] = __float_as_uint(wm);
+    if (t == 0) s.key = 0;
+    __syncthreads();
+    Scale c;
+    c.max = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) c.max = fmaxf(c.max, __uint_as_float(uint32_t(s.part[w])));
+    if (c.max == -INFINITY) {  // every token masked
+        if (t == 0) put(a, r, -1, 0.0f);
+        return;
+    }
     if (!(temp > 0.0f) || top_k == 1 || top_p <= 0.0f) {  // the largest logit's first index
-        u64 best = 0;
-        row.each([&](float l, int i) {
-            if (l == c.max && i < a.vocab) best = max(best, token_key(l, i));
-        });
-        if (best) atomicMax(&s.key, best);
+        if (top == c.max) {
+            u64 best = 0;
+            row.each([&](float l, int i) {
+                if (l == c.max) best = max(best, token_key(l, i));
+            });
+            atomicMax(&s.key, best);
+        }
         __syncthreads();
         if (t == 0) put(a, r, int(~uint32_t(s.key)), 1.0f);
         return;
     }
-    const double cd = fmin(1.4426950408889634 / double(temp), 1e30);
+    // an infinite maximum takes all, whatever the temperature
+    const double cd = c.max < INFINITY ? fmin(1.4426950408889634 / double(temp), 1e30) : 1.0;
     c.hi = float(cd);
     c.lo = cd < 1e30 ? float(cd - double(c.hi)) : 0.0f;
-    float u = a.p.d_uniform[a.state ? a.state[3] : r];
-    u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+    c.least = c.hi > 1e-36f ? -200.0f / c.hi : -3.4028235e38f;
     const bool by_k = top_k > 0 && top_k < a.vocab, by_p = top_p < 1.0f;
     __syncthreads();
 
     if (by_k && top_k <= kFewK) {
         // the top_k threads with the largest maxima hold top_k tokens at least as
-        // large as the least of these: their bins bound the candidates
+        // large as the least of these: it bounds the candidates (to its bin)
         clear_hist(s);
-        if (top > -INFINITY) atomicAdd(&s.hist[bin_of(log_weight(c, top))], u64(1));
+        const int bin = bin_of(log_weight(c, top));
+        if (top > -INFINITY) atomicAdd(&s.hist[bin], u64(1));
         __syncthreads();
         find_in(s, s.hist, kBins, u64(top_k));
-        const int last = s.at < 0 ? kBins - 1 : s.at;
+        const int last = s.at < 0 ? kBins : s.at;
+        __syncthreads();
+        if (t == 0) s.sum = ~u64(0);
+        __syncthreads();
+        if (last < kBins && bin <= last && top > -INFINITY) atomicMin(&s.sum, u64(order_key(top)));
+        __syncthreads();
+        const float least = last < kBins ? key_logit(s.sum << 32) : -INFINITY;
         row.each([&](float l, int i) {
-            if (i < a.vocab && bin_of(log_weight(c, l)) <= last) {
+            if (l >= least && l > -INFINITY) {
                 const int at = atomicAdd(&s.n, 1);
                 if (at < kList) {
                     s.list[at] = token_key(l, i);
@@ -390,11 +423,11 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
             keep = keep && weight(c, key_logit(key)) >= min_p;
             // by index: the kept tokens in front of this one, and all
             if (!keep) w = 0;
-            __syncthreads();
             if (t < n) s.weights[t] = w;
             __syncthreads();
             u64 before = 0, total = 0;
             if (t < n)
+#pragma unroll 8
                 for (int j = 0; j < n; ++j) {
                     const u64 v = s.weights[j];
                     total += v;
@@ -409,36 +442,38 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
     }
 
     u64 cut = 0;  // the last token kept, 0: all
-    if (by_k) {
+#pragma unroll 1
+    for (int mass = 0; mass < 2; ++mass) {  // top-k by counts, then top-p by weights
+        if (!(mass ? by_p : by_k)) continue;
         clear_hist(s);
         row.each([&](float l, int i) {
-            if (i < a.vocab) atomicAdd(&s.hist[bin_of(log_weight(c, l))], u64(1));
+            const float x = log_weight(c, l);
+            if (l > -INFINITY && token_key(l, i) >= cut)
+                atomicAdd(&s.hist[bin_of(x)], mass ? fixed(__builtin_amdgcn_exp2f(x)) : u64(1));
         });
         __syncthreads();
-        cut = find_cut<false>(s, row, c, 0, u64(top_k));
-        __syncthreads();
-    }
-    if (by_p) {
-        clear_hist(s);
-        row.each([&](float l, int i) {
-            if (i < a.vocab && token_key(l, i) >= cut) atomicAdd(&s.hist[bin_of(log_weight(c, l))], fixed(weight(c, l)));
-        });
-        __syncthreads();
-        const u64 whole = find_in(s, s.hist, kBins, ~u64(0));
-        cut = find_cut<true>(s, row, c, cut, max(u64(1), min(whole, u64(ceil(double(top_p) * double(whole))))));
+        u64 target = u64(top_k);
+        if (mass) {
+            const u64 whole = find_in(s, s.hist, kBins, ~u64(0));
+            target = max(u64(1), min(whole, u64(ceil(double(top_p) * double(whole)))));
+        }
+        cut = find_cut(s, row, c, cut, target, mass != 0);
         __syncthreads();
     }
     // the kept weights of each 256 tokens, then the place of u among them
-    auto kept = [&](float l, int i) {
-        if (i >= a.vocab || token_key(l, i) < cut) return u64(0);
+    const float cl = cut ? key_logit(cut) : -INFINITY;
+    const int ci = cut ? int(~uint32_t(cut)) : -1;
+    auto kept = [&](float l, int i) {  // in units of 1, exact in 2^-44
         const float w = weight(c, l);
-        return w >= min_p ? fixed(w) : u64(0);
+        const bool k = (l > cl || (l == cl && i <= ci)) && w >= min_p;
+        return k ? (256.0 + double(w)) - 256.0 : 0.0;
     };
     const int segs = (a.vocab + kSegment - 1) / kSegment;
     row.each4([&](float4 x, int i, int k) {
-        const u64 v = wave_sum(kept(x.x, i) + kept(x.y, i + 1) + kept(x.z, i + 2) + kept(x.w, i + 3));
+        // 256 weights of at most 1: their sum in steps of 2^-44 fits a double
+        const double v = wave_total_f64((kept(x.x, i) + kept(x.y, i + 1)) + (kept(x.z, i + 2) + kept(x.w, i + 3)));
         const int sg = k * kWaves + wave;
-        if (lane == 0 && sg < segs) s.seg[sg] = v;
+        if (lane == 0 && sg < segs) s.seg[sg] = u64(v * 17592186044416.0);
     });
     __syncthreads();
     const u64 total = find_in(s, s.seg, segs, ~u64(0));
@@ -447,8 +482,11 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
     if (wave == 0) {
         const int i = s.at * kSegment + 4 * lane;
         const float4 x = row.at(i);
-        const u64 v[4] = {kept(x.x, i), kept(x.y, i + 1), kept(x.z, i + 2), kept(x.w, i + 3)};
-        const u64 sum = v[0] + v[1] + v[2] + v[3];
+        const float y[4] = {x.x, x.y, x.z, x.w};
+        u64 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = u64(kept(y[j], i + j) * 17592186044416.0);
+        const u64 sum = (v[0] + v[1]) + (v[2] + v[3]);
         u64 before = s.sum + wave_scan(sum) - sum;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -463,13 +501,13 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
 
 int launch_sample(const SampleArgs& a, hipStream_t s) {
     const bool al = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.stride % 4 == 0;
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(unsigned(a.rows)), dim3(kThreads), 0, s, a, al); };
-    if (a.vocab <= 8 * kThreads)
-        go(k_sample<8>);
-    else if (a.vocab <= 32 * kThreads)
-        go(k_sample<32>);
+    auto go = [&](auto kern, size_t lds) {
+        hipLaunchKernelGGL(kern, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(lds), s, a, al);
+    };
+    if (a.vocab <= kResident)
+        go(k_sample<true>, sizeof(Shared<true>));
     else
-        go(k_sample<0>);
+        go(k_sample<false>, sizeof(Shared<false>));
     return int(hipGetLastError());
 }
 
