@@ -480,16 +480,17 @@ int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch *batch, int32_t n_
 
 /* ---- sampling: the next token of each row of logits ---- */
 
-/* How each row's token is drawn: device arrays of one value per row; NULL
- * leaves that step out (d_uniform is always needed). The reference draws on the
- * host (model/sampling/topk.go, model/transformer/generate.go:53-183); here
- * the random numbers are the caller's, so a draw can be repeated. */
+/* How each row's token is drawn: arrays of one value per row (device arrays
+ * for wv_sample_dev, host arrays for the decoder's calls); NULL leaves that
+ * step out (uniform is always needed). The reference draws on the host
+ * (model/sampling/topk.go, model/transformer/generate.go:53-183); here the
+ * random numbers are the caller's, so a draw can be repeated. */
 typedef struct wv_sampling {
-    const float *d_temperature; /* T; NaN or T <= 0: the largest logit's first index */
-    const int32_t *d_top_k;     /* <= 0 or >= vocab: all */
-    const float *d_top_p;       /* >= 1 or NaN: all; <= 0: one token */
-    const float *d_min_p;       /* <= 0 or NaN: all; > 1 is 1 */
-    const float *d_uniform;     /* u in [0, 1); others are clamped into it, NaN is 0 */
+    const float *temperature; /* T; NaN or T <= 0: the largest logit's first index */
+    const int32_t *top_k;     /* <= 0 or >= vocab: all */
+    const float *top_p;       /* >= 1 or NaN: all; <= 0: one token */
+    const float *min_p;       /* <= 0 or NaN: all; > 1 is 1 */
+    const float *uniform;     /* u in [0, 1); others are clamped into it, NaN is 0 */
 } wv_sampling;
 
 /* Draws d_tokens[r] from row r of d_logits (rows of vocab floats, `stride`
@@ -506,6 +507,36 @@ typedef struct wv_sampling {
  * at most 2^19. Device pointers, enqueued on `stream`; allocates nothing. */
 int wv_sample_dev(const float *d_logits, int64_t stride, int32_t rows, int32_t vocab, const wv_sampling *sampling,
                   int32_t *d_tokens, float *d_probs, void *stream);
+
+/* ---- serving: the decoder with drawn tokens and with a shared cache ---- */
+
+/* wv_decoder_generate with advance_pos, each step's token drawn instead of the
+ * largest logit's: temperature, top_k, top_p and min_p of `sampling` are one
+ * host value each (NULL: that step left out), uniform n_steps host values,
+ * one per step. vocab is at most 2^19. Synchronous. */
+int wv_decoder_generate_sampled(uint64_t decoder, int32_t token, int32_t pos, int32_t n_steps,
+                                const wv_sampling *sampling, int32_t *tokens_out, float *last_logits);
+
+/* ForwardTokens (model/transformer/forward.go:26-90) over the new tokens of
+ * several sequences at once, prompt chunks beside single tokens, with their
+ * K/V rows in a shared paged cache (`cache`: as many layers, the decoder's KV
+ * heads and head_dim, same device) instead of the decoder's own. All arrays
+ * are host arrays. Sequence b has n_new[b] new ids (0: idle in this call;
+ * tokens holds those of sequence 0, then 1, ...) after kv_len[b] cached
+ * positions; its position j lies in page pages[b * max_pages + j / page_size].
+ * The new rows are written to the cache, then attended to. next_tokens[b] (may
+ * be NULL) receives the token drawn from the logits of b's last row as
+ * `sampling` (one host value per sequence) says, or with NULL their argmax;
+ * -1 for an idle sequence. logits (n_seqs x vocab, may be NULL) receives those
+ * logits (zeros for an idle one). Projections run as in wv_decoder_prefill (a
+ * block of that many rows), attention as wv_kv_attention_dev, the LM head at
+ * the f32 bar. Errors: WV_E_ARG "empty ids" without any new token, WV_E_SHAPE
+ * for a cache of another shape, positions past the table, a page outside the
+ * pool that holds one of the sequence's positions, or two new tokens for one
+ * position of the pool. Synchronous. */
+int wv_decoder_forward_paged(uint64_t decoder, uint64_t cache, int32_t n_seqs, const int32_t *n_new,
+                             const int32_t *tokens, const int32_t *kv_len, const int32_t *pages, int32_t max_pages,
+                             const wv_sampling *sampling, int32_t *next_tokens, float *logits);
 
 /* ---- streams ---- */
 

@@ -47,6 +47,7 @@ EXPORTS = (
     "wv_decoder_use_graph", "wv_decoder_generate", "wv_decoder_prefill", "wv_decoder_free",
     "wv_kv_create", "wv_kv_info", "wv_kv_free", "wv_kv_write_dev", "wv_kv_read_dev", "wv_kv_attention_dev",
     "wv_kv_attention_scratch", "wv_sample_dev",
+    "wv_decoder_generate_sampled", "wv_decoder_forward_paged",
 )
 
 
@@ -121,6 +122,10 @@ def lib():
                                       ctypes.c_int32, _P, _I64, _P, _SZ, _P]
     L.wv_kv_attention_scratch.argtypes = [ctypes.c_uint64, _P, ctypes.c_int32, ctypes.c_int32, _P]
     L.wv_sample_dev.argtypes = [_P, _I64, ctypes.c_int32, ctypes.c_int32, _P, _P, _P, _P]
+    L.wv_decoder_generate_sampled.argtypes = [ctypes.c_uint64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _P, _P,
+                                              _P]
+    L.wv_decoder_forward_paged.argtypes = [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_int32, _P, _P, _P, _P,
+                                           ctypes.c_int32, _P, _P, _P]
     _lib = L
     return L
 

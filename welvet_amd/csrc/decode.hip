@@ -23,6 +23,8 @@
 
 #include "../../include/welvet_hip.h"
 #include "rt_internal.h"
+#include "kv.h"
+#include "sample.h"
 #include "wave_ops.h"
 
 namespace wv {
@@ -867,6 +869,60 @@ __global__ void __launch_bounds__(256) k_rope_kv_rows(float* __restrict__ q, con
     }
 }
 
+// RoPE of the rows of a batch of sequences, row s at position pos[s] (the
+// arithmetic of k_rope_kv_rows): the q heads go to q, the rotated k heads and
+// the v heads to dense rows kr, vr [n_kv * hd], from where they are written
+// to the paged cache; those may be k and v themselves (a thread reads what it
+// writes before). SPLIT and the strides as there.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) k_rope_rows(float* q, const float* k, const float* v,
+                                                   const float* __restrict__ part, int splits, int64_t pstride,
+                                                   const int32_t* __restrict__ pos, const double* __restrict__ freq_div,
+                                                   float* kr, float* vr, int n_heads, int n_kv, int hd, int qs, int kvs) {
+    const int s = blockIdx.x, half = hd / 2, kvd = n_kv * hd;
+    float* qr = q + int64_t(s) * qs;
+    const float* kin = k + int64_t(s) * kvs;
+    const float* vin = v + int64_t(s) * kvs;
+    const float* pr = SPLIT ? part + int64_t(s) * qs : nullptr;
+    auto rd = [&](const float* r, int off, int j) {
+        if constexpr (!SPLIT) {
+            return r[j];
+        } else {
+            float x = pr[off + j];
+            for (int t = 1; t < splits; ++t) x += pr[int64_t(t) * pstride + off + j];
+            return x;
+        }
+    };
+    const int koff = n_heads * hd, voff = koff + kvd;
+    const int HG = 256 / half, d = threadIdx.x % half;  // half divides 256
+    const double angle = double(pos[s]) / freq_div[d];
+    const double c = cos(angle), sn = sin(angle);
+    float* ko = kr + int64_t(s) * kvd;
+    float* vo = vr + int64_t(s) * kvd;
+    for (int hh = threadIdx.x / half + HG * blockIdx.y; hh < n_heads + n_kv; hh += HG * gridDim.y) {
+        if (hh < n_heads) {
+            const double x0 = rd(qr, 0, hh * hd + d), x1 = rd(qr, 0, hh * hd + d + half);
+            qr[hh * hd + d] = float(x0 * c - x1 * sn);
+            qr[hh * hd + d + half] = float(x0 * sn + x1 * c);
+        } else {
+            const int g = hh - n_heads;
+            const double x0 = rd(kin, koff, g * hd + d), x1 = rd(kin, koff, g * hd + d + half);
+            ko[g * hd + d] = float(x0 * c - x1 * sn);
+            ko[g * hd + d + half] = float(x0 * sn + x1 * c);
+        }
+    }
+    for (int i = threadIdx.x + 256 * blockIdx.y; i < kvd; i += 256 * gridDim.y) vo[i] = rd(vin, voff, i);
+}
+
+// out[b] = h[row] + a[row] of each sequence's last row (zeros where it has none, row < 0).
+__global__ void __launch_bounds__(256) k_last_rows(const float* __restrict__ h, const float* __restrict__ a,
+                                                   const int32_t* __restrict__ rows, float* __restrict__ out,
+                                                   int hidden) {
+    const int b = blockIdx.y, r = rows[b];
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < hidden; i += gridDim.x * 256)
+        out[int64_t(b) * hidden + i] = r < 0 ? 0.0f : h[int64_t(r) * hidden + i] + a[int64_t(r) * hidden + i];
+}
+
 // Causal GQA attention for prompt row s (position pos0 + s) over the cache,
 // which already holds the K and V rows of every prompt position
 // (layers/mha/attn.go:40-118 with the causal mask kPos <= qPos): block (kvh, s)
@@ -1431,6 +1487,22 @@ struct Decoder {
     float* pxh = nullptr;  // the fp16 GEMM operand shared by the projections of one input, then its row factors
     int32_t* ptok = nullptr;
     size_t pscratch_floats = 0, pxh_floats = 0;
+    // drawn tokens: {temperature, top_k, top_p, min_p} and one u per step
+    float* samp = nullptr;
+    // batches over a paged cache: their integers and settings, the sequences' last rows and logits, grown on demand
+    uint8_t* gmeta = nullptr;
+    float *glast = nullptr, *glogits = nullptr;  // grows rows, and their norms; grows rows
+    size_t gmeta_bytes = 0, grows = 0;
+};
+
+// What enqueue_prefill takes of a batch over a paged cache (device pointers).
+struct Paged {
+    KvCache cache;
+    int n_seqs = 0, max_pages = 0, max_q = 0, splits = 1;
+    const int64_t* slots = nullptr;                                                            // [n]
+    const int32_t *pos = nullptr, *cu = nullptr, *kv_len = nullptr, *pages = nullptr, *last = nullptr;
+    wv_sampling samp{};
+    int32_t* next = nullptr;
 };
 
 std::mutex g_dmu;
@@ -1481,6 +1553,9 @@ void release(Decoder* d) {
     if (d->gemv_scratch) (void)hipFree(d->gemv_scratch);
     for (Layer& ly : d->layers) drop_fused(ly);
     for (void* p : d->allocs) (void)hipFree(p);
+    for (void* p : {static_cast<void*>(d->samp), static_cast<void*>(d->gmeta), static_cast<void*>(d->glast),
+                    static_cast<void*>(d->glogits)})
+        if (p) (void)hipFree(p);
     if (d->stream) (void)hipStreamDestroy(d->stream);
     delete d;
 }
@@ -1549,6 +1624,8 @@ void launch_attn(Decoder& d, Layer& ly, int G, float scale) {
                            c.n_heads, c.n_kv_heads, c.max_seq, d.n_chunks, scale, d.k, d.v, d.cs);
 }
 
+// advance: 1 the position moves on, 0 it stays; with kDraw the token is drawn (and the position moves on).
+constexpr int kDraw = 2;
 int enqueue_step(Decoder& d, int advance) {
     const wv_decoder_config& c = d.c;
     const int hd = c.head_dim;
@@ -1620,6 +1697,13 @@ int enqueue_step(Decoder& d, int advance) {
         e = proj(d, d.lm, fin, d.logits, RPL_STORE, nullptr, nullptr);
     }
     if (e) return e;
+    if (advance & kDraw) {
+        SampleArgs a{};
+        a.logits = d.logits, a.stride = c.vocab, a.rows = 1, a.vocab = c.vocab;
+        a.p = {d.samp, reinterpret_cast<const int32_t*>(d.samp + 1), d.samp + 2, d.samp + 3, d.samp + 4};
+        a.state = d.d_state, a.gen = d.d_gen, a.gen_cap = c.max_seq, a.advance = 1;
+        return launch_sample(a, d.stream);
+    }
     hipLaunchKernelGGL(k_argmax_advance, dim3(1), dim3(1024), 0, d.stream, d.logits, c.vocab, d.d_state, d.d_gen,
                        c.max_seq, advance);
     return int(hipGetLastError());
@@ -1728,9 +1812,10 @@ size_t prefill_proj_scratch(const DevBlob& w, int n) {
     return gemm_supported(w, n) ? gemm_scratch_floats(w, n) : matvec_scratch_floats(w, n);
 }
 
-int ensure_prefill(Decoder& d, int n) {
+// more_s: floats of d.pscratch that the caller needs beside the projections'.
+int ensure_prefill(Decoder& d, int n, size_t more_s = 0) {
     const wv_decoder_config& c = d.c;
-    size_t need_s = 0;
+    size_t need_s = more_s;
     size_t need_x = 0;  // the widest fp16 copy of a GEMM input, then its row factors
     for (const Layer& ly : d.layers) {
         auto need = [&](const DevBlob& w) {
@@ -1834,7 +1919,9 @@ bool launch_attn_prefill_mf(Decoder& d, Layer& ly, const float* q, int qstr, int
     return true;
 }
 
-int enqueue_prefill(Decoder& d, int n, int pos0) {
+// With pg the n rows are those of several sequences, each at its own position,
+// over pg's cache; the last row of each goes through the LM head.
+int enqueue_prefill(Decoder& d, int n, int pos0, const Paged* pg = nullptr) {
     const wv_decoder_config& c = d.c;
     const int hd = c.head_dim, hidden = c.hidden;
     const float scale = float(1.0 / std::sqrt(double(hd)));
@@ -1900,7 +1987,26 @@ int enqueue_prefill(Decoder& d, int n, int pos0) {
         // up to 256 / n blocks per row, at most one per pass over the heads
         const int passes = (c.n_heads + c.n_kv_heads + 256 / (hd / 2) - 1) / (256 / (hd / 2));
         const dim3 rg(unsigned(n), unsigned(std::max(1, std::min(passes, 256 / n))));
-        if (qkv_splits > 1)
+        if (pg) {
+            const int64_t ps = int64_t(n) * qstr;
+            if (qkv_splits > 1)
+                hipLaunchKernelGGL(k_rope_rows<true>, rg, dim3(256), 0, d.stream, q, k, v, d.pscratch, qkv_splits, ps,
+                                   pg->pos, d.freq_div, d.pk, d.pv, c.n_heads, c.n_kv_heads, hd, qstr, kvstr);
+            else
+                hipLaunchKernelGGL(k_rope_rows<false>, rg, dim3(256), 0, d.stream, q, k, v, nullptr, 1, ps, pg->pos,
+                                   d.freq_div, d.pk, d.pv, c.n_heads, c.n_kv_heads, hd, qstr, kvstr);
+            const KvView view = pg->cache.layer(L);
+            e = launch_kv_write(view, d.pk, d.pv, kvd, kvd, pg->slots, n, d.stream);
+            if (e) return e;
+            KvAttn a{};
+            a.c = view;
+            a.q = q, a.qs = qstr, a.out = d.patt, a.os = qd, a.part = pg->splits > 1 ? d.pscratch : nullptr;
+            a.cu = pg->cu, a.kv_len = pg->kv_len, a.pages = pg->pages;
+            a.n_seqs = pg->n_seqs, a.n_tokens = n, a.max_pages = pg->max_pages, a.max_q = pg->max_q;
+            a.n_heads = c.n_heads, a.splits = pg->splits, a.scale = scale;
+            e = launch_kv_attn(a, d.stream);
+            if (e) return e;
+        } else if (qkv_splits > 1)
             hipLaunchKernelGGL(k_rope_kv_rows<true>, rg, dim3(256), 0, d.stream, q, k, v, d.pscratch,
                                qkv_splits, int64_t(n) * qstr, ly.kc, ly.vc, d.freq_div, c.n_heads, c.n_kv_heads, hd,
                                c.max_seq, pos0, qstr, kvstr);
@@ -1911,7 +2017,7 @@ int enqueue_prefill(Decoder& d, int n, int pos0) {
         // bf16x3 products where Q, K and V came from the fp16 GEMM (the 2e-3 bar)
         const bool bf = fused || (gemm_supported(ly.w[0], n) && gemm_supported(ly.w[1], n) && gemm_supported(ly.w[2], n));
         int attn_ks = 1;
-        if (!launch_attn_prefill_mf(d, ly, q, qstr, n, pos0, scale, bf, &attn_ks)) {
+        if (!pg && !launch_attn_prefill_mf(d, ly, q, qstr, n, pos0, scale, bf, &attn_ks)) {
             const dim3 ag(unsigned(c.n_kv_heads), unsigned(n));
             if (hd == 128)
                 hipLaunchKernelGGL(k_attn_prefill<128>, ag, dim3(256), 0, d.stream, q, ly.kc, ly.vc, d.patt,
@@ -1959,6 +2065,23 @@ int enqueue_prefill(Decoder& d, int n, int pos0) {
     }
     // the last layer's residual add, for the one row the LM head reads
     sum_splits(down_splits, d.pn);
+    if (pg) {
+        const int B = pg->n_seqs;
+        hipLaunchKernelGGL(k_last_rows, dim3(unsigned((hidden + 255) / 256), unsigned(B)), dim3(256), 0, d.stream, d.ph,
+                           d.pn, pg->last, d.glast, hidden);
+        const float* fin = d.glast;
+        if (d.has_final_norm) {
+            float* y = d.glast + d.grows * size_t(hidden);
+            hipLaunchKernelGGL(k_rmsnorm, dim3(unsigned(B)), dim3(1024), 0, d.stream, d.glast, d.final_norm, y, hidden,
+                               c.rms_eps);
+            fin = y;
+        }
+        const int e = launch_matvec(d.lm, fin, d.glogits, B, d.stream, d.pscratch);
+        if (e) return e;
+        SampleArgs a{};
+        a.logits = d.glogits, a.stride = c.vocab, a.rows = B, a.vocab = c.vocab, a.p = pg->samp, a.tokens = pg->next;
+        return launch_sample(a, d.stream);
+    }
     hipLaunchKernelGGL(k_add, dim3(unsigned((hidden + 255) / 256)), dim3(256), 0, d.stream,
                        d.ph + int64_t(n - 1) * hidden, d.pn + int64_t(n - 1) * hidden, hidden);
     const float* last = d.ph + int64_t(n - 1) * hidden;
@@ -2247,6 +2370,184 @@ int wv_decoder_generate(uint64_t dec, int32_t token, int32_t pos, int32_t n_step
     e = hipStreamSynchronize(d->stream);
     if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_generate: sync");
     return WV_OK;
+}
+
+int wv_decoder_generate_sampled(uint64_t dec, int32_t token, int32_t pos, int32_t n_steps,
+                                const wv_sampling* sampling, int32_t* tokens_out, float* last_logits) {
+    Decoder* d = find(dec);
+    if (!d) return rt_fail(WV_E_HANDLE, "wv_decoder_generate_sampled: unknown decoder %llu", (unsigned long long)dec);
+    const wv_decoder_config& c = d->c;
+    if (!sampling || (n_steps > 0 && !sampling->uniform))
+        return rt_fail(WV_E_ARG, "wv_decoder_generate_sampled: nil sampling/uniform");
+    if (n_steps < 0 || n_steps > c.max_seq)
+        return rt_fail(WV_E_ARG, "wv_decoder_generate_sampled: step count %d outside 0..max_seq", n_steps);
+    if (pos < 0 || int64_t(pos) + n_steps > c.max_seq)
+        return rt_fail(WV_E_SHAPE, "wv_decoder_generate_sampled: positions %d.. exceed max_seq %d", pos, c.max_seq);
+    if (c.vocab > 1 << 19) return rt_fail(WV_E_SHAPE, "wv_decoder_generate_sampled: vocab %d (at most 2^19)", c.vocab);
+    int rc = ready(*d);
+    if (rc) return rc;
+    (void)hipSetDevice(d->device);
+    if (!d->samp) {
+        const hipError_t e = hipMalloc(reinterpret_cast<void**>(&d->samp), (4 + size_t(c.max_seq)) * sizeof(float));
+        if (e != hipSuccess) {
+            d->samp = nullptr;
+            return rt_hip_fail(e, "wv_decoder_generate_sampled: settings");
+        }
+    }
+    struct {
+        float t;
+        int32_t k;
+        float p, m;
+    } set = {sampling->temperature ? *sampling->temperature : 1.0f, sampling->top_k ? *sampling->top_k : 0,
+             sampling->top_p ? *sampling->top_p : 1.0f, sampling->min_p ? *sampling->min_p : 0.0f};
+    const int32_t init[4] = {pos, token, -1, 0};
+    hipError_t e = hipMemcpyAsync(d->d_state, init, sizeof init, hipMemcpyHostToDevice, d->stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(d->samp, &set, sizeof set, hipMemcpyHostToDevice, d->stream);
+    if (e == hipSuccess && n_steps > 0)
+        e = hipMemcpyAsync(d->samp + 4, sampling->uniform, size_t(n_steps) * sizeof(float), hipMemcpyHostToDevice,
+                           d->stream);
+    if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_generate_sampled: state");
+    rc = run_steps(*d, n_steps, 1 | kDraw);
+    if (rc) return rc;
+    if (tokens_out && n_steps > 0)
+        e = hipMemcpyAsync(tokens_out, d->d_gen, size_t(n_steps) * sizeof(int32_t), hipMemcpyDeviceToHost, d->stream);
+    if (e == hipSuccess && last_logits && n_steps > 0)
+        e = hipMemcpyAsync(last_logits, d->logits, size_t(c.vocab) * 4, hipMemcpyDeviceToHost, d->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(d->stream);
+    return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_decoder_generate_sampled: results");
+}
+
+int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const int32_t* n_new, const int32_t* tokens,
+                             const int32_t* kv_len, const int32_t* pages, int32_t max_pages,
+                             const wv_sampling* sampling, int32_t* next_tokens, float* logits) try {
+    Decoder* d = find(dec);
+    if (!d) return rt_fail(WV_E_HANDLE, "wv_decoder_forward_paged: unknown decoder %llu", (unsigned long long)dec);
+    const wv_decoder_config& c = d->c;
+    Paged pg;
+    if (!kv_lookup(cache, pg.cache))
+        return rt_fail(WV_E_HANDLE, "wv_decoder_forward_paged: unknown cache %llu", (unsigned long long)cache);
+    const wv_kv_config& k = pg.cache.c;
+    if (k.n_layers != c.n_layers || k.n_kv_heads != c.n_kv_heads || k.head_dim != c.head_dim ||
+        pg.cache.device != d->device)
+        return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: cache of %d layers, %d KV heads x %d (device %d), want %d, "
+                       "%d x %d (device %d)", k.n_layers, k.n_kv_heads, k.head_dim, pg.cache.device, c.n_layers,
+                       c.n_kv_heads, c.head_dim, d->device);
+    if (n_seqs <= 0 || max_pages <= 0 || n_seqs > 65535)
+        return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: %d sequences (1 to 65535) of up to %d pages", n_seqs, max_pages);
+    if (!n_new || !tokens || !kv_len || !pages || (sampling && !sampling->uniform))
+        return rt_fail(WV_E_ARG, "wv_decoder_forward_paged: nil n_new/tokens/kv_len/pages/uniform");
+    if (c.vocab > 1 << 19) return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: vocab %d (at most 2^19)", c.vocab);
+    const int64_t width = int64_t(max_pages) * k.page_size;
+    int64_t total = 0;
+    for (int b = 0; b < n_seqs; ++b) {
+        if (n_new[b] < 0 || kv_len[b] < 0)
+            return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: sequence %d: %d new tokens after %d", b, n_new[b], kv_len[b]);
+        if (n_new[b] && int64_t(kv_len[b]) + n_new[b] > std::min<int64_t>(width, INT32_MAX))
+            return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: sequence %d: %d new tokens after %d exceed %lld positions",
+                           b, n_new[b], kv_len[b], (long long)width);
+        total += n_new[b];
+        const int64_t used = n_new[b] ? (int64_t(kv_len[b]) + n_new[b] + k.page_size - 1) / k.page_size : 0;
+        for (int64_t j = 0; j < used; ++j)
+            if (const int32_t p = pages[int64_t(b) * max_pages + j]; p < 0 || p >= k.n_pages)
+                return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: sequence %d: page %d of %d", b, p, k.n_pages);
+    }
+    if (!total) return rt_fail(WV_E_ARG, "wv_decoder_forward_paged: empty ids");
+    if (total * c.n_heads >= int64_t(1) << 31 || total > 1 << 20)
+        return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: %lld new tokens in one call", (long long)total);
+    const int n = int(total);
+    // one copy: slots, then 32-bit rows (positions, first rows, lengths, last rows, tables, settings, results)
+    const size_t B = size_t(n_seqs), table = B * size_t(max_pages);
+    const size_t words = 2 * size_t(n) + size_t(n) + (B + 1) + B + B + table + 5 * B + B;
+    std::vector<int32_t> host(words);
+    int64_t* slots = reinterpret_cast<int64_t*>(host.data());
+    int32_t* pos = host.data() + 2 * size_t(n);
+    int32_t *cu = pos + n, *len = cu + B + 1, *last = len + B, *tab = last + B, *set = tab + table;
+    cu[0] = 0;
+    for (int b = 0, t = 0; b < n_seqs; ++b) {
+        pg.max_q = std::max(pg.max_q, n_new[b]);
+        for (int i = 0; i < n_new[b]; ++i, ++t) {
+            const int p = kv_len[b] + i;
+            pos[t] = p;
+            slots[t] = int64_t(pages[int64_t(b) * max_pages + p / k.page_size]) * k.page_size + p % k.page_size;
+        }
+        cu[b + 1] = t;
+        len[b] = kv_len[b] + n_new[b];
+        last[b] = n_new[b] ? t - 1 : -1;
+        const float f[4] = {sampling ? (sampling->temperature ? sampling->temperature[b] : 1.0f) : 0.0f,
+                            sampling && sampling->top_p ? sampling->top_p[b] : 1.0f,
+                            sampling && sampling->min_p ? sampling->min_p[b] : 0.0f,
+                            sampling ? sampling->uniform[b] : 0.0f};
+        for (int i = 0; i < 4; ++i) std::memcpy(set + size_t(i) * B + b, &f[i], 4);
+        set[4 * B + b] = sampling && sampling->top_k ? sampling->top_k[b] : 0;
+    }
+    {
+        std::vector<int64_t> sorted(slots, slots + n);
+        std::sort(sorted.begin(), sorted.end());
+        if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+            return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: two new tokens for one position of the pool");
+    }
+    std::memcpy(tab, pages, table * 4);
+    int rc = ready(*d);
+    if (rc) return rc;
+    (void)hipSetDevice(d->device);
+    pg.n_seqs = n_seqs, pg.max_pages = max_pages;
+    // keys past the longest sequence need no split
+    const int32_t longest = *std::max_element(len, len + B);
+    pg.splits = kv_attn_splits(pg.cache.layer(0), n_seqs, n,
+                               std::min(max_pages, (longest + k.page_size - 1) / k.page_size), pg.max_q, c.n_heads, 0);
+    const size_t more = std::max(kv_attn_part_floats(pg.cache.layer(0), n, c.n_heads, pg.splits),
+                                 matvec_scratch_floats(d->lm, n_seqs));
+    rc = ensure_prefill(*d, n, more);
+    if (rc) return rc;
+    hipError_t e = hipSuccess;
+    if (words * 4 > d->gmeta_bytes) {
+        if (d->gmeta) (void)hipFree(d->gmeta);
+        d->gmeta = nullptr, d->gmeta_bytes = 0;
+        if ((e = hipMalloc(reinterpret_cast<void**>(&d->gmeta), words * 4)) != hipSuccess) {
+            d->gmeta = nullptr;
+            return rt_hip_fail(e, "wv_decoder_forward_paged: batch");
+        }
+        d->gmeta_bytes = words * 4;
+    }
+    if (B > d->grows) {
+        for (float** p : {&d->glast, &d->glogits}) {
+            if (*p) (void)hipFree(*p);
+            *p = nullptr;
+        }
+        d->grows = 0;
+        e = hipMalloc(reinterpret_cast<void**>(&d->glast), 2 * B * size_t(c.hidden) * 4);
+        if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&d->glogits), B * size_t(c.vocab) * 4);
+        if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_forward_paged: logits");
+        d->grows = B;
+    }
+    int32_t* m = reinterpret_cast<int32_t*>(d->gmeta);
+    auto at = [&](const int32_t* p) { return m + (p - host.data()); };
+    pg.slots = reinterpret_cast<const int64_t*>(m);
+    pg.pos = at(pos), pg.cu = at(cu), pg.kv_len = at(len), pg.last = at(last), pg.pages = at(tab);
+    const float* fset = reinterpret_cast<const float*>(at(set));
+    pg.samp = {fset, at(set) + 4 * B, fset + B, fset + 2 * B, fset + 3 * B};
+    pg.next = at(set) + 5 * B;
+    e = hipMemcpyAsync(d->gmeta, host.data(), words * 4, hipMemcpyHostToDevice, d->stream);
+    if (e == hipSuccess) e = hipMemcpyAsync(d->ptok, tokens, size_t(n) * 4, hipMemcpyHostToDevice, d->stream);
+    if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_forward_paged: batch");
+    const int ke = enqueue_prefill(*d, n, 0, &pg);
+    if (ke) {
+        (void)hipStreamSynchronize(d->stream);  // the copies read `host`
+        return rt_hip_fail(hipError_t(ke), "wv_decoder_forward_paged: launch");
+    }
+    if (next_tokens) e = hipMemcpyAsync(next_tokens, pg.next, B * 4, hipMemcpyDeviceToHost, d->stream);
+    if (e == hipSuccess && logits)
+        e = hipMemcpyAsync(logits, d->glogits, B * size_t(c.vocab) * 4, hipMemcpyDeviceToHost, d->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(d->stream);
+    if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_forward_paged: results");
+    for (int b = 0; b < n_seqs; ++b)
+        if (!n_new[b]) {
+            if (next_tokens) next_tokens[b] = -1;
+            if (logits) std::fill_n(logits + size_t(b) * c.vocab, size_t(c.vocab), 0.0f);
+        }
+    return WV_OK;
+} catch (const std::bad_alloc&) {
+    return rt_fail(WV_E_OOM, "wv_decoder_forward_paged: host memory exhausted");
 }
 
 int wv_decoder_prefill(uint64_t dec, const int32_t* tokens, int32_t n_tokens, int32_t pos0, int32_t* next_token,

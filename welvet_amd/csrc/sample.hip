@@ -340,12 +340,12 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
     const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const Row<R> row{a.logits + int64_t(r) * a.stride, s.row, a.vocab, aligned};
 
-    const float temp = a.p.d_temperature ? a.p.d_temperature[r] : 1.0f;
-    const int top_k = a.p.d_top_k ? a.p.d_top_k[r] : 0;
-    const float top_p = a.p.d_top_p ? a.p.d_top_p[r] : 1.0f;
-    float min_p = a.p.d_min_p ? a.p.d_min_p[r] : 0.0f;
+    const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
+    const int top_k = a.p.top_k ? a.p.top_k[r] : 0;
+    const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f;
+    float min_p = a.p.min_p ? a.p.min_p[r] : 0.0f;
     min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
-    float u = a.p.d_uniform[a.state ? a.state[3] : r];
+    float u = a.p.uniform[a.state ? a.state[3] : r];
     u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
 
     float top = -INFINITY;  // this thread's largest
@@ -524,7 +524,7 @@ extern "C" int wv_sample_dev(const float* d_logits, int64_t stride, int32_t rows
     if (stride < vocab)
         return rt_fail(WV_E_SHAPE, "wv_sample: row stride %lld under %d logits", (long long)stride, vocab);
     if (!rows) return WV_OK;
-    if (!d_logits || !d_tokens || !sampling->d_uniform) return rt_fail(WV_E_ARG, "wv_sample: nil logits/tokens/uniform");
+    if (!d_logits || !d_tokens || !sampling->uniform) return rt_fail(WV_E_ARG, "wv_sample: nil logits/tokens/uniform");
     const int rc = rt_ensure_init();
     if (rc) return rc;
     SampleArgs a{};

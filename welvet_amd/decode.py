@@ -8,6 +8,16 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import DeviceBlob, check, lib
+from .kv import KVCache
+from .sampling import Sampling
+
+
+def _host_sampling(n: int, uniform, temperature, top_k, top_p, min_p):
+    """A wv_sampling over host arrays of n values (scalars are repeated), and those arrays."""
+    arr = [None if x is None else np.ascontiguousarray(np.broadcast_to(np.asarray(x, t), (n,)))
+           for x, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+    arr.append(np.ascontiguousarray(uniform, np.float32).reshape(-1))
+    return Sampling(*(None if a is None else a.ctypes.data for a in arr)), arr
 
 
 class DecoderConfig(ctypes.Structure):
@@ -88,6 +98,44 @@ class Decoder:
         check(lib().wv_decoder_generate(self.handle, token, pos, n_steps, 1 if advance_pos else 0, toks.ctypes.data,
                                         None if logits is None else logits.ctypes.data))
         return (toks[:n_steps], logits) if want_logits else toks[:n_steps]
+
+    def generate_sampled(self, token: int, pos: int, uniform, temperature=None, top_k=None, top_p=None, min_p=None,
+                         want_logits: bool = False):
+        """generate() with each step's token drawn: one uniform number per step, the settings one value each
+        (None leaves that step out)."""
+        u = np.ascontiguousarray(uniform, np.float32).reshape(-1)
+        s, keep = _host_sampling(1, u, temperature, top_k, top_p, min_p)
+        toks = np.zeros(max(u.size, 1), np.int32)
+        logits = np.zeros(self.cfg.vocab, np.float32) if want_logits else None
+        check(lib().wv_decoder_generate_sampled(self.handle, token, pos, u.size, ctypes.byref(s), toks.ctypes.data,
+                                                None if logits is None else logits.ctypes.data))
+        del keep
+        return (toks[:u.size], logits) if want_logits else toks[:u.size]
+
+    def forward_paged(self, cache: KVCache, new_tokens, kv_len, pages, uniform=None, temperature=None, top_k=None,
+                      top_p=None, min_p=None, want_logits: bool = False):
+        """The new tokens of several sequences (a list of id lists, [] for an idle one) in one pass, their K/V rows
+        in `cache`: sequence b has kv_len[b] cached positions and the pages pages[b]. Returns each sequence's next
+        token (-1 where idle), drawn with uniform[b] and the settings (a value or one per sequence), or the argmax
+        where uniform is None; and the logits of the last rows."""
+        rows = [np.asarray(t, np.int32).reshape(-1) for t in new_tokens]
+        n = np.ascontiguousarray([r.size for r in rows], np.int32)
+        ids = np.concatenate(rows) if rows else np.zeros(0, np.int32)
+        ids = np.ascontiguousarray(ids if ids.size else np.zeros(1, np.int32))
+        kv = np.ascontiguousarray(kv_len, np.int32).reshape(-1)
+        tab = np.ascontiguousarray(pages, np.int32)
+        if kv.size != n.size or tab.ndim != 2 or tab.shape[0] != n.size:
+            raise ValueError(f"forward_paged: {n.size} sequences, {kv.size} lengths, pages {tab.shape}")
+        s, keep = (None, None) if uniform is None else _host_sampling(n.size, uniform, temperature, top_k, top_p, min_p)
+        if keep is not None and keep[-1].size != n.size:
+            raise ValueError(f"forward_paged: {n.size} sequences, {keep[-1].size} uniform numbers")
+        out = np.zeros(max(n.size, 1), np.int32)
+        logits = np.zeros((n.size, self.cfg.vocab), np.float32) if want_logits else None
+        check(lib().wv_decoder_forward_paged(self.handle, cache.handle, n.size, n.ctypes.data, ids.ctypes.data,
+                                             kv.ctypes.data, tab.ctypes.data, tab.shape[1],
+                                             None if s is None else ctypes.byref(s), out.ctypes.data,
+                                             None if logits is None else logits.ctypes.data))
+        return (out[:n.size], logits) if want_logits else out[:n.size]
 
     def prefill(self, tokens, pos0: int = 0, want_logits: bool = False):
         """ForwardTokens over a prompt block at positions pos0.. (wv_decoder_prefill):

@@ -8,8 +8,8 @@ from . import check, lib
 
 
 class Sampling(ctypes.Structure):
-    _fields_ = [("d_temperature", ctypes.c_void_p), ("d_top_k", ctypes.c_void_p), ("d_top_p", ctypes.c_void_p),
-                ("d_min_p", ctypes.c_void_p), ("d_uniform", ctypes.c_void_p)]
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p), ("uniform", ctypes.c_void_p)]
 
 
 def sample_dev(logits_ptr: int, rows: int, vocab: int, tokens_ptr: int, uniform_ptr: int, *, stride: int = 0,
