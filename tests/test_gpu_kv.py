@@ -287,6 +287,61 @@ def test_attention_long_split_and_deterministic():
     assert p.kv.attention_scratch(b, 4) > 0
 
 
+# The kernel for many rows takes calls of at least 512 blocks of 128 rows (query heads of a KV head x tokens),
+# with a sequence of 1024 rows and more.
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("heads,kv_heads,hd,kv,new", [(32, 8, 64, 2100, 2048), (64, 16, 128, 1100, 1024),
+                                                      (24, 24, 64, 2750, 2747), (32, 8, 128, 4200, 515)])
+def test_many_rows_one_sequence(typ, heads, kv_heads, hd, kv, new):
+    """Whole prompts, a chunk behind cached keys, one cut into key ranges (515 tokens over 4200 keys)."""
+    rng = np.random.default_rng(kv + heads)
+    p = Pool(rng, [kv], kv_heads, hd, 64, typ).fill()
+    a = p.attend([new], heads, max_q=new)
+    p.check(a, [new])
+    assert np.array_equal(a, p.attend([new], heads, max_q=new, q=p.q))
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("window", [0, 200])
+def test_many_rows_ragged_batch(typ, window):
+    """Long chunks beside single tokens and an idle sequence, padding rows, pages outside the pool."""
+    rng = np.random.default_rng(window + 21)
+    lens, new = [1500, 700, 64, 1000, 333, 3], [1100, 0, 1, 1000, 300, 2]
+    p = Pool(rng, lens, 8, 64, 32, typ, layers=2, layer=1).fill()
+    p.check(p.attend(new, 32, window=window, pad=5), new, window=window)
+    table = p.table.copy()
+    table[0, 3], table[3, 7], table[3, 31] = -1, 1 << 30, len(lens) * p.width + 2
+    present = [np.ones(n, bool) for n in lens]
+    present[0][96:128] = present[3][224:256] = present[3][992:] = False
+    p.check(p.attend(new, 32, window=window, table=table, max_q=1100), new, window=window, present=present)
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+def test_many_rows_nan_and_magnitudes(typ):
+    """NaN rows behind the keys and left of the window change nothing, a NaN key the rows that attend to it;
+    V rows far above and below the others, scores of hundreds."""
+    rng = np.random.default_rng(31)
+    p = Pool(rng, [2200], 8, 64, 32, typ)
+    p.v[0][::41] *= np.float32(1e4)
+    p.v[0][7::53] *= np.float32(1e-6)
+    p.k[0][:, ::2] *= np.float32(30)
+    clean = p.k[0].copy(), p.v[0].copy()
+    p.k[0][2100:], p.v[0][2100:] = np.nan, np.inf
+    p.k[0][:20], p.v[0][:20] = np.inf, np.nan
+    p.fill()
+    out = p.attend([2048], 32, window=30, kv_len=[2100])
+    p.k[0], p.v[0] = clean
+    p.check(out, [2048], window=30, lens=[2100])
+    p.k[0][2090, 3], p.v[0][2095, 5] = np.nan, np.nan
+    p.fill()
+    out = p.attend([2048], 32, kv_len=[2100])
+    bad = np.isnan(out)
+    want = np.zeros_like(bad)
+    want[2090 - 52:, 12:16] = want[2095 - 52:, 20:24] = True
+    assert np.array_equal(bad, want)
+
+
 def test_attention_strides_and_in_place():
     rng = np.random.default_rng(12)
     p = Pool(rng, [130], 2, 64, 32, "f16").fill()

@@ -31,7 +31,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;  // m of a row that has met no key
 constexpr int kMaxSplits = 64;
-constexpr int kFewRows = 16;  // query rows of a sequence and KV head up to which the row kernel takes it
+constexpr int kFewRows = 256;  // query rows of a sequence and KV head up to which the row kernel takes it
 
 // 8 biased int8 codes (two words) as fp16: 0x6400 | b is 1024 + b, less 1152
 // the code; one byte permute and half a packed subtraction per code pair.
@@ -824,15 +824,40 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
 
 }  // namespace
 
-int kv_attn_splits(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
-    if (!n_seqs || !n_tokens) return 1;
-    const int64_t G = n_heads / c.n_kv;
-    const int64_t tiles = std::max<int64_t>((n_tokens * G + 15) / 16, std::min(n_seqs, n_tokens));
+namespace {
+
+// How a call is run. The tile kernel reads and converts the keys once for 128
+// rows, but goes through them in steps of 32 keys at 1.4 us a step for one
+// block a CU and 2.0 for two: it pays where two blocks a CU have at least 32
+// key blocks each and some sequence has rows for 8 tiles. Rows of 32 heads
+// over 8, head_dim 128, int8, row against tile kernel at its best split (us):
+// 1 x 512 new over 2048 keys 59 / 66, over 8192 216 / 163; 1 x 2048 over 2048
+// 213 / 102, over 16384 1812 / 975; 16 x 128 over 8192 273 / 281.
+struct Plan {
+    bool many;   // the tile kernel takes the sequences of more than kFewRows rows
+    int splits;
+};
+Plan plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
+    if (!n_seqs || !n_tokens) return {false, 1};
+    const int64_t G = n_heads / c.n_kv, rows = n_tokens * G;
+    const int64_t most_q = max_q ? std::min(max_q, n_tokens) : (n_tokens + n_seqs - 1) / n_seqs;
     const int64_t width = int64_t(max_pages) << c.page_shift;
-    const int64_t keys = window > 0 ? std::min<int64_t>(width, int64_t(window) + 16 / G) : width;
-    const int64_t blocks = (keys + 31) / 32;
-    const int64_t most = std::min<int64_t>(kMaxSplits, (blocks + 3) / 4);
-    return int(std::max<int64_t>(1, std::min<int64_t>(512 / (tiles * c.n_kv), most)));
+    const int64_t keys = window > 0 ? std::min<int64_t>(width, int64_t(window) + most_q) : width;
+    const int64_t blocks = std::max<int64_t>((keys + 31) / 32, 1);
+    const int64_t t128 = (rows + 127) / 128 * c.n_kv;  // tile blocks
+    const int64_t s128 = std::max<int64_t>(1, std::min<int64_t>({512 / t128, blocks / 32, kMaxSplits}));
+    if (most_q * G >= 1024 && t128 * s128 >= 512) return {true, int(s128)};
+    // Row kernel: two blocks a CU; more ranges cost their join more than they gain: a block takes a key
+    // block in about 1 us / 4, a range adds 0.15 us (8192 keys, one token: 8 / 16 / 64 ranges 18.7 / 15.1 / 21.6 us).
+    const int64_t t16 = std::max<int64_t>((rows + 15) / 16, std::min(n_seqs, n_tokens)) * c.n_kv;
+    const int64_t best = int64_t(std::sqrt(1.6 * double(blocks)) + 0.5);
+    return {false, int(std::max<int64_t>(1, std::min<int64_t>({768 / t16, best, kMaxSplits})))};
+}
+
+}  // namespace
+
+int kv_attn_splits(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
+    return plan(c, n_seqs, n_tokens, max_pages, max_q, n_heads, window).splits;
 }
 
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits) {
@@ -847,9 +872,7 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
         const dim3 grid{unsigned(a.c.n_kv), unsigned(tiles), unsigned(a.splits)};
         hipLaunchKernelGGL(kern, grid, dim3(unsigned(threads)), 0, s, a, G, bound);
     };
-    // Sequences with more than kFewRows rows go to the tile kernel, unless none
-    // can have as many; the others to the row kernel, unless there is but one.
-    const bool many = rows > kFewRows && int64_t(a.max_q ? a.max_q : a.n_tokens) * G > kFewRows;
+    const bool many = plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, a.n_heads, a.window).many;
     const bool few = !many || a.n_seqs > 1;
     if (few) {
         const int64_t tiles = (rows + 15) / 16 + a.n_seqs;
