@@ -24,6 +24,9 @@ struct SampleArgs {
     int32_t* gen;
     int gen_cap, advance;
 };
-int launch_sample(const SampleArgs& a, hipStream_t s);
+// Rows of many logits are cut into slices where the caller gives scratch
+// (sample_scratch_floats, 16-byte aligned; 0: none is used).
+size_t sample_scratch_floats(int rows, int vocab);
+int launch_sample(const SampleArgs& a, hipStream_t s, float* scratch = nullptr);
 
 }  // namespace wv

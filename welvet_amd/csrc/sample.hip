@@ -118,19 +118,23 @@ struct Row {
         return x;
     }
     __device__ __forceinline__ int passes() const { return (vocab + kPass - 1) / kPass; }
-    // From memory, four passes' loads on their way.
+    // Passes k0 .. k1 - 1 from memory, four passes' loads on their way.
     template <class F>
-    __device__ __forceinline__ void stream(F f) const {
-        const int n = passes(), i0 = 4 * int(threadIdx.x);
+    __device__ __forceinline__ void range(int k0, int k1, F f) const {
+        const int i0 = 4 * int(threadIdx.x);
         float4 x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = fetch(k * kPass + i0);
-        for (int k = 0; k < n; ++k) {
+        for (int k = 0; k < 4; ++k) x[k] = k0 + k < k1 ? fetch((k0 + k) * kPass + i0) : float4{};
+        for (int k = k0; k < k1; ++k) {
             const float4 y = x[0];
             x[0] = x[1], x[1] = x[2], x[2] = x[3];
-            x[3] = fetch((k + 4) * kPass + i0);
+            if (k + 4 < k1) x[3] = fetch((k + 4) * kPass + i0);
             f(clean(y), k * kPass + i0, k);
         }
+    }
+    template <class F>
+    __device__ __forceinline__ void stream(F f) const {
+        range(0, passes(), f);
     }
     // The first pass over the row, which fills LDS.
     template <class F>
@@ -332,22 +336,118 @@ __device__ __forceinline__ void put(const SampleArgs& a, int row, int token, flo
     }
 }
 
-// One row per block.
+// A row's settings, cleaned.
+struct Settings {
+    float temp, top_p, min_p, u;
+    int top_k;
+    bool greedy, by_k, by_p;
+};
+__device__ __forceinline__ Settings settings(const SampleArgs& a, int r) {
+    Settings x;
+    x.temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
+    x.top_k = a.p.top_k ? a.p.top_k[r] : 0;
+    x.top_p = a.p.top_p ? a.p.top_p[r] : 1.0f;
+    const float m = a.p.min_p ? a.p.min_p[r] : 0.0f;
+    x.min_p = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
+    const float u = a.p.uniform[a.state ? a.state[3] : r];
+    x.u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+    x.greedy = !(x.temp > 0.0f) || x.top_k == 1 || x.top_p <= 0.0f;
+    x.by_k = x.top_k > 0 && x.top_k < a.vocab;
+    x.by_p = x.top_p < 1.0f;
+    return x;
+}
+__device__ __forceinline__ Scale scale_of(float max, float temp) {
+    Scale c;
+    c.max = max;
+    // an infinite maximum takes all, whatever the temperature
+    const double cd = max < INFINITY ? fmin(1.4426950408889634 / double(temp), 1e30) : 1.0;
+    c.hi = float(cd);
+    c.lo = cd < 1e30 ? float(cd - double(c.hi)) : 0.0f;
+    c.least = c.hi > 1e-36f ? -200.0f / c.hi : -3.4028235e38f;
+    return c;
+}
+
+// Which of the tokens in front of a cut (0: all) are kept, and their weights.
+struct Kept {
+    Scale c;
+    float cl, min_p;
+    int ci;
+    __device__ __forceinline__ Kept(const Scale& c, u64 cut, float min_p)
+        : c(c), cl(cut ? key_logit(cut) : -INFINITY), min_p(min_p), ci(cut ? int(~uint32_t(cut)) : -1) {}
+    // in units of 1, a multiple of 2^-44
+    __device__ __forceinline__ double operator()(float l, int i) const {
+        const float w = weight(c, l);
+        const bool k = (l > cl || (l == cl && i <= ci)) && w >= min_p;
+        return k ? (256.0 + double(w)) - 256.0 : 0.0;
+    }
+};
+
+// The place of u among s.seg, the kept weights of each 256 tokens, and in the
+// segment where it lies.
 template <bool R>
-__global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned) {
-    extern __shared__ __align__(16) uint8_t raw[];
-    Shared<R>& s = *reinterpret_cast<Shared<R>*>(raw);
-    const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+__device__ __forceinline__ void pick(const SampleArgs& a, Shared<R>& s, const Row<R>& row, int r, const Kept& kept,
+                                     float u) {
+    const int segs = (a.vocab + kSegment - 1) / kSegment, lane = threadIdx.x & 63;
+    const u64 total = find_in(s, s.seg, segs, ~u64(0));
+    const u64 want = u64(double(u) * double(total));
+    find_in(s, s.seg, segs, want + 1);
+    if (threadIdx.x < 64) {
+        const int i = s.at * kSegment + 4 * lane;
+        const float4 x = row.at(i);
+        const float y[4] = {x.x, x.y, x.z, x.w};
+        u64 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = u64(kept(y[j], i + j) * 17592186044416.0);
+        const u64 sum = (v[0] + v[1]) + (v[2] + v[3]);
+        u64 before = s.sum + wave_scan(sum) - sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (v[j] && before <= want && want < before + v[j])
+                put(a, r, i + j, float(double(v[j]) / double(total)));
+            before += v[j];
+        }
+    }
+}
+
+// The draw among the n tokens of the list, which holds the top_k at least.
+template <bool R>
+__device__ __forceinline__ void pick_from_list(const SampleArgs& a, Shared<R>& s, int r, const Settings& x,
+                                               const Scale& c, int n) {
+    const int t = threadIdx.x;
+    u64 key = 0, w = 0, mass = 0;
+    int rank = kList;
+    if (t < n) {
+        key = s.list[t];
+        w = s.weights[t];
+        rank_list(s, n, key, rank, mass);
+    }
+    if (t < n && rank == min(x.top_k, n) - 1) s.sum = mass + w;  // what the top k hold
+    __syncthreads();
+    bool keep = rank < x.top_k;
+    if (x.by_p) keep = keep && mass < max(u64(1), u64(ceil(double(x.top_p) * double(s.sum))));
+    keep = keep && weight(c, key_logit(key)) >= x.min_p;
+    // by index: the kept tokens in front of this one, and all
+    if (!keep) w = 0;
+    if (t < n) s.weights[t] = w;
+    __syncthreads();
+    u64 before = 0, total = 0;
+    if (t < n)
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+            const u64 v = s.weights[j];
+            total += v;
+            if (uint32_t(s.list[j]) > uint32_t(key)) before += v;  // ~index: larger is earlier
+        }
+    const u64 want = u64(double(x.u) * double(total));
+    if (w && before <= want && want < before + w) put(a, r, int(~uint32_t(key)), float(double(w) / double(total)));
+}
+
+// A whole row by one block.
+template <bool R>
+__device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, int r, bool aligned) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const Row<R> row{a.logits + int64_t(r) * a.stride, s.row, a.vocab, aligned};
-
-    const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
-    const int top_k = a.p.top_k ? a.p.top_k[r] : 0;
-    const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f;
-    float min_p = a.p.min_p ? a.p.min_p[r] : 0.0f;
-    min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
-    float u = a.p.uniform[a.state ? a.state[3] : r];
-    u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-
+    const Settings set = settings(a, r);
     float top = -INFINITY;  // this thread's largest
     row.first([&](float4 x, int, int) { top = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), top); });
     const float wm = wave_maximum(top);
@@ -362,7 +462,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
         if (t == 0) put(a, r, -1, 0.0f);
         return;
     }
-    if (!(temp > 0.0f) || top_k == 1 || top_p <= 0.0f) {  // the largest logit's first index
+    if (set.greedy) {  // the largest logit's first index
         if (top == c.max) {
             u64 best = 0;
             row.each([&](float l, int i) {
@@ -374,22 +474,17 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
         if (t == 0) put(a, r, int(~uint32_t(s.key)), 1.0f);
         return;
     }
-    // an infinite maximum takes all, whatever the temperature
-    const double cd = c.max < INFINITY ? fmin(1.4426950408889634 / double(temp), 1e30) : 1.0;
-    c.hi = float(cd);
-    c.lo = cd < 1e30 ? float(cd - double(c.hi)) : 0.0f;
-    c.least = c.hi > 1e-36f ? -200.0f / c.hi : -3.4028235e38f;
-    const bool by_k = top_k > 0 && top_k < a.vocab, by_p = top_p < 1.0f;
+    c = scale_of(c.max, set.temp);
     __syncthreads();
 
-    if (by_k && top_k <= kFewK) {
+    if (set.by_k && set.top_k <= kFewK) {
         // the top_k threads with the largest maxima hold top_k tokens at least as
         // large as the least of these: it bounds the candidates (to its bin)
         clear_hist(s);
         const int bin = bin_of(log_weight(c, top));
         if (top > -INFINITY) atomicAdd(&s.hist[bin], u64(1));
         __syncthreads();
-        find_in(s, s.hist, kBins, u64(top_k));
+        find_in(s, s.hist, kBins, u64(set.top_k));
         const int last = s.at < 0 ? kBins : s.at;
         __syncthreads();
         if (t == 0) s.sum = ~u64(0);
@@ -408,43 +503,14 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
         });
         __syncthreads();
         const int n = s.n;
-        if (n <= kList) {
-            u64 key = 0, w = 0, mass = 0;
-            int rank = kList;
-            if (t < n) {
-                key = s.list[t];
-                w = s.weights[t];
-                rank_list(s, n, key, rank, mass);
-            }
-            if (t < n && rank == min(top_k, n) - 1) s.sum = mass + w;  // what the top k hold
-            __syncthreads();
-            bool keep = rank < top_k;
-            if (by_p) keep = keep && mass < max(u64(1), u64(ceil(double(top_p) * double(s.sum))));
-            keep = keep && weight(c, key_logit(key)) >= min_p;
-            // by index: the kept tokens in front of this one, and all
-            if (!keep) w = 0;
-            if (t < n) s.weights[t] = w;
-            __syncthreads();
-            u64 before = 0, total = 0;
-            if (t < n)
-#pragma unroll 8
-                for (int j = 0; j < n; ++j) {
-                    const u64 v = s.weights[j];
-                    total += v;
-                    if (uint32_t(s.list[j]) > uint32_t(key)) before += v;  // ~index: larger is earlier
-                }
-            const u64 want = u64(double(u) * double(total));
-            if (w && before <= want && want < before + w)
-                put(a, r, int(~uint32_t(key)), float(double(w) / double(total)));
-            return;
-        }
+        if (n <= kList) return pick_from_list(a, s, r, set, c, n);
         __syncthreads();
     }
 
     u64 cut = 0;  // the last token kept, 0: all
 #pragma unroll 1
     for (int mass = 0; mass < 2; ++mass) {  // top-k by counts, then top-p by weights
-        if (!(mass ? by_p : by_k)) continue;
+        if (!(mass ? set.by_p : set.by_k)) continue;
         clear_hist(s);
         row.each([&](float l, int i) {
             const float x = log_weight(c, l);
@@ -452,22 +518,16 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
                 atomicAdd(&s.hist[bin_of(x)], mass ? fixed(__builtin_amdgcn_exp2f(x)) : u64(1));
         });
         __syncthreads();
-        u64 target = u64(top_k);
+        u64 target = u64(set.top_k);
         if (mass) {
             const u64 whole = find_in(s, s.hist, kBins, ~u64(0));
-            target = max(u64(1), min(whole, u64(ceil(double(top_p) * double(whole)))));
+            target = max(u64(1), min(whole, u64(ceil(double(set.top_p) * double(whole)))));
         }
         cut = find_cut(s, row, c, cut, target, mass != 0);
         __syncthreads();
     }
     // the kept weights of each 256 tokens, then the place of u among them
-    const float cl = cut ? key_logit(cut) : -INFINITY;
-    const int ci = cut ? int(~uint32_t(cut)) : -1;
-    auto kept = [&](float l, int i) {  // in units of 1, exact in 2^-44
-        const float w = weight(c, l);
-        const bool k = (l > cl || (l == cl && i <= ci)) && w >= min_p;
-        return k ? (256.0 + double(w)) - 256.0 : 0.0;
-    };
+    const Kept kept(c, cut, set.min_p);
     const int segs = (a.vocab + kSegment - 1) / kSegment;
     row.each4([&](float4 x, int i, int k) {
         // 256 weights of at most 1: their sum in steps of 2^-44 fits a double
@@ -476,31 +536,240 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
         if (lane == 0 && sg < segs) s.seg[sg] = u64(v * 17592186044416.0);
     });
     __syncthreads();
-    const u64 total = find_in(s, s.seg, segs, ~u64(0));
-    const u64 want = u64(double(u) * double(total));
-    find_in(s, s.seg, segs, want + 1);
-    if (wave == 0) {
-        const int i = s.at * kSegment + 4 * lane;
-        const float4 x = row.at(i);
-        const float y[4] = {x.x, x.y, x.z, x.w};
-        u64 v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = u64(kept(y[j], i + j) * 17592186044416.0);
-        const u64 sum = (v[0] + v[1]) + (v[2] + v[3]);
-        u64 before = s.sum + wave_scan(sum) - sum;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (v[j] && before <= want && want < before + v[j])
-                put(a, r, i + j, float(double(v[j]) / double(total)));
-            before += v[j];
-        }
+    pick(a, s, row, r, kept, set.u);
+}
+
+template <bool R>
+__global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    sample_row(a, *reinterpret_cast<Shared<R>*>(raw), blockIdx.x, aligned);
+}
+
+// ---------------------------------------------------------------------------
+// Rows of many logits, few of them: a row is cut into slices of whole passes,
+// one to a block, in four launches that hand on through memory
+//   max    the slices' maxima
+//   hist   counts (weights) of the slices' tokens by bin, for the first cut
+//   collect  the cut's bin from all slices' histograms; its tokens into the
+//            row's list, the weights of the bins in front of it by segment
+//   finish one block a row: the list's cut, and the place of u
+// Rows that do not fit this (both top_k > kFewK and top_p, a bin of more
+// tokens than the list takes) are done whole by the last launch.
+// ---------------------------------------------------------------------------
+
+struct SliceRow {
+    u64 key;   // greedy: the largest token
+    int n;     // tokens of the list, kList and more: too many
+    int bin;   // the cut's bin, kBins: none
+    u64 left;  // what the cut takes of it (top-p's target for whole rows of top-k lists: unused)
+    float max[64];
+    u64 list[kList], weights[kList];
+    u64 seg[kSegments];
+};
+struct Slices {
+    SliceRow* rows;
+    u64* hist;      // [row][slice][kBins]
+    int n, passes;  // slices of a row, passes of a slice
+};
+
+__device__ __forceinline__ float row_max(const Slices& p, int r) {
+    const int lane = threadIdx.x & 63;
+    return wave_maximum(lane < p.n ? p.rows[r].max[lane] : -INFINITY);
+}
+__device__ __forceinline__ bool sliced(const Settings& x) { return !(x.by_k && x.by_p && x.top_k > kFewK); }
+
+__global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p, bool aligned) {
+    __shared__ float part[kWaves];
+    const int r = blockIdx.y, sl = blockIdx.x;
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    float top = -INFINITY;
+    row.range(sl * p.passes, min((sl + 1) * p.passes, row.passes()),
+              [&](float4 x, int, int) { top = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), top); });
+    top = wave_maximum(top);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, part[w]);
+        p.rows[r].max[sl] = top;
+        if (sl == 0) p.rows[r].key = 0, p.rows[r].n = 0;
     }
+}
+
+__global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p, bool aligned) {
+    __shared__ u64 hist[kBins];
+    const int r = blockIdx.y, sl = blockIdx.x;
+    const Settings set = settings(a, r);
+    const float max = row_max(p, r);
+    if (max == -INFINITY || set.greedy || !(set.by_k || set.by_p) || !sliced(set)) return;
+    const Scale c = scale_of(max, set.temp);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) hist[i] = 0;
+    __syncthreads();
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    auto add = [&](float l) {
+        const float x = log_weight(c, l);
+        if (l > -INFINITY) atomicAdd(&hist[bin_of(x)], set.by_k ? u64(1) : fixed(__builtin_amdgcn_exp2f(x)));
+    };
+    row.range(sl * p.passes, min((sl + 1) * p.passes, row.passes()), [&](float4 x, int, int) {
+        add(x.x);
+        add(x.y);
+        add(x.z);
+        add(x.w);
+    });
+    __syncthreads();
+    u64* out = p.hist + (int64_t(r) * p.n + sl) * kBins;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) out[i] = hist[i];
+}
+
+__global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices p, bool aligned) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
+    const int r = blockIdx.y, sl = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const Settings set = settings(a, r);
+    const float max = row_max(p, r);
+    if (max == -INFINITY || !sliced(set)) return;
+    SliceRow& g = p.rows[r];
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
+    if (set.greedy) {
+        if (g.max[sl] != max) return;
+        u64 best = 0;
+        row.range(k0, k1, [&](float4 x, int i, int) {
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            for (int j = 3; j >= 0; --j)
+                if (v[j] == max) best = best > token_key(max, i + j) ? best : token_key(max, i + j);
+        });
+        if (best) atomicMax(&g.key, best);
+        return;
+    }
+    const Scale c = scale_of(max, set.temp);
+    int bin = kBins;
+    if (set.by_k || set.by_p) {
+        static_assert(kBins == 2 * kThreads, "two bins to a thread");
+        const ulonglong2* h = reinterpret_cast<const ulonglong2*>(p.hist + int64_t(r) * p.n * kBins) + t;
+        u64 v0 = 0, v1 = 0;
+        for (int k = 0; k < p.n; k += 8) {  // eight slices' loads on their way
+            ulonglong2 x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = k + j < p.n ? h[int64_t(k + j) * (kBins / 2)] : ulonglong2{0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v0 += x[j].x, v1 += x[j].y;
+        }
+        s.hist[2 * t] = v0, s.hist[2 * t + 1] = v1;
+        __syncthreads();
+        u64 target = u64(set.top_k);
+        if (!set.by_k) {
+            const u64 whole = find_in(s, s.hist, kBins, ~u64(0));
+            target = u64(ceil(double(set.top_p) * double(whole)));
+            target = target > whole ? whole : target < 1 ? 1 : target;
+        }
+        __syncthreads();
+        find_in(s, s.hist, kBins, target);
+        if (s.at >= 0) bin = s.at;
+        if (sl == 0 && t == 0) {
+            g.bin = bin;
+            g.left = bin < kBins ? target - s.sum : 0;
+        }
+    } else if (sl == 0 && t == 0) {
+        g.bin = kBins;
+    }
+    // few of top-k: the list takes all tokens down to the bin
+    const bool few = set.by_k && set.top_k <= kFewK;
+    auto visit = [&](float l, int i) {
+        const float x = log_weight(c, l);
+        const int b = bin_of(x);
+        if (l == -INFINITY) return 0.0;
+        const float w = __builtin_amdgcn_exp2f(x);
+        if (b == bin || (few && b < bin)) {
+            const int at = atomicAdd(&g.n, 1);
+            if (at < kList) {
+                g.list[at] = token_key(l, i);
+                g.weights[at] = fixed(w);
+            }
+            return 0.0;
+        }
+        return b < bin && w >= set.min_p ? (256.0 + double(w)) - 256.0 : 0.0;
+    };
+    const int segs = (a.vocab + kSegment - 1) / kSegment;
+    row.range(k0, k1, [&](float4 x, int i, int k) {
+        const double v = wave_total_f64((visit(x.x, i) + visit(x.y, i + 1)) + (visit(x.z, i + 2) + visit(x.w, i + 3)));
+        const int sg = k * kWaves + wave;
+        if (lane == 0 && sg < segs) g.seg[sg] = u64(v * 17592186044416.0);
+    });
+}
+
+__global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices p, bool aligned) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
+    const int r = blockIdx.x, t = threadIdx.x;
+    const Settings set = settings(a, r);
+    const float max = row_max(p, r);
+    SliceRow& g = p.rows[r];
+    if (max == -INFINITY) {  // every token masked
+        if (t == 0) put(a, r, -1, 0.0f);
+        return;
+    }
+    if (!sliced(set) || (!set.greedy && g.n > kList)) return sample_row(a, s, r, aligned);
+    if (set.greedy) {
+        if (t == 0) put(a, r, int(~uint32_t(g.key)), 1.0f);
+        return;
+    }
+    const Scale c = scale_of(max, set.temp);
+    const int n = g.n;
+    if (t < n) s.list[t] = g.list[t], s.weights[t] = g.weights[t];
+    const int segs = (a.vocab + kSegment - 1) / kSegment;
+    for (int i = t; i < segs; i += kThreads) s.seg[i] = g.seg[i];
+    if (t == 0) s.key = 0;
+    __syncthreads();
+    if (set.by_k && set.top_k <= kFewK) return pick_from_list(a, s, r, set, c, n);
+    if (n) {
+        // the cut among the bin's tokens, then what it keeps of them into their segments
+        u64 key = 0, mass = 0, w = 0;
+        int rank = 0;
+        if (t < n) {
+            key = s.list[t], w = s.weights[t];
+            rank_list(s, n, key, rank, mass);
+            if (set.by_k ? u64(rank) + 1 == g.left : mass < g.left && mass + w >= g.left) s.key = key;
+        }
+        __syncthreads();
+        if (t < n && key >= s.key && weight(c, key_logit(key)) >= set.min_p)
+            atomicAdd(&s.seg[int(~uint32_t(key)) / kSegment], w);
+        __syncthreads();
+    }
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    pick(a, s, row, r, Kept(c, s.key, set.min_p), set.u);
 }
 
 }  // namespace
 
-int launch_sample(const SampleArgs& a, hipStream_t s) {
+// Slices of a row: enough that the rows fill the GPU, of 8192 logits at
+// least; 0: rows are done whole, where they fit LDS or are many.
+int sample_slices(int rows, int vocab) {
+    if (vocab <= kResident || rows > 128) return 0;
+    const int passes = (vocab + kPass - 1) / kPass;
+    const int want = std::max(1, std::min({64, (passes + 1) / 2, 256 / rows}));
+    const int each = (passes + want - 1) / want;
+    return (passes + each - 1) / each;
+}
+size_t sample_scratch_floats(int rows, int vocab) {
+    const size_t n = size_t(sample_slices(rows, vocab));
+    return n ? size_t(rows) * (sizeof(SliceRow) + n * kBins * sizeof(u64)) / sizeof(float) : 0;
+}
+
+int launch_sample(const SampleArgs& a, hipStream_t s, float* scratch) {
     const bool al = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.stride % 4 == 0;
+    const int n = scratch ? sample_slices(a.rows, a.vocab) : 0;
+    if (n) {
+        const int passes = (a.vocab + kPass - 1) / kPass;
+        Slices p{reinterpret_cast<SliceRow*>(scratch), nullptr, n, (passes + n - 1) / n};
+        p.hist = reinterpret_cast<u64*>(p.rows + a.rows);
+        const dim3 grid{unsigned(n), unsigned(a.rows)};
+        hipLaunchKernelGGL(k_slice_max, grid, dim3(kThreads), 0, s, a, p, al);
+        hipLaunchKernelGGL(k_slice_hist, grid, dim3(kThreads), 0, s, a, p, al);
+        hipLaunchKernelGGL(k_slice_collect, grid, dim3(kThreads), unsigned(sizeof(Shared<false>)), s, a, p, al);
+        hipLaunchKernelGGL(k_slice_finish, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(sizeof(Shared<false>)), s,
+                           a, p, al);
+        return int(hipGetLastError());
+    }
     auto go = [&](auto kern, size_t lds) {
         hipLaunchKernelGGL(kern, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(lds), s, a, al);
     };
@@ -530,6 +799,11 @@ extern "C" int wv_sample_dev(const float* d_logits, int64_t stride, int32_t rows
     SampleArgs a{};
     a.logits = d_logits, a.stride = stride, a.rows = rows, a.vocab = vocab;
     a.p = *sampling, a.tokens = d_tokens, a.probs = d_probs;
-    const int e = launch_sample(a, rt_stream(stream, rt_current_device()));
+    hipStream_t st = rt_stream(stream, rt_current_device());
+    RtScratch sc;  // not under capture: what a replay writes must not lie in a slot that other calls take
+    const size_t floats = rt_capturing(st) ? 0 : sample_scratch_floats(rows, vocab);
+    if (floats)
+        if (const int e = sc.get(floats, st, "wv_sample: scratch")) return e;
+    const int e = launch_sample(a, st, floats ? sc.f() : nullptr);
     return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_sample: kernel launch");
 }
