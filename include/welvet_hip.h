@@ -501,10 +501,13 @@ typedef struct wv_sampling {
  *   the token: the first by index at which the running sum of the kept
  *   weights exceeds u times their total.
  * NaN logits count as -inf; a +inf logit takes all. A row of nothing but -inf
- * gives token -1. Weights are f32 (relative error about 2^-23) and summed
- * exactly in units of 2^-44 of the largest. d_probs (may be NULL): the drawn
- * token's share of the kept weights (1 where T <= 0, 0 for token -1). vocab is
- * at most 2^19. Device pointers, enqueued on `stream`; allocates nothing. */
+ * gives token -1. Weights are f32, the rounding of (l_i - max) / T to 24 bits
+ * included, and summed exactly in units of 2^-44 of the largest: a token that
+ * stands on the edge of top_p or u may fall to either side. d_probs (may be
+ * NULL): the drawn token's share of the kept weights (1 where T <= 0, 0 for
+ * token -1). vocab is at most 2^19. Device pointers, enqueued on `stream`. Up
+ * to 128 rows of more than 32768 logits use the library's own scratch, except
+ * on a stream under capture, where one block draws a row whatever its length. */
 int wv_sample_dev(const float *d_logits, int64_t stride, int32_t rows, int32_t vocab, const wv_sampling *sampling,
                   int32_t *d_tokens, float *d_probs, void *stream);
 

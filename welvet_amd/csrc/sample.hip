@@ -23,7 +23,8 @@ constexpr float kPerUnit = 64.0f;
 constexpr int kList = 512;          // tokens ranked one per thread
 constexpr int kFewK = 128;          // top-k up to which the candidates alone are looked at
 constexpr int kPass = 4 * kThreads; // tokens of a pass of the block, four to a thread
-constexpr int kSegment = 256;       // tokens of a wave's pass, in order of index
+constexpr int kSegment = 1024;      // tokens that a wave goes through in four passes, in order of index
+constexpr int kTurn = 4 * kPass;    // tokens of four passes
 constexpr int kMaxVocab = 1 << 19;  // 2^19 weights of at most 2^44 stay below 2^63
 constexpr int kSegments = kMaxVocab / kSegment;
 constexpr int kResident = 32768;    // logits of a row that stay in LDS
@@ -74,6 +75,11 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {
     return v;
 }
 
+__device__ __forceinline__ u64 last_lane(u64 v) {
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), 63));
+    return u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), 63))) << 32 | lo;
+}
+
 template <bool RESIDENT>
 struct Shared {
     float row[RESIDENT ? kResident : 4];
@@ -88,9 +94,9 @@ struct Shared {
 };
 
 // One row, read from memory once where it fits LDS, else in every pass.
-// each4(f): f(four logits, index of the first, pass) for this thread's ones,
-// 256 consecutive ones to a wave's pass. NaN and what lies behind the row are
-// -inf, which no step counts.
+// each4(f): f(four logits, index of the first, pass) for this thread's ones;
+// in four passes (a turn) a wave meets 1024 consecutive tokens in order, 256
+// a pass. NaN and what lies behind the row are -inf, which no step counts.
 template <bool RESIDENT>
 struct Row {
     const float* p;
@@ -117,19 +123,22 @@ struct Row {
         x.w = fmaxf(x.w, -INFINITY);
         return x;
     }
-    __device__ __forceinline__ int passes() const { return (vocab + kPass - 1) / kPass; }
+    // Whole turns.
+    __device__ __forceinline__ int passes() const { return (vocab + kTurn - 1) / kTurn * 4; }
+    static __device__ __forceinline__ int index(int k) {
+        return (k >> 2) * kTurn + int(threadIdx.x >> 6) * kSegment + (k & 3) * 256 + 4 * int(threadIdx.x & 63);
+    }
     // Passes k0 .. k1 - 1 from memory, four passes' loads on their way.
     template <class F>
     __device__ __forceinline__ void range(int k0, int k1, F f) const {
-        const int i0 = 4 * int(threadIdx.x);
         float4 x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = k0 + k < k1 ? fetch((k0 + k) * kPass + i0) : float4{};
+        for (int k = 0; k < 4; ++k) x[k] = k0 + k < k1 ? fetch(index(k0 + k)) : float4{};
         for (int k = k0; k < k1; ++k) {
             const float4 y = x[0];
             x[0] = x[1], x[1] = x[2], x[2] = x[3];
-            if (k + 4 < k1) x[3] = fetch((k + 4) * kPass + i0);
-            f(clean(y), k * kPass + i0, k);
+            if (k + 4 < k1) x[3] = fetch(index(k + 4));
+            f(clean(y), index(k), k);
         }
     }
     template <class F>
@@ -140,15 +149,14 @@ struct Row {
     template <class F>
     __device__ __forceinline__ void first(F f) const {
         if constexpr (RESIDENT) {
-            const int i0 = 4 * int(threadIdx.x);
             float4 x[kResident / kPass];
 #pragma unroll
-            for (int k = 0; k < kResident / kPass; ++k) x[k] = fetch(k * kPass + i0);
+            for (int k = 0; k < kResident / kPass; ++k) x[k] = fetch(index(k));
 #pragma unroll
             for (int k = 0; k < kResident / kPass; ++k) {
                 x[k] = clean(x[k]);
-                *reinterpret_cast<float4*>(lds + k * kPass + i0) = x[k];
-                f(x[k], k * kPass + i0, k);
+                *reinterpret_cast<float4*>(lds + index(k)) = x[k];
+                f(x[k], index(k), k);
             }
         } else {
             stream(f);
@@ -157,8 +165,8 @@ struct Row {
     template <class F>
     __device__ __forceinline__ void each4(F f) const {
         if constexpr (RESIDENT) {
-            const int n = passes(), i0 = 4 * int(threadIdx.x);
-            for (int k = 0; k < n; ++k) f(*reinterpret_cast<const float4*>(lds + k * kPass + i0), k * kPass + i0, k);
+            const int n = passes();
+            for (int k = 0; k < n; ++k) f(*reinterpret_cast<const float4*>(lds + index(k)), index(k), k);
         } else {
             stream(f);
         }
@@ -220,26 +228,35 @@ template <bool R>
 __device__ __forceinline__ u64 nth_equal(Shared<R>& s, const Row<R>& row, float l, u64 nth) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int segs = (row.vocab + kSegment - 1) / kSegment;
+    int c = 0;
     row.each4([&](float4 x, int, int k) {
-        const int c = (x.x == l) + (x.y == l) + (x.z == l) + (x.w == l);
-        const int n = wave_total_i(c), sg = k * kWaves + wave;
-        if (lane == 0 && sg < segs) s.seg[sg] = u64(n);
+        c += (x.x == l) + (x.y == l) + (x.z == l) + (x.w == l);
+        if ((k & 3) == 3) {
+            const int n = wave_total_i(c), sg = (k >> 2) * kWaves + wave;
+            if (lane == 0 && sg < segs) s.seg[sg] = u64(n);
+            c = 0;
+        }
     });
     __syncthreads();
     find_in(s, s.seg, segs, nth);
     const int sg = s.at;
     const u64 want = nth - s.sum;
     if (wave == 0) {
-        const int i = sg * kSegment + 4 * lane;
-        const float4 x = row.at(i);
-        const float v[4] = {x.x, x.y, x.z, x.w};
-        u64 c = 0;
+        u64 before = 0;
+        for (int q = 0; q < 4; ++q) {
+            const int i = sg * kSegment + q * 256 + 4 * lane;
+            const float4 x = row.at(i);
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            u64 n = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c += v[j] == l;
-        u64 before = wave_scan(c) - c;
+            for (int j = 0; j < 4; ++j) n += v[j] == l;
+            const u64 incl = before + wave_scan(n);
+            u64 at = incl - n;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (v[j] == l && ++before == want) s.key = token_key(l, i + j);
+            for (int j = 0; j < 4; ++j)
+                if (v[j] == l && ++at == want) s.key = token_key(l, i + j);
+            before = last_lane(incl);
+        }
     }
     __syncthreads();
     return s.key;
@@ -382,8 +399,12 @@ struct Kept {
     }
 };
 
-// The place of u among s.seg, the kept weights of each 256 tokens, and in the
+// The place of u among s.seg, the kept weights of each segment, and in the
 // segment where it lies.
+// The wave's sum of doubles that are multiples of 2^-44, in units of it: up to
+// 1024, so in integers.
+__device__ __forceinline__ u64 segment_sum(double v) { return last_lane(wave_scan(u64(v * 17592186044416.0))); }
+
 template <bool R>
 __device__ __forceinline__ void pick(const SampleArgs& a, Shared<R>& s, const Row<R>& row, int r, const Kept& kept,
                                      float u) {
@@ -392,19 +413,26 @@ __device__ __forceinline__ void pick(const SampleArgs& a, Shared<R>& s, const Ro
     const u64 want = u64(double(u) * double(total));
     find_in(s, s.seg, segs, want + 1);
     if (threadIdx.x < 64) {
-        const int i = s.at * kSegment + 4 * lane;
-        const float4 x = row.at(i);
-        const float y[4] = {x.x, x.y, x.z, x.w};
-        u64 v[4];
+        u64 at = s.sum;
+        float4 x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = u64(kept(y[j], i + j) * 17592186044416.0);
-        const u64 sum = (v[0] + v[1]) + (v[2] + v[3]);
-        u64 before = s.sum + wave_scan(sum) - sum;
+        for (int q = 0; q < 4; ++q) x[q] = row.at(s.at * kSegment + q * 256 + 4 * lane);
+        for (int q = 0; q < 4; ++q) {
+            const int i = s.at * kSegment + q * 256 + 4 * lane;
+            const float y[4] = {x[0].x, x[0].y, x[0].z, x[0].w};
+            x[0] = x[1], x[1] = x[2], x[2] = x[3];
+            u64 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (v[j] && before <= want && want < before + v[j])
-                put(a, r, i + j, float(double(v[j]) / double(total)));
-            before += v[j];
+            for (int j = 0; j < 4; ++j) v[j] = u64(kept(y[j], i + j) * 17592186044416.0);
+            const u64 sum = (v[0] + v[1]) + (v[2] + v[3]), incl = at + wave_scan(sum);
+            u64 before = incl - sum;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (v[j] && before <= want && want < before + v[j])
+                    put(a, r, i + j, float(double(v[j]) / double(total)));
+                before += v[j];
+            }
+            at = last_lane(incl);
         }
     }
 }
@@ -529,11 +557,15 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
     // the kept weights of each 256 tokens, then the place of u among them
     const Kept kept(c, cut, set.min_p);
     const int segs = (a.vocab + kSegment - 1) / kSegment;
+    double sum = 0.0;  // a segment's weights of at most 1 in steps of 2^-44 and their sums up to 256 are exact
     row.each4([&](float4 x, int i, int k) {
-        // 256 weights of at most 1: their sum in steps of 2^-44 fits a double
-        const double v = wave_total_f64((kept(x.x, i) + kept(x.y, i + 1)) + (kept(x.z, i + 2) + kept(x.w, i + 3)));
-        const int sg = k * kWaves + wave;
-        if (lane == 0 && sg < segs) s.seg[sg] = u64(v * 17592186044416.0);
+        sum += (kept(x.x, i) + kept(x.y, i + 1)) + (kept(x.z, i + 2) + kept(x.w, i + 3));
+        if ((k & 3) == 3) {
+            const u64 v = segment_sum(sum);
+            const int sg = (k >> 2) * kWaves + wave;
+            if (lane == 0 && sg < segs) s.seg[sg] = v;
+            sum = 0.0;
+        }
     });
     __syncthreads();
     pick(a, s, row, r, kept, set.u);
@@ -559,16 +591,15 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
 
 struct SliceRow {
     u64 key;   // greedy: the largest token
-    int n;     // tokens of the list, kList and more: too many
-    int bin;   // the cut's bin, kBins: none
-    u64 left;  // what the cut takes of it (top-p's target for whole rows of top-k lists: unused)
+    int n;     // tokens of the list; over kList: more than it holds
+    u64 left;  // what the cut keeps of its bin: tokens with top-k, weight with top-p
     float max[64];
     u64 list[kList], weights[kList];
     u64 seg[kSegments];
 };
 struct Slices {
     SliceRow* rows;
-    u64* hist;      // [row][slice][kBins]
+    u64* hist;      // [row][kBins]
     int n, passes;  // slices of a row, passes of a slice
 };
 
@@ -588,6 +619,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p, 
     top = wave_maximum(top);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
+    for (int i = sl * kThreads + threadIdx.x; i < kBins; i += p.n * kThreads) p.hist[int64_t(r) * kBins + i] = 0;
     if (threadIdx.x == 0) {
         for (int w = 1; w < kWaves; ++w) top = fmaxf(top, part[w]);
         p.rows[r].max[sl] = top;
@@ -598,38 +630,40 @@ __global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p, 
 __global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p, bool aligned) {
     __shared__ u64 hist[kBins];
     const int r = blockIdx.y, sl = blockIdx.x;
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
     const Settings set = settings(a, r);
     const float max = row_max(p, r);
     if (max == -INFINITY || set.greedy || !(set.by_k || set.by_p) || !sliced(set)) return;
     const Scale c = scale_of(max, set.temp);
     for (int i = threadIdx.x; i < kBins; i += kThreads) hist[i] = 0;
     __syncthreads();
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
     auto add = [&](float l) {
         const float x = log_weight(c, l);
         if (l > -INFINITY) atomicAdd(&hist[bin_of(x)], set.by_k ? u64(1) : fixed(__builtin_amdgcn_exp2f(x)));
     };
-    row.range(sl * p.passes, min((sl + 1) * p.passes, row.passes()), [&](float4 x, int, int) {
+    row.range(k0, k1, [&](float4 x, int, int) {
         add(x.x);
         add(x.y);
         add(x.z);
         add(x.w);
     });
     __syncthreads();
-    u64* out = p.hist + (int64_t(r) * p.n + sl) * kBins;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) out[i] = hist[i];
+    // sums of integers: the same in any order
+    for (int i = threadIdx.x; i < kBins; i += kThreads)
+        if (hist[i]) atomicAdd(&p.hist[int64_t(r) * kBins + i], hist[i]);
 }
 
 __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices p, bool aligned) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
     const int r = blockIdx.y, sl = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const Settings set = settings(a, r);
-    const float max = row_max(p, r);
-    if (max == -INFINITY || !sliced(set)) return;
     SliceRow& g = p.rows[r];
     const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
     const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
+    const Settings set = settings(a, r);
+    const float max = row_max(p, r);
+    if (max == -INFINITY || !sliced(set)) return;
     if (set.greedy) {
         if (g.max[sl] != max) return;
         u64 best = 0;
@@ -645,16 +679,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices
     int bin = kBins;
     if (set.by_k || set.by_p) {
         static_assert(kBins == 2 * kThreads, "two bins to a thread");
-        const ulonglong2* h = reinterpret_cast<const ulonglong2*>(p.hist + int64_t(r) * p.n * kBins) + t;
-        u64 v0 = 0, v1 = 0;
-        for (int k = 0; k < p.n; k += 8) {  // eight slices' loads on their way
-            ulonglong2 x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = k + j < p.n ? h[int64_t(k + j) * (kBins / 2)] : ulonglong2{0, 0};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v0 += x[j].x, v1 += x[j].y;
-        }
-        s.hist[2 * t] = v0, s.hist[2 * t + 1] = v1;
+        reinterpret_cast<ulonglong2*>(s.hist)[t] = reinterpret_cast<const ulonglong2*>(p.hist + int64_t(r) * kBins)[t];
         __syncthreads();
         u64 target = u64(set.top_k);
         if (!set.by_k) {
@@ -665,59 +690,70 @@ __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices
         __syncthreads();
         find_in(s, s.hist, kBins, target);
         if (s.at >= 0) bin = s.at;
-        if (sl == 0 && t == 0) {
-            g.bin = bin;
-            g.left = bin < kBins ? target - s.sum : 0;
-        }
-    } else if (sl == 0 && t == 0) {
-        g.bin = kBins;
+        if (sl == 0 && t == 0) g.left = bin < kBins ? target - s.sum : 0;
     }
     // few of top-k: the list takes all tokens down to the bin
     const bool few = set.by_k && set.top_k <= kFewK;
+    // bin_of(x) in terms of y = -x kPerUnit: in front of the bin, and in it or (few) not behind it
+    const float front = bin < kBins ? float(bin) : INFINITY;
+    const float lo = few ? -1.0f : front, hi = bin < kBins - 1 ? float(bin + 1) : bin < kBins ? INFINITY : -1.0f;
     auto visit = [&](float l, int i) {
-        const float x = log_weight(c, l);
-        const int b = bin_of(x);
-        if (l == -INFINITY) return 0.0;
+        const float x = log_weight(c, l), y = -x * kPerUnit;
         const float w = __builtin_amdgcn_exp2f(x);
-        if (b == bin || (few && b < bin)) {
-            const int at = atomicAdd(&g.n, 1);
+        if (y >= lo && y < hi && l > -INFINITY) {
+            const int at = atomicAdd(&s.n, 1);
             if (at < kList) {
-                g.list[at] = token_key(l, i);
-                g.weights[at] = fixed(w);
+                s.list[at] = token_key(l, i);
+                s.weights[at] = fixed(w);
             }
             return 0.0;
         }
-        return b < bin && w >= set.min_p ? (256.0 + double(w)) - 256.0 : 0.0;
+        return y < front && l > -INFINITY && w >= set.min_p ? (256.0 + double(w)) - 256.0 : 0.0;
     };
+    if (t == 0) s.n = 0;
+    __syncthreads();
     const int segs = (a.vocab + kSegment - 1) / kSegment;
+    double sum = 0.0;
     row.range(k0, k1, [&](float4 x, int i, int k) {
-        const double v = wave_total_f64((visit(x.x, i) + visit(x.y, i + 1)) + (visit(x.z, i + 2) + visit(x.w, i + 3)));
-        const int sg = k * kWaves + wave;
-        if (lane == 0 && sg < segs) g.seg[sg] = u64(v * 17592186044416.0);
+        sum += (visit(x.x, i) + visit(x.y, i + 1)) + (visit(x.z, i + 2) + visit(x.w, i + 3));
+        if ((k & 3) == 3) {
+            const u64 v = segment_sum(sum);
+            const int sg = (k >> 2) * kWaves + wave;
+            if (lane == 0 && sg < segs) g.seg[sg] = v;
+            sum = 0.0;
+        }
     });
+    __syncthreads();
+    const int n = s.n;  // this slice's share of the row's list
+    if (!n) return;
+    if (t == 0) s.at = atomicAdd(&g.n, n);
+    __syncthreads();
+    if (t < n && s.at + t < kList) g.list[s.at + t] = s.list[t], g.weights[s.at + t] = s.weights[t];
 }
 
 __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices p, bool aligned) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
     const int r = blockIdx.x, t = threadIdx.x;
+    static_assert(kSegments <= kThreads, "a segment to a thread");
+    const SliceRow& g = p.rows[r];
     const Settings set = settings(a, r);
     const float max = row_max(p, r);
-    SliceRow& g = p.rows[r];
     if (max == -INFINITY) {  // every token masked
         if (t == 0) put(a, r, -1, 0.0f);
         return;
     }
-    if (!sliced(set) || (!set.greedy && g.n > kList)) return sample_row(a, s, r, aligned);
+    const int n = g.n;
+    if (!sliced(set) || (!set.greedy && n > kList)) return sample_row(a, s, r, aligned);
     if (set.greedy) {
         if (t == 0) put(a, r, int(~uint32_t(g.key)), 1.0f);
         return;
     }
     const Scale c = scale_of(max, set.temp);
-    const int n = g.n;
     if (t < n) s.list[t] = g.list[t], s.weights[t] = g.weights[t];
     const int segs = (a.vocab + kSegment - 1) / kSegment;
-    for (int i = t; i < segs; i += kThreads) s.seg[i] = g.seg[i];
+    if (t < segs) s.seg[t] = g.seg[t];
+    const u64 left = g.left;
     if (t == 0) s.key = 0;
     __syncthreads();
     if (set.by_k && set.top_k <= kFewK) return pick_from_list(a, s, r, set, c, n);
@@ -728,7 +764,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
         if (t < n) {
             key = s.list[t], w = s.weights[t];
             rank_list(s, n, key, rank, mass);
-            if (set.by_k ? u64(rank) + 1 == g.left : mass < g.left && mass + w >= g.left) s.key = key;
+            if (set.by_k ? u64(rank) + 1 == left : mass < left && mass + w >= left) s.key = key;
         }
         __syncthreads();
         if (t < n && key >= s.key && weight(c, key_logit(key)) >= set.min_p)
@@ -741,26 +777,26 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
 
 }  // namespace
 
-// Slices of a row: enough that the rows fill the GPU, of 8192 logits at
-// least; 0: rows are done whole, where they fit LDS or are many.
+// Slices of a row: enough that the rows fill the GPU, of a turn at least; 0:
+// rows are done whole, where they fit LDS or are many.
 int sample_slices(int rows, int vocab) {
     if (vocab <= kResident || rows > 128) return 0;
-    const int passes = (vocab + kPass - 1) / kPass;
-    const int want = std::max(1, std::min({64, (passes + 1) / 2, 256 / rows}));
-    const int each = (passes + want - 1) / want;
-    return (passes + each - 1) / each;
+    const int turns = (vocab + kTurn - 1) / kTurn;
+    const int want = std::max(1, std::min({64, turns, 512 / rows}));
+    const int each = (turns + want - 1) / want;
+    return (turns + each - 1) / each;
 }
 size_t sample_scratch_floats(int rows, int vocab) {
     const size_t n = size_t(sample_slices(rows, vocab));
-    return n ? size_t(rows) * (sizeof(SliceRow) + n * kBins * sizeof(u64)) / sizeof(float) : 0;
+    return n ? size_t(rows) * (sizeof(SliceRow) + kBins * sizeof(u64)) / sizeof(float) : 0;
 }
 
 int launch_sample(const SampleArgs& a, hipStream_t s, float* scratch) {
     const bool al = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.stride % 4 == 0;
     const int n = scratch ? sample_slices(a.rows, a.vocab) : 0;
     if (n) {
-        const int passes = (a.vocab + kPass - 1) / kPass;
-        Slices p{reinterpret_cast<SliceRow*>(scratch), nullptr, n, (passes + n - 1) / n};
+        const int turns = (a.vocab + kTurn - 1) / kTurn;
+        Slices p{reinterpret_cast<SliceRow*>(scratch), nullptr, n, 4 * ((turns + n - 1) / n)};
         p.hist = reinterpret_cast<u64*>(p.rows + a.rows);
         const dim3 grid{unsigned(n), unsigned(a.rows)};
         hipLaunchKernelGGL(k_slice_max, grid, dim3(kThreads), 0, s, a, p, al);
