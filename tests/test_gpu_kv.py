@@ -178,6 +178,58 @@ def test_write_read_strides(typ, stride_k, stride_v, off):
         assert np.array_equal(out.cpu().numpy(), want)
 
 
+def slot_order(kind, rng, n, pool):
+    """n different slots of the pool in some order, -1 and others outside it among them."""
+    if kind == "shifted":  # runs that begin inside a block and inside a word of four keys
+        cut = [0, 1, 6, 39, 104, n]
+        at = [3, 65, 130, 195, 322, 420]
+        return np.concatenate([np.arange(a, a + j - i) for a, i, j in zip(at, cut, cut[1:])])
+    if kind == "holes":    # every seventh row is padding
+        s = np.arange(5, 5 + n)
+        s[::7] = np.where(np.arange(len(s[::7])) % 2, -1, pool + np.arange(len(s[::7])) % 9)
+        return s
+    if kind == "falling":
+        return np.arange(pool - 1, pool - 1 - n, -1)
+    if kind == "words":    # words of four whole, in any order
+        return (rng.permutation(pool // 4)[:-(-n // 4), None] * 4 + np.arange(4)).ravel()[:n]
+    return rng.permutation(pool)[:n]
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("kind", ["shifted", "holes", "falling", "words", "any"])
+@pytest.mark.parametrize("kv_heads,hd,page,n,odd", [(41, 64, 32, 401, 0), (36, 128, 64, 500, 3), (64, 128, 256, 256, 0)])
+def test_write_read_many_rows(typ, kind, kv_heads, hd, page, n, odd):
+    """Enough rows for whole tiles of them; what no slot names stays."""
+    rng = np.random.default_rng(n)
+    pool = 1024
+    slots = np.asarray(slot_order(kind, rng, n, pool), np.int64)
+    w = kv_heads * hd + odd
+    x = [rows(rng, 1, n, w)[0] for _ in range(2)]
+    x[0][7, 3], x[1][40, 1], x[1][90] = np.nan, np.inf, 0
+    kv = KVCache(1, kv_heads, hd, page, pool // page, typ)
+    base = rows(rng, pool, kv_heads, hd)
+    every = np.arange(pool, dtype=np.int64)
+    db, de, dk, dv, ds = dev(base), dev(every), dev(x[0]), dev(x[1]), dev(slots)
+    torch.cuda.synchronize()
+    kv.write_dev(0, db.data_ptr(), db.data_ptr(), de.data_ptr(), pool)
+    kv.write_dev(0, dk.data_ptr(), dv.data_ptr(), ds.data_ptr(), n, w, w)
+    inside = (slots >= 0) & (slots < pool)
+    for order in (every, slots):
+        m = len(order)
+        out = [torch.full((m + 1, w), 9.0, device="cuda") for _ in range(2)]
+        do = dev(order)
+        torch.cuda.synchronize()
+        kv.read_dev(0, do.data_ptr(), m, out[0].data_ptr(), out[1].data_ptr(), w, w)
+        wv.sync()
+        for o, rows_in in zip(out, x):
+            cache = stored(base, typ)
+            cache[slots[inside]] = stored(rows_in[inside][:, :kv_heads * hd].reshape(-1, kv_heads, hd), typ)
+            want = np.full((m + 1, w), 9.0, np.float32)
+            ok = (order >= 0) & (order < pool)
+            want[:m, :kv_heads * hd] = np.where(ok[:, None], cache[np.where(ok, order, 0)].reshape(m, -1), 0)
+            assert np.array_equal(o.cpu().numpy(), want, equal_nan=True)
+
+
 # ----------------------------------------------------------------- attention
 
 LAYOUTS = [(8, 8, 64), (8, 2, 128), (5, 1, 64), (32, 8, 128), (6, 2, 64), (24, 1, 128)]

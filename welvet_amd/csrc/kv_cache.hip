@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <mutex>
 #include <new>
+#include <type_traits>
 #include <unordered_map>
 
 #include "kv.h"
@@ -47,20 +48,17 @@ __device__ __forceinline__ int q8_code(float x, float s, float inv) {
     return x < 0.0f ? -c : c;
 }
 
-// The largest magnitude of a row over its HD / 4 lanes (32 or 16), and
-// whether any of its values is a NaN or infinity.
+// The largest magnitude of a row over its HD / 4 lanes (32 or 16), as bits:
+// those of NaN and infinity are the largest.
 template <int HD>
 __device__ __forceinline__ float row_amax(const float4 x, bool& bad) {
-    float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-    const float lim = 3.402823466e38f;
-    int b = !(fabsf(x.x) <= lim && fabsf(x.y) <= lim && fabsf(x.z) <= lim && fabsf(x.w) <= lim);
+    constexpr uint32_t A = 0x7fffffff;
+    uint32_t m = max(max(__float_as_uint(x.x) & A, __float_as_uint(x.y) & A),
+                     max(__float_as_uint(x.z) & A, __float_as_uint(x.w) & A));
 #pragma unroll
-    for (int d = HD / 8; d >= 1; d >>= 1) {
-        m = fmaxf(m, __shfl_xor(m, d, 64));
-        b |= __shfl_xor(b, d, 64);
-    }
-    bad = b != 0;
-    return m;
+    for (int d = HD / 8; d >= 1; d >>= 1) m = max(m, uint32_t(__shfl_xor(int(m), d, 64)));
+    bad = m >= 0x7f800000;
+    return __uint_as_float(m);
 }
 
 __device__ __forceinline__ float4 ld4(const float* p, bool aligned) {
@@ -76,6 +74,94 @@ __device__ __forceinline__ bool place(const KvView& c, int64_t slot, int head, i
     block = kv_block(c, page, head, off);
     kk = off & 31;
     return true;
+}
+
+// Stored past the caches: 16384 tokens of 8 heads are read back in 39 us so,
+// in 63 with plain stores.
+__device__ __forceinline__ void st4(float* p, const float4 y, bool aligned) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    if (aligned)
+        __builtin_nontemporal_store(f4{y.x, y.y, y.z, y.w}, reinterpret_cast<f4*>(p));
+    else
+        p[0] = y.x, p[1] = y.y, p[2] = y.z, p[3] = y.w;
+}
+
+// A row's scale, and the codes of this lane's four values of it, the first lowest.
+template <int HD, int TYPE>
+__device__ __forceinline__ uint64_t row_codes(const float4 x, float& s) {
+    bool bad;
+    const float amax = row_amax<HD>(x, bad);
+    float inv;
+    s = row_scale(amax, bad, TYPE, inv);
+    const float f[4] = {x.x, x.y, x.z, x.w};
+    uint64_t c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (TYPE == WV_KV_F16)
+            c |= uint64_t(__builtin_bit_cast(uint16_t, bad ? _Float16(0) : _Float16(f[i] * inv))) << (16 * i);
+        else
+            c |= uint64_t(uint32_t((bad || s == 0.0f ? 0 : q8_code(f[i], s, inv)) + 128)) << (8 * i);
+    }
+    return c;
+}
+template <int TYPE>
+__device__ __forceinline__ void put4(uint8_t* p, uint64_t c) {
+    if (TYPE == WV_KV_F16)
+        *reinterpret_cast<uint64_t*>(p) = c;
+    else
+        *reinterpret_cast<uint32_t*>(p) = uint32_t(c);
+}
+// Four codes' values.
+template <int TYPE>
+__device__ __forceinline__ float4 row_values(uint64_t c, float s) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y[i] = TYPE == WV_KV_F16 ? float(__builtin_bit_cast(_Float16, uint16_t(c >> (16 * i)))) * s
+                                 : float(int(c >> (8 * i) & 255) - 128) * s;
+    return make_float4(y[0], y[1], y[2], y[3]);
+}
+template <int TYPE>
+__device__ __forceinline__ uint64_t get4(const uint8_t* p) {
+    return TYPE == WV_KV_F16 ? *reinterpret_cast<const uint64_t*>(p) : *reinterpret_cast<const uint32_t*>(p);
+}
+
+// From this many rows (tokens times KV heads) on a block takes 32 of them.
+// Fewer do not fill the GPU, and a tile's steps one after the other take
+// longer than a row's. Tiles against row by row, fp16, head dim 128, 8 heads:
+// 64 tokens in order 5.6 to 4.1 us written, 4.6 to 4.1 read; 1024 tokens 6.3
+// to 10.1 and 5.2 to 7.2; 16384 tokens 39 to 98 and 39 to 75, which is a large
+// copy's rate. In no order 1024 tokens 11.3 to 11.4 and 10.4 to 8.8, 16384
+// tokens 135 to 139 and 82 to 97.
+constexpr int kTileRows = 8192;
+
+// Many rows: 32 tokens of one KV head to a block, their codes through LDS, so
+// that K leaves as whole 16-byte units and V as words of four keys, where four
+// rows in a row have the four slots of such a word; the rows left go code by
+// code. `lead`: the rows with which a word begins, `cov`: those in one.
+struct Tile {
+    int64_t block[32];
+    int kk[32];       // -1: outside the pool
+    float sk[32], sv[32];
+    uint32_t lead, cov;
+};
+// By the first wave: places the tile's slots.
+__device__ __forceinline__ void tile_place(const KvView& c, Tile& t, const int64_t* slots, int64_t t0, int n, int head) {
+    if (threadIdx.x >= 64) return;
+    const int r = threadIdx.x & 31;
+    const int64_t slot = t0 + r < n ? slots[t0 + r] : -1;
+    int64_t block = 0;
+    int kk = 0;
+    const bool in = place(c, slot, head, block, kk);
+    bool lead = in && kk % 4 == 0 && r < 29;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) lead = uint64_t(__shfl(slot, (r + i) & 31, 64)) == uint64_t(slot) + i && lead;
+    const uint32_t m = uint32_t(__ballot(lead));
+    if (threadIdx.x < 32) {
+        t.block[r] = block;
+        t.kk[r] = in ? kk : -1;
+        if (r == 0) t.lead = m, t.cov = m | m << 1 | m << 2 | m << 3;
+    }
 }
 
 // One row (token, KV head) per HD / 4 lanes, 4 dims of K and of V each.
@@ -94,38 +180,113 @@ __global__ void __launch_bounds__(256) k_kv_write(KvView c, const float* __restr
     if (!place(c, slots[t], head, block, kk)) return;
     const float4 xk = ld4(k + t * ks + head * HD + d, aligned);
     const float4 xv = ld4(v + t * vs + head * HD + d, aligned);
-    bool bk, bv;
-    const float ak = row_amax<HD>(xk, bk), av = row_amax<HD>(xv, bv);
-    float ik, iv;
-    const float sk = row_scale(ak, bk, TYPE, ik), sv = row_scale(av, bv, TYPE, iv);
+    float sk, sv;
+    const uint64_t ck = row_codes<HD, TYPE>(xk, sk), cv = row_codes<HD, TYPE>(xv, sv);
     int o, j;
     kv_key_octet(kk, o, j);
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
-    uint8_t* kb = c.k + block * (32 * HD * E);
-    uint8_t* vb = c.v + block * (32 * HD * E);
-    const float fk[4] = {xk.x, xk.y, xk.z, xk.w}, fv[4] = {xv.x, xv.y, xv.z, xv.w};
-    if (TYPE == WV_KV_F16) {
-        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-        h4 ck;
+    put4<TYPE>(c.k + block * (32 * HD * E) + (d * E / 16 * 32 + kk) * 16 + d * E % 16, ck);
+    uint8_t* vb = c.v + block * (32 * HD * E) + ((o * HD + d) * 8 + j) * E;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ck[i] = bk ? _Float16(0) : _Float16(fk[i] * ik);
-        *reinterpret_cast<h4*>(kb + ((d / 8) * 32 + kk) * 16 + (d % 8) * 2) = ck;
-        _Float16* vh = reinterpret_cast<_Float16*>(vb) + (o * HD + d) * 8 + j;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vh[8 * i] = bv ? _Float16(0) : _Float16(fv[i] * iv);
-    } else {
-        uint32_t ck = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ck |= uint32_t((bk || sk == 0.0f ? 0 : q8_code(fk[i], sk, ik)) + 128) << (8 * i);
-        *reinterpret_cast<uint32_t*>(kb + ((d / 16) * 32 + kk) * 16 + d % 16) = ck;
-        uint8_t* vq = vb + (o * HD + d) * 8 + j;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vq[8 * i] = uint8_t((bv || sv == 0.0f ? 0 : q8_code(fv[i], sv, iv)) + 128);
+    for (int i = 0; i < 4; ++i) {
+        if (TYPE == WV_KV_F16)
+            *reinterpret_cast<uint16_t*>(vb + 16 * i) = uint16_t(cv >> (16 * i));
+        else
+            vb[8 * i] = uint8_t(cv >> (8 * i));
     }
     if (d == 0) {
         float* sb = c.s + block * kKvScales + o * 16 + j;
         sb[0] = sk;
         sb[8] = sv;
+    }
+}
+
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(256) k_kv_write_tile(KvView c, const float* __restrict__ k,
+                                                       const float* __restrict__ v, int64_t ks, int64_t vs,
+                                                       const int64_t* __restrict__ slots, int n, bool aligned) {
+    constexpr int E = TYPE == WV_KV_F16 ? 2 : 1, LR = HD / 4, RP = 256 / LR, NP = 32 / RP, RS = HD * E + 16;
+    __shared__ Tile tl;
+    __shared__ __align__(16) uint8_t lk[32 * RS], lv[32 * RS];
+    const int64_t t0 = int64_t(blockIdx.x) / c.n_kv * 32;
+    const int head = int(int64_t(blockIdx.x) % c.n_kv);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int d = 4 * (tid % LR), r0 = tid / LR;
+    float4 xk[NP], xv[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int64_t t = t0 + p * RP + r0;
+        xk[p] = t < n ? ld4(k + t * ks + head * HD + d, aligned) : float4{};
+        xv[p] = t < n ? ld4(v + t * vs + head * HD + d, aligned) : float4{};
+    }
+    tile_place(c, tl, slots, t0, n, head);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int r = p * RP + r0;
+        float sk, sv;
+        put4<TYPE>(lk + r * RS + d * E, row_codes<HD, TYPE>(xk[p], sk));
+        put4<TYPE>(lv + r * RS + d * E, row_codes<HD, TYPE>(xv[p], sv));
+        if (d == 0) tl.sk[r] = sk, tl.sv[r] = sv;
+    }
+    __syncthreads();
+    {
+        const int r = tid & 31, kk = tl.kk[r];
+        if (kk >= 0) {
+            const int64_t block = tl.block[r];
+            uint8_t* kb = c.k + block * (32 * HD * E) + kk * 16;
+#pragma unroll
+            for (int u = tid >> 5; u < HD * E / 16; u += 8)
+                *reinterpret_cast<uint4*>(kb + u * 512) = *reinterpret_cast<const uint4*>(lk + r * RS + u * 16);
+            if (tid < 64) {
+                int o, j;
+                kv_key_octet(kk, o, j);
+                c.s[block * kKvScales + o * 16 + 8 * (tid >> 5) + j] = tid < 32 ? tl.sk[r] : tl.sv[r];
+            }
+        }
+    }
+    const int dv = 2 * lane;  // two dims to a lane
+    if (dv >= HD) return;
+    const uint32_t lead = __builtin_amdgcn_readfirstlane(tl.lead), cov = __builtin_amdgcn_readfirstlane(tl.cov);
+    int turn = 0;
+    for (uint32_t m = lead; m; m &= m - 1) {
+        if ((turn++ & 3) != wave) continue;
+        const int r = __builtin_ctz(m);
+        int o, j;
+        kv_key_octet(tl.kk[r], o, j);
+        uint8_t* vb = c.v + tl.block[r] * (32 * HD * E) + ((o * HD + dv) * 8 + j) * E;
+        const uint8_t* x = lv + r * RS + dv * E;
+        if (TYPE == WV_KV_F16) {
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint32_t*>(x + i * RS);
+            *reinterpret_cast<uint2*>(vb) = make_uint2((y[0] & 0xffff) | y[1] << 16, (y[2] & 0xffff) | y[3] << 16);
+            *reinterpret_cast<uint2*>(vb + 16) =
+                make_uint2(y[0] >> 16 | (y[1] & 0xffff0000), y[2] >> 16 | (y[3] & 0xffff0000));
+        } else {
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = *reinterpret_cast<const uint16_t*>(x + i * RS);
+            *reinterpret_cast<uint32_t*>(vb) =
+                (y[0] & 255) | (y[1] & 255) << 8 | (y[2] & 255) << 16 | (y[3] & 255) << 24;
+            *reinterpret_cast<uint32_t*>(vb + 8) = y[0] >> 8 | (y[1] >> 8) << 8 | (y[2] >> 8) << 16 | (y[3] >> 8) << 24;
+        }
+    }
+    for (uint32_t m = ~cov; m; m &= m - 1) {
+        if ((turn++ & 3) != wave) continue;
+        const int r = __builtin_ctz(m), kk = tl.kk[r];
+        if (kk < 0) continue;
+        int o, j;
+        kv_key_octet(kk, o, j);
+        uint8_t* vb = c.v + tl.block[r] * (32 * HD * E) + ((o * HD + dv) * 8 + j) * E;
+        const uint8_t* x = lv + r * RS + dv * E;
+        if (TYPE == WV_KV_F16) {
+            const uint32_t y = *reinterpret_cast<const uint32_t*>(x);
+            *reinterpret_cast<uint16_t*>(vb) = uint16_t(y);
+            *reinterpret_cast<uint16_t*>(vb + 16) = uint16_t(y >> 16);
+        } else {
+            vb[0] = x[0];
+            vb[8] = x[1];
+        }
     }
 }
 
@@ -139,44 +300,110 @@ __global__ void __launch_bounds__(256) k_kv_read(KvView c, const int64_t* __rest
     const int64_t t = row / c.n_kv;
     const int head = int(row % c.n_kv);
     if (t >= n) return;
-    float yk[4] = {0, 0, 0, 0}, yv[4] = {0, 0, 0, 0};
+    float4 yk{}, yv{};
     int64_t block;
     int kk;
     if (place(c, slots[t], head, block, kk)) {
         int o, j;
         kv_key_octet(kk, o, j);
         constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
-        const uint8_t* kb = c.k + block * (32 * HD * E);
-        const uint8_t* vb = c.v + block * (32 * HD * E);
         const float* sb = c.s + block * kKvScales + o * 16 + j;
-        const float sk = sb[0], sv = sb[8];
-        if (TYPE == WV_KV_F16) {
-            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-            const h4 ck = *reinterpret_cast<const h4*>(kb + ((d / 8) * 32 + kk) * 16 + (d % 8) * 2);
-            const _Float16* vh = reinterpret_cast<const _Float16*>(vb) + (o * HD + d) * 8 + j;
+        const uint8_t* vb = c.v + block * (32 * HD * E) + ((o * HD + d) * 8 + j) * E;
+        uint64_t cv = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                yk[i] = float(ck[i]) * sk;
-                yv[i] = float(vh[8 * i]) * sv;
-            }
-        } else {
-            const uint32_t ck = *reinterpret_cast<const uint32_t*>(kb + ((d / 16) * 32 + kk) * 16 + d % 16);
-            const uint8_t* vq = vb + (o * HD + d) * 8 + j;
+        for (int i = 0; i < 4; ++i)
+            cv |= TYPE == WV_KV_F16 ? uint64_t(*reinterpret_cast<const uint16_t*>(vb + 16 * i)) << (16 * i)
+                                    : uint64_t(vb[8 * i]) << (8 * i);
+        yk = row_values<TYPE>(get4<TYPE>(c.k + block * (32 * HD * E) + (d * E / 16 * 32 + kk) * 16 + d * E % 16), sb[0]);
+        yv = row_values<TYPE>(cv, sb[8]);
+    }
+    st4(k + t * ks + head * HD + d, yk, aligned);
+    st4(v + t * vs + head * HD + d, yv, aligned);
+}
+
+// Many rows: the way back, 32 tokens of one KV head to a block.
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(256) k_kv_read_tile(KvView c, const int64_t* __restrict__ slots, int n,
+                                                      float* __restrict__ k, float* __restrict__ v, int64_t ks,
+                                                      int64_t vs, bool aligned) {
+    constexpr int E = TYPE == WV_KV_F16 ? 2 : 1, LR = HD / 4, RP = 256 / LR, NP = 32 / RP, RS = HD * E + 16;
+    __shared__ Tile tl;
+    __shared__ __align__(16) uint8_t lk[32 * RS], lv[32 * RS];
+    const int64_t t0 = int64_t(blockIdx.x) / c.n_kv * 32;
+    const int head = int(int64_t(blockIdx.x) % c.n_kv);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    tile_place(c, tl, slots, t0, n, head);
+    __syncthreads();
+    {
+        const int r = tid & 31, kk = tl.kk[r];
+        if (kk >= 0) {
+            const int64_t block = tl.block[r];
+            const uint8_t* kb = c.k + block * (32 * HD * E) + kk * 16;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                yk[i] = float(int((ck >> (8 * i)) & 255) - 128) * sk;
-                yv[i] = float(int(vq[8 * i]) - 128) * sv;
+            for (int u = tid >> 5; u < HD * E / 16; u += 8)
+                *reinterpret_cast<uint4*>(lk + r * RS + u * 16) = *reinterpret_cast<const uint4*>(kb + u * 512);
+            if (tid < 64) {
+                int o, j;
+                kv_key_octet(kk, o, j);
+                const float x = c.s[block * kKvScales + o * 16 + 8 * (tid >> 5) + j];
+                (tid < 32 ? tl.sk : tl.sv)[r] = x;
             }
         }
     }
-    float* ok = k + t * ks + head * HD + d;
-    float* ov = v + t * vs + head * HD + d;
-    if (aligned) {
-        *reinterpret_cast<float4*>(ok) = make_float4(yk[0], yk[1], yk[2], yk[3]);
-        *reinterpret_cast<float4*>(ov) = make_float4(yv[0], yv[1], yv[2], yv[3]);
-    } else {
+    const int dv = 2 * lane;  // two dims to a lane
+    if (dv < HD) {
+        const uint32_t lead = __builtin_amdgcn_readfirstlane(tl.lead), cov = __builtin_amdgcn_readfirstlane(tl.cov);
+        int turn = 0;
+        for (uint32_t m = lead; m; m &= m - 1) {
+            if ((turn++ & 3) != wave) continue;
+            const int r = __builtin_ctz(m);
+            int o, j;
+            kv_key_octet(tl.kk[r], o, j);
+            const uint8_t* vb = c.v + tl.block[r] * (32 * HD * E) + ((o * HD + dv) * 8 + j) * E;
+            uint8_t* x = lv + r * RS + dv * E;
+            if (TYPE == WV_KV_F16) {
+                const uint2 a = *reinterpret_cast<const uint2*>(vb), b = *reinterpret_cast<const uint2*>(vb + 16);
+                *reinterpret_cast<uint32_t*>(x) = (a.x & 0xffff) | b.x << 16;
+                *reinterpret_cast<uint32_t*>(x + RS) = a.x >> 16 | (b.x & 0xffff0000);
+                *reinterpret_cast<uint32_t*>(x + 2 * RS) = (a.y & 0xffff) | b.y << 16;
+                *reinterpret_cast<uint32_t*>(x + 3 * RS) = a.y >> 16 | (b.y & 0xffff0000);
+            } else {
+                const uint32_t a = *reinterpret_cast<const uint32_t*>(vb), b = *reinterpret_cast<const uint32_t*>(vb + 8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ok[i] = yk[i], ov[i] = yv[i];
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint16_t*>(x + i * RS) =
+                        uint16_t(((a >> (8 * i)) & 255) | ((b >> (8 * i)) & 255) << 8);
+            }
+        }
+        for (uint32_t m = ~cov; m; m &= m - 1) {
+            if ((turn++ & 3) != wave) continue;
+            const int r = __builtin_ctz(m), kk = tl.kk[r];
+            if (kk < 0) continue;
+            int o, j;
+            kv_key_octet(kk, o, j);
+            const uint8_t* vb = c.v + tl.block[r] * (32 * HD * E) + ((o * HD + dv) * 8 + j) * E;
+            uint8_t* x = lv + r * RS + dv * E;
+            if (TYPE == WV_KV_F16)
+                *reinterpret_cast<uint32_t*>(x) = *reinterpret_cast<const uint16_t*>(vb) |
+                                                  uint32_t(*reinterpret_cast<const uint16_t*>(vb + 16)) << 16;
+            else
+                *reinterpret_cast<uint16_t*>(x) = uint16_t(vb[0] | vb[8] << 8);
+        }
+    }
+    __syncthreads();
+    const int d = 4 * (tid % LR), r0 = tid / LR;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int r = p * RP + r0;
+        const int64_t t = t0 + r;
+        if (t >= n) return;
+        float4 yk{}, yv{};
+        if (tl.kk[r] >= 0) {
+            yk = row_values<TYPE>(get4<TYPE>(lk + r * RS + d * E), tl.sk[r]);
+            yv = row_values<TYPE>(get4<TYPE>(lv + r * RS + d * E), tl.sv[r]);
+        }
+        st4(k + t * ks + head * HD + d, yk, aligned);
+        st4(v + t * vs + head * HD + d, yv, aligned);
     }
 }
 
@@ -198,26 +425,44 @@ bool kv_lookup(uint64_t h, KvCache& out) {
 int launch_kv_write(const KvView& c, const float* k, const float* v, int64_t ks, int64_t vs, const int64_t* slots,
                     int n, hipStream_t s) {
     const bool al = rows_aligned(k, v, ks, vs);
+    const bool tile = int64_t(n) * c.n_kv >= kTileRows;
     const int per = 256 / (c.hd / 4);
-    const dim3 grid(unsigned((int64_t(n) * c.n_kv + per - 1) / per));
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, k, v, ks, vs, slots, n, al); };
+    const int64_t blocks = tile ? (int64_t(n) + 31) / 32 * c.n_kv : (int64_t(n) * c.n_kv + per - 1) / per;
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(unsigned(blocks)), dim3(256), 0, s, c, k, v, ks, vs, slots, n, al); };
+    auto pick = [&](auto hd, auto type) {
+        constexpr int HD = decltype(hd)::value, TYPE = decltype(type)::value;
+        tile ? go(k_kv_write_tile<HD, TYPE>) : go(k_kv_write<HD, TYPE>);
+    };
+    std::integral_constant<int, 128> h128;
+    std::integral_constant<int, 64> h64;
+    std::integral_constant<int, WV_KV_F16> f16;
+    std::integral_constant<int, WV_KV_Q8> q8;
     if (c.hd == 128)
-        c.type == WV_KV_F16 ? go(k_kv_write<128, WV_KV_F16>) : go(k_kv_write<128, WV_KV_Q8>);
+        c.type == WV_KV_F16 ? pick(h128, f16) : pick(h128, q8);
     else
-        c.type == WV_KV_F16 ? go(k_kv_write<64, WV_KV_F16>) : go(k_kv_write<64, WV_KV_Q8>);
+        c.type == WV_KV_F16 ? pick(h64, f16) : pick(h64, q8);
     return int(hipGetLastError());
 }
 
 int launch_kv_read(const KvView& c, const int64_t* slots, int n, float* k, float* v, int64_t ks, int64_t vs,
                    hipStream_t s) {
     const bool al = rows_aligned(k, v, ks, vs);
+    const bool tile = int64_t(n) * c.n_kv >= kTileRows;
     const int per = 256 / (c.hd / 4);
-    const dim3 grid(unsigned((int64_t(n) * c.n_kv + per - 1) / per));
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, c, slots, n, k, v, ks, vs, al); };
+    const int64_t blocks = tile ? (int64_t(n) + 31) / 32 * c.n_kv : (int64_t(n) * c.n_kv + per - 1) / per;
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(unsigned(blocks)), dim3(256), 0, s, c, slots, n, k, v, ks, vs, al); };
+    auto pick = [&](auto hd, auto type) {
+        constexpr int HD = decltype(hd)::value, TYPE = decltype(type)::value;
+        tile ? go(k_kv_read_tile<HD, TYPE>) : go(k_kv_read<HD, TYPE>);
+    };
+    std::integral_constant<int, 128> h128;
+    std::integral_constant<int, 64> h64;
+    std::integral_constant<int, WV_KV_F16> f16;
+    std::integral_constant<int, WV_KV_Q8> q8;
     if (c.hd == 128)
-        c.type == WV_KV_F16 ? go(k_kv_read<128, WV_KV_F16>) : go(k_kv_read<128, WV_KV_Q8>);
+        c.type == WV_KV_F16 ? pick(h128, f16) : pick(h128, q8);
     else
-        c.type == WV_KV_F16 ? go(k_kv_read<64, WV_KV_F16>) : go(k_kv_read<64, WV_KV_Q8>);
+        c.type == WV_KV_F16 ? pick(h64, f16) : pick(h64, q8);
     return int(hipGetLastError());
 }
 
