@@ -4,6 +4,18 @@
 // 2^-44 wherever they are summed: the sums are exact, so nothing depends on
 // the order in which threads add. Tokens are ordered by falling logit, equal
 // ones by index; a cut (l*, i*) keeps the tokens in front of it and itself.
+//
+// A row needs its logits once from memory: 33 MB of 64 rows of 128000 take
+// 6.3 us at a large copy's rate. What binds is the passes over them: the
+// maximum; a histogram of the weights (their logarithms in bins, counts for
+// top-k); a pass that collects the cut's bin and sums what is kept in front of
+// it by segments of 1024 tokens, each some 20 instructions a logit; and the
+// steps between them, which one block after the other waits for. Rows of up to
+// 32768 logits stay in LDS meanwhile (256 rows of 32000: greedy 8.9 us, top-k
+// of 40 17, top-p 30, no filter 20). Of larger ones with few rows each is cut
+// over several blocks, below (64 of 128000: top-p 47 us, by whole rows 101).
+// The loops stay small: with the row in registers, unrolled, instruction fetch
+// took most of the time (greedy, one row of 32000: 23 us, from LDS 5).
 #include <algorithm>
 #include <cmath>
 
@@ -399,12 +411,12 @@ struct Kept {
     }
 };
 
-// The place of u among s.seg, the kept weights of each segment, and in the
-// segment where it lies.
 // The wave's sum of doubles that are multiples of 2^-44, in units of it: up to
 // 1024, so in integers.
 __device__ __forceinline__ u64 segment_sum(double v) { return last_lane(wave_scan(u64(v * 17592186044416.0))); }
 
+// The place of u among s.seg, the kept weights of each segment, and in the
+// segment where it lies.
 template <bool R>
 __device__ __forceinline__ void pick(const SampleArgs& a, Shared<R>& s, const Row<R>& row, int r, const Kept& kept,
                                      float u) {
@@ -468,6 +480,73 @@ __device__ __forceinline__ void pick_from_list(const SampleArgs& a, Shared<R>& s
         }
     const u64 want = u64(double(x.u) * double(total));
     if (w && before <= want && want < before + w) put(a, r, int(~uint32_t(key)), float(double(w) / double(total)));
+}
+
+// What a cut in `bin` (kBins: none) does with the tokens from key `floor` on:
+// those of the bin (`few`: down to its end) go into the list, the weights of
+// those in front of it, from min_p on, come back for their segment's sum.
+template <bool FLOOR, bool R>
+struct Visit {
+    Shared<R>& s;
+    const Scale& c;
+    u64 floor;
+    float min_p, front, lo, hi;  // bin_of() in terms of y = -log_weight kPerUnit
+    __device__ __forceinline__ Visit(Shared<R>& s, const Scale& c, u64 floor, float min_p, int bin, bool few)
+        : s(s), c(c), floor(floor), min_p(min_p) {
+        front = bin < kBins ? float(bin) : INFINITY;
+        lo = few ? -1.0f : front;
+        hi = bin < kBins - 1 ? float(bin + 1) : bin < kBins ? INFINITY : -1.0f;
+    }
+    __device__ __forceinline__ double operator()(float l, int i) const {
+        const float x = log_weight(c, l), y = -x * kPerUnit;
+        const float w = __builtin_amdgcn_exp2f(x);
+        const bool in = l > -INFINITY && (!FLOOR || token_key(l, i) >= floor);
+        if (in && y >= lo && y < hi) {
+            const int at = atomicAdd(&s.n, 1);
+            if (at < kList) {
+                s.list[at] = token_key(l, i);
+                s.weights[at] = fixed(w);
+            }
+            return 0.0;
+        }
+        return in && y < front && w >= min_p ? (256.0 + double(w)) - 256.0 : 0.0;
+    }
+    __device__ __forceinline__ double four(float4 x, int i) const {
+        return ((*this)(x.x, i) + (*this)(x.y, i + 1)) + ((*this)(x.z, i + 2) + (*this)(x.w, i + 3));
+    }
+};
+// Adds a pass's weights up and leaves the sum of a segment with its last pass.
+// A segment's weights of at most 1 are steps of 2^-44 and so are a thread's sums of 16.
+struct SegmentSum {
+    u64* seg;
+    int segs;
+    double sum = 0.0;
+    __device__ __forceinline__ SegmentSum(u64* seg, int vocab) : seg(seg), segs((vocab + kSegment - 1) / kSegment) {}
+    __device__ __forceinline__ void operator()(double v, int k) {
+        sum += v;
+        if ((k & 3) != 3) return;
+        const u64 all = segment_sum(sum);
+        const int sg = (k >> 2) * kWaves + int(threadIdx.x >> 6);
+        if ((threadIdx.x & 63) == 0 && sg < segs) seg[sg] = all;
+        sum = 0.0;
+    }
+};
+// The cut among the n tokens of the bin's list, where `left` is what it keeps
+// of them: into s.key; what it keeps, from min_p on, into their segments.
+template <bool R>
+__device__ __forceinline__ void cut_list(Shared<R>& s, const Scale& c, int n, u64 left, bool by_mass, float min_p) {
+    const int t = threadIdx.x;
+    u64 key = 0, mass = 0, w = 0;
+    int rank = 0;
+    if (t < n) {
+        key = s.list[t], w = s.weights[t];
+        rank_list(s, n, key, rank, mass);
+        if (by_mass ? mass < left && mass + w >= left : u64(rank) + 1 == left) s.key = key;
+    }
+    __syncthreads();
+    if (t < n && key >= s.key && weight(c, key_logit(key)) >= min_p)
+        atomicAdd(&s.seg[int(~uint32_t(key)) / kSegment], w);
+    __syncthreads();
 }
 
 // A whole row by one block.
@@ -536,6 +615,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
     }
 
     u64 cut = 0;  // the last token kept, 0: all
+    bool summed = false;
 #pragma unroll 1
     for (int mass = 0; mass < 2; ++mass) {  // top-k by counts, then top-p by weights
         if (!(mass ? set.by_p : set.by_k)) continue;
@@ -551,22 +631,41 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
             const u64 whole = find_in(s, s.hist, kBins, ~u64(0));
             target = max(u64(1), min(whole, u64(ceil(double(set.top_p) * double(whole)))));
         }
+        if (mass || !set.by_p) {  // the last cut: the segments' sums in the same pass
+            find_in(s, s.hist, kBins, target);
+            const int bin = s.at < 0 ? kBins : s.at;
+            const u64 left = target - s.sum;
+            __syncthreads();
+            if (t == 0) s.key = cut;
+            SegmentSum sums(s.seg, a.vocab);
+            if (cut) {
+                const Visit<true, R> visit(s, c, cut, set.min_p, bin, false);
+                row.each4([&](float4 x, int i, int k) { sums(visit.four(x, i), k); });
+            } else {
+                const Visit<false, R> visit(s, c, cut, set.min_p, bin, false);
+                row.each4([&](float4 x, int i, int k) { sums(visit.four(x, i), k); });
+            }
+            __syncthreads();
+            const int n = s.n;
+            if (n <= kList) {
+                if (n) cut_list(s, c, n, left, mass != 0, set.min_p);
+                cut = s.key;
+                summed = true;
+                break;
+            }
+            __syncthreads();
+        }
         cut = find_cut(s, row, c, cut, target, mass != 0);
         __syncthreads();
     }
-    // the kept weights of each 256 tokens, then the place of u among them
+    // the kept weights of each segment, then the place of u among them
     const Kept kept(c, cut, set.min_p);
-    const int segs = (a.vocab + kSegment - 1) / kSegment;
-    double sum = 0.0;  // a segment's weights of at most 1 in steps of 2^-44 and their sums up to 256 are exact
-    row.each4([&](float4 x, int i, int k) {
-        sum += (kept(x.x, i) + kept(x.y, i + 1)) + (kept(x.z, i + 2) + kept(x.w, i + 3));
-        if ((k & 3) == 3) {
-            const u64 v = segment_sum(sum);
-            const int sg = (k >> 2) * kWaves + wave;
-            if (lane == 0 && sg < segs) s.seg[sg] = v;
-            sum = 0.0;
-        }
-    });
+    if (!summed) {
+        SegmentSum sums(s.seg, a.vocab);
+        row.each4([&](float4 x, int i, int k) {
+            sums((kept(x.x, i) + kept(x.y, i + 1)) + (kept(x.z, i + 2) + kept(x.w, i + 3)), k);
+        });
+    }
     __syncthreads();
     pick(a, s, row, r, kept, set.u);
 }
@@ -586,7 +685,10 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned)
 //            row's list, the weights of the bins in front of it by segment
 //   finish one block a row: the list's cut, and the place of u
 // Rows that do not fit this (both top_k > kFewK and top_p, a bin of more
-// tokens than the list takes) are done whole by the last launch.
+// tokens than the list takes) are done whole by the last launch. 64 rows of
+// 128000 with top-p: 5.8, 11.9, 17.7 and 12.3 us; loading a pass's logits in
+// front of the wait for the maximum costs registers, and so a block a CU (25
+// for 17.7).
 // ---------------------------------------------------------------------------
 
 struct SliceRow {
@@ -657,7 +759,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p,
 __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices p, bool aligned) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
-    const int r = blockIdx.y, sl = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int r = blockIdx.y, sl = blockIdx.x, t = threadIdx.x;
     SliceRow& g = p.rows[r];
     const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
     const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
@@ -694,35 +796,11 @@ __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices
     }
     // few of top-k: the list takes all tokens down to the bin
     const bool few = set.by_k && set.top_k <= kFewK;
-    // bin_of(x) in terms of y = -x kPerUnit: in front of the bin, and in it or (few) not behind it
-    const float front = bin < kBins ? float(bin) : INFINITY;
-    const float lo = few ? -1.0f : front, hi = bin < kBins - 1 ? float(bin + 1) : bin < kBins ? INFINITY : -1.0f;
-    auto visit = [&](float l, int i) {
-        const float x = log_weight(c, l), y = -x * kPerUnit;
-        const float w = __builtin_amdgcn_exp2f(x);
-        if (y >= lo && y < hi && l > -INFINITY) {
-            const int at = atomicAdd(&s.n, 1);
-            if (at < kList) {
-                s.list[at] = token_key(l, i);
-                s.weights[at] = fixed(w);
-            }
-            return 0.0;
-        }
-        return y < front && l > -INFINITY && w >= set.min_p ? (256.0 + double(w)) - 256.0 : 0.0;
-    };
     if (t == 0) s.n = 0;
     __syncthreads();
-    const int segs = (a.vocab + kSegment - 1) / kSegment;
-    double sum = 0.0;
-    row.range(k0, k1, [&](float4 x, int i, int k) {
-        sum += (visit(x.x, i) + visit(x.y, i + 1)) + (visit(x.z, i + 2) + visit(x.w, i + 3));
-        if ((k & 3) == 3) {
-            const u64 v = segment_sum(sum);
-            const int sg = (k >> 2) * kWaves + wave;
-            if (lane == 0 && sg < segs) g.seg[sg] = v;
-            sum = 0.0;
-        }
-    });
+    const Visit<false, false> visit(s, c, 0, set.min_p, bin, few);
+    SegmentSum sums(g.seg, a.vocab);
+    row.range(k0, k1, [&](float4 x, int i, int k) { sums(visit.four(x, i), k); });
     __syncthreads();
     const int n = s.n;  // this slice's share of the row's list
     if (!n) return;
@@ -757,20 +835,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
     if (t == 0) s.key = 0;
     __syncthreads();
     if (set.by_k && set.top_k <= kFewK) return pick_from_list(a, s, r, set, c, n);
-    if (n) {
-        // the cut among the bin's tokens, then what it keeps of them into their segments
-        u64 key = 0, mass = 0, w = 0;
-        int rank = 0;
-        if (t < n) {
-            key = s.list[t], w = s.weights[t];
-            rank_list(s, n, key, rank, mass);
-            if (set.by_k ? u64(rank) + 1 == left : mass < left && mass + w >= left) s.key = key;
-        }
-        __syncthreads();
-        if (t < n && key >= s.key && weight(c, key_logit(key)) >= set.min_p)
-            atomicAdd(&s.seg[int(~uint32_t(key)) / kSegment], w);
-        __syncthreads();
-    }
+    if (n) cut_list(s, c, n, left, !set.by_k, set.min_p);
     const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
     pick(a, s, row, r, Kept(c, s.key, set.min_p), set.u);
 }
