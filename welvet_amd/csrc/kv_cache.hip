@@ -61,9 +61,11 @@ __device__ __forceinline__ float row_amax(const float4 x, bool& bad) {
     return __uint_as_float(m);
 }
 
-__device__ __forceinline__ float4 ld4(const float* p, bool aligned) {
-    if (aligned) return *reinterpret_cast<const float4*>(p);
-    return make_float4(p[0], p[1], p[2], p[3]);
+// Rows lie at any multiple of 4 bytes.
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ float4 ld4(const float* p) {
+    const f4 x = *reinterpret_cast<const f4*>(p);
+    return make_float4(x.x, x.y, x.z, x.w);
 }
 
 // Where a slot lies: its block and the key in it; false outside the pool.
@@ -78,12 +80,8 @@ __device__ __forceinline__ bool place(const KvView& c, int64_t slot, int head, i
 
 // Stored past the caches: 16384 tokens of 8 heads are read back in 39 us so,
 // in 63 with plain stores.
-__device__ __forceinline__ void st4(float* p, const float4 y, bool aligned) {
-    typedef float f4 __attribute__((ext_vector_type(4)));
-    if (aligned)
-        __builtin_nontemporal_store(f4{y.x, y.y, y.z, y.w}, reinterpret_cast<f4*>(p));
-    else
-        p[0] = y.x, p[1] = y.y, p[2] = y.z, p[3] = y.w;
+__device__ __forceinline__ void st4(float* p, const float4 y) {
+    __builtin_nontemporal_store(f4{y.x, y.y, y.z, y.w}, reinterpret_cast<f4*>(p));
 }
 
 // A row's scale, and the codes of this lane's four values of it, the first lowest.
@@ -167,8 +165,7 @@ __device__ __forceinline__ void tile_place(const KvView& c, Tile& t, const int64
 // One row (token, KV head) per HD / 4 lanes, 4 dims of K and of V each.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256) k_kv_write(KvView c, const float* __restrict__ k, const float* __restrict__ v,
-                                                  int64_t ks, int64_t vs, const int64_t* __restrict__ slots, int n,
-                                                  bool aligned) {
+                                                  int64_t ks, int64_t vs, const int64_t* __restrict__ slots, int n) {
     constexpr int LR = HD / 4;
     const int64_t row = int64_t(blockIdx.x) * (256 / LR) + threadIdx.x / LR;
     const int d = 4 * (threadIdx.x % LR);
@@ -178,8 +175,8 @@ __global__ void __launch_bounds__(256) k_kv_write(KvView c, const float* __restr
     int64_t block;
     int kk;
     if (!place(c, slots[t], head, block, kk)) return;
-    const float4 xk = ld4(k + t * ks + head * HD + d, aligned);
-    const float4 xv = ld4(v + t * vs + head * HD + d, aligned);
+    const float4 xk = ld4(k + t * ks + head * HD + d);
+    const float4 xv = ld4(v + t * vs + head * HD + d);
     float sk, sv;
     const uint64_t ck = row_codes<HD, TYPE>(xk, sk), cv = row_codes<HD, TYPE>(xv, sv);
     int o, j;
@@ -204,7 +201,7 @@ __global__ void __launch_bounds__(256) k_kv_write(KvView c, const float* __restr
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256) k_kv_write_tile(KvView c, const float* __restrict__ k,
                                                        const float* __restrict__ v, int64_t ks, int64_t vs,
-                                                       const int64_t* __restrict__ slots, int n, bool aligned) {
+                                                       const int64_t* __restrict__ slots, int n) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1, LR = HD / 4, RP = 256 / LR, NP = 32 / RP, RS = HD * E + 16;
     __shared__ Tile tl;
     __shared__ __align__(16) uint8_t lk[32 * RS], lv[32 * RS];
@@ -216,8 +213,8 @@ __global__ void __launch_bounds__(256) k_kv_write_tile(KvView c, const float* __
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
         const int64_t t = t0 + p * RP + r0;
-        xk[p] = t < n ? ld4(k + t * ks + head * HD + d, aligned) : float4{};
-        xv[p] = t < n ? ld4(v + t * vs + head * HD + d, aligned) : float4{};
+        xk[p] = t < n ? ld4(k + t * ks + head * HD + d) : float4{};
+        xv[p] = t < n ? ld4(v + t * vs + head * HD + d) : float4{};
     }
     tile_place(c, tl, slots, t0, n, head);
 #pragma unroll
@@ -292,8 +289,7 @@ __global__ void __launch_bounds__(256) k_kv_write_tile(KvView c, const float* __
 
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256) k_kv_read(KvView c, const int64_t* __restrict__ slots, int n,
-                                                 float* __restrict__ k, float* __restrict__ v, int64_t ks, int64_t vs,
-                                                 bool aligned) {
+                                                 float* __restrict__ k, float* __restrict__ v, int64_t ks, int64_t vs) {
     constexpr int LR = HD / 4;
     const int64_t row = int64_t(blockIdx.x) * (256 / LR) + threadIdx.x / LR;
     const int d = 4 * (threadIdx.x % LR);
@@ -317,15 +313,15 @@ __global__ void __launch_bounds__(256) k_kv_read(KvView c, const int64_t* __rest
         yk = row_values<TYPE>(get4<TYPE>(c.k + block * (32 * HD * E) + (d * E / 16 * 32 + kk) * 16 + d * E % 16), sb[0]);
         yv = row_values<TYPE>(cv, sb[8]);
     }
-    st4(k + t * ks + head * HD + d, yk, aligned);
-    st4(v + t * vs + head * HD + d, yv, aligned);
+    st4(k + t * ks + head * HD + d, yk);
+    st4(v + t * vs + head * HD + d, yv);
 }
 
 // Many rows: the way back, 32 tokens of one KV head to a block.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256) k_kv_read_tile(KvView c, const int64_t* __restrict__ slots, int n,
                                                       float* __restrict__ k, float* __restrict__ v, int64_t ks,
-                                                      int64_t vs, bool aligned) {
+                                                      int64_t vs) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1, LR = HD / 4, RP = 256 / LR, NP = 32 / RP, RS = HD * E + 16;
     __shared__ Tile tl;
     __shared__ __align__(16) uint8_t lk[32 * RS], lv[32 * RS];
@@ -402,14 +398,9 @@ __global__ void __launch_bounds__(256) k_kv_read_tile(KvView c, const int64_t* _
             yk = row_values<TYPE>(get4<TYPE>(lk + r * RS + d * E), tl.sk[r]);
             yv = row_values<TYPE>(get4<TYPE>(lv + r * RS + d * E), tl.sv[r]);
         }
-        st4(k + t * ks + head * HD + d, yk, aligned);
-        st4(v + t * vs + head * HD + d, yv, aligned);
+        st4(k + t * ks + head * HD + d, yk);
+        st4(v + t * vs + head * HD + d, yv);
     }
-}
-
-// Rows that float4 accesses reach: base and stride multiples of 16 bytes.
-bool rows_aligned(const void* a, const void* b, int64_t sa, int64_t sb) {
-    return !((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) && sa % 4 == 0 && sb % 4 == 0;
 }
 
 }  // namespace
@@ -424,11 +415,10 @@ bool kv_lookup(uint64_t h, KvCache& out) {
 
 int launch_kv_write(const KvView& c, const float* k, const float* v, int64_t ks, int64_t vs, const int64_t* slots,
                     int n, hipStream_t s) {
-    const bool al = rows_aligned(k, v, ks, vs);
     const bool tile = int64_t(n) * c.n_kv >= kTileRows;
     const int per = 256 / (c.hd / 4);
     const int64_t blocks = tile ? (int64_t(n) + 31) / 32 * c.n_kv : (int64_t(n) * c.n_kv + per - 1) / per;
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(unsigned(blocks)), dim3(256), 0, s, c, k, v, ks, vs, slots, n, al); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(unsigned(blocks)), dim3(256), 0, s, c, k, v, ks, vs, slots, n); };
     auto pick = [&](auto hd, auto type) {
         constexpr int HD = decltype(hd)::value, TYPE = decltype(type)::value;
         tile ? go(k_kv_write_tile<HD, TYPE>) : go(k_kv_write<HD, TYPE>);
@@ -446,11 +436,10 @@ int launch_kv_write(const KvView& c, const float* k, const float* v, int64_t ks,
 
 int launch_kv_read(const KvView& c, const int64_t* slots, int n, float* k, float* v, int64_t ks, int64_t vs,
                    hipStream_t s) {
-    const bool al = rows_aligned(k, v, ks, vs);
     const bool tile = int64_t(n) * c.n_kv >= kTileRows;
     const int per = 256 / (c.hd / 4);
     const int64_t blocks = tile ? (int64_t(n) + 31) / 32 * c.n_kv : (int64_t(n) * c.n_kv + per - 1) / per;
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(unsigned(blocks)), dim3(256), 0, s, c, slots, n, k, v, ks, vs, al); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(unsigned(blocks)), dim3(256), 0, s, c, slots, n, k, v, ks, vs); };
     auto pick = [&](auto hd, auto type) {
         constexpr int HD = decltype(hd)::value, TYPE = decltype(type)::value;
         tile ? go(k_kv_read_tile<HD, TYPE>) : go(k_kv_read<HD, TYPE>);

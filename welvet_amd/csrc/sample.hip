@@ -114,12 +114,13 @@ struct Row {
     const float* p;
     float* lds;
     int vocab;
-    bool aligned;
 
     __device__ __forceinline__ float4 fetch(int i) const {
         float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        if (aligned && i + 3 < vocab) {
-            x = *reinterpret_cast<const float4*>(p + i);
+        if (i + 3 < vocab) {  // one load at any multiple of 4 bytes
+            typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+            const f4 y = *reinterpret_cast<const f4*>(p + i);
+            x = make_float4(y.x, y.y, y.z, y.w);
         } else {
             if (i < vocab) x.x = p[i];
             if (i + 1 < vocab) x.y = p[i + 1];
@@ -551,9 +552,9 @@ __device__ __forceinline__ void cut_list(Shared<R>& s, const Scale& c, int n, u6
 
 // A whole row by one block.
 template <bool R>
-__device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, int r, bool aligned) {
+__device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, int r) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const Row<R> row{a.logits + int64_t(r) * a.stride, s.row, a.vocab, aligned};
+    const Row<R> row{a.logits + int64_t(r) * a.stride, s.row, a.vocab};
     const Settings set = settings(a, r);
     float top = -INFINITY;  // this thread's largest
     row.first([&](float4 x, int, int) { top = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), top); });
@@ -671,9 +672,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
 }
 
 template <bool R>
-__global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a, bool aligned) {
+__global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
-    sample_row(a, *reinterpret_cast<Shared<R>*>(raw), blockIdx.x, aligned);
+    sample_row(a, *reinterpret_cast<Shared<R>*>(raw), blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -711,10 +712,10 @@ __device__ __forceinline__ float row_max(const Slices& p, int r) {
 }
 __device__ __forceinline__ bool sliced(const Settings& x) { return !(x.by_k && x.by_p && x.top_k > kFewK); }
 
-__global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p, bool aligned) {
+__global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p) {
     __shared__ float part[kWaves];
     const int r = blockIdx.y, sl = blockIdx.x;
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     float top = -INFINITY;
     row.range(sl * p.passes, min((sl + 1) * p.passes, row.passes()),
               [&](float4 x, int, int) { top = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), top); });
@@ -729,10 +730,10 @@ __global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p, 
     }
 }
 
-__global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p, bool aligned) {
+__global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p) {
     __shared__ u64 hist[kBins];
     const int r = blockIdx.y, sl = blockIdx.x;
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
     const Settings set = settings(a, r);
     const float max = row_max(p, r);
@@ -756,12 +757,12 @@ __global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p,
         if (hist[i]) atomicAdd(&p.hist[int64_t(r) * kBins + i], hist[i]);
 }
 
-__global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices p, bool aligned) {
+__global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices p) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
     const int r = blockIdx.y, sl = blockIdx.x, t = threadIdx.x;
     SliceRow& g = p.rows[r];
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
     const Settings set = settings(a, r);
     const float max = row_max(p, r);
@@ -809,7 +810,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices
     if (t < n && s.at + t < kList) g.list[s.at + t] = s.list[t], g.weights[s.at + t] = s.weights[t];
 }
 
-__global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices p, bool aligned) {
+__global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices p) {
     extern __shared__ __align__(16) uint8_t raw[];
     Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
     const int r = blockIdx.x, t = threadIdx.x;
@@ -822,7 +823,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
         return;
     }
     const int n = g.n;
-    if (!sliced(set) || (!set.greedy && n > kList)) return sample_row(a, s, r, aligned);
+    if (!sliced(set) || (!set.greedy && n > kList)) return sample_row(a, s, r);
     if (set.greedy) {
         if (t == 0) put(a, r, int(~uint32_t(g.key)), 1.0f);
         return;
@@ -836,7 +837,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
     __syncthreads();
     if (set.by_k && set.top_k <= kFewK) return pick_from_list(a, s, r, set, c, n);
     if (n) cut_list(s, c, n, left, !set.by_k, set.min_p);
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab, aligned};
+    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     pick(a, s, row, r, Kept(c, s.key, set.min_p), set.u);
 }
 
@@ -857,22 +858,21 @@ size_t sample_scratch_floats(int rows, int vocab) {
 }
 
 int launch_sample(const SampleArgs& a, hipStream_t s, float* scratch) {
-    const bool al = !(reinterpret_cast<uintptr_t>(a.logits) & 15) && a.stride % 4 == 0;
     const int n = scratch ? sample_slices(a.rows, a.vocab) : 0;
     if (n) {
         const int turns = (a.vocab + kTurn - 1) / kTurn;
         Slices p{reinterpret_cast<SliceRow*>(scratch), nullptr, n, 4 * ((turns + n - 1) / n)};
         p.hist = reinterpret_cast<u64*>(p.rows + a.rows);
         const dim3 grid{unsigned(n), unsigned(a.rows)};
-        hipLaunchKernelGGL(k_slice_max, grid, dim3(kThreads), 0, s, a, p, al);
-        hipLaunchKernelGGL(k_slice_hist, grid, dim3(kThreads), 0, s, a, p, al);
-        hipLaunchKernelGGL(k_slice_collect, grid, dim3(kThreads), unsigned(sizeof(Shared<false>)), s, a, p, al);
+        hipLaunchKernelGGL(k_slice_max, grid, dim3(kThreads), 0, s, a, p);
+        hipLaunchKernelGGL(k_slice_hist, grid, dim3(kThreads), 0, s, a, p);
+        hipLaunchKernelGGL(k_slice_collect, grid, dim3(kThreads), unsigned(sizeof(Shared<false>)), s, a, p);
         hipLaunchKernelGGL(k_slice_finish, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(sizeof(Shared<false>)), s,
-                           a, p, al);
+                           a, p);
         return int(hipGetLastError());
     }
     auto go = [&](auto kern, size_t lds) {
-        hipLaunchKernelGGL(kern, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(lds), s, a, al);
+        hipLaunchKernelGGL(kern, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(lds), s, a);
     };
     if (a.vocab <= kResident)
         go(k_sample<true>, sizeof(Shared<true>));
