@@ -432,7 +432,8 @@ int wv_kv_free(uint64_t cache);
  * rows back to back), their position d_slots[t]. A slot outside the pool (-1
  * for the padding rows of a batch) is skipped. The slots of one call have to
  * differ: of two rows for one slot, which codes and scale end there is not
- * defined. Device pointers, enqueued on `stream`; allocates nothing. */
+ * defined. n * n_kv_heads is at most 2^28. Device pointers, enqueued on
+ * `stream`; allocates nothing. */
 int wv_kv_write_dev(uint64_t cache, int32_t layer, const float *d_k, const float *d_v, int64_t k_stride,
                     int64_t v_stride, const int64_t *d_slots, int32_t n, void *stream);
 /* Reads n positions back into f32 rows (laid out as in wv_kv_write_dev); rows
@@ -505,8 +506,8 @@ typedef struct wv_sampling {
  * included, and summed exactly in units of 2^-44 of the largest: a token that
  * stands on the edge of top_p or u may fall to either side. d_probs (may be
  * NULL): the drawn token's share of the kept weights (1 where T <= 0, 0 for
- * token -1). vocab is at most 2^19. Device pointers, enqueued on `stream`. Up
- * to 128 rows of more than 32768 logits use the library's own scratch, except
+ * token -1). vocab is at most 2^19, rows 2^20. Device pointers, enqueued on
+ * `stream`. Up to 128 rows of more than 32768 logits use the library's own scratch, except
  * on a stream under capture, where one block draws a row whatever its length. */
 int wv_sample_dev(const float *d_logits, int64_t stride, int32_t rows, int32_t vocab, const wv_sampling *sampling,
                   int32_t *d_tokens, float *d_probs, void *stream);
@@ -535,8 +536,8 @@ int wv_decoder_generate_sampled(uint64_t decoder, int32_t token, int32_t pos, in
  * block of that many rows), attention as wv_kv_attention_dev, the LM head at
  * the f32 bar. Errors: WV_E_ARG "empty ids" without any new token, WV_E_SHAPE
  * for a cache of another shape, positions past the table, a page outside the
- * pool that holds one of the sequence's positions, or two new tokens for one
- * position of the pool. Synchronous. */
+ * pool that holds one of the sequence's positions, two new tokens for one
+ * position of the pool, or over 65535 new tokens. Synchronous. */
 int wv_decoder_forward_paged(uint64_t decoder, uint64_t cache, int32_t n_seqs, const int32_t *n_new,
                              const int32_t *tokens, const int32_t *kv_len, const int32_t *pages, int32_t max_pages,
                              const wv_sampling *sampling, int32_t *next_tokens, float *logits);

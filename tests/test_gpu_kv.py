@@ -445,6 +445,16 @@ def test_attention_graph_replays(scratch):
         p.check(eager, [1], scale=0.125, lens=[length])
 
 
+@pytest.mark.parametrize("new", [3, 600])
+def test_attention_of_zero_queries(new):
+    """Queries of zeros and a scale that underflows: the plain mean of the values, the masked keys left out."""
+    p = Pool(np.random.default_rng(new), [700], 2, 64, 32, "f16").fill()
+    q = np.zeros((new, 8, 64), np.float32)
+    out = p.attend([new], 8, scale=1e-12, q=q, max_q=new)
+    p.check(out, [new], scale=1e-12)
+    assert np.isfinite(out).all()
+
+
 def test_attention_two_streams():
     """Split calls on two streams at once do not share partials."""
     rng = np.random.default_rng(14)
@@ -478,6 +488,8 @@ def test_refusals_with_a_cache():
     assert L.wv_kv_write_dev(kv.handle, -1, P, P, 0, 0, I, 1, None) == -1
     assert L.wv_kv_write_dev(kv.handle, 0, P, P, 0, 0, I, -1, None) == -2
     assert L.wv_kv_write_dev(kv.handle, 0, P, P, 127, 0, I, 1, None) == -2
+    assert L.wv_kv_write_dev(kv.handle, 0, P, P, 0, 0, I, (1 << 27) + 1, None) == -2
+    assert L.wv_kv_read_dev(kv.handle, 0, I, (1 << 27) + 1, P, P, 0, 0, None) == -2
     assert L.wv_kv_write_dev(kv.handle, 0, None, P, 0, 0, I, 1, None) == -1
     assert L.wv_kv_read_dev(kv.handle, 0, None, 1, P, P, 0, 0, None) == -1
     assert L.wv_kv_write_dev(kv.handle, 0, None, None, 0, 0, None, 0, None) == 0

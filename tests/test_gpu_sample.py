@@ -1,8 +1,9 @@
 """wv_sample_dev against the definition in float64: every setting alone and together, ties, masked and
 non-finite logits, row strides, vocabularies from one token to 2^19, borders of u and of the cuts.
 
-Weights on the device are off by a relative 2^-22 at most (f32 exponential and its argument), sums are
-exact: a running sum over a total is off by 2^-21 (OFF). A draw has to be the reference's token, or one
+Weights on the device are off by a step of the f32 exponential and by the rounding of its argument a, 2^-24 |a|
+ln 2, whose sign changes from token to token: weights down to 2^-5 by 2^-22 each, and sums of smaller ones, which
+take many, by less. Sums are exact: a running sum over a total is off by 2^-21 (OFF). A draw has to be the reference's token, or one
 that the reference gives when its borders (the sum at u, the top-p prefix, min_p) move by that much."""
 import ctypes
 
@@ -227,6 +228,40 @@ def test_repeatable_and_replayed():
         a, b = draw(x, t=0.9, p=0.9, u=y)
         assert np.array_equal(a, tok.cpu().numpy()) and np.array_equal(b, prob.cpu().numpy())
         check(x, t=0.9, p=0.9, u=y)
+
+
+def test_many_rows_of_a_large_vocab():
+    """More rows than are cut over blocks: each by one block that reads it from memory in every pass."""
+    rng = np.random.default_rng(12)
+    r, v = 131, 33001
+    x = logits(rng, r, v)
+    x[3] = -np.inf
+    x[7, 5:] = x[7, 5]
+    pick = lambda *a: rng.choice(np.array(a, np.float32), r)  # noqa: E731
+    check(x, t=pick(0.0, 0.7, 1.0), k=pick(0, 1, 40, 500).astype(np.int32), p=pick(0.5, 0.95, 1.0),
+          m=pick(0, 0.01), u=rng.random(r, np.float32))
+
+
+def test_two_streams():
+    """Calls on two streams at once, each with scratch of its own: the bits of calls one after the other."""
+    rng = np.random.default_rng(13)
+    v, st = 70000, [torch.cuda.Stream() for _ in range(2)]
+    sets = []
+    for r in (17, 40):
+        x, u = logits(rng, r, v), rng.random(r, np.float32)
+        want = draw(x, t=0.9, p=0.9, u=u)
+        sets.append((r, torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(), torch.full((r,), 0.9, device="cuda"), want,
+                     [torch.zeros(r, dtype=torch.int32, device="cuda") for _ in range(6)],
+                     [torch.zeros(r, device="cuda") for _ in range(6)]))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for s, (r, x, u, a, _, tok, prob) in zip(st, sets):
+            sample_dev(x.data_ptr(), r, v, tok[i].data_ptr(), u.data_ptr(), temperature_ptr=a.data_ptr(),
+                       top_p_ptr=a.data_ptr(), probs_ptr=prob[i].data_ptr(), stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for r, _, _, _, want, tok, prob in sets:
+        for i in range(6):
+            assert np.array_equal(tok[i].cpu().numpy(), want[0]) and np.array_equal(prob[i].cpu().numpy(), want[1])
 
 
 def test_no_probs_and_refusals():

@@ -205,3 +205,25 @@ def test_generate_sampled():
         dec.prefill(prompt)
         assert dec.generate_sampled(first, 20, u[:6], temperature=0.0).tolist() == greedy
     assert dec.generate_sampled(first, 20, []).size == 0
+
+
+def test_generate_sampled_large_vocab():
+    """More logits than one block holds: the draw is cut over blocks, eager and in the replayed graph."""
+    cfg = config(vocab=40000, n_layers=1)
+    dec, _ = build(cfg, "Q4_K", 11)
+    u = np.random.default_rng(12).random(6, np.float32)
+    kw = dict(temperature=1.1, top_p=0.97, min_p=0.0001)
+    tok, one = 5, []
+    for i in range(6):
+        t, logits = dec.generate_sampled(tok, i, u[i:i + 1], want_logits=True, **kw)
+        assert reference(logits, np.float32(1.1), 0, np.float32(0.97), np.float32(0.0001), u[i])[2](int(t[0]))
+        tok = int(t[0])
+        one.append(tok)
+    for graph in (False, True, True):
+        dec.use_graph(graph)
+        assert dec.generate_sampled(5, 0, u, **kw).tolist() == one
+    s = Server(cfg, "Q4_K", "q8", 3, seed=11)
+    tokens, logits = s.step([[1, 2], [], [7]], uniform=[0.3, 0.5, 0.8], temperature=1.1, top_k=900, top_p=0.9)
+    for b, un in ((0, 0.3), (2, 0.8)):
+        assert reference(logits[b], np.float32(1.1), 900, np.float32(0.9), 0, np.float32(un))[2](int(tokens[b]))
+    assert tokens[1] == -1

@@ -14,6 +14,7 @@ def test_refusals_without_device():
     assert L.wv_sample_dev(16, 0, -1, 100, by, 16, None, None) == -2
     assert L.wv_sample_dev(16, 0, 1, 0, by, 16, None, None) == -2
     assert L.wv_sample_dev(16, 0, 1, (1 << 19) + 1, by, 16, None, None) == -2
+    assert L.wv_sample_dev(16, 0, (1 << 20) + 1, 100, by, 16, None, None) == -2
     assert L.wv_sample_dev(16, 99, 1, 100, by, 16, None, None) == -2
     assert b"stride" in L.wv_last_error()
     assert L.wv_sample_dev(None, 0, 1, 100, by, 16, None, None) == -1

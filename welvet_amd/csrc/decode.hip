@@ -1487,7 +1487,7 @@ struct Decoder {
     float* pxh = nullptr;  // the fp16 GEMM operand shared by the projections of one input, then its row factors
     int32_t* ptok = nullptr;
     size_t pscratch_floats = 0, pxh_floats = 0;
-    // drawn tokens: {temperature, top_k, top_p, min_p} and one u per step
+    // drawn tokens: {temperature, top_k, top_p, min_p} and one u per step; behind samp_head floats the draw's scratch
     float* samp = nullptr;
     // batches over a paged cache: their integers and settings, the sequences' last rows and logits, grown on demand
     uint8_t* gmeta = nullptr;
@@ -1624,6 +1624,7 @@ void launch_attn(Decoder& d, Layer& ly, int G, float scale) {
                            c.n_heads, c.n_kv_heads, c.max_seq, d.n_chunks, scale, d.k, d.v, d.cs);
 }
 
+size_t samp_head(const wv_decoder_config& c) { return (4 + size_t(c.max_seq) + 3) / 4 * 4; }
 // advance: 1 the position moves on, 0 it stays; with kDraw the token is drawn (and the position moves on).
 constexpr int kDraw = 2;
 int enqueue_step(Decoder& d, int advance) {
@@ -1702,7 +1703,7 @@ int enqueue_step(Decoder& d, int advance) {
         a.logits = d.logits, a.stride = c.vocab, a.rows = 1, a.vocab = c.vocab;
         a.p = {d.samp, reinterpret_cast<const int32_t*>(d.samp + 1), d.samp + 2, d.samp + 3, d.samp + 4};
         a.state = d.d_state, a.gen = d.d_gen, a.gen_cap = c.max_seq, a.advance = 1;
-        return launch_sample(a, d.stream);
+        return launch_sample(a, d.stream, d.samp + samp_head(c));
     }
     hipLaunchKernelGGL(k_argmax_advance, dim3(1), dim3(1024), 0, d.stream, d.logits, c.vocab, d.d_state, d.d_gen,
                        c.max_seq, advance);
@@ -2080,7 +2081,7 @@ int enqueue_prefill(Decoder& d, int n, int pos0, const Paged* pg = nullptr) {
         if (e) return e;
         SampleArgs a{};
         a.logits = d.glogits, a.stride = c.vocab, a.rows = B, a.vocab = c.vocab, a.p = pg->samp, a.tokens = pg->next;
-        return launch_sample(a, d.stream);
+        return launch_sample(a, d.stream, d.pscratch);
     }
     hipLaunchKernelGGL(k_add, dim3(unsigned((hidden + 255) / 256)), dim3(256), 0, d.stream,
                        d.ph + int64_t(n - 1) * hidden, d.pn + int64_t(n - 1) * hidden, hidden);
@@ -2388,7 +2389,8 @@ int wv_decoder_generate_sampled(uint64_t dec, int32_t token, int32_t pos, int32_
     if (rc) return rc;
     (void)hipSetDevice(d->device);
     if (!d->samp) {
-        const hipError_t e = hipMalloc(reinterpret_cast<void**>(&d->samp), (4 + size_t(c.max_seq)) * sizeof(float));
+        const hipError_t e = hipMalloc(reinterpret_cast<void**>(&d->samp),
+                                       (samp_head(c) + sample_scratch_floats(1, c.vocab)) * sizeof(float));
         if (e != hipSuccess) {
             d->samp = nullptr;
             return rt_hip_fail(e, "wv_decoder_generate_sampled: settings");
@@ -2452,7 +2454,7 @@ int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const
                 return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: sequence %d: page %d of %d", b, p, k.n_pages);
     }
     if (!total) return rt_fail(WV_E_ARG, "wv_decoder_forward_paged: empty ids");
-    if (total * c.n_heads >= int64_t(1) << 31 || total > 1 << 20)
+    if (total > 65535)
         return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: %lld new tokens in one call", (long long)total);
     const int n = int(total);
     // one copy: slots, then 32-bit rows (positions, first rows, lengths, last rows, tables, settings, results)
@@ -2495,8 +2497,8 @@ int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const
     const int32_t longest = *std::max_element(len, len + B);
     pg.splits = kv_attn_splits(pg.cache.layer(0), n_seqs, n,
                                std::min(max_pages, (longest + k.page_size - 1) / k.page_size), pg.max_q, c.n_heads, 0);
-    const size_t more = std::max(kv_attn_part_floats(pg.cache.layer(0), n, c.n_heads, pg.splits),
-                                 matvec_scratch_floats(d->lm, n_seqs));
+    const size_t more = std::max({kv_attn_part_floats(pg.cache.layer(0), n, c.n_heads, pg.splits),
+                                  matvec_scratch_floats(d->lm, n_seqs), sample_scratch_floats(n_seqs, c.vocab)});
     rc = ensure_prefill(*d, n, more);
     if (rc) return rc;
     hipError_t e = hipSuccess;

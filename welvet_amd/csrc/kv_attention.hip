@@ -30,7 +30,9 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;  // m of a row that has met no key
+constexpr float kLeast = 1.4e-45f;  // of a row's factor: times the -inf of a masked key it stays -inf
 constexpr int kMaxSplits = 64;
+constexpr int kMaxGridY = 1 << 15;  // tiles of a launch
 constexpr int kFewRows = 256;  // query rows of a sequence and KV head up to which the row kernel takes it
 
 // 8 biased int8 codes (two words) as fp16: 0x6400 | b is 1024 + b, less 1152
@@ -184,7 +186,7 @@ __device__ __forceinline__ float row_unit(float amax, float& inv) {
 // lane (row l & 15, octet l >> 4) with the 8 keys of its octet, which are its
 // operand of O^T += V^T P^T. The waves' sums meet in LDS.
 template <int HD, int TYPE>
-__global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int max_rows) {
+__global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int max_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
     constexpr int S = HD / 32;                   // k steps of a score product
     constexpr int NK = S / (TYPE == WV_KV_F16 ? 1 : 2);   // 16-byte K loads of a 16-key tile
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 
     const int kvh = blockIdx.x, sp = blockIdx.z;
     Tile t;
-    if (!find_tile<16>(a, G, blockIdx.y, 1, max_rows, t)) return;
+    if (!find_tile<16>(a, G, tile0 + int(blockIdx.y), 1, max_rows, t)) return;
     const Range rg = tile_range<16>(a, t, G, sp, 4);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
                 m = fmaxf(m, fabsf(x[s][j]));
             }
         float inv;
-        qs = row_unit(max_over_quads(m), inv) * a.scale * kLog2e;
+        qs = fmaxf(row_unit(max_over_quads(m), inv) * a.scale * kLog2e, kLeast);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
 #pragma unroll
@@ -433,7 +435,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // on their way into registers. The V scales are staged as s_j 2^-E already,
 // with the factor by which E moved.
 template <int HD, int TYPE>
-__global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows) {
+__global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
     constexpr int BB = 32 * HD * E;   // bytes of a block's codes
     constexpr int S = HD / 16;        // k steps of a score product
@@ -453,9 +455,9 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     // of a CU walk about as many keys as those of any other
     const int half = (gridDim.y + 1) / 2, y = int(blockIdx.y);
     const bool once = gridDim.x * gridDim.y * gridDim.z <= 512;
-    const int idx = once && y >= half ? y - half : int(gridDim.y) - 1 - y;
+    const int idx = tile0 + (once && y >= half ? y - half : int(gridDim.y) - 1 - y);
     Tile t;
-    if (!find_tile<128>(a, G, idx, min_rows, 1 << 30, t)) return;
+    if (!find_tile<128>(a, G, idx, min_rows, INT32_MAX, t)) return;
     const Range rg = tile_range<128>(a, t, G, sp, 8);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
             }
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
         float inv;
-        qs = row_unit(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), inv) * a.scale * kLog2e;
+        qs = fmaxf(row_unit(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), inv) * a.scale * kLog2e, kLeast);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
 #pragma unroll
@@ -784,7 +786,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
     constexpr int LD = HD + 4, W = HD / 64;
     __shared__ float red[4][HD];
     const int tok = blockIdx.x, head = blockIdx.y;
-    if (tok >= min(a.cu[a.n_seqs], a.n_tokens)) return;
+    if (tok < a.cu[0] || tok >= min(a.cu[a.n_seqs], a.n_tokens)) return;
     const float* p = a.part + (int64_t(tok) * a.n_heads + head) * a.splits * LD;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float m = -INFINITY, l = 0.0f;
@@ -868,15 +870,17 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
     const int G = a.n_heads / a.c.n_kv;
     const int64_t rows = int64_t(a.n_tokens) * G;
     const bool f16 = a.c.type == WV_KV_F16;
-    auto go = [&](auto kern, int64_t tiles, int bound, int threads = 256) {
-        const dim3 grid{unsigned(a.c.n_kv), unsigned(tiles), unsigned(a.splits)};
-        hipLaunchKernelGGL(kern, grid, dim3(unsigned(threads)), 0, s, a, G, bound);
+    auto go = [&](auto kern, int64_t tiles, int bound) {
+        for (int64_t t0 = 0; t0 < tiles; t0 += kMaxGridY) {
+            const dim3 grid{unsigned(a.c.n_kv), unsigned(std::min<int64_t>(tiles - t0, kMaxGridY)), unsigned(a.splits)};
+            hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, G, bound, int(t0));
+        }
     };
     const bool many = plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, a.n_heads, a.window).many;
     const bool few = !many || a.n_seqs > 1;
     if (few) {
         const int64_t tiles = (rows + 15) / 16 + a.n_seqs;
-        const int most = many ? kFewRows : 1 << 30;
+        const int most = many ? kFewRows : INT32_MAX;
         if (a.c.hd == 128)
             f16 ? go(k_kv_attn_rows<128, WV_KV_F16>, tiles, most) : go(k_kv_attn_rows<128, WV_KV_Q8>, tiles, most);
         else

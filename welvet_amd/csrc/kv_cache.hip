@@ -474,7 +474,7 @@ int check_rows(const char* what, uint64_t cache, int32_t layer, const void* k, c
         return rt_fail(WV_E_SHAPE, "%s: row strides %lld and %lld under the row's %lld floats", what, (long long)ks,
                        (long long)vs, (long long)w);
     if (n && (!k || !v || !slots)) return rt_fail(WV_E_ARG, "%s: nil k/v/slots", what);
-    if (int64_t(n) * c.c.n_kv_heads >= int64_t(1) << 31)
+    if (int64_t(n) * c.c.n_kv_heads > int64_t(1) << 28)
         return rt_fail(WV_E_SHAPE, "%s: %d rows of %d heads in one call", what, n, c.c.n_kv_heads);
     return WV_OK;
 }

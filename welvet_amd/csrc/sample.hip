@@ -888,8 +888,8 @@ using namespace wv;
 extern "C" int wv_sample_dev(const float* d_logits, int64_t stride, int32_t rows, int32_t vocab,
                              const wv_sampling* sampling, int32_t* d_tokens, float* d_probs, void* stream) {
     if (!sampling) return rt_fail(WV_E_ARG, "wv_sample: nil sampling");
-    if (rows < 0 || vocab <= 0 || vocab > kMaxVocab)
-        return rt_fail(WV_E_SHAPE, "wv_sample: %d rows of %d logits (1 to %d)", rows, vocab, kMaxVocab);
+    if (rows < 0 || rows > 1 << 20 || vocab <= 0 || vocab > kMaxVocab)
+        return rt_fail(WV_E_SHAPE, "wv_sample: %d rows (at most 2^20) of %d logits (1 to %d)", rows, vocab, kMaxVocab);
     if (!stride) stride = vocab;
     if (stride < vocab)
         return rt_fail(WV_E_SHAPE, "wv_sample: row stride %lld under %d logits", (long long)stride, vocab);
