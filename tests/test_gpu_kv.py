@@ -339,12 +339,12 @@ def test_attention_long_split_and_deterministic():
     assert p.kv.attention_scratch(b, 4) > 0
 
 
-# The kernel for many rows takes calls of at least 512 blocks of 128 rows (query heads of a KV head x tokens),
-# with a sequence of 1024 rows and more.
+# The kernel for many rows takes long chunks: these shapes, of whatever type.
 
 @pytest.mark.parametrize("typ", ["f16", "q8"])
 @pytest.mark.parametrize("heads,kv_heads,hd,kv,new", [(32, 8, 64, 2100, 2048), (64, 16, 128, 1100, 1024),
-                                                      (24, 24, 64, 2750, 2747), (32, 8, 128, 4200, 515)])
+                                                      (24, 24, 64, 2750, 2747), (32, 8, 128, 4200, 515),
+                                                      (24, 4, 128, 9001, 203), (64, 16, 64, 1900, 1900)])
 def test_many_rows_one_sequence(typ, heads, kv_heads, hd, kv, new):
     """Whole prompts, a chunk behind cached keys, one cut into key ranges (515 tokens over 4200 keys)."""
     rng = np.random.default_rng(kv + heads)

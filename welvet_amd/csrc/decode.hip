@@ -1498,7 +1498,8 @@ struct Decoder {
 // What enqueue_prefill takes of a batch over a paged cache (device pointers).
 struct Paged {
     KvCache cache;
-    int n_seqs = 0, max_pages = 0, max_q = 0, splits = 1;
+    int n_seqs = 0, max_pages = 0, max_q = 0;
+    KvPlan plan{};
     const int64_t* slots = nullptr;                                                            // [n]
     const int32_t *pos = nullptr, *cu = nullptr, *kv_len = nullptr, *pages = nullptr, *last = nullptr;
     wv_sampling samp{};
@@ -2001,10 +2002,10 @@ int enqueue_prefill(Decoder& d, int n, int pos0, const Paged* pg = nullptr) {
             if (e) return e;
             KvAttn a{};
             a.c = view;
-            a.q = q, a.qs = qstr, a.out = d.patt, a.os = qd, a.part = pg->splits > 1 ? d.pscratch : nullptr;
+            a.q = q, a.qs = qstr, a.out = d.patt, a.os = qd, a.part = pg->plan.splits > 1 ? d.pscratch : nullptr;
             a.cu = pg->cu, a.kv_len = pg->kv_len, a.pages = pg->pages;
             a.n_seqs = pg->n_seqs, a.n_tokens = n, a.max_pages = pg->max_pages, a.max_q = pg->max_q;
-            a.n_heads = c.n_heads, a.splits = pg->splits, a.scale = scale;
+            a.n_heads = c.n_heads, a.splits = pg->plan.splits, a.many = pg->plan.many, a.scale = scale;
             e = launch_kv_attn(a, d.stream);
             if (e) return e;
         } else if (qkv_splits > 1)
@@ -2493,11 +2494,10 @@ int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const
     if (rc) return rc;
     (void)hipSetDevice(d->device);
     pg.n_seqs = n_seqs, pg.max_pages = max_pages;
-    // keys past the longest sequence need no split
     const int32_t longest = *std::max_element(len, len + B);
-    pg.splits = kv_attn_splits(pg.cache.layer(0), n_seqs, n,
-                               std::min(max_pages, (longest + k.page_size - 1) / k.page_size), pg.max_q, c.n_heads, 0);
-    const size_t more = std::max({kv_attn_part_floats(pg.cache.layer(0), n, c.n_heads, pg.splits),
+    pg.plan = kv_attn_plan(pg.cache.layer(0), n_seqs, n, std::min(max_pages, (longest + k.page_size - 1) / k.page_size),
+                           pg.max_q, c.n_heads, 0);
+    const size_t more = std::max({kv_attn_part_floats(pg.cache.layer(0), n, c.n_heads, pg.plan.splits),
                                   matvec_scratch_floats(d->lm, n_seqs), sample_scratch_floats(n_seqs, c.vocab)});
     rc = ensure_prefill(*d, n, more);
     if (rc) return rc;

@@ -83,10 +83,16 @@ struct KvAttn {
     int n_seqs, n_tokens, max_pages, max_q;
     int n_heads, window;
     int splits;
+    bool many;  // long sequences by the kernel of 128-row tiles
     float scale;
 };
-// The number of key ranges a call is cut into, and the floats of its partials.
-int kv_attn_splits(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window);
+// Which kernels a call takes and into how many key ranges it is cut (max_pages: as many as sequences hold), and
+// the floats of its partials.
+struct KvPlan {
+    bool many;
+    int splits;
+};
+KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window);
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits);
 int launch_kv_attn(const KvAttn& a, hipStream_t s);
 

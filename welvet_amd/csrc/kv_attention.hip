@@ -32,6 +32,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNoMax = -3.0e38f;  // m of a row that has met no key
 constexpr float kLeast = 1.4e-45f;  // of a row's factor: times the -inf of a masked key it stays -inf
 constexpr int kMaxSplits = 64;
+constexpr int kTileRows = 512;      // rows of a sequence from which on the tile kernel is thought of
 constexpr int kMaxGridY = 1 << 15;  // tiles of a launch
 constexpr int kFewRows = 256;  // query rows of a sequence and KV head up to which the row kernel takes it
 
@@ -826,40 +827,49 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
 
 }  // namespace
 
-namespace {
-
 // How a call is run. The tile kernel reads and converts the keys once for 128
-// rows, but goes through them in steps of 32 keys at 1.4 us a step for one
-// block a CU and 2.0 for two: it pays where two blocks a CU have at least 32
-// key blocks each and some sequence has rows for 8 tiles. Rows of 32 heads
-// over 8, head_dim 128, int8, row against tile kernel at its best split (us):
-// 1 x 512 new over 2048 keys 59 / 66, over 8192 216 / 163; 1 x 2048 over 2048
-// 213 / 102, over 16384 1812 / 975; 16 x 128 over 8192 273 / 281.
-struct Plan {
-    bool many;   // the tile kernel takes the sequences of more than kFewRows rows
-    int splits;
-};
-Plan plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
+// rows and the row kernel for 16, but a tile steps through its key blocks one
+// after the other, 1.4 us each for one block a CU and 2.0 for two, so that few
+// tiles, or short ones, leave the GPU waiting. This compares what the two
+// take, in us, fitted to calls of 128 to 3500 new tokens over 300 to 50000
+// keys. Row against tile kernel as measured, 32 heads over 8, head_dim 128: 512
+// new over 512 keys 23 / 32, over 16384 552 / 302; 1024 over 1024 50 / 56, over
+// 4096 230 / 172; 1508 over 1508 98 / 84; 1900 over 16384 2460 / 957; 1900 with
+// a window of 512 96 / 54; head_dim 64, 1900 over 1900 76 / 91. Of a batch, the
+// tile kernel takes the sequences of more than kFewRows rows.
+KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
     if (!n_seqs || !n_tokens) return {false, 1};
     const int64_t G = n_heads / c.n_kv, rows = n_tokens * G;
     const int64_t most_q = max_q ? std::min(max_q, n_tokens) : (n_tokens + n_seqs - 1) / n_seqs;
     const int64_t width = int64_t(max_pages) << c.page_shift;
+    const int64_t seqs = std::min(n_seqs, n_tokens);
+    // key blocks that the last tile of `RT` rows walks, and one on average
+    const auto last = [&](int64_t RT) {
+        return double(window > 0 ? std::min<int64_t>(width, window + RT / G + 31) : width) / 32.0;
+    };
+    const double causal = window > 0 ? 0.0 : double(std::min(most_q, width)) / 64.0;
     const int64_t keys = window > 0 ? std::min<int64_t>(width, int64_t(window) + most_q) : width;
     const int64_t blocks = std::max<int64_t>((keys + 31) / 32, 1);
-    const int64_t t128 = (rows + 127) / 128 * c.n_kv;  // tile blocks
-    const int64_t s128 = std::max<int64_t>(1, std::min<int64_t>({512 / t128, blocks / 32, kMaxSplits}));
-    if (most_q * G >= 1024 && t128 * s128 >= 512) return {true, int(s128)};
+    const int64_t t16 = std::max<int64_t>((rows + 15) / 16, seqs) * c.n_kv;
+    if (most_q * G >= kTileRows) {
+        const int64_t t128 = std::max<int64_t>((rows + 127) / 128, seqs) * c.n_kv;
+        const int64_t s128 = std::max<int64_t>(1, std::min<int64_t>({512 / t128, blocks / 32, kMaxSplits}));
+        const bool wide = c.hd == 128;
+        // what the last tile takes, or all of them at two blocks a CU, and the join's partial rows
+        double tile = (wide ? 15.0 : 10.0) + std::max(last(128) / double(s128) * (wide ? 1.6 : 1.25),
+                                                      double(t128) * (last(128) - causal) / 256.0 * (wide ? 1.15 : 0.9));
+        if (s128 > 1) tile += 5.0 + double(t128 * s128) * 128.0 * double(c.hd + 4) * 8.0 / 5.2e6;
+        const double steps = double(t16) * (last(16) - 0.65 * causal);
+        double row = 3.0 + double(t16) * (1.8 / 512.0) + steps / (wide ? 1150.0 : 2300.0);
+        const double block_bytes = 64.0 * c.hd * kv_code_bytes(c.type);
+        if (last(16) * block_bytes > 2e6)  // more than stays in an L2
+            row = std::max(row, double(t16) * (last(16) - causal) * block_bytes / 11e6);
+        if (tile < row) return {true, int(s128)};
+    }
     // Row kernel: two blocks a CU; more ranges cost their join more than they gain: a block takes a key
     // block in about 1 us / 4, a range adds 0.15 us (8192 keys, one token: 8 / 16 / 64 ranges 18.7 / 15.1 / 21.6 us).
-    const int64_t t16 = std::max<int64_t>((rows + 15) / 16, std::min(n_seqs, n_tokens)) * c.n_kv;
     const int64_t best = int64_t(std::sqrt(1.6 * double(blocks)) + 0.5);
     return {false, int(std::max<int64_t>(1, std::min<int64_t>({768 / t16, best, kMaxSplits})))};
-}
-
-}  // namespace
-
-int kv_attn_splits(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
-    return plan(c, n_seqs, n_tokens, max_pages, max_q, n_heads, window).splits;
 }
 
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits) {
@@ -876,8 +886,7 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
             hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, G, bound, int(t0));
         }
     };
-    const bool many = plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, a.n_heads, a.window).many;
-    const bool few = !many || a.n_seqs > 1;
+    const bool many = a.many, few = !many || a.n_seqs > 1;
     if (few) {
         const int64_t tiles = (rows + 15) / 16 + a.n_seqs;
         const int most = many ? kFewRows : INT32_MAX;
@@ -941,7 +950,8 @@ int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch* batch, int32_t n_
     if (rc) return rc;
     if (!bytes) return rt_fail(WV_E_ARG, "wv_kv_attention_scratch: nil bytes");
     const KvView v = c.layer(0);
-    const int sp = kv_attn_splits(v, batch->n_seqs, batch->n_tokens, batch->max_pages, batch->max_q, n_heads, window);
+    const int sp =
+        kv_attn_plan(v, batch->n_seqs, batch->n_tokens, batch->max_pages, batch->max_q, n_heads, std::min(window, 1 << 30)).splits;
     *bytes = kv_attn_part_floats(v, batch->n_tokens, n_heads, sp) * sizeof(float);
     return WV_OK;
 }
@@ -972,7 +982,8 @@ int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch* batch,
     a.cu = batch->d_cu_q, a.kv_len = batch->d_kv_len, a.pages = batch->d_pages;
     a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages, a.max_q = batch->max_q;
     a.n_heads = n_heads, a.window = std::min(window, 1 << 30), a.scale = scale;
-    a.splits = kv_attn_splits(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, n_heads, window);
+    const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, n_heads, a.window);
+    a.splits = plan.splits, a.many = plan.many;
     const size_t floats = kv_attn_part_floats(a.c, a.n_tokens, n_heads, a.splits);
     RtScratch sc;
     if (d_scratch) {
