@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
                 pin(up);
             }
         };
-        h8 x = k_at(0);
+        h8 x[2] = {k_at(0), k_at(1)};
         f4 vs[2];
         vs[0] = *reinterpret_cast<const f4*>(&ls[ring][h * 16 + 8]);
 #pragma unroll
@@ -700,9 +700,9 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
         float add[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < S; ++c) {
-            h8 y = x;
+            h8 y = x[c & 1];
             pin(y);
-            if (c + 1 < S) x = k_at(c + 1);
+            if (c + 2 < S) x[c & 1] = k_at(c + 2);
             if (c % (S / 4) == 0 && c < S - S / 4)
                 vs[(4 * c / S + 1) & 1] = *reinterpret_cast<const f4*>(
                     &ls[ring][(2 * ((4 * c / S + 1) >> 1) + h) * 16 + 8 + 4 * ((4 * c / S + 1) & 1)]);
