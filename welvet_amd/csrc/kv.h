@@ -84,12 +84,13 @@ struct KvAttn {
     int n_heads, window;
     int splits;
     bool many;  // long sequences by the kernel of 128-row tiles
+    bool once;  // one block reads a sequence's keys of a KV head
     float scale;
 };
 // Which kernels a call takes and into how many key ranges it is cut (max_pages: as many as sequences hold), and
 // the floats of its partials.
 struct KvPlan {
-    bool many;
+    bool many, once;
     int splits;
 };
 KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window);

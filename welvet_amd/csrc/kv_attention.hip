@@ -185,8 +185,15 @@ __device__ __forceinline__ float row_unit(float amax, float& inv) {
 // registers from the cache to the sums: a lane's 16-byte loads are operands
 // of the 16x16x32 products as they lie in the cache. S^T = K Q^T leaves a
 // lane (row l & 15, octet l >> 4) with the 8 keys of its octet, which are its
-// operand of O^T += V^T P^T. The waves' sums meet in LDS.
-template <int HD, int TYPE>
+// operand of O^T += V^T P^T. The waves' sums meet in LDS. A single token's row
+// is bound by the codes' bytes: 64 sequences of 1 to 8192 int8 keys, 32 heads
+// over 8 of 128, 134 us, 5.2 TB/s; one of 131071 fp16 keys 106 us, 5.2 TB/s. A
+// short one by the chain of loads before its first product and by the join's
+// launch: 2048 int8 keys 8 + 3 us.
+// ONCE: no other block reads a sequence's keys, and they are loaded past the
+// caches (131071 fp16 keys 106 us, else 112); not where several tiles read them
+// (64 tokens of 32 heads over 8000 fp16 keys 56 us so, else 43).
+template <int HD, int TYPE, bool ONCE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int max_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
     constexpr int S = HD / 32;                   // k steps of a score product
@@ -253,17 +260,28 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     uint4 kr[2][NK], vr[NV];
     float4 sk[2], sv[2];
     auto load_k = [&](int64_t b) {
-        const uint8_t* p = a.c.k + b * BB;
+        const uint4* p = reinterpret_cast<const uint4*>(a.c.k + b * BB) + g * 32 + key0;
+        if (ONCE) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int i = 0; i < NK; ++i)
-                kr[x][i] = ld_nt16(reinterpret_cast<const uint4*>(p + ((4 * i + g) * 32 + key0 + 8 * x) * 16));
+                for (int i = 0; i < NK; ++i) kr[x][i] = ld_nt16(p + 128 * i + 8 * x);
+        } else {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < NK; ++i) kr[x][i] = p[128 * i + 8 * x];
+        }
     };
     auto load_v = [&](int64_t b) {
-        const uint8_t* p = a.c.v + b * BB + g * HD * 8 * E;
+        const uint4* p = reinterpret_cast<const uint4*>(a.c.v + b * BB + g * HD * 8 * E) + n;
+        if (ONCE) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) vr[i] = ld_nt16(reinterpret_cast<const uint4*>(p + (16 * i + n) * 16));
+            for (int i = 0; i < NV; ++i) vr[i] = ld_nt16(p + 16 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) vr[i] = p[16 * i];
+        }
     };
     auto load_s = [&](int64_t b) {
         const float4* p = reinterpret_cast<const float4*>(a.c.s + b * kKvScales + g * 16);
@@ -435,6 +453,14 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // exponentials of the one between. The codes of the key block after those are
 // on their way into registers. The V scales are staged as s_j 2^-E already,
 // with the factor by which E moved.
+// 2048 tokens of 32 heads over 16384 int8 keys: 972 us, 1060 TFLOP/s of two-term
+// products, where an fp16 library product of 8192^3 reaches 1155. The matrix
+// unit is busy half of the cycles and the vector unit's issue the other half;
+// without the exponentials it would take 0.79 of that, without the products
+// 0.80. A prompt of 2047 tokens: 99 us, for half of which the longest tile runs
+// alone on its CU. Tried and dropped: two groups of four waves half a tile
+// apart, or on halves of the keys; a barrier every second step; both blocks'
+// keys in steps of 64.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
@@ -782,6 +808,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 
 // The key ranges of one (token, head) row joined: the ranges' maxima and sums
 // weigh their partial rows, added in the order of the ranges by four waves.
+// 3 us for one token's 32 rows of 10 ranges: a launch.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
     constexpr int LD = HD + 4, W = HD / 64;
@@ -838,7 +865,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
 // a window of 512 96 / 54; head_dim 64, 1900 over 1900 76 / 91. Of a batch, the
 // tile kernel takes the sequences of more than kFewRows rows.
 KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
-    if (!n_seqs || !n_tokens) return {false, 1};
+    if (!n_seqs || !n_tokens) return {false, false, 1};
     const int64_t G = n_heads / c.n_kv, rows = n_tokens * G;
     const int64_t most_q = max_q ? std::min(max_q, n_tokens) : (n_tokens + n_seqs - 1) / n_seqs;
     const int64_t width = int64_t(max_pages) << c.page_shift;
@@ -864,12 +891,12 @@ KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, in
         const double block_bytes = 64.0 * c.hd * kv_code_bytes(c.type);
         if (last(16) * block_bytes > 2e6)  // more than stays in an L2
             row = std::max(row, double(t16) * (last(16) - causal) * block_bytes / 11e6);
-        if (tile < row) return {true, int(s128)};
+        if (tile < row) return {true, false, int(s128)};
     }
     // Row kernel: two blocks a CU; more ranges cost their join more than they gain: a block takes a key
     // block in about 1 us / 4, a range adds 0.15 us (8192 keys, one token: 8 / 16 / 64 ranges 18.7 / 15.1 / 21.6 us).
     const int64_t best = int64_t(std::sqrt(1.6 * double(blocks)) + 0.5);
-    return {false, int(std::max<int64_t>(1, std::min<int64_t>({768 / t16, best, kMaxSplits})))};
+    return {false, most_q * G <= 16, int(std::max<int64_t>(1, std::min<int64_t>({768 / t16, best, kMaxSplits})))};
 }
 
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits) {
@@ -890,10 +917,13 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
     if (few) {
         const int64_t tiles = (rows + 15) / 16 + a.n_seqs;
         const int most = many ? kFewRows : INT32_MAX;
+        auto rows_go = [&](auto once, auto again) { a.once ? go(once, tiles, most) : go(again, tiles, most); };
         if (a.c.hd == 128)
-            f16 ? go(k_kv_attn_rows<128, WV_KV_F16>, tiles, most) : go(k_kv_attn_rows<128, WV_KV_Q8>, tiles, most);
+            f16 ? rows_go(k_kv_attn_rows<128, WV_KV_F16, true>, k_kv_attn_rows<128, WV_KV_F16, false>)
+                : rows_go(k_kv_attn_rows<128, WV_KV_Q8, true>, k_kv_attn_rows<128, WV_KV_Q8, false>);
         else
-            f16 ? go(k_kv_attn_rows<64, WV_KV_F16>, tiles, most) : go(k_kv_attn_rows<64, WV_KV_Q8>, tiles, most);
+            f16 ? rows_go(k_kv_attn_rows<64, WV_KV_F16, true>, k_kv_attn_rows<64, WV_KV_F16, false>)
+                : rows_go(k_kv_attn_rows<64, WV_KV_Q8, true>, k_kv_attn_rows<64, WV_KV_Q8, false>);
     }
     if (many) {
         const int64_t tiles = (rows + 127) / 128 + a.n_seqs;
@@ -983,7 +1013,7 @@ int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch* batch,
     a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages, a.max_q = batch->max_q;
     a.n_heads = n_heads, a.window = std::min(window, 1 << 30), a.scale = scale;
     const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, n_heads, a.window);
-    a.splits = plan.splits, a.many = plan.many;
+    a.splits = plan.splits, a.many = plan.many, a.once = plan.once;
     const size_t floats = kv_attn_part_floats(a.c, a.n_tokens, n_heads, a.splits);
     RtScratch sc;
     if (d_scratch) {
