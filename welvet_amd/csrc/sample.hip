@@ -12,8 +12,9 @@
 // it by segments of 1024 tokens, each some 20 instructions a logit; and the
 // steps between them, which one block after the other waits for. Rows of up to
 // 32768 logits stay in LDS meanwhile (256 rows of 32000: greedy 8.9 us, top-k
-// of 40 17, top-p 30, no filter 20). Of larger ones with few rows each is cut
-// over several blocks, below (64 of 128000: top-p 47 us, by whole rows 101).
+// of 40 17, top-p 30, top-k of 400 and top-p 37, no filter 20). Of larger ones,
+// where rows are few, each is cut over several blocks, below (64 of 128000:
+// top-p 47 us, by whole rows 101).
 // The loops stay small: with the row in registers, unrolled, instruction fetch
 // took most of the time (greedy, one row of 32000: 23 us, from LDS 5).
 #include <algorithm>
@@ -616,17 +617,20 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
     }
 
     u64 cut = 0;  // the last token kept, 0: all
-    bool summed = false;
+    bool ready = false, summed = false;
 #pragma unroll 1
     for (int mass = 0; mass < 2; ++mass) {  // top-k by counts, then top-p by weights
         if (!(mass ? set.by_p : set.by_k)) continue;
-        clear_hist(s);
-        row.each([&](float l, int i) {
-            const float x = log_weight(c, l);
-            if (l > -INFINITY && token_key(l, i) >= cut)
-                atomicAdd(&s.hist[bin_of(x)], mass ? fixed(__builtin_amdgcn_exp2f(x)) : u64(1));
-        });
-        __syncthreads();
+        auto histogram = [&] {
+            clear_hist(s);
+            row.each([&](float l, int i) {
+                const float x = log_weight(c, l);
+                if (l > -INFINITY && token_key(l, i) >= cut)
+                    atomicAdd(&s.hist[bin_of(x)], mass ? fixed(__builtin_amdgcn_exp2f(x)) : u64(1));
+            });
+            __syncthreads();
+        };
+        if (!ready) histogram();
         u64 target = u64(set.top_k);
         if (mass) {
             const u64 whole = find_in(s, s.hist, kBins, ~u64(0));
@@ -655,6 +659,45 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
                 break;
             }
             __syncthreads();
+        } else {  // top-k in front of top-p: the weights' histogram in the pass that collects the cut's bin
+            find_in(s, s.hist, kBins, target);
+            const int bin = s.at;
+            const u64 left = target - s.sum;
+            __syncthreads();
+            if (bin >= 0) {
+                clear_hist(s);
+                row.each([&](float l, int i) {
+                    const float x = log_weight(c, l);
+                    const int at_bin = bin_of(x);
+                    if (at_bin > bin || l == -INFINITY) return;
+                    const u64 w = fixed(__builtin_amdgcn_exp2f(x));
+                    if (at_bin < bin) {
+                        atomicAdd(&s.hist[at_bin], w);
+                    } else if (const int at = atomicAdd(&s.n, 1); at < kList) {
+                        s.list[at] = token_key(l, i);
+                        s.weights[at] = w;
+                    }
+                });
+                __syncthreads();
+                const int n = s.n;
+                if (n <= kList) {
+                    if (t < n) {
+                        u64 before;
+                        int rank;
+                        rank_list(s, n, s.list[t], rank, before);
+                        if (u64(rank) < left) atomicAdd(&s.hist[bin], s.weights[t]);
+                        if (u64(rank) + 1 == left) s.key = s.list[t];
+                    }
+                    __syncthreads();
+                    cut = s.key;
+                    ready = true;
+                    if (t == 0) s.n = 0;
+                    __syncthreads();
+                    continue;
+                }
+                __syncthreads();
+                histogram();
+            }
         }
         cut = find_cut(s, row, c, cut, target, mass != 0);
         __syncthreads();
