@@ -11,7 +11,8 @@
 // top-k); a pass that collects the cut's bin and sums what is kept in front of
 // it by segments of 1024 tokens, each some 20 instructions a logit; and the
 // steps between them, which one block after the other waits for. Rows of up to
-// 32768 logits stay in LDS meanwhile (256 rows of 32000: greedy 8.9 us, top-k
+// 32768 logits stay in LDS meanwhile, those of up to 4096 and 8192 dealt out so
+// that all waves have some (10 rows of 1530, top-k of 400 and top-p: 21 to 13 us) (256 rows of 32000: greedy 8.9 us, top-k
 // of 40 17, top-p 30, top-k of 400 and top-p 37, no filter 20). Of larger ones,
 // where rows are few, each is cut over several blocks, below (64 of 128000:
 // top-p 47 us, by whole rows 101).
@@ -41,6 +42,10 @@ constexpr int kTurn = 4 * kPass;    // tokens of four passes
 constexpr int kMaxVocab = 1 << 19;  // 2^19 weights of at most 2^44 stay below 2^63
 constexpr int kSegments = kMaxVocab / kSegment;
 constexpr int kResident = 32768;    // logits of a row that stay in LDS
+// Where a row lies: in memory, read in every pass; or in LDS, of so many passes
+// at most that a turn takes them all, or of up to kResident logits.
+enum { kStream, kLong, kTwo, kOne };
+constexpr int row_floats(int R) { return R == kLong ? kResident : R == kTwo ? 2 * kPass : R == kOne ? kPass : 4; }
 
 // Order-preserving integer of a float (NaN does not occur).
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -93,13 +98,13 @@ __device__ __forceinline__ u64 last_lane(u64 v) {
     return u64(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), 63))) << 32 | lo;
 }
 
-template <bool RESIDENT>
+template <int R>
 struct Shared {
-    float row[RESIDENT ? kResident : 4];
+    float row[row_floats(R)];
     u64 hist[kBins];
     u64 list[kList];
     u64 weights[kList];
-    u64 seg[RESIDENT ? kResident / kSegment : kSegments];
+    u64 seg[R != kStream ? kResident / kSegment : kSegments];
     u64 part[kWaves];
     u64 key;   // a result of one thread for all
     u64 sum;
@@ -108,9 +113,9 @@ struct Shared {
 
 // One row, read from memory once where it fits LDS, else in every pass.
 // each4(f): f(four logits, index of the first, pass) for this thread's ones;
-// in four passes (a turn) a wave meets 1024 consecutive tokens in order, 256
-// a pass. NaN and what lies behind the row are -inf, which no step counts.
-template <bool RESIDENT>
+// in a turn (four passes; for short rows two or one) a wave meets a segment,
+// 1024 (512, 256) consecutive tokens in order, 256 a pass. NaN and what lies behind the row are -inf, which no step counts.
+template <int R>
 struct Row {
     const float* p;
     float* lds;
@@ -137,10 +142,19 @@ struct Row {
         x.w = fmaxf(x.w, -INFINITY);
         return x;
     }
+    // log2 of a turn's passes; a segment is 256 tokens times them. Short rows spread over all waves.
+    static constexpr __device__ int lg() { return R == kOne ? 0 : R == kTwo ? 1 : 2; }
+    static constexpr __device__ int segment() { return 256 << lg(); }
+    __device__ __forceinline__ int segments() const { return (vocab + segment() - 1) >> (8 + lg()); }
+    __device__ __forceinline__ bool ends_segment(int k) const { return (k & ((1 << lg()) - 1)) == (1 << lg()) - 1; }
     // Whole turns.
-    __device__ __forceinline__ int passes() const { return (vocab + kTurn - 1) / kTurn * 4; }
-    static __device__ __forceinline__ int index(int k) {
-        return (k >> 2) * kTurn + int(threadIdx.x >> 6) * kSegment + (k & 3) * 256 + 4 * int(threadIdx.x & 63);
+    __device__ __forceinline__ int passes() const { return (vocab + (kPass << lg()) - 1) / (kPass << lg()) << lg(); }
+    // Where the wave's segment of pass k begins.
+    __device__ __forceinline__ int begin(int k) const {
+        return (k >> lg()) * (kPass << lg()) + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)) * segment();
+    }
+    __device__ __forceinline__ int index(int k) const {
+        return begin(k) + (k & ((1 << lg()) - 1)) * 256 + 4 * int(threadIdx.x & 63);
     }
     // Passes k0 .. k1 - 1 from memory, four passes' loads on their way.
     template <class F>
@@ -162,12 +176,13 @@ struct Row {
     // The first pass over the row, which fills LDS.
     template <class F>
     __device__ __forceinline__ void first(F f) const {
-        if constexpr (RESIDENT) {
-            float4 x[kResident / kPass];
+        if constexpr (R != kStream) {
+            float4 x[row_floats(R) / kPass];
 #pragma unroll
-            for (int k = 0; k < kResident / kPass; ++k) x[k] = fetch(index(k));
+            for (int k = 0; k < row_floats(R) / kPass; ++k) x[k] = fetch(index(k));
 #pragma unroll
-            for (int k = 0; k < kResident / kPass; ++k) {
+            for (int k = 0; k < row_floats(R) / kPass; ++k) {
+                if (begin(k) >= vocab) continue;
                 x[k] = clean(x[k]);
                 *reinterpret_cast<float4*>(lds + index(k)) = x[k];
                 f(x[k], index(k), k);
@@ -178,9 +193,12 @@ struct Row {
     }
     template <class F>
     __device__ __forceinline__ void each4(F f) const {
-        if constexpr (RESIDENT) {
+        if constexpr (R != kStream) {
             const int n = passes();
-            for (int k = 0; k < n; ++k) f(*reinterpret_cast<const float4*>(lds + index(k)), index(k), k);
+            for (int k = 0; k < n; ++k) {
+                if (begin(k) >= vocab) continue;  // nor the rest of the segment
+                f(*reinterpret_cast<const float4*>(lds + index(k)), index(k), k);
+            }
         } else {
             stream(f);
         }
@@ -196,12 +214,12 @@ struct Row {
     }
     // Four logits from index i (a multiple of 4) on.
     __device__ __forceinline__ float4 at(int i) const {
-        if constexpr (RESIDENT) return *reinterpret_cast<const float4*>(lds + i);
+        if constexpr (R != kStream) return *reinterpret_cast<const float4*>(lds + i);
         return clean(fetch(i));
     }
 };
 
-template <bool R>
+template <int R>
 __device__ __forceinline__ void clear_hist(Shared<R>& s) {
 #pragma unroll
     for (int i = 0; i < kBins / kThreads; ++i) s.hist[threadIdx.x + i * kThreads] = 0;
@@ -212,7 +230,7 @@ __device__ __forceinline__ void clear_hist(Shared<R>& s) {
 // v[0 .. n) (n at most 2 * 1024) added up in order: the index where the sum
 // reaches `target` (> 0) into s.at, the sum in front of it into s.sum, and the
 // whole sum returned. s.at is -1 where the whole is less.
-template <bool R>
+template <int R>
 __device__ __forceinline__ u64 find_in(Shared<R>& s, const u64* v, int n, u64 target) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     if (t == 0) s.at = -1;
@@ -238,15 +256,15 @@ __device__ __forceinline__ u64 find_in(Shared<R>& s, const u64* v, int n, u64 ta
 }
 
 // Where tokens of one logit l share the cut: the `nth` (from 1) of them by index.
-template <bool R>
+template <int R>
 __device__ __forceinline__ u64 nth_equal(Shared<R>& s, const Row<R>& row, float l, u64 nth) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int segs = (row.vocab + kSegment - 1) / kSegment;
+    const int segs = row.segments();
     int c = 0;
     row.each4([&](float4 x, int, int k) {
         c += (x.x == l) + (x.y == l) + (x.z == l) + (x.w == l);
-        if ((k & 3) == 3) {
-            const int n = wave_total_i(c), sg = (k >> 2) * kWaves + wave;
+        if (row.ends_segment(k)) {
+            const int n = wave_total_i(c), sg = (k >> row.lg()) * kWaves + wave;
             if (lane == 0 && sg < segs) s.seg[sg] = u64(n);
             c = 0;
         }
@@ -257,8 +275,8 @@ __device__ __forceinline__ u64 nth_equal(Shared<R>& s, const Row<R>& row, float 
     const u64 want = nth - s.sum;
     if (wave == 0) {
         u64 before = 0;
-        for (int q = 0; q < 4; ++q) {
-            const int i = sg * kSegment + q * 256 + 4 * lane;
+        for (int q = 0; q < 1 << row.lg(); ++q) {
+            const int i = sg * row.segment() + q * 256 + 4 * lane;
             const float4 x = row.at(i);
             const float v[4] = {x.x, x.y, x.z, x.w};
             u64 n = 0;
@@ -278,7 +296,7 @@ __device__ __forceinline__ u64 nth_equal(Shared<R>& s, const Row<R>& row, float 
 
 // Ranks the n tokens of the list, one per thread: how many of them, and how
 // much weight, come before this thread's in the tokens' order.
-template <bool R>
+template <int R>
 __device__ __forceinline__ void rank_list(const Shared<R>& s, int n, u64 key, int& rank, u64& mass) {
     rank = 0;
     mass = 0;
@@ -293,7 +311,7 @@ __device__ __forceinline__ void rank_list(const Shared<R>& s, int n, u64 key, in
 // The cut that keeps, of the tokens down to `floor` (0: all), the first
 // `target` (by_mass: the shortest prefix whose weights reach target); floor
 // where there are not as many. s.hist holds their counts (weights) by bin.
-template <bool R>
+template <int R>
 __device__ __forceinline__ u64 find_cut(Shared<R>& s, const Row<R>& row, const Scale& c, u64 floor, u64 target,
                                      bool by_mass) {
     find_in(s, s.hist, kBins, target);
@@ -419,10 +437,10 @@ __device__ __forceinline__ u64 segment_sum(double v) { return last_lane(wave_sca
 
 // The place of u among s.seg, the kept weights of each segment, and in the
 // segment where it lies.
-template <bool R>
+template <int R>
 __device__ __forceinline__ void pick(const SampleArgs& a, Shared<R>& s, const Row<R>& row, int r, const Kept& kept,
                                      float u) {
-    const int segs = (a.vocab + kSegment - 1) / kSegment, lane = threadIdx.x & 63;
+    const int segs = row.segments(), lane = threadIdx.x & 63;
     const u64 total = find_in(s, s.seg, segs, ~u64(0));
     const u64 want = u64(double(u) * double(total));
     find_in(s, s.seg, segs, want + 1);
@@ -430,9 +448,10 @@ __device__ __forceinline__ void pick(const SampleArgs& a, Shared<R>& s, const Ro
         u64 at = s.sum;
         float4 x[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) x[q] = row.at(s.at * kSegment + q * 256 + 4 * lane);
-        for (int q = 0; q < 4; ++q) {
-            const int i = s.at * kSegment + q * 256 + 4 * lane;
+        for (int q = 0; q < 4; ++q)
+            if (q < 1 << row.lg()) x[q] = row.at(s.at * row.segment() + q * 256 + 4 * lane);
+        for (int q = 0; q < 1 << row.lg(); ++q) {
+            const int i = s.at * row.segment() + q * 256 + 4 * lane;
             const float y[4] = {x[0].x, x[0].y, x[0].z, x[0].w};
             x[0] = x[1], x[1] = x[2], x[2] = x[3];
             u64 v[4];
@@ -452,7 +471,7 @@ __device__ __forceinline__ void pick(const SampleArgs& a, Shared<R>& s, const Ro
 }
 
 // The draw among the n tokens of the list, which holds the top_k at least.
-template <bool R>
+template <int R>
 __device__ __forceinline__ void pick_from_list(const SampleArgs& a, Shared<R>& s, int r, const Settings& x,
                                                const Scale& c, int n) {
     const int t = threadIdx.x;
@@ -487,7 +506,7 @@ __device__ __forceinline__ void pick_from_list(const SampleArgs& a, Shared<R>& s
 // What a cut in `bin` (kBins: none) does with the tokens from key `floor` on:
 // those of the bin (`few`: down to its end) go into the list, the weights of
 // those in front of it, from min_p on, come back for their segment's sum.
-template <bool FLOOR, bool R>
+template <bool FLOOR, int R>
 struct Visit {
     Shared<R>& s;
     const Scale& c;
@@ -519,24 +538,25 @@ struct Visit {
 };
 // Adds a pass's weights up and leaves the sum of a segment with its last pass.
 // A segment's weights of at most 1 are steps of 2^-44 and so are a thread's sums of 16.
+template <int R>
 struct SegmentSum {
+    const Row<R>& row;
     u64* seg;
-    int segs;
     double sum = 0.0;
-    __device__ __forceinline__ SegmentSum(u64* seg, int vocab) : seg(seg), segs((vocab + kSegment - 1) / kSegment) {}
+    __device__ __forceinline__ SegmentSum(const Row<R>& row, u64* seg) : row(row), seg(seg) {}
     __device__ __forceinline__ void operator()(double v, int k) {
         sum += v;
-        if ((k & 3) != 3) return;
+        if (!row.ends_segment(k)) return;
         const u64 all = segment_sum(sum);
-        const int sg = (k >> 2) * kWaves + int(threadIdx.x >> 6);
-        if ((threadIdx.x & 63) == 0 && sg < segs) seg[sg] = all;
+        const int sg = (k >> row.lg()) * kWaves + int(threadIdx.x >> 6);
+        if ((threadIdx.x & 63) == 0 && sg < row.segments()) seg[sg] = all;
         sum = 0.0;
     }
 };
 // The cut among the n tokens of the bin's list, where `left` is what it keeps
 // of them: into s.key; what it keeps, from min_p on, into their segments.
-template <bool R>
-__device__ __forceinline__ void cut_list(Shared<R>& s, const Scale& c, int n, u64 left, bool by_mass, float min_p) {
+template <int R>
+__device__ __forceinline__ void cut_list(Shared<R>& s, const Row<R>& row, const Scale& c, int n, u64 left, bool by_mass, float min_p) {
     const int t = threadIdx.x;
     u64 key = 0, mass = 0, w = 0;
     int rank = 0;
@@ -547,12 +567,12 @@ __device__ __forceinline__ void cut_list(Shared<R>& s, const Scale& c, int n, u6
     }
     __syncthreads();
     if (t < n && key >= s.key && weight(c, key_logit(key)) >= min_p)
-        atomicAdd(&s.seg[int(~uint32_t(key)) / kSegment], w);
+        atomicAdd(&s.seg[int(~uint32_t(key)) >> (8 + row.lg())], w);
     __syncthreads();
 }
 
 // A whole row by one block.
-template <bool R>
+template <int R>
 __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, int r) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const Row<R> row{a.logits + int64_t(r) * a.stride, s.row, a.vocab};
@@ -642,7 +662,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
             const u64 left = target - s.sum;
             __syncthreads();
             if (t == 0) s.key = cut;
-            SegmentSum sums(s.seg, a.vocab);
+            SegmentSum<R> sums(row, s.seg);
             if (cut) {
                 const Visit<true, R> visit(s, c, cut, set.min_p, bin, false);
                 row.each4([&](float4 x, int i, int k) { sums(visit.four(x, i), k); });
@@ -653,7 +673,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
             __syncthreads();
             const int n = s.n;
             if (n <= kList) {
-                if (n) cut_list(s, c, n, left, mass != 0, set.min_p);
+                if (n) cut_list(s, row, c, n, left, mass != 0, set.min_p);
                 cut = s.key;
                 summed = true;
                 break;
@@ -705,7 +725,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
     // the kept weights of each segment, then the place of u among them
     const Kept kept(c, cut, set.min_p);
     if (!summed) {
-        SegmentSum sums(s.seg, a.vocab);
+        SegmentSum<R> sums(row, s.seg);
         row.each4([&](float4 x, int i, int k) {
             sums((kept(x.x, i) + kept(x.y, i + 1)) + (kept(x.z, i + 2) + kept(x.w, i + 3)), k);
         });
@@ -714,7 +734,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, Shared<R>& s, in
     pick(a, s, row, r, kept, set.u);
 }
 
-template <bool R>
+template <int R>
 __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     sample_row(a, *reinterpret_cast<Shared<R>*>(raw), blockIdx.x);
@@ -758,7 +778,7 @@ __device__ __forceinline__ bool sliced(const Settings& x) { return !(x.by_k && x
 __global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p) {
     __shared__ float part[kWaves];
     const int r = blockIdx.y, sl = blockIdx.x;
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
+    const Row<kStream> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     float top = -INFINITY;
     row.range(sl * p.passes, min((sl + 1) * p.passes, row.passes()),
               [&](float4 x, int, int) { top = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), top); });
@@ -776,7 +796,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p) 
 __global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p) {
     __shared__ u64 hist[kBins];
     const int r = blockIdx.y, sl = blockIdx.x;
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
+    const Row<kStream> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
     const Settings set = settings(a, r);
     const float max = row_max(p, r);
@@ -802,10 +822,10 @@ __global__ void __launch_bounds__(kThreads) k_slice_hist(SampleArgs a, Slices p)
 
 __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices p) {
     extern __shared__ __align__(16) uint8_t raw[];
-    Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
+    Shared<kStream>& s = *reinterpret_cast<Shared<kStream>*>(raw);
     const int r = blockIdx.y, sl = blockIdx.x, t = threadIdx.x;
     SliceRow& g = p.rows[r];
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
+    const Row<kStream> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     const int k0 = sl * p.passes, k1 = min((sl + 1) * p.passes, row.passes());
     const Settings set = settings(a, r);
     const float max = row_max(p, r);
@@ -842,8 +862,8 @@ __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices
     const bool few = set.by_k && set.top_k <= kFewK;
     if (t == 0) s.n = 0;
     __syncthreads();
-    const Visit<false, false> visit(s, c, 0, set.min_p, bin, few);
-    SegmentSum sums(g.seg, a.vocab);
+    const Visit<false, kStream> visit(s, c, 0, set.min_p, bin, few);
+    SegmentSum<kStream> sums(row, g.seg);
     row.range(k0, k1, [&](float4 x, int i, int k) { sums(visit.four(x, i), k); });
     __syncthreads();
     const int n = s.n;  // this slice's share of the row's list
@@ -855,7 +875,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices
 
 __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices p) {
     extern __shared__ __align__(16) uint8_t raw[];
-    Shared<false>& s = *reinterpret_cast<Shared<false>*>(raw);
+    Shared<kStream>& s = *reinterpret_cast<Shared<kStream>*>(raw);
     const int r = blockIdx.x, t = threadIdx.x;
     static_assert(kSegments <= kThreads, "a segment to a thread");
     const SliceRow& g = p.rows[r];
@@ -879,8 +899,8 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
     if (t == 0) s.key = 0;
     __syncthreads();
     if (set.by_k && set.top_k <= kFewK) return pick_from_list(a, s, r, set, c, n);
-    if (n) cut_list(s, c, n, left, !set.by_k, set.min_p);
-    const Row<false> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
+    const Row<kStream> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
+    if (n) cut_list(s, row, c, n, left, !set.by_k, set.min_p);
     pick(a, s, row, r, Kept(c, s.key, set.min_p), set.u);
 }
 
@@ -909,18 +929,22 @@ int launch_sample(const SampleArgs& a, hipStream_t s, float* scratch) {
         const dim3 grid{unsigned(n), unsigned(a.rows)};
         hipLaunchKernelGGL(k_slice_max, grid, dim3(kThreads), 0, s, a, p);
         hipLaunchKernelGGL(k_slice_hist, grid, dim3(kThreads), 0, s, a, p);
-        hipLaunchKernelGGL(k_slice_collect, grid, dim3(kThreads), unsigned(sizeof(Shared<false>)), s, a, p);
-        hipLaunchKernelGGL(k_slice_finish, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(sizeof(Shared<false>)), s,
+        hipLaunchKernelGGL(k_slice_collect, grid, dim3(kThreads), unsigned(sizeof(Shared<kStream>)), s, a, p);
+        hipLaunchKernelGGL(k_slice_finish, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(sizeof(Shared<kStream>)), s,
                            a, p);
         return int(hipGetLastError());
     }
     auto go = [&](auto kern, size_t lds) {
         hipLaunchKernelGGL(kern, dim3(unsigned(a.rows)), dim3(kThreads), unsigned(lds), s, a);
     };
-    if (a.vocab <= kResident)
-        go(k_sample<true>, sizeof(Shared<true>));
+    if (a.vocab <= row_floats(kOne))
+        go(k_sample<kOne>, sizeof(Shared<kOne>));
+    else if (a.vocab <= row_floats(kTwo))
+        go(k_sample<kTwo>, sizeof(Shared<kTwo>));
+    else if (a.vocab <= kResident)
+        go(k_sample<kLong>, sizeof(Shared<kLong>));
     else
-        go(k_sample<false>, sizeof(Shared<false>));
+        go(k_sample<kStream>, sizeof(Shared<kStream>));
     return int(hipGetLastError());
 }
 
