@@ -11,11 +11,11 @@
 // top-k); a pass that collects the cut's bin and sums what is kept in front of
 // it by segments of 1024 tokens, each some 20 instructions a logit; and the
 // steps between them, which one block after the other waits for. Rows of up to
-// 32768 logits stay in LDS meanwhile, those of up to 4096 and 8192 dealt out so
-// that all waves have some (10 rows of 1530, top-k of 400 and top-p: 21 to 13 us) (256 rows of 32000: greedy 8.9 us, top-k
-// of 40 17, top-p 30, top-k of 400 and top-p 37, no filter 20). Of larger ones,
-// where rows are few, each is cut over several blocks, below (64 of 128000:
-// top-p 47 us, by whole rows 101).
+// 32768 logits stay in LDS meanwhile (256 rows of 32000: greedy 8.9 us, top-k
+// of 40 17, top-p 30, top-k of 400 and top-p 37, no filter 20), those of up to
+// 4096 and 8192 dealt out so that all waves have some (10 of 1530, top-k of 400
+// and top-p: 21 to 13 us). Of larger ones, where rows are few, each is cut over
+// several blocks, below (64 of 128000: top-p 47 us, by whole rows 101).
 // The loops stay small: with the row in registers, unrolled, instruction fetch
 // took most of the time (greedy, one row of 32000: 23 us, from LDS 5).
 #include <algorithm>
@@ -182,7 +182,6 @@ struct Row {
             for (int k = 0; k < row_floats(R) / kPass; ++k) x[k] = fetch(index(k));
 #pragma unroll
             for (int k = 0; k < row_floats(R) / kPass; ++k) {
-                if (begin(k) >= vocab) continue;
                 x[k] = clean(x[k]);
                 *reinterpret_cast<float4*>(lds + index(k)) = x[k];
                 f(x[k], index(k), k);
@@ -194,11 +193,9 @@ struct Row {
     template <class F>
     __device__ __forceinline__ void each4(F f) const {
         if constexpr (R != kStream) {
-            const int n = passes();
-            for (int k = 0; k < n; ++k) {
-                if (begin(k) >= vocab) continue;  // nor the rest of the segment
-                f(*reinterpret_cast<const float4*>(lds + index(k)), index(k), k);
-            }
+            // as far as the wave has segments of the row
+            const int n = (vocab - begin(0) + (kPass << lg()) - 1) / (kPass << lg()) << lg();
+            for (int k = 0; k < n; ++k) f(*reinterpret_cast<const float4*>(lds + index(k)), index(k), k);
         } else {
             stream(f);
         }
