@@ -178,6 +178,18 @@ def test_masked_and_non_finite():
         assert tok[3] % 2 == 1 and tok[4] % 7 != 5 and tok[5] in (77, 1300) and tok[7] >= 1990
 
 
+@pytest.mark.parametrize("v", [70, 6000, 20000, 33000, 150000])
+@pytest.mark.parametrize("s", [dict(k=40), dict(k=40, p=0.9), dict(k=500), dict(k=500, p=0.9), dict(p=0.9), dict()])
+def test_few_unmasked(v, s):
+    """Fewer tokens that are not -inf than top_k asks for, one alone among them."""
+    rng = np.random.default_rng(v)
+    l = np.full((7, v), -np.inf, np.float32)
+    for r, n in enumerate((1, 2, 5, 17, 30, 39, 40)):
+        at = rng.permutation(v)[:n]
+        l[r, at] = logits(rng, 1, n)[0]
+    check(l, t=0.9, u=rng.random(7, np.float32), **s)
+
+
 def test_settings_out_of_range():
     rng = np.random.default_rng(6)
     l = logits(rng, 10, 777)

@@ -513,7 +513,7 @@ struct Visit {
         : s(s), c(c), floor(floor), min_p(min_p) {
         front = bin < kBins ? float(bin) : INFINITY;
         lo = few ? -1.0f : front;
-        hi = bin < kBins - 1 ? float(bin + 1) : bin < kBins ? INFINITY : -1.0f;
+        hi = bin < kBins - 1 ? float(bin + 1) : bin < kBins || few ? INFINITY : -1.0f;
     }
     __device__ __forceinline__ double operator()(float l, int i) const {
         const float x = log_weight(c, l), y = -x * kPerUnit;
