@@ -893,10 +893,18 @@ KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, in
             row = std::max(row, double(t16) * (last(16) - causal) * block_bytes / 11e6);
         if (tile < row) return {true, false, int(s128)};
     }
-    // Row kernel: two blocks a CU; more ranges cost their join more than they gain: a block takes a key
-    // block in about 1 us / 4, a range adds 0.15 us (8192 keys, one token: 8 / 16 / 64 ranges 18.7 / 15.1 / 21.6 us).
+    // Row kernel: ranges for two blocks a CU; more cost their join more than they gain (8192 keys, one token:
+    // 8 / 16 / 64 ranges 18.7 / 15.1 / 21.6 us). Its waves take four key blocks at a time, in 1.1 to 1.6 us, or
+    // what the bytes take of sequences half as long as the longest; ranges add a launch of 4.5 us. One token,
+    // 32 heads over 8, without and with ranges: 100 keys 6.3 / 11.1 us, 500 9.3 / 11.0, 1000 13.7 / 12.4, 2048
+    // 22.1 / 12.6; 48 tokens of 2048 keys each 41.5 / 43.6.
+    const double block_us = 64.0 * c.hd * kv_code_bytes(c.type) * double(seqs * c.n_kv) / 5.2e6;
+    const auto walk = [&](int64_t n) {
+        return std::max(double(blocks) / (4.0 * double(n)) * (c.hd == 128 ? 1.5 : 1.1), 0.5 * double(blocks) * block_us);
+    };
     const int64_t best = int64_t(std::sqrt(1.6 * double(blocks)) + 0.5);
-    return {false, most_q * G <= 16, int(std::max<int64_t>(1, std::min<int64_t>({768 / t16, best, kMaxSplits})))};
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({768 / t16, best, blocks / 4, kMaxSplits}));
+    return {false, most_q * G <= 16, walk(1) <= walk(n) + 4.5 + 0.15 * double(n) ? 1 : int(n)};
 }
 
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits) {
