@@ -370,6 +370,21 @@ def test_many_rows_ragged_batch(typ, window):
 
 
 @pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("new", [6, 1900])
+def test_more_tokens_than_keys_and_short_tables(typ, new):
+    """A sequence whose first tokens stand in front of the keys, and one whose table ends before its keys do."""
+    rng = np.random.default_rng(new)
+    p = Pool(rng, [max(new // 2, 3)], 16, 64, 64, typ).fill()
+    out = p.attend([new], 64, max_q=new)
+    p.check(out, [new])
+    assert not out[:new - p.lens[0]].any()
+    p = Pool(rng, [new + 200], 16, 64, 64, typ).fill()
+    cut = (new + 150) // 64
+    present = [np.arange(new + 200) < 64 * cut]
+    p.check(p.attend([new], 64, max_q=new, table=p.table[:, :cut].copy()), [new], present=present)
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
 def test_many_rows_nan_and_magnitudes(typ):
     """NaN rows behind the keys and left of the window change nothing, a NaN key the rows that attend to it;
     V rows far above and below the others, scores of hundreds."""
