@@ -102,8 +102,8 @@ template <int R>
 struct Shared {
     float row[row_floats(R)];
     u64 hist[kBins];
-    u64 list[kList];
-    u64 weights[kList];
+    alignas(16) u64 list[kList];
+    alignas(16) u64 weights[kList];
     u64 seg[R != kStream ? kResident / kSegment : kSegments];
     u64 part[kWaves];
     u64 key;   // a result of one thread for all
@@ -297,11 +297,18 @@ template <int R>
 __device__ __forceinline__ void rank_list(const Shared<R>& s, int n, u64 key, int& rank, u64& mass) {
     rank = 0;
     mass = 0;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-        const bool b = s.list[j] > key;
+    const ulonglong2* keys = reinterpret_cast<const ulonglong2*>(s.list);
+    const ulonglong2* weights = reinterpret_cast<const ulonglong2*>(s.weights);
+#pragma unroll 4
+    for (int j = 0; j < n / 2; ++j) {
+        const ulonglong2 k = keys[j], w = weights[j];
+        rank += (k.x > key) + (k.y > key);
+        mass += (k.x > key ? w.x : 0) + (k.y > key ? w.y : 0);
+    }
+    if (n & 1) {
+        const bool b = s.list[n - 1] > key;
         rank += b;
-        mass += b ? s.weights[j] : 0;
+        mass += b ? s.weights[n - 1] : 0;
     }
 }
 
@@ -489,13 +496,22 @@ __device__ __forceinline__ void pick_from_list(const SampleArgs& a, Shared<R>& s
     if (t < n) s.weights[t] = w;
     __syncthreads();
     u64 before = 0, total = 0;
-    if (t < n)
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) {
-            const u64 v = s.weights[j];
-            total += v;
-            if (uint32_t(s.list[j]) > uint32_t(key)) before += v;  // ~index: larger is earlier
+    if (t < n) {
+        const ulonglong2* keys = reinterpret_cast<const ulonglong2*>(s.list);
+        const ulonglong2* weights = reinterpret_cast<const ulonglong2*>(s.weights);
+        const uint32_t mine = uint32_t(key);  // ~index: larger is earlier
+#pragma unroll 4
+        for (int j = 0; j < n / 2; ++j) {
+            const ulonglong2 k = keys[j], v = weights[j];
+            total += v.x + v.y;
+            before += (uint32_t(k.x) > mine ? v.x : 0) + (uint32_t(k.y) > mine ? v.y : 0);
         }
+        if (n & 1) {
+            const u64 v = s.weights[n - 1];
+            total += v;
+            if (uint32_t(s.list[n - 1]) > mine) before += v;
+        }
+    }
     const u64 want = u64(double(x.u) * double(total));
     if (w && before <= want && want < before + w) put(a, r, int(~uint32_t(key)), float(double(w) / double(total)));
 }
@@ -745,8 +761,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a) {
 //   collect  the cut's bin from all slices' histograms; its tokens into the
 //            row's list, the weights of the bins in front of it by segment
 //   finish one block a row: the list's cut, and the place of u
-// Rows that do not fit this (both top_k > kFewK and top_p, a bin of more
-// tokens than the list takes) are done whole by the last launch. 64 rows of
+// Rows that do not fit this (top_p with a larger top_k than the list takes, a
+// bin of more tokens than that) are done whole by the last launch. 64 rows of
 // 128000 with top-p: 5.8, 11.9, 17.7 and 12.3 us; loading a pass's logits in
 // front of the wait for the maximum costs registers, and so a block a CU (25
 // for 17.7).
@@ -770,7 +786,9 @@ __device__ __forceinline__ float row_max(const Slices& p, int r) {
     const int lane = threadIdx.x & 63;
     return wave_maximum(lane < p.n ? p.rows[r].max[lane] : -INFINITY);
 }
-__device__ __forceinline__ bool sliced(const Settings& x) { return !(x.by_k && x.by_p && x.top_k > kFewK); }
+// The list takes all tokens down to the bin of the top-k cut, and the draw is among them.
+__device__ __forceinline__ bool few(const Settings& x) { return x.by_k && (x.top_k <= kFewK || (x.by_p && x.top_k <= kList)); }
+__device__ __forceinline__ bool sliced(const Settings& x) { return !(x.by_k && x.by_p && x.top_k > kList); }
 
 __global__ void __launch_bounds__(kThreads) k_slice_max(SampleArgs a, Slices p) {
     __shared__ float part[kWaves];
@@ -855,11 +873,9 @@ __global__ void __launch_bounds__(kThreads) k_slice_collect(SampleArgs a, Slices
         if (s.at >= 0) bin = s.at;
         if (sl == 0 && t == 0) g.left = bin < kBins ? target - s.sum : 0;
     }
-    // few of top-k: the list takes all tokens down to the bin
-    const bool few = set.by_k && set.top_k <= kFewK;
     if (t == 0) s.n = 0;
     __syncthreads();
-    const Visit<false, kStream> visit(s, c, 0, set.min_p, bin, few);
+    const Visit<false, kStream> visit(s, c, 0, set.min_p, bin, few(set));
     SegmentSum<kStream> sums(row, g.seg);
     row.range(k0, k1, [&](float4 x, int i, int k) { sums(visit.four(x, i), k); });
     __syncthreads();
@@ -895,7 +911,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
     const u64 left = g.left;
     if (t == 0) s.key = 0;
     __syncthreads();
-    if (set.by_k && set.top_k <= kFewK) return pick_from_list(a, s, r, set, c, n);
+    if (few(set)) return pick_from_list(a, s, r, set, c, n);
     const Row<kStream> row{a.logits + int64_t(r) * a.stride, nullptr, a.vocab};
     if (n) cut_list(s, row, c, n, left, !set.by_k, set.min_p);
     pick(a, s, row, r, Kept(c, s.key, set.min_p), set.u);
