@@ -12,10 +12,10 @@
 // it by segments of 1024 tokens, each some 20 instructions a logit; and the
 // steps between them, which one block after the other waits for. Rows of up to
 // 32768 logits stay in LDS meanwhile (256 rows of 32000: greedy 8.9 us, top-k
-// of 40 17, top-p 30, top-k of 400 and top-p 37, no filter 20), those of up to
+// of 40 15, top-p 29, top-k of 400 and top-p 37, no filter 20), those of up to
 // 4096 and 8192 dealt out so that all waves have some (10 of 1530, top-k of 400
 // and top-p: 21 to 13 us). Of larger ones, where rows are few, each is cut over
-// several blocks, below (64 of 128000: top-p 47 us, by whole rows 101).
+// several blocks, below (64 of 128000: top-p 45 us, by whole rows 101).
 // The loops stay small: with the row in registers, unrolled, instruction fetch
 // took most of the time (greedy, one row of 32000: 23 us, from LDS 5).
 #include <algorithm>
@@ -292,7 +292,8 @@ __device__ __forceinline__ u64 nth_equal(Shared<R>& s, const Row<R>& row, float 
 }
 
 // Ranks the n tokens of the list, one per thread: how many of them, and how
-// much weight, come before this thread's in the tokens' order.
+// much weight, come before this thread's in the tokens' order. LDS reads bind:
+// some 20 us for 400 tokens, so that whole rows cut such a top-k by bins instead.
 template <int R>
 __device__ __forceinline__ void rank_list(const Shared<R>& s, int n, u64 key, int& rank, u64& mass) {
     rank = 0;
