@@ -460,6 +460,19 @@ def test_attention_graph_replays(scratch):
         p.check(eager, [1], scale=0.125, lens=[length])
 
 
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("max_q", [0, 1])
+def test_attention_one_chunk_among_tokens(typ, max_q):
+    """Many single tokens, idle sequences, and one or two chunks that the batch's average (or a max_q too small)
+    does not let expect."""
+    rng = np.random.default_rng(max_q + 77)
+    new = [1] * 30 + [0, 100, 1, 0, 0, 37] + [1] * 25
+    lens = [int(n) for n in rng.integers(1, 300, len(new))]
+    lens[31], lens[35] = 250, 37
+    p = Pool(rng, lens, 2, 64, 32, typ).fill()
+    p.check(p.attend(new, 4, max_q=max_q, pad=3), new)
+
+
 @pytest.mark.parametrize("new", [3, 600])
 def test_attention_of_zero_queries(new):
     """Queries of zeros and a scale that underflows: the plain mean of the values, the masked keys left out."""

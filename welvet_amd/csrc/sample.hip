@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a) {
 // for 17.7).
 // ---------------------------------------------------------------------------
 
-struct SliceRow {
+struct alignas(16) SliceRow {
     u64 key;   // greedy: the largest token
     int n;     // tokens of the list; over kList: more than it holds
     u64 left;  // what the cut keeps of its bin: tokens with top-k, weight with top-p
