@@ -190,8 +190,8 @@ __device__ __forceinline__ float row_unit(float amax, float& inv) {
 // operand of O^T += V^T P^T. The waves' sums meet in LDS. A single token's row
 // is bound by the codes' bytes: 64 sequences of 1 to 8192 int8 keys, 32 heads
 // over 8 of 128, 134 us, 5.2 TB/s; one of 131071 fp16 keys 106 us, 5.2 TB/s. A
-// short one by the chain of loads before its first product and by the join's
-// launch: 2048 int8 keys 8 + 3 us.
+// short one by a wave's chain from score to second product, 1.1 to 1.5 us a key
+// block, and by the join's launch: 2048 int8 keys 8 + 3 us.
 // ONCE: no other block reads a sequence's keys, and they are loaded past the
 // caches (131071 fp16 keys 106 us, else 112); not where several tiles read them
 // (64 tokens of 32 heads over 8000 fp16 keys 56 us so, else 43).
@@ -471,14 +471,14 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // exponentials of the one between. The codes of the key block after those are
 // on their way into registers. The V scales are staged as s_j 2^-E already,
 // with the factor by which E moved.
-// 2048 tokens of 32 heads over 16384 int8 keys: 972 us, 1060 TFLOP/s of two-term
-// products, where an fp16 library product of 8192^3 reaches 1155. The matrix
-// unit is busy half of the cycles and the vector unit's issue the other half;
-// without the exponentials it would take 0.79 of that, without the products
-// 0.80. A prompt of 2047 tokens: 99 us, for half of which the longest tile runs
-// alone on its CU. Tried and dropped: two groups of four waves half a tile
-// apart, or on halves of the keys; a barrier every second step; both blocks'
-// keys in steps of 64.
+// 2048 tokens of 32 heads over 16384 int8 keys: 970 to 1000 us across cards, up
+// to 1060 TFLOP/s of two-term products, where an fp16 library product of 8192^3
+// reaches 1155. The matrix unit is busy half of the cycles, the vector unit's
+// issue the other half; without the exponentials it would take 0.79 of that,
+// without the products 0.80. A prompt of 2047 tokens: 100 us, for half of which
+// the longest tile runs alone on its CU. Dropped, since they gained nothing: two
+// groups of four waves half a tile apart, or on halves of the keys; a barrier
+// every second step; steps of 64 keys.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
