@@ -154,6 +154,31 @@ def test_same_call_again_gives_the_same_bits():
     assert np.array_equal(out[0][0], out[1][0]) and np.array_equal(out[0][1], out[1][1])
 
 
+def test_follows_the_librarys_stream():
+    """Rows that calls without a stream still have to write when the forward is called are there for it."""
+    cfg = config()
+    s = Server(cfg, "Q4_K", "f16", 1)
+    s.step([np.random.default_rng(3).integers(0, cfg.vocab, 60)])
+    n = len(s.ids[0])
+    j = np.arange(n)
+    sl = torch.from_numpy(s.pages[0][j // s.page].astype(np.int64) * s.page + j % s.page).cuda()
+    rows = [[torch.zeros(n, cfg.kv_dim, device="cuda") for _ in range(2)] for _ in range(cfg.n_layers)]
+    zero, sink = torch.zeros(n, cfg.kv_dim, device="cuda"), torch.zeros(1 << 17, cfg.kv_dim, device="cuda")
+    every = torch.zeros(1 << 17, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    for L, (k, v) in enumerate(rows):
+        s.kv.read_dev(L, sl.data_ptr(), n, k.data_ptr(), v.data_ptr())
+    _, want = s.dec.forward_paged(s.kv, [[7]], [n], s.pages, want_logits=True)
+    for L in range(cfg.n_layers):
+        s.kv.write_dev(L, zero.data_ptr(), zero.data_ptr(), sl.data_ptr(), n)
+    for _ in range(50):  # some milliseconds of other work in front of the rows
+        s.kv.read_dev(0, every.data_ptr(), 1 << 17, sink.data_ptr(), sink.data_ptr())
+    for L, (k, v) in enumerate(rows):
+        s.kv.write_dev(L, k.data_ptr(), v.data_ptr(), sl.data_ptr(), n)
+    _, got = s.dec.forward_paged(s.kv, [[7]], [n], s.pages, want_logits=True)
+    assert np.array_equal(got, want)
+
+
 def test_refusals():
     cfg = config()
     s = Server(cfg, "Q4_K", "q8", 2, width=1)

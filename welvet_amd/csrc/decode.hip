@@ -2502,7 +2502,9 @@ int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const
                                   matvec_scratch_floats(d->lm, n_seqs), sample_scratch_floats(n_seqs, c.vocab)});
     rc = ensure_prefill(*d, n, more);
     if (rc) return rc;
-    hipError_t e = hipSuccess;
+    // what was enqueued on the library's stream may write the cache
+    hipError_t e = hipStreamSynchronize(rt_stream(nullptr, d->device));
+    if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_forward_paged: wait");
     if (words * 4 > d->gmeta_bytes) {
         if (d->gmeta) (void)hipFree(d->gmeta);
         d->gmeta = nullptr, d->gmeta_bytes = 0;
