@@ -921,7 +921,9 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
 }  // namespace
 
 // Slices of a row: enough that the rows fill the GPU, of a turn at least; 0:
-// rows are done whole, where they fit LDS or are many.
+// rows are done whole, where they fit LDS or are many. By slices and whole, 64
+// rows of 128000 logits: top-p 45 and 101 us, top-k of 40 39 and 37; 200 rows:
+// 90 and 95, 85 and 42.
 int sample_slices(int rows, int vocab) {
     if (vocab <= kResident || rows > 128) return 0;
     const int turns = (vocab + kTurn - 1) / kTurn;
