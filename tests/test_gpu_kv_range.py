@@ -1,0 +1,81 @@
+"""Attention over the paged cache where values, keys or queries lie far from 1, and that a row's bits come from the
+keys it attends alone: row and tile kernel, whole and cut into key ranges."""
+import numpy as np
+import pytest
+
+import welvet_amd as wv
+from kv_ref import stored
+from test_gpu_kv import Pool, rows
+from welvet_amd.kv import KVBatch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    print(f"[gpu] {__name__}: init device 0", flush=True)
+    wv.init(0)
+    yield
+
+
+# heads, kv heads, hd, keys, new tokens, cut into key ranges
+ROW = [(8, 2, 128, 1, 1, False), (8, 2, 128, 40, 1, False), (8, 2, 64, 300, 40, False), (4, 1, 128, 9001, 1, True)]
+TILE = [(64, 16, 64, 1900, 1900, False), (32, 8, 128, 4200, 515, True)]
+
+
+def reference(q, k, v, n, scale, window=0):
+    """The rows in float64 over held K and V, and what each value may be off by: a score by
+    d = (2^-21 + (hd + 2) 2^-24) scale sum|q k| (fp16 pairs, hd products summed in f32, two scales), an exponential by
+    a relative d + 2^-21, sums over L keys and their quotient by L 2^-24 each; the fp16 pair of a probability times
+    its V scale also by 2^-25 in units of 2^-14 of the largest scale that the ROW attends: 2^-37 of its largest |V|
+    per key. 2^-149 for results that are subnormal."""
+    q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
+    H, hd, L = q.shape[1], q.shape[2], k.shape[0]
+    G = H // k.shape[1]
+    pos, key = L - n + np.arange(n)[:, None], np.arange(L)[None]
+    seen = key <= pos
+    if window:
+        seen &= key > pos - window
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    for h in range(H):
+        kk, vv = k[:, h // G], v[:, h // G]
+        s = np.where(seen, q[:, h] @ kk.T * scale, -np.inf)
+        w = np.exp(s - s.max(1, keepdims=True))
+        w /= w.sum(1, keepdims=True)
+        out[:, h] = w @ vv
+        big = np.where(seen, np.abs(q[:, h]) @ np.abs(kk).T * scale, 0.0).max(1, keepdims=True)
+        d = (2.0 ** -21 + (hd + 2) * 2.0 ** -24) * big + 2.0 ** -21 + L * 2.0 ** -24
+        top = np.where(seen, np.abs(vv).max(1)[None], 0.0).max(1, keepdims=True)
+        tol[:, h] = 2 * d * (w @ np.abs(vv)) + L * 2.0 ** -37 * top + 2.0 ** -149
+    return out, tol
+
+
+def close(got, p, n, scale, window=0, only=slice(None)):
+    ref, tol = reference(p.q, stored(p.k[0], p.typ), stored(p.v[0], p.typ), n, np.float64(np.float32(scale)), window)
+    off = np.abs(got.astype(np.float64) - ref)[only]
+    assert np.isfinite(got[only]).all(), f"{(~np.isfinite(got[only])).sum()} values not finite"
+    bad = off > tol[only]
+    assert not bad.any(), f"{bad.sum()} values, by up to {(off / tol[only]).max():.3g} of the bound"
+
+
+def pool(seed, typ, shape):
+    heads, kvh, hd, kv, new, cut = shape
+    p = Pool(np.random.default_rng(seed), [kv], kvh, hd, 64, typ)
+    assert (p.kv.attention_scratch(KVBatch(1, new, p.width, 0, 0, 0, max_q=new), heads) > 0) == cut
+    return p
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("shape", ROW + TILE)
+@pytest.mark.parametrize("even", [False, True])
+def test_large_values(typ, shape, even):
+    """V up to the end of the range: the sums of the weights' multiples of it never lie above the largest |V|."""
+    heads, kvh, hd, kv, new, _ = shape
+    p = pool(41, typ, shape)
+    if even:  # equal weights, one sign: the mean of values next to f32's largest
+        p.k[0][:] = 0
+        p.v[0] = np.float32(3e38) * (1 - np.abs(p.v[0]) * np.float32(0.01))
+    else:
+        p.v[0] *= np.float32(2e37)
+    p.fill()
+    close(p.attend([new], heads, max_q=new), p, new, 1 / np.sqrt(hd))

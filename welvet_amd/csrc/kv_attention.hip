@@ -393,16 +393,17 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
         ok = nok;
     }
 
-    // the waves' sums: out = sum_w 2^(m_w - M) O_w / sum_w 2^(m_w - M) l_w
+    // the waves' rows y_w = O_w / l_w, each of its own keys' V, weighed by their shares of L = sum_w 2^(m_w - M) l_w:
+    // no value on the way is larger than the largest |V|
     l = sum_over_quads(l);
-    const float back = ldexpf(1.0f, max(eo, -126));
+    const float back = ldexpf(1.0f, max(eo, -126)), wl = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int i = 0; i < T; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int md = 4 * g + k;
             const int d = TYPE == WV_KV_F16 ? 16 * i + md : 32 * (i / 2) + 2 * md + i % 2;
-            red[wave][n][d] = o[i][k] * back;
+            red[wave][n][d] = o[i][k] * wl * back;
         }
     if (g == 0) {
         rm[wave][n] = mx;
@@ -418,11 +419,13 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
         if (rl[i][r] != 0.0f) M = fmaxf(M, rm[i][r]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        w[i] = rl[i][r] != 0.0f ? __builtin_amdgcn_exp2f(rm[i][r] - M) : 0.0f;
-        L += w[i] * rl[i][r];
+        w[i] = rl[i][r] != 0.0f ? __builtin_amdgcn_exp2f(rm[i][r] - M) * rl[i][r] : 0.0f;
+        L += w[i];
     }
     const int tok = t.q0 + orow / G, head = kvh * G + orow % G;
-    const float inv = a.part ? 1.0f : L != 0.0f ? 1.0f / L : 0.0f;
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] *= inv;
     float* dst = a.part ? a.part + ((int64_t(tok) * a.n_heads + head) * a.splits + sp) * LD
                         : a.out + int64_t(tok) * a.os + head * HD;
 #pragma unroll
@@ -431,7 +434,7 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (w[i] != 0.0f) x += w[i] * red[i][r][d];
-        dst[d] = x * inv;
+        dst[d] = x;
     }
     if (a.part && c == 0) {
         dst[HD] = M;
@@ -800,7 +803,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const int64_t orow = int64_t(t.q0 + row / G);
     const int head = kvh * G + row % G;
     const float back = ldexpf(1.0f, max(le, -126));
-    const float inv = a.part ? back : l != 0.0f ? back / l : 0.0f;
+    const float inv = l != 0.0f ? back / l : 0.0f;
     float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
     const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
 #pragma unroll
@@ -825,7 +828,8 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 }
 
 // The key ranges of one (token, head) row joined: the ranges' maxima and sums
-// weigh their partial rows, added in the order of the ranges by four waves.
+// weigh their rows, each divided by its own sum already, added in the order of
+// the ranges by four waves.
 // 3 us for one token's 32 rows of 10 ranges: a launch.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
@@ -841,8 +845,9 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
         l = p[lane * LD + HD + 1];
     }
     const float M = wave_maximum(l != 0.0f ? m : -INFINITY);
-    const float w = l != 0.0f ? __builtin_amdgcn_exp2f(m - M) : 0.0f;
-    const float L = wave_total(w * l);
+    float w = l != 0.0f ? __builtin_amdgcn_exp2f(m - M) * l : 0.0f;
+    const float L = wave_total(w);
+    w = L != 0.0f ? w / L : 0.0f;
     float x[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) x[i] = 0.0f;
@@ -866,7 +871,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
     if (threadIdx.x < HD) {
         const int d = threadIdx.x;
         const float y = red[0][d] + red[1][d] + red[2][d] + red[3][d];
-        a.out[int64_t(tok) * a.os + head * HD + d] = L != 0.0f ? y / L : 0.0f;
+        a.out[int64_t(tok) * a.os + head * HD + d] = y;
     }
 }
 
