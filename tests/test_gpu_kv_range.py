@@ -79,3 +79,20 @@ def test_large_values(typ, shape, even):
         p.v[0] *= np.float32(2e37)
     p.fill()
     close(p.attend([new], heads, max_q=new), p, new, 1 / np.sqrt(hd))
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("shape", ROW + TILE)
+def test_small_values(typ, shape):
+    """V rows next to 2^-100, equal weights, one sign: a mean that loses nothing on the way. Every weight is exactly
+    2^14 and its scale at most split in 22 bits; two sums for every 16 keys, roundings of 2^-24 each, and 8 more."""
+    heads, kvh, hd, kv, new, _ = shape
+    p = pool(42, typ, shape)
+    p.k[0][:] = 0
+    p.v[0] = np.float32(2.0 ** -99) * (1 + np.abs(p.v[0]) / 8)
+    p.fill()
+    got = p.attend([new], heads, max_q=new).astype(np.float64)
+    v = np.repeat(stored(p.v[0], typ), heads // kvh, 1)
+    ref = (np.cumsum(v, 0) / np.arange(1, kv + 1)[:, None, None])[kv - new:]
+    off = np.abs(got - ref).max() / np.abs(ref).max()
+    assert off <= 2.0 ** -22 + (kv / 8 + 8) * 2.0 ** -24, off

@@ -803,7 +803,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const int64_t orow = int64_t(t.q0 + row / G);
     const int head = kvh * G + row % G;
     const float back = ldexpf(1.0f, max(le, -126));
-    const float inv = l != 0.0f ? back / l : 0.0f;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // back / l may be subnormal
     float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
     const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
 #pragma unroll
@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
         for (int q = 0; q < 4; ++q) {
             f4 x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = o[i][4 * q + k] * inv;
+            for (int k = 0; k < 4; ++k) x[k] = o[i][4 * q + k] * inv * back;
             float* d = dst + 32 * i + 8 * q + 4 * h;
             if (al) {
                 *reinterpret_cast<f4*>(d) = x;
