@@ -96,3 +96,18 @@ def test_small_values(typ, shape):
     ref = (np.cumsum(v, 0) / np.arange(1, kv + 1)[:, None, None])[kv - new:]
     off = np.abs(got - ref).max() / np.abs(ref).max()
     assert off <= 2.0 ** -22 + (kv / 8 + 8) * 2.0 ** -24, off
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("shape", ROW + TILE)
+@pytest.mark.parametrize("key,query,factor", [(1e33, 1e-33, 1), (1e36, 1e-36, 1), (1e-29, 1e29, 1), (1e35, 1, 1e-35),
+                                              (1e36, 1e-20, 1e-16), (1e-20, 1e-15, 1e35), (1e-29, 1e36, 1e-7)])
+def test_scores_of_large_and_small_factors(typ, shape, key, query, factor):
+    """Keys, queries and the scale far from 1, their product and so the scores ordinary."""
+    heads, kvh, hd, kv, new, _ = shape
+    p = pool(43, typ, shape)
+    p.k[0] *= np.float32(key)
+    p.fill()
+    q = rows(p.rng, new, heads, hd) * np.float32(query)
+    scale = factor / np.sqrt(hd)
+    close(p.attend([new], heads, max_q=new, q=q, scale=scale), p, new, scale)

@@ -28,7 +28,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 constexpr float kNoMax = -3.0e38f;  // m of a row that has met no key
 constexpr float kLeast = 1.4e-45f;  // of a row's factor: times the -inf of a masked key it stays -inf
 constexpr int kMaxSplits = 64;
@@ -174,12 +174,15 @@ __device__ __forceinline__ Range tile_range(const KvAttn& a, const Tile& t, int 
     return r;
 }
 
-// The power of two that brings a row of magnitude amax into fp16's range
-// ([2^14, 2^15)), and its inverse.
-__device__ __forceinline__ float row_unit(float amax, float& inv) {
-    const int e = min(max(int(__float_as_uint(amax) >> 23) - 127, -100), 127);
+// A query row of magnitude amax: the power of two `inv` that brings it into
+// fp16's range ([2^14, 2^15)), and the factor from its scores in units of
+// 1 / kScore to t. Sums of codes times queries reach 2^37 and K scales 2^113,
+// so scores are held 2^-23 times as large until they meet this factor.
+constexpr float kScore = 1.1920929e-7f;  // 2^-23, on the K scales
+__device__ __forceinline__ float row_unit(float amax, float scale, float& inv) {
+    const int e = min(max(int(__float_as_uint(amax) >> 23) - 127, -113), 127);
     inv = __uint_as_float(uint32_t(14 - e + 127) << 23);
-    return __uint_as_float(uint32_t(e - 14 + 127) << 23);
+    return float(fmin(fmax(ldexp(double(scale) * kLog2e, e - 14 + 23), double(kLeast)), 3.4028234e38));
 }
 
 // Few rows: 16 query rows of one sequence and KV head per block, each of its
@@ -232,7 +235,7 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
                 m = fmaxf(m, fabsf(x[s][j]));
             }
         float inv;
-        qs = fmaxf(row_unit(max_over_quads(m), inv) * a.scale * kLog2e, kLeast);
+        qs = row_unit(max_over_quads(m), a.scale, inv);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
 #pragma unroll
@@ -321,7 +324,7 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
         float vs[8] = {sv[0].x, sv[0].y, sv[0].z, sv[0].w, sv[1].x, sv[1].y, sv[1].z, sv[1].w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // a NaN V scale makes the score NaN, where the mask can drop it
-            ks[j] = vs[j] == vs[j] ? ks[j] : vs[j];
+            ks[j] = vs[j] == vs[j] ? ks[j] * kScore : vs[j];
             vs[j] = fmaxf(vs[j], 0.0f);
         }
         if (next < rg.end) {
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
         const int en = max(eo, et);
         if (lane < 32) {
             float* d = &ls[ring][(n >> 3) * 16 + (n & 7)];
-            d[0] = sv == sv ? sk : sv;  // a NaN V scale makes the score NaN, where the mask can drop it
+            d[0] = sv == sv ? sk * kScore : sv;  // a NaN V scale makes the score NaN, where the mask can drop it
             d[8] = v * exp2_int(-en);
         }
         if (lane == 0) lf[ring] = exp2_int(eo - en);
@@ -612,7 +615,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
             }
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
         float inv;
-        qs = fmaxf(row_unit(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), inv) * a.scale * kLog2e, kLeast);
+        qs = row_unit(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), a.scale, inv);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
 #pragma unroll
