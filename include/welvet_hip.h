@@ -466,8 +466,10 @@ typedef struct wv_kv_batch {
  * t * stride floats (0: n_heads * head_dim), n_heads a multiple of n_kv_heads;
  * out may be q. The codes enter the matrix products exactly, queries and
  * probabilities in two fp16 terms each (22 bits), sums are f32: within a few
- * 1e-7 normwise of the same sums in f64. Keys, queries, values and scale may be
- * of any size; the scores scale q.K themselves have to stay below 1e38.
+ * 1e-7 of the largest |V| that the row attends from the same sums in f64. Keys,
+ * queries, values and scale may be of any size; the scores scale q.K themselves
+ * have to stay below 1e38. Keys that a row does not attend have no part in its
+ * bits.
  * Long key ranges are split over blocks and joined in order; the partial rows
  * lie in d_scratch (wv_kv_attention_scratch bytes, 16-byte aligned, held by
  * the call until its work is done), or, with NULL, in the library's own

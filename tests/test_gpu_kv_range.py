@@ -111,3 +111,27 @@ def test_scores_of_large_and_small_factors(typ, shape, key, query, factor):
     q = rows(p.rng, new, heads, hd) * np.float32(query)
     scale = factor / np.sqrt(hd)
     close(p.attend([new], heads, max_q=new, q=q, scale=scale), p, new, scale)
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("shape", [(8, 2, 128, 300, 12), (8, 2, 64, 300, 40), (32, 8, 128, 4200, 515),
+                                   (64, 16, 64, 1900, 1900)])
+@pytest.mark.parametrize("power", [3, 20, 110])
+@pytest.mark.parametrize("left", [False, True])
+def test_rows_come_from_their_own_keys(typ, shape, power, left):
+    """Values that a row does not attend, behind it or left of its window, 2^power times the others: its bits stay."""
+    heads, kvh, hd, kv, new = shape
+    window = new // 3 + 1 if left else 0
+    p = Pool(np.random.default_rng(44), [kv], kvh, hd, 64, typ).fill()
+    half = new // 2
+    a = p.attend([new], heads, max_q=new, window=window)
+    if left:  # rows from `half` on attend nothing at or in front of half's position less the window
+        keep, swap = slice(half, None), slice(0, kv - new + half - window + 1)
+    else:
+        keep, swap = slice(0, half), slice(kv - new + half, None)
+    p.v[0][swap] *= np.float32(2.0 ** power)
+    p.fill()
+    b = p.attend([new], heads, max_q=new, window=window, q=p.q)
+    close(b, p, new, 1 / np.sqrt(hd), window, keep)
+    assert np.array_equal(a[keep], b[keep]), f"{(a[keep] != b[keep]).sum()} values changed"
+    close(b, p, new, 1 / np.sqrt(hd), window)

@@ -10,8 +10,9 @@
 //   t_j = (c_j.qh + c_j.ql) s_j * (2^e scale log2 e)
 // on the fp16 matrix cores with f32 sums. For the second product the
 // probabilities take the V scales, P_j = 2^14 p_j s_j 2^-E, with E the running
-// exponent of the largest scale met (P_j then fills fp16's range whatever the
-// values' magnitude), and are split as ph + pl the same way.
+// exponent of the largest scale that the row has met among the keys it attends
+// (P_j then fills fp16's range whatever the values' magnitude, and nothing else
+// in the block has a part in a row's bits), and are split as ph + pl the same way.
 #include <algorithm>
 #include <cmath>
 
@@ -101,10 +102,6 @@ __device__ __forceinline__ uint32_t max_of_32(float v) {
     x = max(x, uint32_t(dpp_i<kDppRowShr8>(0, int(x))));
     x = max(x, uint32_t(dpp_i<kDppRowBcast15>(0, int(x))));
     return uint32_t(__builtin_amdgcn_readlane(int(x), 31));
-}
-// 2^e for a uniform e, clamped to what a normal float holds (0 below).
-__device__ __forceinline__ float exp2_int(int e) {
-    return e < -126 ? 0.0f : __uint_as_float(uint32_t(min(e, 127) + 127) << 23);
 }
 
 // A tile of query rows: row = token * G + head of the group, in one sequence.
@@ -248,7 +245,7 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
 #pragma unroll
     for (int i = 0; i < T; ++i) o[i] = f4{0, 0, 0, 0};
     float mx = kNoMax, l = 0.0f;
-    int eo = -200;  // E: the outputs are in units of 2^eo
+    int eo = -200;  // E of the lane's row: its outputs are in units of 2^eo
 
     const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
     const int pb = a.c.page_shift - 5;  // log2 blocks per page
@@ -343,8 +340,7 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = k0 + kv_octet_key(g, j);
-                    if (key > pos || key < first || key >= rg.limit) p[j] = -INFINITY;
-                    if (key >= rg.limit) vs[j] = 0.0f;
+                    if (key > pos || key < first || key >= rg.limit) p[j] = -INFINITY, vs[j] = 0.0f;
                 }
             }
 #pragma unroll
@@ -354,15 +350,11 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
             }
             m = max_over_quads(m);
             top = max_over_quads(top);
-            const int et = __builtin_amdgcn_readfirstlane(int(__float_as_uint(top) >> 23) - 126);  // top < 2^et
+            const int en = max(eo, int(__float_as_uint(top) >> 23) - 126);  // top < 2^en
             m = fmaxf(mx, ceilf(m * qs));
-            float f = __builtin_amdgcn_exp2f(mx - m);
             float add = 0.0f;
-            const float al = f;
-            if (et > eo) {
-                f *= ldexpf(1.0f, max(eo - et, -250));
-                eo = et;
-            }
+            const float al = __builtin_amdgcn_exp2f(mx - m), f = al * ldexpf(1.0f, max(eo - en, -250));
+            eo = en;
             mx = m;
             const float unit = ldexpf(1.0f, -eo), up = 14.0f - m;
 #pragma unroll
@@ -475,8 +467,8 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // about as long on the vector unit, so one iteration holds three key blocks:
 // the products O += V P of the last one and S of the next one run under the
 // exponentials of the one between. The codes of the key block after those are
-// on their way into registers. The V scales are staged as s_j 2^-E already,
-// with the factor by which E moved.
+// on their way into registers. With the scales lies the exponent of their
+// largest, which is what E takes of a key block that a wave's rows attend whole.
 // 2048 tokens of 32 heads over 16384 int8 keys: 970 to 1000 us across cards, up
 // to 1060 TFLOP/s of two-term products, where an fp16 library product of 8192^3
 // reaches 1155. The matrix unit is busy half of the cycles, the vector unit's
@@ -496,9 +488,8 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     constexpr int NU = (CU + 255) / 256;  // 16-byte loads of a thread
     constexpr int LD = HD + 4;
     __shared__ u4 lk[2][UN], lv[2][UN];
-    __shared__ float ls[4][kKvScales];  // K scales, V scales / 2^E, by octet
-    __shared__ float lf[4];             // 2^(E before - E)
-    __shared__ int le;
+    __shared__ float ls[4][kKvScales];  // K and V scales by octet
+    __shared__ float lt[4];             // exponent of the largest V scale
 
     const int kvh = blockIdx.x, sp = blockIdx.z;
     // a sequence's later tiles walk more keys and start first; where all blocks
@@ -554,7 +545,6 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
             for (int i = 0; i < NU; ++i)
                 vr[i] = *reinterpret_cast<const u4*>(a.c.v + blk * BB + (i * 256 + tid) * 16);
     };
-    int eo = -126;  // of wave 0, which stages the scales
     auto stage_k = [&](int buf) {
         if (loads)
 #pragma unroll
@@ -573,14 +563,12 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
         const int key = (kb << 5) + kv_octet_key(n >> 3, n & 7);
         const float v = ok && key < rg.limit ? fmaxf(sv, 0.0f) : 0.0f;
         const int et = int(max_of_32(v) >> 23) - 126;  // the largest is below 2^et
-        const int en = max(eo, et);
         if (lane < 32) {
             float* d = &ls[ring][(n >> 3) * 16 + (n & 7)];
             d[0] = sv == sv ? sk * kScore : sv;  // a NaN V scale makes the score NaN, where the mask can drop it
-            d[8] = v * exp2_int(-en);
+            d[8] = v;
         }
-        if (lane == 0) lf[ring] = exp2_int(eo - en);
-        eo = en;
+        if (lane == 0) lt[ring] = float(et);
     };
     auto stage_v = [&](int buf) {
         if (loads)
@@ -628,7 +616,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     for (int i = 0; i < T; ++i)
 #pragma unroll
         for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
-    float mx = kNoMax, l = 0.0f;
+    float mx = kNoMax, l = 0.0f, er = -113.0f;  // er: E of the lane's row (no scale is smaller)
     u4 ph[2] = {}, pl[2] = {};  // the probabilities that wait for their product, as fp16
 
     auto qk = [&](int buf, f16v& s) {
@@ -686,7 +674,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             ks[q] = *reinterpret_cast<const f4*>(&ls[ring][(2 * (q >> 1) + h) * 16 + 4 * (q & 1)]);
-        const float fe = lf[ring];
+        const float et = lt[ring];
         auto v_at = [&](int f) { return as_half(lv[cur ^ 1][(2 * (f / T) + h) * HD + 32 * (f % T) + n]); };
         auto k_at = [&](int c) { return as_half(lk[cur ^ 1][(2 * c + h) * 32 + n]); };
         h8 f0 = v_at(0), f1 = v_at(1);
@@ -728,8 +716,6 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
             }
         };
         h8 x[2] = {k_at(0), k_at(1)};
-        f4 vs[2];
-        vs[0] = *reinterpret_cast<const f4*>(&ls[ring][h * 16 + 8]);
 #pragma unroll
         for (int f = 0; f < 2 * T; f += 2) {
             const int q = f / T, i = f % T;
@@ -744,10 +730,29 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
             o[i + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g1, as_half(ph[q]), o[i + 1], 0, 0, 0);
             piece(f + 1);
         }
+        float en = er;
+        if (whole) {
+            en = fmaxf(er, et);
+        } else if (live) {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f4 v = *reinterpret_cast<const f4*>(&ls[ring][(2 * (i >> 1) + h) * 16 + 8 + 4 * (i & 1)]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top = fmaxf(top, s0[4 * i + k] != -INFINITY ? v[k] : 0.0f);
+            }
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            en = fmaxf(er, float(int(max(r[0], r[1]) >> 23) - 126));
+        }
+        const float f = al * __builtin_amdgcn_exp2f(er - en), unit = __builtin_amdgcn_exp2f(-en);
+        l *= al;
+        er = en;
         // The scores of b + 1; between the products the probabilities of b, some keys at a time
 #pragma unroll
         for (int e = 0; e < 16; ++e) s1[e] = 0.0f;
         float add[2] = {0.0f, 0.0f};
+        f4 vs[2];
+        vs[0] = *reinterpret_cast<const f4*>(&ls[ring][h * 16 + 8]);
 #pragma unroll
         for (int c = 0; c < S; ++c) {
             h8 y = x[c & 1];
@@ -765,7 +770,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
                 const float e1 = __builtin_amdgcn_exp2f(fmaf(s0[e + 1], qs, up));
                 add[q] += e0;
                 add[q] += e1;
-                const float p0 = e0 * vs[(e >> 2) & 1][e & 3], p1 = e1 * vs[(e >> 2) & 1][(e + 1) & 3];
+                const float p0 = e0 * unit * vs[(e >> 2) & 1][e & 3], p1 = e1 * unit * vs[(e >> 2) & 1][(e + 1) & 3];
                 const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
                 const h2 lo = {_Float16(fmaf(float(hi[0]), -1.0f, p0)), _Float16(fmaf(float(hi[1]), -1.0f, p1))};
                 uint32_t wh = __builtin_bit_cast(uint32_t, hi), wl = __builtin_bit_cast(uint32_t, lo);
@@ -773,8 +778,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
                 ph[q][i] = wh, pl[q][i] = wl;
             }
         }
-        l = fmaf(l, al, add[0] + add[1]);
-        const float f = fe * al;
+        l += add[0] + add[1];
         if (wave == 0) {
             stage_s(rg.begin + b + 2, ok2, (b + 2) & 3);
             load_s(kblk);
@@ -798,14 +802,12 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     }
     if (b < nb) step(b++, sa, sb);
     if (nb) pv((nb - 1) & 1);
-    if (tid == 0) le = eo;
-    __syncthreads();
     if (!busy || wr0 + n >= t.rows) return;
     const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
     const int64_t orow = int64_t(t.q0 + row / G);
     const int head = kvh * G + row % G;
-    const float back = ldexpf(1.0f, max(le, -126));
+    const float back = ldexpf(1.0f, int(er));
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // back / l may be subnormal
     float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
     const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
