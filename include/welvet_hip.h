@@ -464,7 +464,7 @@ typedef struct wv_kv_batch {
  * with KV head h / (n_heads / n_kv_heads). A row without keys comes out as
  * zeros; padding rows are left as they are. q and out are f32, row t at
  * t * stride floats (0: n_heads * head_dim), n_heads a multiple of n_kv_heads;
- * out may be q. The codes enter the matrix products exactly, queries and
+ * out may be q, at q's stride. The codes enter the matrix products exactly, queries and
  * probabilities in two fp16 terms each (22 bits), sums are f32: within a few
  * 1e-7 of the largest |V| that the row attends from the same sums in f64. Keys,
  * queries, values and scale may be of any size; the scores scale q.K themselves

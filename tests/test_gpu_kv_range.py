@@ -1,7 +1,10 @@
 """Attention over the paged cache where values, keys or queries lie far from 1, and that a row's bits come from the
 keys it attends alone: row and tile kernel, whole and cut into key ranges."""
+import ctypes
+
 import numpy as np
 import pytest
+import torch
 
 import welvet_amd as wv
 from kv_ref import stored
@@ -135,3 +138,19 @@ def test_rows_come_from_their_own_keys(typ, shape, power, left):
     close(b, p, new, 1 / np.sqrt(hd), window, keep)
     assert np.array_equal(a[keep], b[keep]), f"{(a[keep] != b[keep]).sum()} values changed"
     close(b, p, new, 1 / np.sqrt(hd), window)
+
+
+def test_in_place_at_another_stride_is_refused():
+    """out = q needs q's stride: rows written at another one would be queries that other blocks still read."""
+    p = pool(45, "q8", ROW[1])
+    L, x = wv.lib(), torch.zeros(1 << 16, device="cuda")
+    i = torch.zeros(64, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    b = KVBatch(1, 9, 1, i.data_ptr(), i.data_ptr(), i.data_ptr())
+
+    def call(qs, os, out):
+        return L.wv_kv_attention_dev(p.kv.handle, 0, ctypes.byref(b), x.data_ptr(), qs, 8, 1.0, 0, out, os, None, 0, None)
+    assert call(1025, 0, x.data_ptr()) == -2 and b"out is q" in L.wv_last_error()
+    assert call(0, 2048, x.data_ptr()) == -2
+    assert call(1024, 0, x.data_ptr()) == 0 and call(1025, 0, x.data_ptr() + 4 * 16384) == 0
+    wv.sync()

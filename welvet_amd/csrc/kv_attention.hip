@@ -1037,6 +1037,9 @@ int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch* batch,
     if (q_stride < w || out_stride < w)
         return rt_fail(WV_E_SHAPE, "wv_kv_attention: row strides %lld and %lld under the row's %lld floats",
                        (long long)q_stride, (long long)out_stride, (long long)w);
+    if (d_q && d_q == d_out && q_stride != out_stride)  // rows written would be others' queries still to be read
+        return rt_fail(WV_E_SHAPE, "wv_kv_attention: out is q, at row strides of %lld and %lld", (long long)out_stride,
+                       (long long)q_stride);
     if (!batch->n_seqs || !batch->n_tokens) return WV_OK;
     if (!d_q || !d_out || !batch->d_cu_q || !batch->d_kv_len || (batch->max_pages && !batch->d_pages))
         return rt_fail(WV_E_ARG, "wv_kv_attention: nil q/out/cu_q/kv_len/pages");
