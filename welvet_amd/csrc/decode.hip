@@ -2495,9 +2495,12 @@ int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const
     if (rc) return rc;
     (void)hipSetDevice(d->device);
     pg.n_seqs = n_seqs, pg.max_pages = max_pages;
-    const int32_t longest = *std::max_element(len, len + B);
-    pg.plan = kv_attn_plan(pg.cache.layer(0), n_seqs, n, std::min(max_pages, (longest + k.page_size - 1) / k.page_size),
-                           pg.max_q, c.n_heads, 0);
+    // planned for the sequences that run: an idle one's length is not even bounded by the table
+    int32_t longest = 0;
+    for (int b = 0; b < n_seqs; ++b)
+        if (n_new[b]) longest = std::max(longest, len[b]);
+    const int64_t most_pages = (int64_t(longest) + k.page_size - 1) / k.page_size;
+    pg.plan = kv_attn_plan(pg.cache.layer(0), n_seqs, n, int(most_pages), pg.max_q, c.n_heads, 0);
     const size_t more = std::max({kv_attn_part_floats(pg.cache.layer(0), n, c.n_heads, pg.plan.splits),
                                   matvec_scratch_floats(d->lm, n_seqs), sample_scratch_floats(n_seqs, c.vocab)});
     rc = ensure_prefill(*d, n, more);
