@@ -538,11 +538,11 @@ int wv_decoder_generate_sampled(uint64_t decoder, int32_t token, int32_t pos, in
  * logits (zeros for an idle one). Projections run as in wv_decoder_prefill (a
  * block of that many rows), attention as wv_kv_attention_dev, the LM head at
  * the f32 bar. Errors: WV_E_ARG "empty ids" without any new token, WV_E_SHAPE
- * for a cache of another shape, positions past the table, a page outside the
- * pool that holds one of the sequence's positions, two new tokens for one
- * position of the pool, or over 65535 new tokens. Synchronous; it waits for the
- * library's own stream first (calls on the cache with stream NULL), work on
- * other streams has to be done. */
+ * for a cache of another shape, a table of 2^31 positions or more, positions
+ * past the table, a page outside the pool that holds one of the sequence's
+ * positions, two new tokens for one position of the pool, or over 65535 new
+ * tokens. Synchronous; it waits for the library's own stream first (calls on the
+ * cache with stream NULL), work on other streams has to be done. */
 int wv_decoder_forward_paged(uint64_t decoder, uint64_t cache, int32_t n_seqs, const int32_t *n_new,
                              const int32_t *tokens, const int32_t *kv_len, const int32_t *pages, int32_t max_pages,
                              const wv_sampling *sampling, int32_t *next_tokens, float *logits);

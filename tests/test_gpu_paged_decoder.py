@@ -29,3 +29,14 @@ def test_idle_sequences_do_not_steer(idle):
         want = s.dec.forward_paged(s.kv, [[7], []], [n, 0], table, want_logits=True)[1]
         got = s.dec.forward_paged(s.kv, [[7], []], [n, idle], table, want_logits=True)[1]
         assert np.array_equal(got[0], want[0])
+
+
+def test_table_of_2_31_positions():
+    """Positions are 32-bit numbers: a table of more is refused, as wv_kv_attention_dev does."""
+    s = Server(config(8, 2, 64), "Q4_K", "q8", 1, page=256, width=1)
+    table = np.full((1, 1 << 23), -1, np.int32)
+    table[0, 0] = s.pages[0, 0]
+    with pytest.raises(wv.WelvetError) as e:
+        s.dec.forward_paged(s.kv, [[1]], [0], table)
+    assert e.value.code == -2 and "2^31" in str(e.value)
+    s.dec.forward_paged(s.kv, [[1]], [0], table[:, :-1])

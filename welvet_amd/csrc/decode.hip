@@ -2442,11 +2442,14 @@ int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const
         return rt_fail(WV_E_ARG, "wv_decoder_forward_paged: nil n_new/tokens/kv_len/pages/uniform");
     if (c.vocab > 1 << 19) return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: vocab %d (at most 2^19)", c.vocab);
     const int64_t width = int64_t(max_pages) * k.page_size;
+    if (width >= int64_t(1) << 31)
+        return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: a table of %d pages of %d positions (2^31 and more)", max_pages,
+                       k.page_size);
     int64_t total = 0;
     for (int b = 0; b < n_seqs; ++b) {
         if (n_new[b] < 0 || kv_len[b] < 0)
             return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: sequence %d: %d new tokens after %d", b, n_new[b], kv_len[b]);
-        if (n_new[b] && int64_t(kv_len[b]) + n_new[b] > std::min<int64_t>(width, INT32_MAX))
+        if (n_new[b] && int64_t(kv_len[b]) + n_new[b] > width)
             return rt_fail(WV_E_SHAPE, "wv_decoder_forward_paged: sequence %d: %d new tokens after %d exceed %lld positions",
                            b, n_new[b], kv_len[b], (long long)width);
         total += n_new[b];
