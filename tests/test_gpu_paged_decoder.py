@@ -2,6 +2,7 @@
 stay over many calls, attention cut into key ranges and on tiles inside the decoder."""
 import numpy as np
 import pytest
+import torch
 
 import welvet_amd as wv
 from test_gpu_serving import Server, config
@@ -40,3 +41,32 @@ def test_table_of_2_31_positions():
         s.dec.forward_paged(s.kv, [[1]], [0], table)
     assert e.value.code == -2 and "2^31" in str(e.value)
     s.dec.forward_paged(s.kv, [[1]], [0], table[:, :-1])
+
+
+def test_buffers_stay():
+    """A prompt of many rows and a chunk of fewer that needs more scratch (its attention's key ranges), in turn:
+    neither frees what the other made."""
+    cfg = config(32, 8, 128, n_layers=1, max_seq=1024)
+    s = Server(cfg, "Q4_K", "q8", 1, width=256)
+    ids, free = np.random.default_rng(6).integers(0, cfg.vocab, 600), []
+    for _ in range(3):
+        for call in (lambda: s.dec.prefill(ids), lambda: s.dec.forward_paged(s.kv, [ids[:256]], [7936], s.pages)):
+            call()
+            torch.cuda.synchronize()
+            free.append(torch.cuda.mem_get_info()[0])
+    print("[gpu] free", [f >> 20 for f in free], flush=True)
+    assert len(set(free[1:])) == 1, free
+
+
+def test_buffers_grow_by_more_than_a_row():
+    """A sequence more in every call: buffers are not made anew for each."""
+    cfg = config(8, 2, 64, n_layers=1, hidden=512, ffn=131072)
+    s = Server(cfg, "Q4_K", "q8", 96, width=1)
+    free = []
+    for n in range(40, 97):
+        s.dec.forward_paged(s.kv, [[1]] * n, [0] * n, s.pages[:n])
+        torch.cuda.synchronize()
+        free.append(torch.cuda.mem_get_info()[0])
+    print("[gpu] free", [f >> 20 for f in free], flush=True)
+    # rows, scratch, operands and logits: each by half at least, so three times from 40 to 96
+    assert len(set(free)) <= 13, free

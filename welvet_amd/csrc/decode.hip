@@ -17,6 +17,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <unordered_map>
 #include <vector>
@@ -1481,7 +1482,7 @@ struct Decoder {
     hipGraphExec_t exec = nullptr;
     hipGraph_t graph = nullptr;
     // prompt forward (wv_decoder_prefill): rows of every prompt token, grown on demand
-    int pcap = 0;
+    size_t pcap = 0;
     float *ph = nullptr, *pn = nullptr, *pq = nullptr, *pk = nullptr, *pv = nullptr, *patt = nullptr;
     float *pg = nullptr, *pu = nullptr, *pt = nullptr, *pscratch = nullptr;
     float* pxh = nullptr;  // the fp16 GEMM operand shared by the projections of one input, then its row factors
@@ -1814,6 +1815,40 @@ size_t prefill_proj_scratch(const DevBlob& w, int n) {
     return gemm_supported(w, n) ? gemm_scratch_floats(w, n) : matvec_scratch_floats(w, n);
 }
 
+// Buffers of `have` units each, made anew where `need` is more: by half of what they held at least, so that batches
+// a row longer every time do not free and allocate every time (a free waits for the device).
+struct Grown {
+    void** p;
+    size_t unit;  // bytes
+    template <class T>
+    Grown(T** p, size_t unit) : p(reinterpret_cast<void**>(p)), unit(unit) {}
+};
+hipError_t grow(size_t& have, size_t need, std::initializer_list<Grown> bufs) {
+    if (need <= have) return hipSuccess;
+    auto drop = [&] {
+        for (const Grown& b : bufs) {
+            if (*b.p) (void)hipFree(*b.p);
+            *b.p = nullptr;
+        }
+    };
+    drop();
+    const size_t ample = std::max(need, have + have / 2);
+    have = 0;
+    hipError_t e = hipSuccess;
+    for (const size_t n : {ample, need}) {  // where there is no room to spare, what is needed
+        e = hipSuccess;
+        for (const Grown& b : bufs)
+            if (e == hipSuccess && (e = hipMalloc(b.p, std::max<size_t>(n * b.unit, 256))) != hipSuccess) *b.p = nullptr;
+        if (e == hipSuccess) {
+            have = n;
+            return e;
+        }
+        drop();
+        (void)hipGetLastError();
+    }
+    return e;
+}
+
 // more_s: floats of d.pscratch that the caller needs beside the projections'.
 int ensure_prefill(Decoder& d, int n, size_t more_s = 0) {
     const wv_decoder_config& c = d.c;
@@ -1828,37 +1863,15 @@ int ensure_prefill(Decoder& d, int n, size_t more_s = 0) {
         if (ly.has_qkv) need(ly.qkv);
     }
     need_s = std::max(need_s, attn_part_floats(c, n));  // the key-split attention's ranges (between RoPE and O)
-    if (n <= d.pcap && need_s <= d.pscratch_floats && need_x <= d.pxh_floats) return WV_OK;
-    drop_prefill(d);
     const size_t qd = size_t(c.n_heads) * c.head_dim, kvd = size_t(c.n_kv_heads) * c.head_dim;
-    const size_t wide = std::max({size_t(c.hidden), size_t(c.ffn), qd});
-    struct {
-        void** p;
-        size_t bytes;
-    } bufs[] = {{reinterpret_cast<void**>(&d.ph), n * size_t(c.hidden) * 4},
-                {reinterpret_cast<void**>(&d.pn), n * size_t(c.hidden) * 4},
-                {reinterpret_cast<void**>(&d.pq), n * (qd + 2 * kvd) * 4},  // q | k | v rows of the fused GEMM
-                {reinterpret_cast<void**>(&d.pk), n * kvd * 4},
-                {reinterpret_cast<void**>(&d.pv), n * kvd * 4},
-                {reinterpret_cast<void**>(&d.patt), n * qd * 4},
-                {reinterpret_cast<void**>(&d.pg), n * size_t(c.ffn) * 4},
-                {reinterpret_cast<void**>(&d.pu), n * size_t(c.ffn) * 4},
-                {reinterpret_cast<void**>(&d.pt), n * wide * 4},
-                {reinterpret_cast<void**>(&d.pscratch), std::max<size_t>(need_s, 1) * 4},
-                {reinterpret_cast<void**>(&d.pxh), std::max<size_t>(need_x, 1) * 4},
-                {reinterpret_cast<void**>(&d.ptok), size_t(n) * 4}};
-    for (auto& b : bufs) {
-        const hipError_t e = hipMalloc(b.p, std::max<size_t>(b.bytes, 256));
-        if (e != hipSuccess) {
-            *b.p = nullptr;
-            drop_prefill(d);
-            return rt_hip_fail(e, "wv_decoder_prefill: buffers");
-        }
-    }
-    d.pcap = n;
-    d.pscratch_floats = std::max<size_t>(need_s, 1);
-    d.pxh_floats = std::max<size_t>(need_x, 1);
-    return WV_OK;
+    const size_t wide = std::max({size_t(c.hidden), size_t(c.ffn), qd}), hidden = size_t(c.hidden), ffn = size_t(c.ffn);
+    hipError_t e = grow(d.pcap, size_t(n), {{&d.ph, hidden * 4}, {&d.pn, hidden * 4},
+                                            {&d.pq, (qd + 2 * kvd) * 4},  // q | k | v rows of the fused GEMM
+                                            {&d.pk, kvd * 4}, {&d.pv, kvd * 4}, {&d.patt, qd * 4}, {&d.pg, ffn * 4},
+                                            {&d.pu, ffn * 4}, {&d.pt, wide * 4}, {&d.ptok, 4}});
+    if (e == hipSuccess) e = grow(d.pscratch_floats, std::max<size_t>(need_s, 1), {{&d.pscratch, 4}});
+    if (e == hipSuccess) e = grow(d.pxh_floats, std::max<size_t>(need_x, 1), {{&d.pxh, 4}});
+    return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_decoder_prefill: buffers");
 }
 
 // ForwardTokens over n prompt tokens at positions pos0 .. pos0+n-1
@@ -2511,26 +2524,9 @@ int wv_decoder_forward_paged(uint64_t dec, uint64_t cache, int32_t n_seqs, const
     // what was enqueued on the library's stream may write the cache
     hipError_t e = hipStreamSynchronize(rt_stream(nullptr, d->device));
     if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_forward_paged: wait");
-    if (words * 4 > d->gmeta_bytes) {
-        if (d->gmeta) (void)hipFree(d->gmeta);
-        d->gmeta = nullptr, d->gmeta_bytes = 0;
-        if ((e = hipMalloc(reinterpret_cast<void**>(&d->gmeta), words * 4)) != hipSuccess) {
-            d->gmeta = nullptr;
-            return rt_hip_fail(e, "wv_decoder_forward_paged: batch");
-        }
-        d->gmeta_bytes = words * 4;
-    }
-    if (B > d->grows) {
-        for (float** p : {&d->glast, &d->glogits}) {
-            if (*p) (void)hipFree(*p);
-            *p = nullptr;
-        }
-        d->grows = 0;
-        e = hipMalloc(reinterpret_cast<void**>(&d->glast), 2 * B * size_t(c.hidden) * 4);
-        if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&d->glogits), B * size_t(c.vocab) * 4);
-        if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_forward_paged: logits");
-        d->grows = B;
-    }
+    e = grow(d->gmeta_bytes, words * 4, {{&d->gmeta, 1}});
+    if (e == hipSuccess) e = grow(d->grows, B, {{&d->glast, 2 * size_t(c.hidden) * 4}, {&d->glogits, size_t(c.vocab) * 4}});
+    if (e != hipSuccess) return rt_hip_fail(e, "wv_decoder_forward_paged: buffers");
     int32_t* m = reinterpret_cast<int32_t*>(d->gmeta);
     auto at = [&](const int32_t* p) { return m + (p - host.data()); };
     pg.slots = reinterpret_cast<const int64_t*>(m);
