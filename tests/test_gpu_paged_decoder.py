@@ -6,6 +6,7 @@ import torch
 
 import welvet_amd as wv
 from test_gpu_serving import Server, config
+from welvet_amd.kv import KVBatch
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +71,35 @@ def test_buffers_grow_by_more_than_a_row():
     print("[gpu] free", [f >> 20 for f in free], flush=True)
     # rows, scratch, operands and logits: each by half at least, so three times from 40 to 96
     assert len(set(free)) <= 13, free
+
+
+def splits(s, new):
+    """Whether attention over the longest sequence's pages is cut into key ranges for these new tokens."""
+    longest = max(len(i) + n for i, n in zip(s.ids, new) if n)
+    b = KVBatch(len(new), sum(new), -(-longest // s.page), 0, 0, 0, max_q=max(new))
+    return s.kv.attention_scratch(b, s.cfg.n_heads) > 0
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+def test_key_ranges(typ):
+    """Tokens behind a prompt of some hundreds: ranges and their join, in the buffer of the projections' partials."""
+    cfg = config(8, 2, 64, n_layers=2)
+    s = Server(cfg, "Q4_K", typ, 2, width=32)
+    rng = np.random.default_rng(3)
+    s.step([rng.integers(0, cfg.vocab, 900), rng.integers(0, cfg.vocab, 20)])
+    for lens in ((1, 1), (2, 0)):
+        new = [rng.integers(0, cfg.vocab, n) for n in lens]
+        assert splits(s, lens)
+        tokens, logits = s.step(new)
+        s.check(new, tokens, logits, 2e-3)
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+def test_tiles(typ):
+    """A prompt that the tile kernel takes beside a short one."""
+    cfg = config(32, 8, 128, n_layers=1)
+    s = Server(cfg, "Q4_K", typ, 2, width=52)
+    rng = np.random.default_rng(4)
+    new = [rng.integers(0, cfg.vocab, n) for n in (1600, 3)]
+    tokens, logits = s.step(new)
+    s.check(new, tokens, logits, 2e-3)
