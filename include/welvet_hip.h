@@ -404,9 +404,10 @@ int wv_decoder_free(uint64_t decoder);
  * Rows are held as codes with one f32 scale per position and KV head, for K
  * and V each. For a row x of head_dim values with amax = max |x|:
  *   WV_KV_F16  scale = 2^(floor(log2 amax) - 14), code = fp16(x / scale)
- *              (nearest, ties to even): 2 bytes per value, no overflow
+ *              (nearest, ties to even): 2 bytes per value
  *   WV_KV_Q8   scale = f32(amax / 127), code = x / scale rounded half away
  *              from zero (the exact quotient; Q8_0's rule): 1 byte per value
+ * both no larger than leaves code * scale finite (rows that reach 3.4e38),
  * and a row reads back as code * scale. A row with amax < 2^-100 is held as
  * zeros. A row that holds a NaN or an infinity reads back as NaN in every
  * value (and what attends to it is NaN). Positions never written read back 0. */

@@ -8,8 +8,8 @@ import torch
 
 import welvet_amd as wv
 from kv_ref import stored
-from test_gpu_kv import Pool, rows
-from welvet_amd.kv import KVBatch
+from test_gpu_kv import Pool, dev, rows
+from welvet_amd.kv import KVBatch, KVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -154,3 +154,24 @@ def test_in_place_at_another_stride_is_refused():
     assert call(0, 2048, x.data_ptr()) == -2
     assert call(1024, 0, x.data_ptr()) == 0 and call(1025, 0, x.data_ptr() + 4 * 16384) == 0
     wv.sync()
+
+
+@pytest.mark.parametrize("typ", ["f16", "q8"])
+@pytest.mark.parametrize("n", [5, 1024])  # row by row, and tiles of 32 rows
+def test_the_largest_rows_read_back_finite(typ, n):
+    """Rows up to f32's largest value: a code times its scale never rounds to infinity. In between the codes are the
+    nearest ones: half a step of an 11-bit fp16 code or of 1 / 127, a whole one at the very end."""
+    rng, big = np.random.default_rng(46), np.finfo(np.float32).max
+    x = (rng.uniform(-1, 1, (n, 8, 64)) * big).astype(np.float32)
+    x[:, :, 0] = np.float32(big) * np.where(rng.random((n, 8)) < 0.5, -1, 1)
+    x[1, :, 1] = np.float32(3.4021e38)
+    kv = KVCache(1, 8, 64, 32, n // 32 + 1, typ)
+    dx, ds = dev(x), dev(np.arange(n), np.int64)
+    k, v = (torch.zeros(n, 8, 64, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    kv.write_dev(0, dx.data_ptr(), dx.data_ptr(), ds.data_ptr(), n)
+    kv.read_dev(0, ds.data_ptr(), n, k.data_ptr(), v.data_ptr())
+    wv.sync()
+    for got in (k, v):
+        off = np.abs(got.cpu().numpy().astype(np.float64) - x) / np.float64(big)
+        assert off.max() <= (2.0 ** -11 if typ == "f16" else 0.5 / 127 + 2.0 ** -23)

@@ -18,6 +18,9 @@ uint64_t g_next = 1;
 
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100: rows below it are held as zeros
 
+constexpr float kMostQ8 = 8454659.0f * 3.1691265005705735e29f;  // 8454659 2^98: the largest with a finite 127-fold
+constexpr float kMostF16 = 1.0384593717069655e34f;  // 2^113, a row's largest scale: codes end under 2^15 there
+
 // A row's scale from its largest magnitude (bad: it holds a NaN or infinity)
 // and the factor its values take before rounding. F16: powers of two, so the
 // product is exact and amax / scale lies in [2^14, 2^15). Q8: amax / 127 in
@@ -31,7 +34,7 @@ __device__ __forceinline__ float row_scale(float amax, bool bad, int type, float
         inv = __uint_as_float(uint32_t(14 - e + 127) << 23);
         return __uint_as_float(uint32_t(e - 14 + 127) << 23);
     }
-    const float s = amax / 127.0f;
+    const float s = fminf(amax / 127.0f, kMostQ8);
     inv = 1.0f / s;
     return s;
 }
@@ -91,12 +94,13 @@ __device__ __forceinline__ uint64_t row_codes(const float4 x, float& s) {
     const float amax = row_amax<HD>(x, bad);
     float inv;
     s = row_scale(amax, bad, TYPE, inv);
-    const float f[4] = {x.x, x.y, x.z, x.w};
+    const float f[4] = {x.x, x.y, x.z, x.w}, most = s == kMostF16 ? 32752.0f : 32768.0f;
     uint64_t c = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (TYPE == WV_KV_F16)
-            c |= uint64_t(__builtin_bit_cast(uint16_t, bad ? _Float16(0) : _Float16(f[i] * inv))) << (16 * i);
+            c |= uint64_t(__builtin_bit_cast(uint16_t, bad ? _Float16(0) : _Float16(fminf(fmaxf(f[i] * inv, -most), most))))
+                 << (16 * i);
         else
             c |= uint64_t(uint32_t((bad || s == 0.0f ? 0 : q8_code(f[i], s, inv)) + 128)) << (8 * i);
     }
