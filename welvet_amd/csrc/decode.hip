@@ -2017,7 +2017,7 @@ int enqueue_prefill(Decoder& d, int n, int pos0, const Paged* pg = nullptr) {
             a.c = view;
             a.q = q, a.qs = qstr, a.out = d.patt, a.os = qd, a.part = pg->plan.splits > 1 ? d.pscratch : nullptr;
             a.cu = pg->cu, a.kv_len = pg->kv_len, a.pages = pg->pages;
-            a.n_seqs = pg->n_seqs, a.n_tokens = n, a.max_pages = pg->max_pages, a.max_q = pg->max_q;
+            a.n_seqs = pg->n_seqs, a.n_tokens = n, a.max_pages = pg->max_pages;
             a.n_heads = c.n_heads, a.scale = scale;
             a.splits = pg->plan.splits, a.many = pg->plan.many, a.once = pg->plan.once;
             e = launch_kv_attn(a, d.stream);

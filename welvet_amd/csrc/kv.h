@@ -80,7 +80,7 @@ struct KvAttn {
     float* part;
     const int32_t *cu, *kv_len, *pages;
     int64_t qs, os;
-    int n_seqs, n_tokens, max_pages, max_q;
+    int n_seqs, n_tokens, max_pages;
     int n_heads, window;
     int splits;
     bool many;  // long sequences by the kernel of 128-row tiles

@@ -1049,9 +1049,9 @@ int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch* batch,
     a.c = c.layer(layer);
     a.q = d_q, a.out = d_out, a.qs = q_stride, a.os = out_stride;
     a.cu = batch->d_cu_q, a.kv_len = batch->d_kv_len, a.pages = batch->d_pages;
-    a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages, a.max_q = batch->max_q;
+    a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages;
     a.n_heads = n_heads, a.window = std::min(window, 1 << 30), a.scale = scale;
-    const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, a.max_q, n_heads, a.window);
+    const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, batch->max_q, n_heads, a.window);
     a.splits = plan.splits, a.many = plan.many, a.once = plan.once;
     const size_t floats = kv_attn_part_floats(a.c, a.n_tokens, n_heads, a.splits);
     RtScratch sc;
