@@ -99,8 +99,8 @@ __device__ __forceinline__ uint64_t row_codes(const float4 x, float& s) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if (TYPE == WV_KV_F16)
-            c |= uint64_t(__builtin_bit_cast(uint16_t, bad ? _Float16(0) : _Float16(fminf(fmaxf(f[i] * inv, -most), most))))
-                 << (16 * i);
+            c |= uint64_t(__builtin_bit_cast(
+                     uint16_t, bad ? _Float16(0) : _Float16(__builtin_amdgcn_fmed3f(f[i] * inv, -most, most)))) << (16 * i);
         else
             c |= uint64_t(uint32_t((bad || s == 0.0f ? 0 : q8_code(f[i], s, inv)) + 128)) << (8 * i);
     }
