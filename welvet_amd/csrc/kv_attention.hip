@@ -469,14 +469,17 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // exponentials of the one between. The codes of the key block after those are
 // on their way into registers. With the scales lies the exponent of their
 // largest, which is what E takes of a key block that a wave's rows attend whole.
-// 2048 tokens of 32 heads over 16384 int8 keys: 970 to 1000 us across cards, up
-// to 1060 TFLOP/s of two-term products, where an fp16 library product of 8192^3
-// reaches 1155. The matrix unit is busy half of the cycles, the vector unit's
-// issue the other half; without the exponentials it would take 0.79 of that,
-// without the products 0.80. A prompt of 2047 tokens: 100 us, for half of which
-// the longest tile runs alone on its CU. Dropped, since they gained nothing: two
-// groups of four waves half a tile apart, or on halves of the keys; a barrier
-// every second step; steps of 64 keys.
+// A row's E is its own: one multiplication a probability, 2.6 % of a long chunk
+// against an E for the whole block, which took bits from rows whose mask hides a
+// large V. A second copy of the step for such rows costs the others as much.
+// 2048 tokens of 32 heads over 16384 int8 keys: 982 to 994 us across cards, up
+// to 1050 TFLOP/s of two-term products, where an fp16 library product of 8192^3
+// reaches 1155. The matrix unit is busy 48 % of the cycles, the vector unit's
+// issue 53 %; without the exponentials it would take 0.95 of that, without the
+// products 0.90. A prompt of 2047 tokens: 100 us, for half of which the longest
+// tile runs alone on its CU. Dropped, since they gained nothing: two groups of
+// four waves half a tile apart, or on halves of the keys; a barrier every second
+// step; steps of 64 keys.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;

@@ -15,7 +15,7 @@
 // of 40 15, top-p 29, top-k of 400 and top-p 37, no filter 20), those of up to
 // 4096 and 8192 dealt out so that all waves have some (10 of 1530, top-k of 400
 // and top-p: 21 to 13 us). Of larger ones, where rows are few, each is cut over
-// several blocks, below (64 of 128000: top-p 45 us, by whole rows 101).
+// several blocks, below (64 of 128000: top-p 46 us, by whole rows 92).
 // The loops stay small: with the row in registers, unrolled, instruction fetch
 // took most of the time (greedy, one row of 32000: 23 us, from LDS 5).
 #include <algorithm>
@@ -764,7 +764,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(SampleArgs a) {
 //   finish one block a row: the list's cut, and the place of u
 // Rows that do not fit this (top_p with a larger top_k than the list takes, a
 // bin of more tokens than that) are done whole by the last launch. 64 rows of
-// 128000 with top-p: 5.8, 11.9, 17.7 and 12.3 us; loading a pass's logits in
+// 128000 with top-p: 5.7, 12.2, 17.4 and 10.1 us; loading a pass's logits in
 // front of the wait for the maximum costs registers, and so a block a CU (25
 // for 17.7).
 // ---------------------------------------------------------------------------
@@ -922,7 +922,7 @@ __global__ void __launch_bounds__(kThreads) k_slice_finish(SampleArgs a, Slices 
 
 // Slices of a row: enough that the rows fill the GPU, of a turn at least; 0:
 // rows are done whole, where they fit LDS or are many. By slices and whole, 64
-// rows of 128000 logits: top-p 45 and 101 us, top-k of 40 39 and 37; 200 rows:
+// rows of 128000 logits: top-p 46 and 92 us, top-k of 40 39 and 37; 200 rows:
 // 90 and 95, 85 and 42.
 int sample_slices(int rows, int vocab) {
     if (vocab <= kResident || rows > 128) return 0;
