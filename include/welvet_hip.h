@@ -510,9 +510,10 @@ typedef struct wv_sampling {
  * included, and summed exactly in units of 2^-44 of the largest: a token that
  * stands on the edge of top_p or u may fall to either side. d_probs (may be
  * NULL): the drawn token's share of the kept weights (1 where T <= 0, 0 for
- * token -1). vocab is at most 2^19, rows 2^20. Device pointers, enqueued on
- * `stream`. Up to 128 rows of more than 32768 logits use the library's own scratch, except
- * on a stream under capture, where one block draws a row whatever its length. */
+ * token -1). vocab is at most 2^19, rows 2^20. Pointers of the device of
+ * `stream` (NULL: the current one), enqueued there. Up to 128 rows of more than
+ * 32768 logits use the library's own scratch on that device, except on a stream
+ * under capture, where one block draws a row whatever its length. */
 int wv_sample_dev(const float *d_logits, int64_t stride, int32_t rows, int32_t vocab, const wv_sampling *sampling,
                   int32_t *d_tokens, float *d_probs, void *stream);
 

@@ -2,9 +2,11 @@
 of several slices meet in one list, up to the list's end and past it, and rows done whole."""
 import numpy as np
 import pytest
+import torch
 
 import welvet_amd as wv
-from test_gpu_sample import check, logits
+from test_gpu_sample import check, draw, logits
+from welvet_amd.sampling import sample_dev
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +46,20 @@ def test_mixed_lists():
     x[11], x[12, 6:] = -np.inf, -np.inf
     check(x, t=rng.choice([0, 0.7, 1.2], r), k=rng.choice([0, 1, 128, 129, 400, 512, 513, 4000], r),
           p=rng.choice([0.5, 0.95, 1.0], r), m=rng.choice([0, 0.01], r), u=rng.random(r, np.float32))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="two devices")
+def test_on_another_device_than_the_current_one():
+    """Rows on the stream's device while another is the library's current one: the scratch is that device's too."""
+    rng = np.random.default_rng(6)
+    x, u = logits(rng, 5, 50000), rng.random(5, np.float32)
+    want = draw(x, p=np.full(5, 0.9), u=u)[0]
+    wv.init(1)
+    wv.init(0)
+    with torch.cuda.device(1):
+        l, uu, p = (torch.from_numpy(a).cuda() for a in (x, u, np.full(5, 0.9, np.float32)))
+        tok, st = torch.zeros(5, dtype=torch.int32, device="cuda"), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        sample_dev(l.data_ptr(), 5, 50000, tok.data_ptr(), uu.data_ptr(), top_p_ptr=p.data_ptr(), stream=st.cuda_stream)
+        st.synchronize()
+        assert tok.cpu().numpy().tolist() == want.tolist()

@@ -983,7 +983,11 @@ extern "C" int wv_sample_dev(const float* d_logits, int64_t stride, int32_t rows
     SampleArgs a{};
     a.logits = d_logits, a.stride = stride, a.rows = rows, a.vocab = vocab;
     a.p = *sampling, a.tokens = d_tokens, a.probs = d_probs;
-    hipStream_t st = rt_stream(stream, rt_current_device());
+    // no handle says where the rows lie: on the stream's device, whose scratch the call then takes
+    int dev = rt_current_device();
+    hipStream_t st = rt_stream(stream, dev);
+    if (hipDevice_t of; stream && hipStreamGetDevice(st, &of) == hipSuccess) dev = of;
+    (void)hipSetDevice(dev);
     RtScratch sc;  // not under capture: what a replay writes must not lie in a slot that other calls take
     const size_t floats = rt_capturing(st) ? 0 : sample_scratch_floats(rows, vocab);
     if (floats)
