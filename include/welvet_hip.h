@@ -442,6 +442,52 @@ int wv_kv_write_dev(uint64_t cache, int32_t layer, const float *d_k, const float
 int wv_kv_read_dev(uint64_t cache, int32_t layer, const int64_t *d_slots, int32_t n, float *d_k, float *d_v,
                    int64_t k_stride, int64_t v_stride, void *stream);
 
+/* Who holds which page: a page table on the device, and how many sequences
+ * hold each page of the pool (0: free). Sequence b holds d_kv_len[b] positions
+ * in the pages d_pages[b * max_pages ..]; entries that it does not hold are -1
+ * (the calls below keep it so; a new table is -1 everywhere, lengths and
+ * counts 0). The calls on one table run one after the other: on one stream, or
+ * ordered by the caller. They allocate nothing, need no host in between, and
+ * can be captured. n_seqs is at most 16384. */
+typedef struct wv_kv_tables {
+    int32_t n_seqs, max_pages;
+    int32_t *d_pages;  /* [n_seqs][max_pages] */
+    int32_t *d_kv_len; /* [n_seqs] */
+    int32_t *d_refs;   /* [n_pages of the cache] */
+    int32_t *d_work;   /* wv_kv_tables_work bytes that belong to this table, any contents */
+} wv_kv_tables;
+int wv_kv_tables_work(uint64_t cache, int32_t n_seqs, int32_t max_pages, size_t *bytes);
+
+/* Every sequence b becomes sequence d_parent[b] as it was before the call, all
+ * at once: forked, or traded places as beams do. The pages are shared, not
+ * copied; what b alone held becomes free. -1 empties b; b itself, or an index
+ * outside the table, leaves it as it is. */
+int wv_kv_fork_dev(uint64_t cache, const wv_kv_tables *tables, const int32_t *d_parent, void *stream);
+
+/* Every sequence b to d_len[b] positions (negative: 0), and what lies behind
+ * its old length its own to write:
+ *   first the ones that shrink give the pages back that they no longer need;
+ *   then the ones that grow take the lowest free pages, in order of b: one for
+ *   the page that its next position lies in, where that has rows already and
+ *   other sequences hold it too (its rows are copied, in all layers; of
+ *   sequences that grow out of one page and are all its holders, the last
+ *   keeps it), and the new pages.
+ * The first sequence that does not find enough, and all growing ones behind it,
+ * stay as they are, as does one that the table has no room for: d_ok[b] is 0
+ * there, else 1. */
+int wv_kv_resize_dev(uint64_t cache, const wv_kv_tables *tables, const int32_t *d_len, int32_t *d_ok, void *stream);
+
+/* Moves pages so that the U pages that are held come first in the pool: the
+ * i-th held page from U on goes to the i-th free one below U, in all layers,
+ * and the table follows (every holder of the pool's pages has to be in it).
+ * *d_used (device, may be NULL) receives U. */
+int wv_kv_compact_dev(uint64_t cache, const wv_kv_tables *tables, int32_t *d_used, void *stream);
+
+/* Copies page d_src[i] to page d_dst[i], in all layers, i < n. Pairs outside
+ * the pool are skipped. No page may be the target of two pairs, or of one and
+ * the source of another. */
+int wv_kv_copy_pages_dev(uint64_t cache, const int32_t *d_src, const int32_t *d_dst, int32_t n, void *stream);
+
 /* New tokens of n_seqs sequences in one batch. Sequence b owns the query rows
  * d_cu_q[b] .. d_cu_q[b+1]-1 of n_tokens rows (ascending from 0; rows behind
  * the last sequence are padding) and the keys 0 .. d_kv_len[b]-1, its new
@@ -456,6 +502,12 @@ typedef struct wv_kv_batch {
     const int32_t *d_kv_len; /* [n_seqs] */
     const int32_t *d_pages;  /* [n_seqs][max_pages] */
 } wv_kv_batch;
+
+/* Slot and position of every row of a batch (whose kv_len counts its new
+ * tokens), as wv_kv_write_dev and wv_rope_dev take them: d_slots[t] and d_pos[t]
+ * (may be NULL), n_tokens each. Padding rows get slot -1 and position 0, rows
+ * whose page is outside the pool or past the table slot -1. */
+int wv_kv_slots_dev(uint64_t cache, const wv_kv_batch *batch, int64_t *d_slots, int32_t *d_pos, void *stream);
 
 /* Causal grouped-query attention of a batch's new tokens over the cache
  * (layers/mha/attn.go:40-118 with its causal and sliding-window masks). Token
@@ -482,6 +534,61 @@ int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch *batch,
  * n_seqs, n_tokens, max_pages and max_q are read. */
 int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch *batch, int32_t n_heads, int32_t window,
                             size_t *bytes);
+
+/* ---- rotary positions ---- */
+
+/* A rotation of heads of head_dim values (2 to 1024): with t = pos f_i, pair i
+ * of the first rot_dim (even) becomes gain (a cos t - b sin t, a sin t +
+ * b cos t); the values behind rot_dim stay. (layers/mha/rope.go:6-21 is
+ * WV_ROPE_HALF over the whole head, WV_ROPE_NONE, gain 1, as the decoder calls
+ * do it.) f_i = theta^(-2i / rot_dim), for contexts longer than the trained
+ * one scaled:
+ *   WV_ROPE_LINEAR      f_i / factor
+ *   WV_ROPE_BASE        theta * factor^(rot_dim / (rot_dim - 2)) in theta's place
+ *   WV_ROPE_RAMP_TURNS  f_i (1 - r) / factor + f_i r, r = (n_i - low) / (high -
+ *                       low) within [0, 1], n_i = trained f_i / 2 pi the turns
+ *                       that pair i makes over the trained positions
+ *   WV_ROPE_RAMP_DIMS   the same with r falling from 1 to 0 between the pairs
+ *                       i0 and i1: r = 1 - (i - i0) / max(i1 - i0, 0.001) within
+ *                       [0, 1], i0 the floor of the i at which n_i = high, i1
+ *                       the ceiling of that for low, both within 0 .. rot_dim/2 - 1 */
+#define WV_ROPE_HALF 0  /* pair i at (i, i + rot_dim / 2) */
+#define WV_ROPE_PAIRS 1 /* pair i at (2i, 2i + 1) */
+#define WV_ROPE_NONE 0
+#define WV_ROPE_LINEAR 1
+#define WV_ROPE_BASE 2
+#define WV_ROPE_RAMP_DIMS 3
+#define WV_ROPE_RAMP_TURNS 4
+typedef struct wv_rope_config {
+    int32_t head_dim, rot_dim;
+    int32_t layout;    /* WV_ROPE_HALF, WV_ROPE_PAIRS */
+    int32_t scaling;   /* WV_ROPE_NONE .. WV_ROPE_RAMP_TURNS */
+    int32_t trained;   /* ramps: positions of the training */
+    double theta;      /* > 1 */
+    double factor;     /* every scaling: > 0, that of the context's length */
+    double low, high;  /* ramps: turns, 0 < low < high */
+    double gain;       /* > 0; 1: none */
+} wv_rope_config;
+int wv_rope_create(const wv_rope_config *cfg, uint64_t *rope);
+/* Releases a rotation once its work is done (waits for the device). */
+int wv_rope_free(uint64_t rope);
+
+/* Rows of n_heads heads, row t at t * stride floats (0: n_heads * head_dim).
+ * d_y NULL: in place; d_y may also be d_x at x_stride, but not overlap it
+ * otherwise. */
+typedef struct wv_rope_rows {
+    const float *d_x;
+    float *d_y;
+    int64_t x_stride, y_stride;
+    int32_t n_heads;
+} wv_rope_rows;
+/* Turns row t of q and of k (either may be NULL) to position d_pos[t], t < n.
+ * A negative position turns back, which is also the gradient of the call at
+ * the positive one. Angles are taken in f64 modulo a turn, sine, cosine and
+ * products in f32: within 6e-7 gain of a pair's length (positions up to 2^24; at
+ * 2^31 within 2e-6 gain). Device pointers, enqueued on `stream`. */
+int wv_rope_dev(uint64_t rope, const int32_t *d_pos, int32_t n, const wv_rope_rows *q, const wv_rope_rows *k,
+                void *stream);
 
 /* ---- sampling: the next token of each row of logits ---- */
 

@@ -28,6 +28,16 @@ class KVBatch(ctypes.Structure):
         super().__init__(n_seqs, n_tokens, max_pages, max_q, cu_q_ptr, kv_len_ptr, pages_ptr)
 
 
+class KVTables(ctypes.Structure):
+    """wv_kv_tables: which pages each sequence holds, how many positions, and how many sequences hold each page of
+    the pool; int32 device arrays (a new one: -1, 0, 0), and the table's own work array (KVCache.tables_work)."""
+    _fields_ = [("n_seqs", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("d_pages", ctypes.c_void_p),
+                ("d_kv_len", ctypes.c_void_p), ("d_refs", ctypes.c_void_p), ("d_work", ctypes.c_void_p)]
+
+    def __init__(self, n_seqs: int, max_pages: int, pages_ptr: int, kv_len_ptr: int, refs_ptr: int, work_ptr: int):
+        super().__init__(n_seqs, max_pages, pages_ptr, kv_len_ptr, refs_ptr, work_ptr)
+
+
 class KVCache:
     """Owns a wv_kv cache handle; freed with free() or on GC."""
 
@@ -67,6 +77,33 @@ class KVCache:
         nb = ctypes.c_size_t()
         check(lib().wv_kv_attention_scratch(self.handle, ctypes.byref(batch), n_heads, window, ctypes.byref(nb)))
         return nb.value
+
+    def tables_work(self, n_seqs: int, max_pages: int) -> int:
+        """Bytes of a table's work array."""
+        nb = ctypes.c_size_t()
+        check(lib().wv_kv_tables_work(self.handle, n_seqs, max_pages, ctypes.byref(nb)))
+        return nb.value
+
+    def fork_dev(self, tables: KVTables, parent_ptr: int, stream: int | None = None) -> None:
+        """Sequence b becomes sequence parent[b] (int32) as it was, all at once, sharing its pages; -1 empties it."""
+        check(lib().wv_kv_fork_dev(self.handle, ctypes.byref(tables), parent_ptr, stream))
+
+    def resize_dev(self, tables: KVTables, len_ptr: int, ok_ptr: int, stream: int | None = None) -> None:
+        """Sequence b to len[b] positions (int32): pages given back, or the lowest free ones taken and a shared last
+        page copied. ok[b] (int32) is 0 where the pool or the table had no room and b stayed as it was."""
+        check(lib().wv_kv_resize_dev(self.handle, ctypes.byref(tables), len_ptr, ok_ptr, stream))
+
+    def compact_dev(self, tables: KVTables, used_ptr: int | None = None, stream: int | None = None) -> None:
+        """Moves the pages that are held to the front of the pool; used (int32): how many there are."""
+        check(lib().wv_kv_compact_dev(self.handle, ctypes.byref(tables), used_ptr, stream))
+
+    def copy_pages_dev(self, src_ptr: int, dst_ptr: int, n: int, stream: int | None = None) -> None:
+        """n pages copied in all layers, src to dst (int32)."""
+        check(lib().wv_kv_copy_pages_dev(self.handle, src_ptr, dst_ptr, n, stream))
+
+    def slots_dev(self, batch: KVBatch, slots_ptr: int, pos_ptr: int | None = None, stream: int | None = None) -> None:
+        """Slot (int64) and position (int32) of every row of a batch."""
+        check(lib().wv_kv_slots_dev(self.handle, ctypes.byref(batch), slots_ptr, pos_ptr, stream))
 
     def free(self) -> None:
         if self.handle:
