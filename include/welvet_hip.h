@@ -590,6 +590,60 @@ typedef struct wv_rope_rows {
 int wv_rope_dev(uint64_t rope, const int32_t *d_pos, int32_t n, const wv_rope_rows *q, const wv_rope_rows *k,
                 void *stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection ---- */
+
+/* A handle holds the adapters of one projection (rows x cols): A, rank x cols,
+ * and B, rows x rank, as 16-bit floats, and a scale, for each of n_adapters. */
+#define WV_ADAPTER_F16 0
+#define WV_ADAPTER_BF16 1
+typedef struct wv_adapters_config {
+    int32_t rows, cols;  /* at most 2^24 */
+    int32_t max_rank;    /* 1 to 256 */
+    int32_t n_adapters;  /* at most 2^20 */
+    int32_t type;        /* WV_ADAPTER_* */
+} wv_adapters_config;
+/* Allocates on the current device; every adapter is unset (rank 0). */
+int wv_adapters_create(const wv_adapters_config *cfg, uint64_t *adapters);
+/* Adapter `index`: host arrays a [rank][cols] and b [rows][rank] of the set's
+ * type (copied), its scale; rank 0 unsets it. Waits for the device's work, so
+ * that calls before it see the old adapter and those after it the new one. */
+int wv_adapters_set(uint64_t adapters, int32_t index, int32_t rank, float scale, const uint16_t *a,
+                    const uint16_t *b);
+/* Releases a set once its work is done (waits for the device). */
+int wv_adapters_free(uint64_t adapters);
+
+/* The token rows of n_seqs sequences in one batch, laid out as in wv_kv_batch:
+ * sequence b owns rows d_cu_q[b] .. d_cu_q[b+1]-1 of n_tokens (at most 65535)
+ * and adapter d_adapter[b] (outside the set, -1 say, or unset: none). Device
+ * arrays, read when the work runs. */
+typedef struct wv_adapter_batch {
+    int32_t n_seqs, n_tokens;
+    int32_t max_q;            /* most tokens of one sequence, 0: unknown. Steers the launch only. */
+    const int32_t *d_cu_q;    /* [n_seqs + 1] */
+    const int32_t *d_adapter; /* [n_seqs] */
+} wv_adapter_batch;
+/* What one set adds to: row t of y at t * y_stride floats (0: rows), of base at
+ * t * base_stride. d_base NULL: y itself. Otherwise y may be base at the same
+ * stride, but overlap neither it nor x in another way. */
+typedef struct wv_adapter_rows {
+    uint64_t adapters;
+    float *d_y;
+    const float *d_base;
+    int64_t y_stride, base_stride;
+} wv_adapter_rows;
+/* y_t = base_t + scale_a B_a (A_a x_t) for each of 1 to 4 sets over the same
+ * rows x (Q, K and V; gate and up): as many columns, one type, one device.
+ * Rows of a sequence without an adapter are base_t, padding rows are left as
+ * they are. x, base and y are f32 (row t of x at t * x_stride, 0: cols); the
+ * products A x lie in f32 in d_scratch (wv_adapters_scratch bytes, 16-byte
+ * aligned, held by the call until its work is done), or, with NULL, in the
+ * library's own scratch, which a call under capture is refused. The sums have a
+ * fixed order. Device pointers, enqueued on `stream`. */
+int wv_adapters_dev(const wv_adapter_batch *batch, const float *d_x, int64_t x_stride, const wv_adapter_rows *sets,
+                    int32_t n_sets, void *d_scratch, size_t scratch_bytes, void *stream);
+/* Scratch bytes of such a call. Only the batch's sizes and the sets' handles are read. */
+int wv_adapters_scratch(const wv_adapter_batch *batch, const wv_adapter_rows *sets, int32_t n_sets, size_t *bytes);
+
 /* ---- sampling: the next token of each row of logits ---- */
 
 /* How each row's token is drawn: arrays of one value per row (device arrays

@@ -30,7 +30,7 @@ HIP_FLAGS = [
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-pthread", "-ffp-contract=off", "-Wall"]
 
 HIP_SOURCES = ["runtime.hip", "gemv.hip", "gemv_rpl.hip", "gemv_batch.hip", "gemm_rpl.hip", "decode.hip", "native.hip", "kv_cache.hip",
-               "kv_attention.hip", "kv_pages.hip", "rope.hip", "sample.hip"]
+               "kv_attention.hip", "kv_pages.hip", "rope.hip", "adapters.hip", "sample.hip"]
 CXX_SOURCES = ["pack.cpp"]
 GEMM_PARTS = 8  # kGemmParts of csrc/gemm_tiles.h
 
