@@ -535,6 +535,31 @@ int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch *batch,
 int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch *batch, int32_t n_heads, int32_t window,
                             size_t *bytes);
 
+/* Sequences of a batch that share their first keys (one prompt sampled many
+ * times, one instruction before many requests). Group g is the sequences
+ * d_cu_seq[g] .. d_cu_seq[g+1]-1 (ascending; sequences before the first and
+ * behind the last group stand alone) and its positions 0 .. d_shared[g]-1: all
+ * of its sequences hold the same rows there, in the same pages or in copies. */
+typedef struct wv_kv_groups {
+    int32_t n_groups;
+    int32_t max_shared; /* most shared positions of a group, 0: unknown. Steers the launch only. */
+    const int32_t *d_cu_seq; /* [n_groups + 1] */
+    const int32_t *d_shared; /* [n_groups] */
+} wv_kv_groups;
+/* wv_kv_attention_dev where the shared keys of a group are read once for all of
+ * its rows (from the pages of its first sequence), with every sequence's own
+ * keys behind them: the same arguments, results within the same bounds. The
+ * shared and the own keys' partial rows lie in d_scratch
+ * (wv_kv_attention_shared_scratch bytes, as there), or, with NULL, in the
+ * library's own; a call with NULL on a stream under capture reads the shared
+ * keys once for each sequence. Device arrays, read when the work runs. */
+int wv_kv_attention_shared_dev(uint64_t cache, int32_t layer, const wv_kv_batch *batch, const wv_kv_groups *groups,
+                               const float *d_q, int64_t q_stride, int32_t n_heads, float scale, int32_t window,
+                               float *d_out, int64_t out_stride, void *d_scratch, size_t scratch_bytes, void *stream);
+/* Scratch bytes of such a call. Only the batch's and the groups' sizes are read. */
+int wv_kv_attention_shared_scratch(uint64_t cache, const wv_kv_batch *batch, const wv_kv_groups *groups,
+                                   int32_t n_heads, int32_t window, size_t *bytes);
+
 /* ---- rotary positions ---- */
 
 /* A rotation of heads of head_dim values (2 to 1024): with t = pos f_i, pair i

@@ -46,7 +46,7 @@ EXPORTS = (
     "wv_decoder_create", "wv_decoder_set_layer", "wv_decoder_set_output", "wv_decoder_set_kv",
     "wv_decoder_use_graph", "wv_decoder_generate", "wv_decoder_prefill", "wv_decoder_free",
     "wv_kv_create", "wv_kv_info", "wv_kv_free", "wv_kv_write_dev", "wv_kv_read_dev", "wv_kv_attention_dev",
-    "wv_kv_attention_scratch", "wv_kv_tables_work", "wv_kv_fork_dev", "wv_kv_resize_dev", "wv_kv_compact_dev",
+    "wv_kv_attention_scratch", "wv_kv_attention_shared_dev", "wv_kv_attention_shared_scratch", "wv_kv_tables_work", "wv_kv_fork_dev", "wv_kv_resize_dev", "wv_kv_compact_dev",
     "wv_kv_copy_pages_dev", "wv_kv_slots_dev", "wv_rope_create", "wv_rope_free", "wv_rope_dev",
     "wv_adapters_create", "wv_adapters_set", "wv_adapters_free", "wv_adapters_dev", "wv_adapters_scratch",
     "wv_sample_dev",
@@ -124,6 +124,9 @@ def lib():
     L.wv_kv_attention_dev.argtypes = [ctypes.c_uint64, ctypes.c_int32, _P, _P, _I64, ctypes.c_int32, ctypes.c_float,
                                       ctypes.c_int32, _P, _I64, _P, _SZ, _P]
     L.wv_kv_attention_scratch.argtypes = [ctypes.c_uint64, _P, ctypes.c_int32, ctypes.c_int32, _P]
+    L.wv_kv_attention_shared_dev.argtypes = [ctypes.c_uint64, ctypes.c_int32, _P, _P, _P, _I64, ctypes.c_int32,
+                                             ctypes.c_float, ctypes.c_int32, _P, _I64, _P, _SZ, _P]
+    L.wv_kv_attention_shared_scratch.argtypes = [ctypes.c_uint64, _P, _P, ctypes.c_int32, ctypes.c_int32, _P]
     L.wv_kv_tables_work.argtypes = [ctypes.c_uint64, ctypes.c_int32, ctypes.c_int32, _P]
     L.wv_kv_fork_dev.argtypes = [ctypes.c_uint64, _P, _P, _P]
     L.wv_kv_resize_dev.argtypes = [ctypes.c_uint64, _P, _P, _P, _P]

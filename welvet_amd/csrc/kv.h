@@ -86,6 +86,10 @@ struct KvAttn {
     bool many;  // long sequences by the kernel of 128-row tiles
     bool once;  // one block reads a sequence's keys of a KV head
     float scale;
+    // Sequences in groups that share their first keys: of the splits the first `lead` are ranges of a group's shared
+    // keys, which all of its rows take from its first sequence's pages, the others ranges of a sequence's own.
+    const int32_t *group_cu, *group_shared;
+    int n_groups, lead;
 };
 // Which kernels a call takes and into how many key ranges it is cut (max_pages: as many as sequences hold), and
 // the floats of its partials.
@@ -96,5 +100,14 @@ struct KvPlan {
 KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window);
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits);
 int launch_kv_attn(const KvAttn& a, hipStream_t s);
+// With groups: whether they are worth it, the shared keys' rows by the kernel of 128-row tiles, and into how many
+// ranges the shared and the own keys are cut.
+struct KvGroupPlan {
+    bool use, lead_many;
+    int lead, own;
+};
+KvGroupPlan kv_attn_group_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads,
+                               int window, int n_groups, int max_shared);
+int launch_kv_attn_groups(const KvAttn& a, const KvGroupPlan& p, hipStream_t s);
 
 }  // namespace wv

@@ -15,6 +15,7 @@
 // in the block has a part in a row's bits), and are split as ph + pl the same way.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv.h"
 #include "rt_internal.h"
@@ -108,7 +109,29 @@ __device__ __forceinline__ uint32_t max_of_32(float v) {
 struct Tile {
     int seq = -1, r0 = 0, rows = 0;  // first row of the tile, rows of the sequence
     int q0 = 0, n = 0, kv_len = 0;   // the sequence's first token row, new tokens, keys
+    int from = 0, seq_end = 0;       // first key of its own; a group's sequences are seq .. seq_end - 1
 };
+
+// What a block's rows attend over: a sequence's keys; its own keys alone, where it is in a group; the keys that a
+// group shares.
+constexpr int kWhole = 0, kOwn = 1, kLead = 2;
+
+// Keys that group g shares, as whole blocks: the rest are taken as each sequence's own.
+__device__ __forceinline__ int group_keys(const KvAttn& a, int g) {
+    return min(max(a.group_shared[g], 0), a.max_pages << a.c.page_shift) & ~31;
+}
+// The group of a sequence: 64 at a time. False: none.
+__device__ __forceinline__ bool find_group(const KvAttn& a, int seq, int& g) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.n_groups; base += 64) {
+        const int i = base + lane;
+        const uint64_t m = __ballot(i < a.n_groups && a.group_cu[i + 1] > seq);
+        if (!m) continue;
+        g = base + __builtin_ctzll(m);
+        return a.group_cu[g] <= seq;
+    }
+    return false;
+}
 
 // Tile `idx` of the batch's tiles of RT rows, over the sequences with at
 // least min_rows and at most max_rows rows, in order of the sequences: every
@@ -149,23 +172,110 @@ __device__ __forceinline__ bool find_tile(const KvAttn& a, int G, int idx, int m
     return false;
 }
 
-// The 32-key blocks [begin, end) that split `sp` of a tile's rows
-// r0 .. r0 + RT - 1 walks, and the positions of its first and last row.
+// The same over the groups' rows (kLead), or over the sequences with the first key of their own (kOwn).
+template <int RT, int MODE>
+__device__ __forceinline__ bool find_group_tile(const KvAttn& a, int G, int idx, int min_rows, int max_rows, Tile& t) {
+    if constexpr (MODE == kOwn) {
+        if (!find_tile<RT>(a, G, idx, min_rows, max_rows, t)) return false;
+        int g;
+        if (find_group(a, t.seq, g)) t.from = group_keys(a, g);
+        return true;
+    }
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.n_groups; base += 64) {
+        const int g = base + lane;
+        int s0 = 0, s1 = 0, c0 = 0, n = 0, tiles = 0;
+        if (g < a.n_groups) {
+            s0 = min(max(a.group_cu[g], 0), a.n_seqs);
+            s1 = min(max(a.group_cu[g + 1], s0), a.n_seqs);
+            c0 = min(max(a.cu[s0], 0), a.n_tokens);
+            n = min(max(a.cu[s1], c0), a.n_tokens) - c0;
+            const int rows = n * G;
+            if (rows >= min_rows && rows <= max_rows) tiles = (rows + RT - 1) / RT;
+        }
+        int incl = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += o;
+        }
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        if (idx < total) {
+            const int w = __builtin_ctzll(__ballot(incl > idx));
+            t.seq = __builtin_amdgcn_readlane(s0, w);
+            t.seq_end = __builtin_amdgcn_readlane(s1, w);
+            t.q0 = __builtin_amdgcn_readlane(c0, w);
+            t.n = __builtin_amdgcn_readlane(n, w);
+            t.rows = t.n * G;
+            t.r0 = (idx - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(tiles, w))) * RT;
+            t.kv_len = group_keys(a, base + w);
+            return true;
+        }
+        idx -= total;
+    }
+    return false;
+}
+
+// The 32-key blocks [begin, end) of range `sp` that a tile walks, and the positions of its first and last row (of a
+// group's: the least and the largest).
 struct Range {
     int begin, end, p_first, p_last, limit;
 };
-template <int RT>
-__device__ __forceinline__ Range tile_range(const KvAttn& a, const Tile& t, int G, int sp, int least) {
+// The sequences of a group's token rows tok0 .. tok1 (counted from its first): the lane's own position, the least and
+// the largest. 64 sequences at a time, one turn for each that the rows touch.
+__device__ __forceinline__ void group_positions(const KvAttn& a, const Tile& t, int tok0, int tok1, int mine, int& pos,
+                                                int& least, int& most) {
+    const int lane = threadIdx.x & 63;
+    pos = -1, least = INT32_MAX, most = -1;
+    int tok = tok0;
+    for (int base = t.seq; base < t.seq_end && tok <= tok1; base += 64) {
+        const int s = base + lane;
+        int end = INT32_MAX, len = 0;
+        if (s < t.seq_end) {
+            end = min(a.cu[s + 1], a.n_tokens);
+            len = max(a.kv_len[s], 0);
+        }
+        while (tok <= tok1) {
+            const uint64_t m = __ballot(end > t.q0 + tok);
+            if (!m) break;
+            const int w = __builtin_ctzll(m);
+            const int e = __builtin_amdgcn_readlane(end, w), at = __builtin_amdgcn_readlane(len, w) - e + t.q0;
+            if (e == INT32_MAX) return;
+            const int last = min(tok1, e - t.q0 - 1);
+            if (mine >= tok && mine <= last) pos = at + mine;
+            least = min(least, at + tok);
+            most = max(most, at + last);
+            tok = last + 1;
+        }
+    }
+}
+// Positions of the rows r0 .. r0 + count - 1 of a tile, and of the lane's row.
+template <int MODE>
+__device__ __forceinline__ void row_positions(const KvAttn& a, const Tile& t, int G, int r0, int count, int row,
+                                              int& pos, int& first, int& last) {
+    const int end = min(r0 + count - 1, t.rows - 1);
+    if constexpr (MODE == kLead) {
+        group_positions(a, t, r0 / G, end / G, row / G, pos, first, last);
+    } else {
+        pos = t.kv_len - t.n + row / G;
+        first = t.kv_len - t.n + r0 / G;
+        last = t.kv_len - t.n + end / G;
+    }
+}
+template <int MODE>
+__device__ __forceinline__ Range tile_range(const KvAttn& a, const Tile& t, int p_first, int p_last, int sp, int least) {
     Range r;
-    r.limit = min(t.kv_len, a.max_pages << a.c.page_shift);
-    r.p_first = t.kv_len - t.n + t.r0 / G;
-    r.p_last = t.kv_len - t.n + min(t.r0 + RT - 1, t.rows - 1) / G;
-    const int lo = a.window > 0 ? max(0, r.p_first - a.window + 1) : 0;
+    r.limit = MODE == kLead ? t.kv_len : min(t.kv_len, a.max_pages << a.c.page_shift);
+    r.p_first = p_first;
+    r.p_last = p_last;
+    int lo = a.window > 0 ? max(0, r.p_first - a.window + 1) : 0;
+    if (MODE == kOwn) lo = max(lo, t.from);
     const int hi = min(r.limit - 1, r.p_last);
     r.begin = lo >> 5;
     r.end = hi >= lo ? (hi >> 5) + 1 : r.begin;
     const int nb = r.end - r.begin;
-    const int chunk = max(least, (nb + a.splits - 1) / a.splits);
+    const int ranges = MODE == kLead ? a.lead : MODE == kOwn ? a.splits - a.lead : a.splits;
+    const int chunk = max(least, (nb + ranges - 1) / ranges);
     r.begin = min(r.begin + sp * chunk, r.end);
     r.end = min(r.begin + chunk, r.end);
     return r;
@@ -195,7 +305,7 @@ __device__ __forceinline__ float row_unit(float amax, float scale, float& inv) {
 // ONCE: no other block reads a sequence's keys, and they are loaded past the
 // caches (131071 fp16 keys 106 us, else 112); not where several tiles read them
 // (64 tokens of 32 heads over 8000 fp16 keys 56 us so, else 43).
-template <int HD, int TYPE, bool ONCE>
+template <int HD, int TYPE, bool ONCE, int MODE>
 __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t, int kvh, int sp) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
     constexpr int S = HD / 32;                   // k steps of a score product
@@ -207,13 +317,14 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
     __shared__ float red[4][16][LD];
     __shared__ float rm[4][16], rl[4][16];
 
-    const Range rg = tile_range<16>(a, t, G, sp, 4);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
 
     const int row = t.r0 + n;
     const bool live = row < t.rows;
-    const int pos = t.kv_len - t.n + (live ? row : t.r0) / G;
+    int pos, p_first, p_last;
+    row_positions<MODE>(a, t, G, t.r0, 16, live ? row : t.r0, pos, p_first, p_last);
+    const Range rg = tile_range<MODE>(a, t, p_first, p_last, sp, 4);
     const int first = a.window > 0 ? pos - a.window + 1 : 0;
 
     // the query row: dims of lane group g in the order of the K codes
@@ -421,7 +532,7 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] *= inv;
-    float* dst = a.part ? a.part + ((int64_t(tok) * a.n_heads + head) * a.splits + sp) * LD
+    float* dst = a.part ? a.part + ((int64_t(tok) * a.n_heads + head) * a.splits + sp + (MODE == kOwn ? a.lead : 0)) * LD
                         : a.out + int64_t(tok) * a.os + head * HD;
 #pragma unroll
     for (int d = c; d < HD; d += 16) {
@@ -453,7 +564,15 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     } else if (!find_tile<16>(a, G, ONCE ? y - a.n_seqs : y, 1, max_rows, t, ONCE)) {
         return;
     }
-    attn_rows<HD, TYPE, ONCE>(a, G, t, blockIdx.x, blockIdx.z);
+    attn_rows<HD, TYPE, ONCE, kWhole>(a, G, t, blockIdx.x, blockIdx.z);
+}
+
+// The same rows with their sequences in groups. MODE kLead: a tile's rows are of a group, over the keys it shares.
+template <int HD, int TYPE, bool ONCE, int MODE>
+__global__ void __launch_bounds__(256, 2) k_kv_attn_group_rows(KvAttn a, int G, int max_rows, int tile0) {
+    Tile t;
+    if (!find_group_tile<16, MODE>(a, G, tile0 + int(blockIdx.y), 1, max_rows, t)) return;
+    attn_rows<HD, TYPE, ONCE, MODE>(a, G, t, blockIdx.x, blockIdx.z);
 }
 
 // Many rows: 128 query rows of one sequence and KV head per block, 32 to a
@@ -480,7 +599,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // tile runs alone on its CU. Dropped, since they gained nothing: two groups of
 // four waves half a tile apart, or on halves of the keys; a barrier every second
 // step; steps of 64 keys.
-template <int HD, int TYPE>
+template <int HD, int TYPE, int MODE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
     constexpr int BB = 32 * HD * E;   // bytes of a block's codes
@@ -502,18 +621,25 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const bool once = gridDim.x * gridDim.y * gridDim.z <= 512;
     const int idx = tile0 + (once && y >= half ? y - half : int(gridDim.y) - 1 - y);
     Tile t;
-    if (!find_tile<128>(a, G, idx, min_rows, INT32_MAX, t)) return;
-    const Range rg = tile_range<128>(a, t, G, sp, 8);
+    if constexpr (MODE == kWhole) {
+        if (!find_tile<128>(a, G, idx, min_rows, INT32_MAX, t)) return;
+    } else {
+        if (!find_group_tile<128, MODE>(a, G, idx, min_rows, INT32_MAX, t)) return;
+    }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
 
     const int wr0 = t.r0 + 32 * wave;  // the wave's first row
     const bool busy = wr0 < t.rows;
     const int row = min(wr0 + n, t.rows - 1);
-    const int pos = t.kv_len - t.n + row / G;
+    int pos, w_first, w_last, p_first, p_last;  // positions of the lane's row, of the wave's rows, of the tile's
+    row_positions<MODE>(a, t, G, t.r0, 128, row, pos, p_first, p_last);
+    if constexpr (MODE == kLead)
+        row_positions<MODE>(a, t, G, min(wr0, t.rows - 1), 32, row, pos, w_first, w_last);
+    else
+        w_first = t.kv_len - t.n + min(wr0, t.rows - 1) / G, w_last = t.kv_len - t.n + min(wr0 + 31, t.rows - 1) / G;
+    const Range rg = tile_range<MODE>(a, t, p_first, p_last, sp, 8);
     const int first = a.window > 0 ? pos - a.window + 1 : 0;
-    const int w_first = t.kv_len - t.n + min(wr0, t.rows - 1) / G;       // positions of the wave's first
-    const int w_last = t.kv_len - t.n + min(wr0 + 31, t.rows - 1) / G;   // and last row
 
     const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
     const int pb = a.c.page_shift - 5;
@@ -812,7 +938,8 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const int head = kvh * G + row % G;
     const float back = ldexpf(1.0f, int(er));
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // back / l may be subnormal
-    float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
+    float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp + (MODE == kOwn ? a.lead : 0)) * LD
+                        : a.out + orow * a.os + head * HD;
     const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
 #pragma unroll
     for (int i = 0; i < T; ++i)
@@ -838,17 +965,22 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
 // The key ranges of one (token, head) row joined: the ranges' maxima and sums
 // weigh their rows, each divided by its own sum already, added in the order of
 // the ranges by four waves.
-// 3 us for one token's 32 rows of 10 ranges: a launch.
-template <int HD>
+// 3 us for one token's 32 rows of 10 ranges: a launch. GROUPS: rows of no group
+// have no shared keys' ranges.
+template <int HD, bool GROUPS>
 __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
     constexpr int LD = HD + 4, W = HD / 64;
     __shared__ float red[4][HD];
     const int tok = blockIdx.x, head = blockIdx.y;
     if (tok < a.cu[0] || tok >= min(a.cu[a.n_seqs], a.n_tokens)) return;
     const float* p = a.part + (int64_t(tok) * a.n_heads + head) * a.splits * LD;
+    int splits = a.splits;
+    if (GROUPS && (tok < a.cu[min(max(a.group_cu[0], 0), a.n_seqs)] ||
+                   tok >= a.cu[min(max(a.group_cu[a.n_groups], 0), a.n_seqs)]))
+        p += a.lead * LD, splits -= a.lead;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float m = -INFINITY, l = 0.0f;
-    if (lane < a.splits) {
+    if (lane < splits) {
         m = p[lane * LD + HD];
         l = p[lane * LD + HD + 1];
     }
@@ -859,18 +991,18 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
     float x[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) x[i] = 0.0f;
-    for (int s0 = wave; s0 < a.splits; s0 += 16) {  // four ranges' rows in flight
+    for (int s0 = wave; s0 < splits; s0 += 16) {  // four ranges' rows in flight
         float y[4][W];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int i = 0; i < W; ++i) y[k][i] = s0 + 4 * k < a.splits ? p[(s0 + 4 * k) * LD + W * lane + i] : 0.0f;
+            for (int i = 0; i < W; ++i) y[k][i] = s0 + 4 * k < splits ? p[(s0 + 4 * k) * LD + W * lane + i] : 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (s0 + 4 * k) & 63));
 #pragma unroll
             for (int i = 0; i < W; ++i)
-                if (s0 + 4 * k < a.splits) x[i] += ws * y[k][i];
+                if (s0 + 4 * k < splits) x[i] += ws * y[k][i];
         }
     }
 #pragma unroll
@@ -968,19 +1100,67 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
         const int64_t tiles = (rows + 127) / 128 + a.n_seqs;
         const int least = few ? kFewRows + 1 : 1;
         if (a.c.hd == 128)
-            f16 ? go(k_kv_attn_tile<128, WV_KV_F16>, tiles, least)
-                : go(k_kv_attn_tile<128, WV_KV_Q8>, tiles, least);
+            f16 ? go(k_kv_attn_tile<128, WV_KV_F16, kWhole>, tiles, least)
+                : go(k_kv_attn_tile<128, WV_KV_Q8, kWhole>, tiles, least);
         else
-            f16 ? go(k_kv_attn_tile<64, WV_KV_F16>, tiles, least)
-                : go(k_kv_attn_tile<64, WV_KV_Q8>, tiles, least);
+            f16 ? go(k_kv_attn_tile<64, WV_KV_F16, kWhole>, tiles, least)
+                : go(k_kv_attn_tile<64, WV_KV_Q8, kWhole>, tiles, least);
     }
     if (a.splits > 1) {
         const dim3 jg{unsigned(a.n_tokens), unsigned(a.n_heads)};
         if (a.c.hd == 128)
-            hipLaunchKernelGGL(k_kv_attn_join<128>, jg, dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_kv_attn_join<128, false>), jg, dim3(256), 0, s, a);
         else
-            hipLaunchKernelGGL(k_kv_attn_join<64>, jg, dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_kv_attn_join<64, false>), jg, dim3(256), 0, s, a);
     }
+    return int(hipGetLastError());
+}
+
+// The same for a batch whose sequences are in groups: the groups' rows over the shared keys, then every sequence's
+// rows over its own.
+KvGroupPlan kv_attn_group_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads,
+                               int window, int n_groups, int max_shared) {
+    KvGroupPlan p{};
+    const int64_t width = int64_t(max_pages) << c.page_shift;
+    const int64_t shared = max_shared > 0 ? std::min<int64_t>(max_shared, width) : width;
+    if (n_groups <= 0 || n_tokens <= 0 || n_seqs <= 1 || shared < 32) return p;
+    const int64_t G = n_heads / c.n_kv, rows = n_tokens * G;
+    const int64_t t16 = (rows + 15) / 16 * c.n_kv, t128 = (rows + 127) / 128 * c.n_kv;
+    const int64_t blocks = shared / 32, own = std::max<int64_t>((width - shared + 31) / 32, 1);
+    p.use = true;
+    p.lead_many = rows / n_groups >= 1024;
+    p.lead = int(std::max<int64_t>(1, std::min<int64_t>({p.lead_many ? 512 / t128 : 1024 / t16, blocks / 4, 48})));
+    p.own = int(std::max<int64_t>(1, std::min<int64_t>({1024 / t16, own / 8, 16})));
+    return p;
+}
+
+int launch_kv_attn_groups(const KvAttn& a, const KvGroupPlan& p, hipStream_t s) {
+    const int G = a.n_heads / a.c.n_kv;
+    const int64_t rows = int64_t(a.n_tokens) * G;
+    const bool f16 = a.c.type == WV_KV_F16;
+    auto go = [&](auto kern, int64_t tiles, int ranges, int bound) {
+        for (int64_t t0 = 0; t0 < tiles; t0 += kMaxGridY) {
+            const dim3 grid{unsigned(a.c.n_kv), unsigned(std::min<int64_t>(tiles - t0, kMaxGridY)), unsigned(ranges)};
+            hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, G, bound, int(t0));
+        }
+    };
+    auto pick = [&](auto hd, auto type) {
+        constexpr int HD = decltype(hd)::value, TYPE = decltype(type)::value;
+        if (p.lead_many)
+            go(k_kv_attn_tile<HD, TYPE, kLead>, (rows + 127) / 128 + a.n_groups, p.lead, 1);
+        else
+            go(k_kv_attn_group_rows<HD, TYPE, false, kLead>, (rows + 15) / 16 + a.n_groups, p.lead, INT32_MAX);
+        go(k_kv_attn_group_rows<HD, TYPE, true, kOwn>, (rows + 15) / 16 + a.n_seqs, p.own, INT32_MAX);
+        hipLaunchKernelGGL((k_kv_attn_join<HD, true>), dim3(unsigned(a.n_tokens), unsigned(a.n_heads)), dim3(256), 0, s, a);
+    };
+    std::integral_constant<int, 128> h128;
+    std::integral_constant<int, 64> h64;
+    std::integral_constant<int, WV_KV_F16> t16;
+    std::integral_constant<int, WV_KV_Q8> t8;
+    if (a.c.hd == 128)
+        f16 ? pick(h128, t16) : pick(h128, t8);
+    else
+        f16 ? pick(h64, t16) : pick(h64, t8);
     return int(hipGetLastError());
 }
 
@@ -1008,6 +1188,74 @@ int check_batch(const char* what, uint64_t cache, const wv_kv_batch* b, int32_t 
     return WV_OK;
 }
 
+int check_groups(const char* what, const wv_kv_groups* g) {
+    if (!g) return rt_fail(WV_E_ARG, "%s: nil groups", what);
+    if (g->n_groups < 0 || g->n_groups > 1 << 24 || g->max_shared < 0)
+        return rt_fail(WV_E_SHAPE, "%s: %d groups, max_shared %d", what, g->n_groups, g->max_shared);
+    if (g->n_groups && (!g->d_cu_seq || !g->d_shared)) return rt_fail(WV_E_ARG, "%s: nil cu_seq/shared", what);
+    return WV_OK;
+}
+
+// wv_kv_attention_dev, and with groups wv_kv_attention_shared_dev.
+int attention(const char* what, uint64_t cache, int32_t layer, const wv_kv_batch* batch, const wv_kv_groups* groups,
+              const float* d_q, int64_t q_stride, int32_t n_heads, float scale, int32_t window, float* d_out,
+              int64_t out_stride, void* d_scratch, size_t scratch_bytes, void* stream) {
+    KvCache c;
+    int rc = check_batch(what, cache, batch, n_heads, window, c);
+    if (rc) return rc;
+    if (layer < 0 || layer >= c.c.n_layers)
+        return rt_fail(WV_E_ARG, "%s: layer %d of %d", what, layer, c.c.n_layers);
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return rt_fail(WV_E_ARG, "%s: scale %g", what, double(scale));
+    const int64_t w = int64_t(n_heads) * c.c.head_dim;
+    if (!q_stride) q_stride = w;
+    if (!out_stride) out_stride = w;
+    if (q_stride < w || out_stride < w)
+        return rt_fail(WV_E_SHAPE, "%s: row strides %lld and %lld under the row's %lld floats", what,
+                       (long long)q_stride, (long long)out_stride, (long long)w);
+    if (d_q && d_q == d_out && q_stride != out_stride)  // rows written would be others' queries still to be read
+        return rt_fail(WV_E_SHAPE, "%s: out is q, at row strides of %lld and %lld", what, (long long)out_stride,
+                       (long long)q_stride);
+    if (!batch->n_seqs || !batch->n_tokens) return WV_OK;
+    if (!d_q || !d_out || !batch->d_cu_q || !batch->d_kv_len || (batch->max_pages && !batch->d_pages))
+        return rt_fail(WV_E_ARG, "%s: nil q/out/cu_q/kv_len/pages", what);
+    (void)hipSetDevice(c.device);
+    hipStream_t s = rt_stream(stream, c.device);
+    KvAttn a{};
+    a.c = c.layer(layer);
+    a.q = d_q, a.out = d_out, a.qs = q_stride, a.os = out_stride;
+    a.cu = batch->d_cu_q, a.kv_len = batch->d_kv_len, a.pages = batch->d_pages;
+    a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages;
+    a.n_heads = n_heads, a.window = std::min(window, 1 << 30), a.scale = scale;
+    KvGroupPlan gp{};
+    if (groups && groups->n_groups) {
+        gp = kv_attn_group_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, batch->max_q, n_heads, a.window,
+                                groups->n_groups, groups->max_shared);
+        a.group_cu = groups->d_cu_seq, a.group_shared = groups->d_shared, a.n_groups = groups->n_groups;
+        // its ranges are joined in scratch: a captured call without any attends over whole sequences
+        if (!d_scratch && rt_capturing(s)) gp.use = false;
+    }
+    const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, batch->max_q, n_heads, a.window);
+    a.splits = plan.splits, a.many = plan.many, a.once = plan.once;
+    if (gp.use) a.lead = gp.lead, a.splits = gp.lead + gp.own;
+    const size_t floats = kv_attn_part_floats(a.c, a.n_tokens, n_heads, a.splits);
+    RtScratch sc;
+    if (d_scratch) {
+        if (reinterpret_cast<uintptr_t>(d_scratch) & 15)
+            return rt_fail(WV_E_ARG, "%s: scratch not 16-byte aligned", what);
+        if (scratch_bytes < floats * sizeof(float))
+            return rt_fail(WV_E_SHAPE, "%s: %zu bytes of scratch, needs %zu", what, scratch_bytes,
+                           floats * sizeof(float));
+        if (floats) a.part = static_cast<float*>(d_scratch);
+    } else if (floats && rt_capturing(s)) {
+        a.splits = 1;  // what a replay writes must not lie in a slot that other calls take
+    } else if (floats) {
+        if ((rc = sc.get(floats, s, "wv_kv_attention: scratch"))) return rc;
+        a.part = sc.f();
+    }
+    const int e = gp.use ? launch_kv_attn_groups(a, gp, s) : launch_kv_attn(a, s);
+    return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_kv_attention: kernel launch");
+}
+
 }  // namespace
 
 extern "C" {
@@ -1028,51 +1276,32 @@ int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch* batch, int32_t n_
 int wv_kv_attention_dev(uint64_t cache, int32_t layer, const wv_kv_batch* batch, const float* d_q, int64_t q_stride,
                         int32_t n_heads, float scale, int32_t window, float* d_out, int64_t out_stride,
                         void* d_scratch, size_t scratch_bytes, void* stream) {
+    return attention("wv_kv_attention", cache, layer, batch, nullptr, d_q, q_stride, n_heads, scale, window, d_out,
+                     out_stride, d_scratch, scratch_bytes, stream);
+}
+
+int wv_kv_attention_shared_scratch(uint64_t cache, const wv_kv_batch* batch, const wv_kv_groups* groups,
+                                   int32_t n_heads, int32_t window, size_t* bytes) {
     KvCache c;
-    int rc = check_batch("wv_kv_attention", cache, batch, n_heads, window, c);
+    int rc = check_batch("wv_kv_attention_shared_scratch", cache, batch, n_heads, window, c);
+    if (!rc) rc = check_groups("wv_kv_attention_shared_scratch", groups);
     if (rc) return rc;
-    if (layer < 0 || layer >= c.c.n_layers)
-        return rt_fail(WV_E_ARG, "wv_kv_attention: layer %d of %d", layer, c.c.n_layers);
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return rt_fail(WV_E_ARG, "wv_kv_attention: scale %g", double(scale));
-    const int64_t w = int64_t(n_heads) * c.c.head_dim;
-    if (!q_stride) q_stride = w;
-    if (!out_stride) out_stride = w;
-    if (q_stride < w || out_stride < w)
-        return rt_fail(WV_E_SHAPE, "wv_kv_attention: row strides %lld and %lld under the row's %lld floats",
-                       (long long)q_stride, (long long)out_stride, (long long)w);
-    if (d_q && d_q == d_out && q_stride != out_stride)  // rows written would be others' queries still to be read
-        return rt_fail(WV_E_SHAPE, "wv_kv_attention: out is q, at row strides of %lld and %lld", (long long)out_stride,
-                       (long long)q_stride);
-    if (!batch->n_seqs || !batch->n_tokens) return WV_OK;
-    if (!d_q || !d_out || !batch->d_cu_q || !batch->d_kv_len || (batch->max_pages && !batch->d_pages))
-        return rt_fail(WV_E_ARG, "wv_kv_attention: nil q/out/cu_q/kv_len/pages");
-    (void)hipSetDevice(c.device);
-    hipStream_t s = rt_stream(stream, c.device);
-    KvAttn a{};
-    a.c = c.layer(layer);
-    a.q = d_q, a.out = d_out, a.qs = q_stride, a.os = out_stride;
-    a.cu = batch->d_cu_q, a.kv_len = batch->d_kv_len, a.pages = batch->d_pages;
-    a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages;
-    a.n_heads = n_heads, a.window = std::min(window, 1 << 30), a.scale = scale;
-    const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, batch->max_q, n_heads, a.window);
-    a.splits = plan.splits, a.many = plan.many, a.once = plan.once;
-    const size_t floats = kv_attn_part_floats(a.c, a.n_tokens, n_heads, a.splits);
-    RtScratch sc;
-    if (d_scratch) {
-        if (reinterpret_cast<uintptr_t>(d_scratch) & 15)
-            return rt_fail(WV_E_ARG, "wv_kv_attention: scratch not 16-byte aligned");
-        if (scratch_bytes < floats * sizeof(float))
-            return rt_fail(WV_E_SHAPE, "wv_kv_attention: %zu bytes of scratch, needs %zu", scratch_bytes,
-                           floats * sizeof(float));
-        if (floats) a.part = static_cast<float*>(d_scratch);
-    } else if (floats && rt_capturing(s)) {
-        a.splits = 1;  // what a replay writes must not lie in a slot that other calls take
-    } else if (floats) {
-        if ((rc = sc.get(floats, s, "wv_kv_attention: scratch"))) return rc;
-        a.part = sc.f();
-    }
-    const int e = launch_kv_attn(a, s);
-    return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_kv_attention: kernel launch");
+    if (!bytes) return rt_fail(WV_E_ARG, "wv_kv_attention_shared_scratch: nil bytes");
+    const KvView v = c.layer(0);
+    const KvGroupPlan gp = kv_attn_group_plan(v, batch->n_seqs, batch->n_tokens, batch->max_pages, batch->max_q, n_heads,
+                                              std::min(window, 1 << 30), groups->n_groups, groups->max_shared);
+    if (!gp.use) return wv_kv_attention_scratch(cache, batch, n_heads, window, bytes);
+    *bytes = kv_attn_part_floats(v, batch->n_tokens, n_heads, gp.lead + gp.own) * sizeof(float);
+    return WV_OK;
+}
+
+int wv_kv_attention_shared_dev(uint64_t cache, int32_t layer, const wv_kv_batch* batch, const wv_kv_groups* groups,
+                               const float* d_q, int64_t q_stride, int32_t n_heads, float scale, int32_t window,
+                               float* d_out, int64_t out_stride, void* d_scratch, size_t scratch_bytes, void* stream) {
+    const int rc = check_groups("wv_kv_attention_shared", groups);
+    if (rc) return rc;
+    return attention("wv_kv_attention_shared", cache, layer, batch, groups, d_q, q_stride, n_heads, scale, window, d_out,
+                     out_stride, d_scratch, scratch_bytes, stream);
 }
 
 }  // extern "C"

@@ -28,6 +28,16 @@ class KVBatch(ctypes.Structure):
         super().__init__(n_seqs, n_tokens, max_pages, max_q, cu_q_ptr, kv_len_ptr, pages_ptr)
 
 
+class KVGroups(ctypes.Structure):
+    """wv_kv_groups: group g is the sequences cu_seq[g] .. cu_seq[g+1]-1 of a batch, which hold the same rows at their
+    first shared[g] positions; int32 device arrays. max_shared (most of these, 0: unknown) only steers the launch."""
+    _fields_ = [("n_groups", ctypes.c_int32), ("max_shared", ctypes.c_int32), ("d_cu_seq", ctypes.c_void_p),
+                ("d_shared", ctypes.c_void_p)]
+
+    def __init__(self, n_groups: int, cu_seq_ptr: int, shared_ptr: int, max_shared: int = 0):
+        super().__init__(n_groups, max_shared, cu_seq_ptr, shared_ptr)
+
+
 class KVTables(ctypes.Structure):
     """wv_kv_tables: which pages each sequence holds, how many positions, and how many sequences hold each page of
     the pool; int32 device arrays (a new one: -1, 0, 0), and the table's own work array (KVCache.tables_work)."""
@@ -76,6 +86,22 @@ class KVCache:
         """Bytes of scratch an attention call may be given (needed only for calls under graph capture)."""
         nb = ctypes.c_size_t()
         check(lib().wv_kv_attention_scratch(self.handle, ctypes.byref(batch), n_heads, window, ctypes.byref(nb)))
+        return nb.value
+
+    def attention_shared_dev(self, layer: int, batch: KVBatch, groups: KVGroups, q_ptr: int, out_ptr: int, n_heads: int,
+                             scale: float, window: int = 0, q_stride: int = 0, out_stride: int = 0,
+                             scratch_ptr: int | None = None, scratch_bytes: int = 0,
+                             stream: int | None = None) -> None:
+        """attention_dev with the keys that a group's sequences share read once for all of them."""
+        check(lib().wv_kv_attention_shared_dev(self.handle, layer, ctypes.byref(batch), ctypes.byref(groups), q_ptr,
+                                               q_stride, n_heads, scale, window, out_ptr, out_stride, scratch_ptr,
+                                               scratch_bytes, stream))
+
+    def attention_shared_scratch(self, batch: KVBatch, groups: KVGroups, n_heads: int, window: int = 0) -> int:
+        """Bytes of scratch such a call may be given (needed under graph capture to read shared keys once)."""
+        nb = ctypes.c_size_t()
+        check(lib().wv_kv_attention_shared_scratch(self.handle, ctypes.byref(batch), ctypes.byref(groups), n_heads,
+                                                   window, ctypes.byref(nb)))
         return nb.value
 
     def tables_work(self, n_seqs: int, max_pages: int) -> int:
