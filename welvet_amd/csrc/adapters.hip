@@ -9,6 +9,7 @@
 #include <cstring>
 #include <mutex>
 #include <new>
+#include <type_traits>
 #include <unordered_map>
 #include <vector>
 
@@ -21,7 +22,9 @@ namespace {
 
 constexpr int kMaxSets = 4;      // of a call
 constexpr int kMaxRank = 256;
-constexpr int kChunk = 512;      // columns that a wave takes at a time, 8 to a lane
+constexpr int kTile = 32;        // token rows of a block
+constexpr int kFew = 4;          // rows of a tile up to which they go one by one
+constexpr int kChunk = 512;      // columns that a wave takes at a time of such a row, 8 to a lane
 constexpr int kMaxRanges = 32;   // of the columns
 
 struct Set {
@@ -46,6 +49,8 @@ bool set_lookup(uint64_t h, Set& out) {
 }
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float g4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 // One set of a call as the kernels see it.
 struct SetArgs {
@@ -75,125 +80,434 @@ __device__ __forceinline__ float high(uint32_t w) {
     return TYPE == WV_ADAPTER_BF16 ? __uint_as_float(w & 0xffff0000) : float(__builtin_bit_cast(_Float16, uint16_t(w >> 16)));
 }
 
-// The sequence of row t, -1 behind the last one: 64 at a time, after a look at sequence t itself, which it is
-// wherever every sequence has one token.
-__device__ __forceinline__ int sequence_of(const Args& a, int t) {
-    if (t < a.n_seqs && a.cu[t] == t && a.cu[t + 1] == t + 1) return t;
-    const int lane = threadIdx.x & 63;
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-        const int s = s0 + lane;
-        const int end = s < a.n_seqs ? a.cu[s + 1] : INT32_MAX;
-        const uint64_t behind = __ballot(end > t);
-        if (!behind) continue;
-        const int b = s0 + __builtin_ctzll(behind);
-        return b < a.n_seqs && a.cu[b] <= t ? b : -1;
+// Up to 32 token rows of one sequence.
+struct Tile {
+    int t0, n, seq;
+};
+// Tile `idx`: the first one of sequence idx, then all further ones in order of the sequences, found 64 sequences at a
+// time (a decode step has none, and its blocks no search). False: there is none.
+__device__ __forceinline__ bool find_tile(const Args& a, int idx, Tile& t) {
+    if (idx < a.n_seqs) {
+        t.seq = idx;
+        t.t0 = min(max(a.cu[idx], 0), a.n_tokens);
+        t.n = min(min(max(a.cu[idx + 1], t.t0), a.n_tokens) - t.t0, kTile);
+        return t.n > 0;
     }
-    return -1;
+    idx -= a.n_seqs;
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < a.n_seqs; base += 64) {
+        const int s = base + lane;
+        int c0 = 0, n = 0;
+        if (s < a.n_seqs) {
+            c0 = min(max(a.cu[s], 0), a.n_tokens);
+            n = min(max(a.cu[s + 1], c0), a.n_tokens) - c0;
+        }
+        const int tiles = max((n + kTile - 1) / kTile - 1, 0);
+        int incl = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d, 64);
+            if (lane >= d) incl += o;
+        }
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        if (idx < total) {
+            const int w = __builtin_ctzll(__ballot(incl > idx));
+            const int skip = kTile * (1 + idx - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(tiles, w)));
+            t.seq = base + w;
+            t.t0 = __builtin_amdgcn_readlane(c0, w) + skip;
+            t.n = min(__builtin_amdgcn_readlane(n, w) - skip, kTile);
+            return true;
+        }
+        idx -= total;
+    }
+    return false;
 }
 
-// A token's h: a wave takes every fourth group of ranks, a lane 8 columns at a time.
+// What this wave's lanes wrote to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// 8 consecutive floats of a row, zeros behind its end.
+__device__ __forceinline__ void load8(const float* x, int c, int cols, float* v) {
+    if (c + 8 <= cols) {
+        const f4 lo = *reinterpret_cast<const f4*>(x + c), hi = *reinterpret_cast<const f4*>(x + c + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? x[c + i] : 0.0f;
+    }
+}
 template <int TYPE>
-__global__ void __launch_bounds__(256) k_adapt_down(Args a) {
-    const int t = blockIdx.y, range = blockIdx.x;
-    const SetArgs& s = a.set[blockIdx.z];
-    const int b = sequence_of(a, t);
-    if (b < 0) return;
-    const int id = a.which[b];
-    if (unsigned(id) >= unsigned(s.n_adapters)) return;
-    const int rank = s.rank[id];
+__device__ __forceinline__ void wide8(uint4 w, float* v) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = low<TYPE>(u[i]), v[2 * i + 1] = high<TYPE>(u[i]);
+}
+
+// h of a few tokens, one after the other: a wave takes every fourth group of four ranks, a lane 8 columns at a time.
+// The first loads do not wait for the adapter's rank (there are 16 rows in A at least).
+template <int TYPE>
+__device__ __forceinline__ void down_few(const Args& a, const SetArgs& s, const Tile& t, int id, int c0, int c1, float* h) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint16_t* A = s.a + int64_t(id) * s.R * s.C;
-    const float* x = a.x + int64_t(t) * a.xs;
-    float* h = s.h + (int64_t(range) * a.n_tokens + t) * s.R;
-    const int c0 = range * a.range, c1 = min(c0 + a.range, a.cols);
-    for (int r0 = 4 * wave; r0 < rank; r0 += 16) {
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int c = c0 + 8 * lane; c < c1; c += kChunk) {
-            float v[8];
-            if (c + 8 <= a.cols) {
-                const f4 lo = *reinterpret_cast<const f4*>(x + c), hi = *reinterpret_cast<const f4*>(x + c + 4);
+    const uint16_t* A = s.a + int64_t(id) * s.R * s.C + c0 + 8 * lane;
+    const int cl = c0 + 8 * lane;
+    uint4 w[4];
+    float v[8];
+    auto load = [&](const float* x, int r0, int c) {
+        load8(x, cl + c, a.cols, v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
-            } else {
+        for (int k = 0; k < 4; ++k)
+            w[k] = cl + c < c1 ? *reinterpret_cast<const uint4*>(A + int64_t(r0 + k) * s.C + c) : uint4{};
+    };
+    load(a.x + int64_t(t.t0) * a.xs, 4 * wave, 0);
+    const int rank = s.rank[id];
+    for (int n = 0; n < t.n; ++n) {
+        const float* x = a.x + int64_t(t.t0 + n) * a.xs;
+        for (int r0 = 4 * wave; r0 < rank; r0 += 16) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c = 0; c < c1 - c0; c += kChunk) {
+                if (n || c || r0 >= 16) load(x, r0, c);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = c + i < a.cols ? x[c + i] : 0.0f;
+                for (int k = 0; k < 4; ++k) {
+                    float f[8];
+                    wide8<TYPE>(w[k], f);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[k] = fmaf(f[i], v[i], sum[k]);
+                }
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint4 w = *reinterpret_cast<const uint4*>(A + int64_t(r0 + k) * s.C + c);
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sum[k] = fmaf(low<TYPE>(u[i]), v[2 * i], sum[k]);
-                    sum[k] = fmaf(high<TYPE>(u[i]), v[2 * i + 1], sum[k]);
-                }
+                const float y = wave_total(sum[k]);
+                if (lane == 0 && r0 + k < rank) h[int64_t(n) * s.R + r0 + k] = y;
             }
         }
+    }
+}
+
+// h of a tile of tokens, 32 NR ranks at a time, on f32 products of 32 ranks x 32 tokens x 2 columns: a lane holds the
+// same 16 columns of its rank's row and of its token's (lanes from 32 on the 16 behind those), straight from memory.
+// The block's waves take every fourth 32 columns and meet in LDS.
+template <int TYPE, int NR>
+__device__ __forceinline__ void down_tile(const Args& a, const SetArgs& s, const Tile& t, const uint16_t* A, int rank,
+                                          int c0, int c1, float* h, float* lds) {
+    constexpr int LD = 32 * NR + 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, hi = lane >> 5;
+    const float* x = a.x + int64_t(t.t0 + min(n, t.n - 1)) * a.xs;
+    for (int r0 = 0; r0 < rank; r0 += 32 * NR) {
+        f16v acc[NR];
+        const uint16_t* row[NR];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float y = wave_total(sum[k]);
-            if (lane == 0 && r0 + k < rank) h[r0 + k] = y;
+        for (int k = 0; k < NR; ++k) {
+            row[k] = A + int64_t(min(r0 + 32 * k + n, s.R - 1)) * s.C;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[k][i] = 0.0f;
+        }
+        float v[16];
+        uint4 w[NR][2];
+        auto load = [&](int c) {
+            load8(x, c, a.cols, v);
+            load8(x, c + 8, a.cols, v + 8);
+#pragma unroll
+            for (int k = 0; k < NR; ++k) {
+                w[k][0] = *reinterpret_cast<const uint4*>(row[k] + c);
+                w[k][1] = *reinterpret_cast<const uint4*>(row[k] + c + 8);
+            }
+        };
+        int c = c0 + 32 * wave + 16 * hi;
+        const int end = c1 + 16 * hi;  // c1 is a multiple of 32, and C one of 64: A is there
+        if (c < end) load(c);
+        while (c < end) {
+            float xv[16], wv[NR][16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) xv[i] = v[i];
+#pragma unroll
+            for (int k = 0; k < NR; ++k) wide8<TYPE>(w[k][0], wv[k]), wide8<TYPE>(w[k][1], wv[k] + 8);
+            c += 128;
+            if (c < end) load(c);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int k = 0; k < NR; ++k)
+                    acc[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(wv[k][i], xv[i], acc[k], 0, 0, 0);
+        }
+        // waves 2 and 3 to 0 and 1, then 1 to 0
+#pragma unroll
+        for (int step = 2; step >= 1; step /= 2) {
+            float* mine = lds + ((wave & (step - 1)) * 32 + n) * LD + 4 * hi;
+            __syncthreads();
+            if (wave >= step && wave < 2 * step) {
+#pragma unroll
+                for (int k = 0; k < NR; ++k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) mine[32 * k + 8 * q + i] = acc[k][4 * q + i];
+            }
+            __syncthreads();
+            if (wave < step) {
+#pragma unroll
+                for (int k = 0; k < NR; ++k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[k][4 * q + i] += mine[32 * k + 8 * q + i];
+            }
+        }
+        if (wave == 0 && n < t.n) {
+            float* d = h + int64_t(n) * s.R + r0 + 4 * hi;
+#pragma unroll
+            for (int k = 0; k < NR; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (r0 + 32 * k + 8 * q < s.R)
+                        *reinterpret_cast<f4*>(d + 32 * k + 8 * q) =
+                            f4{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
         }
     }
 }
 
-// y of 256 rows of one token.
-template <int TYPE>
-__global__ void __launch_bounds__(256) k_adapt_up(Args a) {
-    __shared__ float h[kMaxRank];
-    const int t = blockIdx.y, o = blockIdx.x * 256 + threadIdx.x;
+// FEW: the caller says that no sequence has more than kFew rows (if one has, its rows go one by one all the same).
+template <int TYPE, int NR, bool FEW>
+__global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
+    constexpr int ND = NR < 4 ? NR : 4;  // more would take all of a SIMD's registers for one wave
+    __shared__ float lds[FEW ? 1 : 2 * 32 * (32 * ND + 4)];
     const SetArgs& s = a.set[blockIdx.z];
-    if (blockIdx.x * 256 >= s.rows) return;
-    const int b = sequence_of(a, t);
-    if (b < 0) return;
-    const int id = a.which[b];
-    const int rank = unsigned(id) < unsigned(s.n_adapters) ? s.rank[id] : 0;
-    for (int r = threadIdx.x; r < s.R && rank; r += 256) {
-        float x = 0.0f;
-        if (r < rank)
-            for (int i = 0; i < a.ranges; ++i) x += s.h[(int64_t(i) * a.n_tokens + t) * s.R + r];
-        h[r] = x * s.scale[id];
-    }
-    __syncthreads();
-    if (o >= s.rows) return;
-    const float* base = s.base + t * s.bs + o;
-    float* y = s.y + t * s.ys + o;
-    if (!rank) {
-        if (base != y) *y = *base;
-        return;
-    }
-    const uint16_t* B = s.b + (int64_t(id) * s.rows + o) * s.R;
-    float sum = 0.0f;
-    for (int r = 0; r < rank; r += 8) {
-        const uint4 w = *reinterpret_cast<const uint4*>(B + r);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    Tile t;
+    if (!find_tile(a, tile0 + int(blockIdx.y), t)) return;
+    const int id = a.which[t.seq];
+    if (unsigned(id) >= unsigned(s.n_adapters)) return;
+    const int range = blockIdx.x, c0 = range * a.range;
+    float* h = s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R;
+    if (FEW || t.n <= kFew)
+        down_few<TYPE>(a, s, t, id, c0, min(c0 + a.range, a.cols), h);
+    else
+        down_tile<TYPE, ND>(a, s, t, s.a + int64_t(id) * s.R * s.C, s.rank[id], c0, min(c0 + a.range, s.C), h, lds);
+}
+
+// Rows of h into LDS (NR * 32 + 4 floats each), the ranges summed in their order, with the adapter's scale. What lies
+// behind the adapter's own ranks is anything until it is masked.
+template <int NR>
+__device__ __forceinline__ void stage_h(const Args& a, const SetArgs& s, const Tile& t, int n0, int rows, int rank,
+                                        float scale, float* h) {
+    constexpr int LD = 32 * NR + 4;
+    for (int i = threadIdx.x; i < 8 * NR * rows; i += 256) {
+        const int n = i / (8 * NR), r = 4 * (i % (8 * NR));
+        f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < s.R && n0 + n < t.n) {
+            const float* p = s.h + (int64_t(t.t0) + n0 + n) * s.R + r;
+            const int64_t step = int64_t(a.n_tokens) * s.R;
+            int k = 0;
+            for (; k + 4 <= a.ranges; k += 4) {
+                f4 y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sum = fmaf(low<TYPE>(u[i]), h[r + 2 * i], sum);
-            sum = fmaf(high<TYPE>(u[i]), h[r + 2 * i + 1], sum);
+                for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const f4*>(p + (k + j) * step);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x += y[j];
+            }
+            for (; k < a.ranges; ++k) x += *reinterpret_cast<const f4*>(p + k * step);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = r + j < rank ? x[j] * scale : 0.0f;
+        }
+        *reinterpret_cast<f4*>(h + n * LD + r) = x;
+    }
+}
+
+// y of the block's outputs for a few tokens, kFew at a time: a thread takes an output, and has its row of B on the
+// way before it looks at anything else.
+template <int TYPE, int NR>
+__device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Tile& t, int id, int first, int last,
+                                       const float* base, float* y, float* h) {
+    constexpr int LD = 32 * NR + 4, NB = NR < 2 ? 4 : 8;  // 16-byte units of B that are loaded ahead
+    const uint16_t* B = s.b + (int64_t(id) * s.rows + first) * s.R;
+    const int rank = s.rank[id];
+    const float scale = s.scale[id];
+    for (int n0 = 0; n0 < t.n; n0 += kFew) {
+        const int rows = min(t.n - n0, kFew);
+        for (int o = threadIdx.x; o - int(threadIdx.x) < last - first; o += 256) {
+            const bool in = o < last - first;
+            const uint16_t* row = B + int64_t(in ? o : 0) * s.R;
+            uint4 w[NB];
+#pragma unroll
+            for (int k = 0; k < NB; ++k) w[k] = 8 * k < s.R ? *reinterpret_cast<const uint4*>(row + 8 * k) : uint4{};
+            float sum[kFew];
+#pragma unroll
+            for (int n = 0; n < kFew; ++n) sum[n] = in && n < rows ? base[(n0 + n) * s.bs + first + o] : 0.0f;
+            if (o == int(threadIdx.x)) {
+                if (n0) __syncthreads();
+                stage_h<NR>(a, s, t, n0, rows, rank, scale, h);
+                __syncthreads();
+            }
+            float add[kFew] = {};
+            auto unit = [&](uint4 u, int r) {
+                float f[8];
+                wide8<TYPE>(u, f);
+#pragma unroll
+                for (int n = 0; n < kFew; ++n)
+                    if (n < rows)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) add[n] = fmaf(f[i], h[n * LD + r + i], add[n]);
+            };
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+                if (8 * k < rank) unit(w[k], 8 * k);
+            for (int r = 8 * NB; r < rank; r += 8) unit(*reinterpret_cast<const uint4*>(row + r), r);
+#pragma unroll
+            for (int n = 0; n < kFew; ++n)
+                if (in && n < rows) y[(n0 + n) * s.ys + first + o] = sum[n] + add[n];
         }
     }
-    *y = *base + sum;
 }
+
+// y of the block's outputs for a tile, on f32 products of 32 outputs x 32 tokens x 2 ranks. A lane ends with 16 outputs
+// of one token; through LDS they become four times 4 side by side, 8 lanes a row, as base and y are read and written.
+// The next outputs' B and base are on their way under the products.
+template <int TYPE, int NR>
+__device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const Tile& t, int id, int first, int last,
+                                        const float* base, float* y, float* h, float* swap) {
+    constexpr int LD = 32 * NR + 4, SW = 36;  // rows of 36 floats: 16 lanes' 16-byte accesses reach all banks
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, hi = lane >> 5, m = lane >> 3, o4 = 4 * (lane & 7);
+    const uint16_t* B = s.b + int64_t(id) * s.rows * s.R + 8 * hi;
+    uint4 w[2 * NR];
+    f4 was[4];
+    auto load = [&](int o0) {
+        const uint16_t* row = B + int64_t(min(o0 + n, last - 1)) * s.R;
+#pragma unroll
+        for (int k = 0; k < 2 * NR; ++k)
+            if (16 * k < s.R) w[k] = *reinterpret_cast<const uint4*>(row + 16 * k);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float* p = base + (8 * q + m) * s.bs + o0 + o4;
+            if (8 * q + m >= t.n) continue;
+            if (o0 + o4 + 4 <= last) {
+                was[q] = *reinterpret_cast<const f4*>(p);
+            } else {
+                for (int i = 0; i < 4; ++i)
+                    if (o0 + o4 + i < last) was[q][i] = p[i];
+            }
+        }
+    };
+    int o0 = first + 32 * wave;
+    if (o0 < last) load(o0);
+    stage_h<NR>(a, s, t, 0, 32, s.rank[id], s.scale[id], h);
+    __syncthreads();
+    float hv[2 * NR][8];
+#pragma unroll
+    for (int k = 0; k < 2 * NR; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hv[k][i] = h[n * LD + 16 * k + 8 * hi + i];
+    swap += wave * 32 * SW;
+    for (; o0 < last; o0 += 128) {
+        f16v acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+        f4 old[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) old[q] = was[q];
+        uint4 u[2 * NR];
+#pragma unroll
+        for (int k = 0; k < 2 * NR; ++k) u[k] = w[k];
+        if (o0 + 128 < last) load(o0 + 128);
+#pragma unroll
+        for (int k = 0; k < 2 * NR; ++k) {
+            if (16 * k >= s.R) continue;
+            float v[8];
+            wide8<TYPE>(u[k], v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v[i], hv[k][i], acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<g4*>(swap + n * SW + 8 * q + 4 * hi) = g4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+        wave_sync();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f4 x = old[q] + f4(*reinterpret_cast<const g4*>(swap + (8 * q + m) * SW + o4));
+            if (8 * q + m >= t.n) continue;
+            float* p = y + (8 * q + m) * s.ys + o0 + o4;
+            if (o0 + o4 + 4 <= last) {
+                *reinterpret_cast<f4*>(p) = x;
+            } else {
+                for (int i = 0; i < 4; ++i)
+                    if (o0 + o4 + i < last) p[i] = x[i];
+            }
+        }
+        wave_sync();
+    }
+}
+
+template <int TYPE, int NR, bool FEW>
+__global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) {
+    constexpr int LD = 32 * NR + 4;
+    __shared__ __align__(16) float h[(FEW ? kFew : 32) * LD];
+    __shared__ __align__(16) float swap[FEW ? 4 : 4 * 32 * 36];
+    const SetArgs& s = a.set[blockIdx.z];
+    const int first = blockIdx.x * 256 * turns;
+    if (first >= s.rows) return;
+    Tile t;
+    if (!find_tile(a, tile0 + int(blockIdx.y), t)) return;
+    const int id = a.which[t.seq];
+    const int last = min(first + 256 * turns, s.rows);
+    const float* base = s.base + t.t0 * s.bs;
+    float* y = s.y + t.t0 * s.ys;
+    const bool known = unsigned(id) < unsigned(s.n_adapters);
+    if (known && (FEW || t.n <= kFew)) {
+        up_few<TYPE, NR>(a, s, t, id, first, last, base, y, h);
+    } else if (!FEW && known && s.rank[id]) {
+        up_tile<TYPE, NR>(a, s, t, id, first, last, base, y, h, swap);
+    } else if (base != y) {
+        for (int n = 0; n < t.n; ++n)
+            for (int o = first + int(threadIdx.x); o < last; o += 256) y[n * s.ys + o] = base[n * s.bs + o];
+    }
+}
+
+// Tiles of a call, at most.
+int64_t adapt_tiles(int n_seqs, int n_tokens) { return int64_t(n_seqs) + n_tokens / kTile; }
 
 // Into how many ranges the columns are cut: about eight blocks a CU, and ranges of whole chunks.
-int adapt_ranges(int cols, int n_tokens, int n_sets, int& range) {
+int adapt_ranges(int cols, int n_seqs, int n_tokens, int n_sets, int& range) {
     const int chunks = (cols + kChunk - 1) / kChunk;
-    const int want = std::max<int>(1, std::min({int(2048 / std::min<int64_t>(int64_t(n_tokens) * n_sets, 2048)), chunks, kMaxRanges}));
+    const int64_t tiles = std::min<int64_t>(n_tokens, adapt_tiles(n_seqs, n_tokens)) * n_sets;
+    const int want = int(std::max<int64_t>(1, std::min<int64_t>({2048 / std::max<int64_t>(tiles, 1), chunks, kMaxRanges})));
     const int each = (chunks + want - 1) / want;
     range = each * kChunk;
     return (chunks + each - 1) / each;
 }
 
-template <int TYPE>
+template <int TYPE, int NR, bool FEW>
 int launch_adapters(const Args& a, int n_sets, hipStream_t s) {
     int rows = 0;
     for (int i = 0; i < n_sets; ++i) rows = std::max(rows, a.set[i].rows);
-    hipLaunchKernelGGL(k_adapt_down<TYPE>, dim3(unsigned(a.ranges), unsigned(a.n_tokens), unsigned(n_sets)), dim3(256),
-                       0, s, a);
-    hipLaunchKernelGGL(k_adapt_up<TYPE>, dim3(unsigned((rows + 255) / 256), unsigned(a.n_tokens), unsigned(n_sets)),
-                       dim3(256), 0, s, a);
+    const int64_t tiles = adapt_tiles(a.n_seqs, a.n_tokens), cols = (rows + 255) / 256;
+    const int turns = int(std::max<int64_t>(1, std::min<int64_t>(4, cols * tiles * n_sets / 2048)));
+    auto go = [&](auto kern, int64_t x, auto... more) {
+        for (int64_t t0 = 0; t0 < tiles; t0 += 1 << 15) {
+            const dim3 grid{unsigned(x), unsigned(std::min<int64_t>(tiles - t0, 1 << 15)), unsigned(n_sets)};
+            hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, int(t0), more...);
+        }
+    };
+    go(k_adapt_down<TYPE, NR, FEW>, a.ranges);
+    go(k_adapt_up<TYPE, NR, FEW>, (cols + turns - 1) / turns, turns);
     return int(hipGetLastError());
+}
+int launch_adapters(const Args& a, int n_sets, int type, bool few, hipStream_t s) {
+    int R = 0;
+    for (int i = 0; i < n_sets; ++i) R = std::max(R, a.set[i].R);
+    auto pick = [&](auto nr) {
+        constexpr int NR = decltype(nr)::value;
+        if (type == WV_ADAPTER_BF16)
+            return few ? launch_adapters<WV_ADAPTER_BF16, NR, true>(a, n_sets, s)
+                       : launch_adapters<WV_ADAPTER_BF16, NR, false>(a, n_sets, s);
+        return few ? launch_adapters<WV_ADAPTER_F16, NR, true>(a, n_sets, s)
+                   : launch_adapters<WV_ADAPTER_F16, NR, false>(a, n_sets, s);
+    };
+    return R <= 32 ? pick(std::integral_constant<int, 1>{}) : R <= 64 ? pick(std::integral_constant<int, 2>{})
+         : R <= 128 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 8>{});
 }
 
 }  // namespace
@@ -326,7 +640,7 @@ int wv_adapters_scratch(const wv_adapter_batch* batch, const wv_adapter_rows* se
     if (rc) return rc;
     if (!bytes) return rt_fail(WV_E_ARG, "wv_adapters_scratch: nil bytes");
     int range;
-    *bytes = scratch_floats(s, n_sets, batch->n_tokens, adapt_ranges(s[0].c.cols, std::max(batch->n_tokens, 1), n_sets, range)) * 4;
+    *bytes = scratch_floats(s, n_sets, batch->n_tokens, adapt_ranges(s[0].c.cols, batch->n_seqs, batch->n_tokens, n_sets, range)) * 4;
     return WV_OK;
 }
 
@@ -362,7 +676,7 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
     for (int i = 0; i < n_sets; ++i)
         if (!a.set[i].y) return rt_fail(WV_E_ARG, "wv_adapters: nil y");
     a.x = d_x, a.xs = x_stride, a.cu = batch->d_cu_q, a.which = batch->d_adapter;
-    a.ranges = adapt_ranges(a.cols, a.n_tokens, n_sets, a.range);
+    a.ranges = adapt_ranges(a.cols, a.n_seqs, a.n_tokens, n_sets, a.range);
     (void)hipSetDevice(s[0].device);
     hipStream_t st = rt_stream(stream, s[0].device);
     const size_t floats = scratch_floats(s, n_sets, a.n_tokens, a.ranges);
@@ -382,8 +696,8 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
         a.set[i].h = h;
         h += size_t(a.ranges) * size_t(a.n_tokens) * size_t(a.set[i].R);
     }
-    const int e = s[0].c.type == WV_ADAPTER_BF16 ? launch_adapters<WV_ADAPTER_BF16>(a, n_sets, st)
-                                                 : launch_adapters<WV_ADAPTER_F16>(a, n_sets, st);
+    const bool few = batch->max_q ? batch->max_q <= kFew : a.n_tokens <= kFew;
+    const int e = launch_adapters(a, n_sets, s[0].c.type, few, st);
     return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_adapters: kernel launch");
 }
 
