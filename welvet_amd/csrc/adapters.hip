@@ -49,6 +49,9 @@ bool set_lookup(uint64_t h, Set& out) {
 }
 
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float g4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
@@ -148,6 +151,58 @@ __device__ __forceinline__ void wide8(uint4 w, float* v) {
     for (int i = 0; i < 4; ++i) v[2 * i] = low<TYPE>(u[i]), v[2 * i + 1] = high<TYPE>(u[i]);
 }
 
+// Eight f32 values as NT terms of the weights' type, whose products with a weight are exact in f32. bf16: three terms
+// hold all 24 bits, whatever the exponent. fp16: two hold 22, of values that a power of two has brought into its range.
+template <int TYPE>
+struct Terms {
+    static constexpr int N = TYPE == WV_ADAPTER_BF16 ? 3 : 2;
+    uint4 t[N];
+};
+template <int TYPE>
+__device__ __forceinline__ Terms<TYPE> split8(const float* x) {
+    Terms<TYPE> r;
+    uint32_t w[Terms<TYPE>::N][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x[2 * i], b = x[2 * i + 1];
+        if constexpr (TYPE == WV_ADAPTER_BF16) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {  // truncated, the rest exactly
+                w[k][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+            }
+        } else {
+            const auto hi = __builtin_amdgcn_cvt_pkrtz(a, b);
+            const h2 lo = {_Float16(fmaf(float(hi[0]), -1.0f, a)), _Float16(fmaf(float(hi[1]), -1.0f, b))};
+            w[0][i] = __builtin_bit_cast(uint32_t, hi);
+            w[1][i] = __builtin_bit_cast(uint32_t, lo);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < Terms<TYPE>::N; ++k) r.t[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    return r;
+}
+// acc += 32 rows of weights x 32 columns of values, 16 deep: the smallest terms first.
+template <int TYPE>
+__device__ __forceinline__ f16v product(uint4 w, const Terms<TYPE>& x, f16v acc) {
+#pragma unroll
+    for (int k = Terms<TYPE>::N - 1; k >= 0; --k) {
+        if constexpr (TYPE == WV_ADAPTER_BF16)
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, w), __builtin_bit_cast(b8, x.t[k]), acc, 0, 0, 0);
+        else
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, w), __builtin_bit_cast(h8, x.t[k]), acc, 0, 0, 0);
+    }
+    return acc;
+}
+// Exponent e with |x| < 2^(e + 1), of the larger of this lane's and lane ^ 32's magnitude, within what a power of two
+// in f32 can bring to 2^14 and back.
+__device__ __forceinline__ int pair_exponent(float m) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    return min(max(int(max(r[0], r[1]) >> 23) - 127, -113), 127);
+}
+__device__ __forceinline__ float power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
+
 // h of a few tokens, one after the other: a wave takes every fourth group of four ranks, a lane 8 columns at a time.
 // The first loads do not wait for the adapter's rank (there are 16 rows in A at least).
 template <int TYPE>
@@ -188,7 +243,7 @@ __device__ __forceinline__ void down_few(const Args& a, const SetArgs& s, const 
     }
 }
 
-// h of a tile of tokens, 32 NR ranks at a time, on f32 products of 32 ranks x 32 tokens x 2 columns: a lane holds the
+// h of a tile of tokens, 32 NR ranks at a time, on products of 32 ranks x 32 tokens x 16 columns: a lane holds the
 // same 16 columns of its rank's row and of its token's (lanes from 32 on the 16 behind those), straight from memory.
 // The block's waves take every fourth 32 columns and meet in LDS.
 template <int TYPE, int NR>
@@ -220,20 +275,38 @@ __device__ __forceinline__ void down_tile(const Args& a, const SetArgs& s, const
         };
         int c = c0 + 32 * wave + 16 * hi;
         const int end = c1 + 16 * hi;  // c1 is a multiple of 32, and C one of 64: A is there
+        int e = -113;                  // fp16: the token's sums so far are in units of 2^(e - 14)
         if (c < end) load(c);
         while (c < end) {
-            float xv[16], wv[NR][16];
+            if constexpr (TYPE == WV_ADAPTER_F16) {
+                float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) xv[i] = v[i];
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+                const int en = max(e, pair_exponent(m));
+                if (__ballot(en != e)) {
+                    const float f = ldexpf(1.0f, max(e - en, -200));
 #pragma unroll
-            for (int k = 0; k < NR; ++k) wide8<TYPE>(w[k][0], wv[k]), wide8<TYPE>(w[k][1], wv[k] + 8);
+                    for (int k = 0; k < NR; ++k) acc[k] *= f;
+                }
+                e = en;
+                const float up = power(14 - e);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] *= up;
+            }
+            const Terms<TYPE> x0 = split8<TYPE>(v), x1 = split8<TYPE>(v + 8);
+            uint4 u[NR][2];
+#pragma unroll
+            for (int k = 0; k < NR; ++k) u[k][0] = w[k][0], u[k][1] = w[k][1];
             c += 128;
             if (c < end) load(c);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][0], x0, acc[k]);
 #pragma unroll
-                for (int k = 0; k < NR; ++k)
-                    acc[k] = __builtin_amdgcn_mfma_f32_32x32x2f32(wv[k][i], xv[i], acc[k], 0, 0, 0);
+            for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][1], x1, acc[k]);
+        }
+        if constexpr (TYPE == WV_ADAPTER_F16) {
+#pragma unroll
+            for (int k = 0; k < NR; ++k) acc[k] *= power(e - 14);
         }
         // waves 2 and 3 to 0 and 1, then 1 to 0
 #pragma unroll
@@ -363,7 +436,7 @@ __device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Ti
     }
 }
 
-// y of the block's outputs for a tile, on f32 products of 32 outputs x 32 tokens x 2 ranks. A lane ends with 16 outputs
+// y of the block's outputs for a tile, on products of 32 outputs x 32 tokens x 16 ranks. A lane ends with 16 outputs
 // of one token; through LDS they become four times 4 side by side, 8 lanes a row, as base and y are read and written.
 // The next outputs' B and base are on their way under the products.
 template <int TYPE, int NR>
@@ -396,11 +469,23 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
     if (o0 < last) load(o0);
     stage_h<NR>(a, s, t, 0, 32, s.rank[id], s.scale[id], h);
     __syncthreads();
-    float hv[2 * NR][8];
+    float unit = 1.0f, up = 1.0f;
+    if constexpr (TYPE == WV_ADAPTER_F16) {
+        float m = 0.0f;
+        for (int r = 8 * hi; r < s.R; r += 16)
 #pragma unroll
-    for (int k = 0; k < 2 * NR; ++k)
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(h[n * LD + r + i]));
+        const int e = pair_exponent(m);
+        up = power(14 - e), unit = power(e - 14);
+    }
+    Terms<TYPE> hv[2 * NR];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hv[k][i] = h[n * LD + 16 * k + 8 * hi + i];
+    for (int k = 0; k < 2 * NR; ++k) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = h[n * LD + 16 * k + 8 * hi + i] * up;
+        hv[k] = split8<TYPE>(v);
+    }
     swap += wave * 32 * SW;
     for (; o0 < last; o0 += 128) {
         f16v acc;
@@ -415,12 +500,9 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
         if (o0 + 128 < last) load(o0 + 128);
 #pragma unroll
         for (int k = 0; k < 2 * NR; ++k) {
-            if (16 * k >= s.R) continue;
-            float v[8];
-            wide8<TYPE>(u[k], v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v[i], hv[k][i], acc, 0, 0, 0);
+            if (16 * k < s.R) acc = product<TYPE>(u[k], hv[k], acc);
         }
+        if constexpr (TYPE == WV_ADAPTER_F16) acc *= unit;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             *reinterpret_cast<g4*>(swap + n * SW + 8 * q + 4 * hi) = g4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
