@@ -79,11 +79,22 @@ class Adapters:
 
 def _rows(sets, y_ptrs, base_ptrs, y_strides, base_strides):
     n = len(sets)
-    y, base = list(y_ptrs or [None] * n), list(base_ptrs or [None] * n)
-    ys, bs = list(y_strides or [0] * n), list(base_strides or [0] * n)
-    if not n == len(y) == len(base) == len(ys) == len(bs):
-        raise ValueError(f"adapters: {n} sets, {len(y)} outputs, {len(base)} bases, {len(ys)} and {len(bs)} strides")
-    return (AdapterRows * max(n, 1))(*[AdapterRows(s.handle, *r) for s, *r in zip(sets, y, base, ys, bs)])
+    for x in (y_ptrs, base_ptrs, y_strides, base_strides):
+        if x is not None and len(x) != n:
+            raise ValueError(f"adapters: {n} sets, {len(x)} pointers or strides")
+    rows = (AdapterRows * n)()
+    for i in range(n):
+        r = rows[i]
+        r.adapters = sets[i].handle
+        if y_ptrs is not None:
+            r.d_y = y_ptrs[i]
+        if base_ptrs is not None:
+            r.d_base = base_ptrs[i]
+        if y_strides is not None:
+            r.y_stride = y_strides[i]
+        if base_strides is not None:
+            r.base_stride = base_strides[i]
+    return rows
 
 
 def apply_dev(sets, batch: AdapterBatch, x_ptr: int, y_ptrs, *, base_ptrs=None, x_stride: int = 0, y_strides=None,

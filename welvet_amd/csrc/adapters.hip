@@ -85,13 +85,13 @@ __device__ __forceinline__ float high(uint32_t w) {
 
 // Up to 32 token rows of one sequence.
 struct Tile {
-    int t0, n, seq;
+    int t0, n, id;  // its adapter
 };
 // Tile `idx`: the first one of sequence idx, then all further ones in order of the sequences, found 64 sequences at a
 // time (a decode step has none, and its blocks no search). False: there is none.
 __device__ __forceinline__ bool find_tile(const Args& a, int idx, Tile& t) {
     if (idx < a.n_seqs) {
-        t.seq = idx;
+        t.id = a.which[idx];
         t.t0 = min(max(a.cu[idx], 0), a.n_tokens);
         t.n = min(min(max(a.cu[idx + 1], t.t0), a.n_tokens) - t.t0, kTile);
         return t.n > 0;
@@ -116,7 +116,7 @@ __device__ __forceinline__ bool find_tile(const Args& a, int idx, Tile& t) {
         if (idx < total) {
             const int w = __builtin_ctzll(__ballot(incl > idx));
             const int skip = kTile * (1 + idx - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(tiles, w)));
-            t.seq = base + w;
+            t.id = a.which[base + w];
             t.t0 = __builtin_amdgcn_readlane(c0, w) + skip;
             t.n = min(__builtin_amdgcn_readlane(n, w) - skip, kTile);
             return true;
@@ -195,11 +195,12 @@ __device__ __forceinline__ f16v product(uint4 w, const Terms<TYPE>& x, f16v acc)
     }
     return acc;
 }
-// Exponent e with |x| < 2^(e + 1), of the larger of this lane's and lane ^ 32's magnitude, within what a power of two
-// in f32 can bring to 2^14 and back.
+// Exponent e of a magnitude's bits (it is below 2^(e + 1)), within what a power of two in f32 can bring to 2^14 and
+// back; of the larger of this lane's and lane ^ 32's.
+__device__ __forceinline__ int exponent(uint32_t bits) { return min(max(int(bits >> 23) - 127, -113), 127); }
 __device__ __forceinline__ int pair_exponent(float m) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    return min(max(int(max(r[0], r[1]) >> 23) - 127, -113), 127);
+    return exponent(max(r[0], r[1]));
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 
@@ -264,20 +265,23 @@ __device__ __forceinline__ void down_tile(const Args& a, const SetArgs& s, const
         }
         float v[16];
         uint4 w[NR][2];
-        auto load = [&](int c) {
-            load8(x, c, a.cols, v);
-            load8(x, c + 8, a.cols, v + 8);
+        auto load_a = [&](int c) {
 #pragma unroll
             for (int k = 0; k < NR; ++k) {
                 w[k][0] = *reinterpret_cast<const uint4*>(row[k] + c);
                 w[k][1] = *reinterpret_cast<const uint4*>(row[k] + c + 8);
             }
         };
-        int c = c0 + 32 * wave + 16 * hi;
-        const int end = c1 + 16 * hi;  // c1 is a multiple of 32, and C one of 64: A is there
-        int e = -113;                  // fp16: the token's sums so far are in units of 2^(e - 14)
-        if (c < end) load(c);
-        while (c < end) {
+        auto load_x = [&](int c) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f4 y = *reinterpret_cast<const f4*>(x + c + 4 * q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 * q + i] = y[i];
+            }
+        };
+        int e = -113;  // fp16: the token's sums so far are in units of 2^(e - 14)
+        auto step = [&](auto next) {
             if constexpr (TYPE == WV_ADAPTER_F16) {
                 float m = 0.0f;
 #pragma unroll
@@ -297,12 +301,28 @@ __device__ __forceinline__ void down_tile(const Args& a, const SetArgs& s, const
             uint4 u[NR][2];
 #pragma unroll
             for (int k = 0; k < NR; ++k) u[k][0] = w[k][0], u[k][1] = w[k][1];
-            c += 128;
-            if (c < end) load(c);
+            next();
 #pragma unroll
             for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][0], x0, acc[k]);
 #pragma unroll
             for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][1], x1, acc[k]);
+        };
+        // whole steps without a branch (what would be loaded behind the last one is that one again), then what is left
+        // of a row, where A, padded with zeros to multiples of 64 columns, goes on
+        const int steps = (min(c1, a.cols) - c0) / 32, mine = (steps - wave + 3) / 4;
+        const int at = c0 + 32 * wave + 16 * hi;
+        if (mine > 0) {
+            load_x(at), load_a(at);
+            for (int i = 0; i < mine; ++i) {
+                const int c = at + 128 * min(i + 1, mine - 1);
+                step([&] { load_x(c), load_a(c); });
+            }
+        }
+        if (const int c = c0 + 32 * steps + 16 * hi; c0 + 32 * steps < min(c1, a.cols) && (steps & 3) == wave) {
+            load8(x, c, a.cols, v);
+            load8(x, c + 8, a.cols, v + 8);
+            load_a(c);
+            step([] {});
         }
         if constexpr (TYPE == WV_ADAPTER_F16) {
 #pragma unroll
@@ -352,7 +372,7 @@ __global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
     const SetArgs& s = a.set[blockIdx.z];
     Tile t;
     if (!find_tile(a, tile0 + int(blockIdx.y), t)) return;
-    const int id = a.which[t.seq];
+    const int id = t.id;
     if (unsigned(id) >= unsigned(s.n_adapters)) return;
     const int range = blockIdx.x, c0 = range * a.range;
     float* h = s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R;
@@ -375,12 +395,12 @@ __device__ __forceinline__ void stage_h(const Args& a, const SetArgs& s, const T
             const float* p = s.h + (int64_t(t.t0) + n0 + n) * s.R + r;
             const int64_t step = int64_t(a.n_tokens) * s.R;
             int k = 0;
-            for (; k + 4 <= a.ranges; k += 4) {
-                f4 y[4];
+            for (; k + 8 <= a.ranges; k += 8) {
+                f4 y[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const f4*>(p + (k + j) * step);
+                for (int j = 0; j < 8; ++j) y[j] = *reinterpret_cast<const f4*>(p + (k + j) * step);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x += y[j];
+                for (int j = 0; j < 8; ++j) x += y[j];
             }
             for (; k < a.ranges; ++k) x += *reinterpret_cast<const f4*>(p + k * step);
 #pragma unroll
@@ -436,116 +456,209 @@ __device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Ti
     }
 }
 
-// y of the block's outputs for a tile, on products of 32 outputs x 32 tokens x 16 ranks. A lane ends with 16 outputs
-// of one token; through LDS they become four times 4 side by side, 8 lanes a row, as base and y are read and written.
-// The next outputs' B and base are on their way under the products.
+// What up_tile keeps in LDS: the tile's h as operands, [16 ranks][term][lane] units of 16 bytes, the tokens' scales,
+// and rows of 36 floats in which a wave's outputs change lanes (16 lanes' 16-byte accesses reach all banks).
+constexpr int kSwap = 36;
 template <int TYPE, int NR>
-__device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const Tile& t, int id, int first, int last,
-                                        const float* base, float* y, float* h, float* swap) {
-    constexpr int LD = 32 * NR + 4, SW = 36;  // rows of 36 floats: 16 lanes' 16-byte accesses reach all banks
+struct UpLds {
+    uint4 h[2 * NR][Terms<TYPE>::N][64];
+    uint32_t most[32];
+    float swap[4][32 * kSwap];
+};
+
+// The tile's h: the ranges summed in their order, with the adapter's scale, as operands of the products. What lies
+// behind the adapter's own ranks is anything until it is masked.
+template <int TYPE, int NR>
+__device__ __forceinline__ void stage_operands(const Args& a, const SetArgs& s, const Tile& t, int rank, float scale,
+                                               UpLds<TYPE, NR>& l) {
+    f4 x[NR];
+    const int64_t step = int64_t(a.n_tokens) * s.R;
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int i = threadIdx.x + 256 * j, n = i / (8 * NR), r = 4 * (i % (8 * NR));
+        x[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (r < s.R && n < t.n) {
+            const float* p = s.h + (int64_t(t.t0) + n) * s.R + r;
+            int k = 0;
+            for (; k + 4 <= a.ranges; k += 4) {
+                f4 y[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) y[c] = *reinterpret_cast<const f4*>(p + (k + c) * step);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[j] += y[c];
+            }
+            for (; k < a.ranges; ++k) x[j] += *reinterpret_cast<const f4*>(p + k * step);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[j][c] = r + c < rank ? x[j][c] * scale : 0.0f;
+        }
+    }
+    if constexpr (TYPE == WV_ADAPTER_F16) {  // the token's largest, which its power of two goes by
+        if (threadIdx.x < 32) l.most[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            const int n = (threadIdx.x + 256 * j) / (8 * NR);
+            const float m = fmaxf(fmaxf(fabsf(x[j][0]), fabsf(x[j][1])), fmaxf(fabsf(x[j][2]), fabsf(x[j][3])));
+            atomicMax(&l.most[n], __float_as_uint(m));
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < NR; ++j) {
+        const int i = threadIdx.x + 256 * j, n = i / (8 * NR), r = 4 * (i % (8 * NR));
+        float v[8] = {x[j][0], x[j][1], x[j][2], x[j][3]};
+        if constexpr (TYPE == WV_ADAPTER_F16) {
+            const float up = power(14 - exponent(l.most[n]));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] *= up;
+        }
+        const Terms<TYPE> w = split8<TYPE>(v);
+#pragma unroll
+        for (int k = 0; k < Terms<TYPE>::N; ++k)
+            reinterpret_cast<uint2*>(&l.h[r / 16][k][n + 32 * ((r / 8) & 1)])[(r / 4) & 1] = make_uint2(w.t[k].x, w.t[k].y);
+    }
+    __syncthreads();
+}
+
+// y of the block's outputs for a tile, on products of 32 outputs x 32 tokens x 16 ranks. A lane ends with 16 outputs
+// of one token; through LDS they become four times 4 side by side, 8 lanes a row, as base and y are read and written,
+// past the caches (a prompt's rows are more than they hold). The base of the next two steps is on its way meanwhile.
+template <int TYPE, int NR>
+__device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const Tile& t, int id, int rank, int first,
+                                        int last, const float* base, float* y, UpLds<TYPE, NR>& l) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hi = lane >> 5, m = lane >> 3, o4 = 4 * (lane & 7);
     const uint16_t* B = s.b + int64_t(id) * s.rows * s.R + 8 * hi;
-    uint4 w[2 * NR];
-    f4 was[4];
-    auto load = [&](int o0) {
+    float* swap = l.swap[wave];
+    // Nothing in a step branches, so that loads stay on their way: rows behind the tile's last are that one again (to
+    // the same place), ranks behind the stored ones the last ones (times h = 0), what would be loaded behind the last
+    // whole 32 outputs are those again.
+    const int whole = first + ((last - first) & ~31);
+    int64_t rb[4], ry[4];
+    int rs[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int r = min(8 * q + m, t.n - 1);
+        rb[q] = r * s.bs + o4, ry[q] = r * s.ys + o4, rs[q] = r * kSwap + o4;
+    }
+    constexpr int D = NR <= 2 ? 2 : 1;  // steps ahead that B is loaded, as registers allow
+    uint4 w[D][2 * NR];
+    f4 was[2][4];
+    auto load_b = [&](int o0, uint4* w) {
         const uint16_t* row = B + int64_t(min(o0 + n, last - 1)) * s.R;
 #pragma unroll
-        for (int k = 0; k < 2 * NR; ++k)
-            if (16 * k < s.R) w[k] = *reinterpret_cast<const uint4*>(row + 16 * k);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float* p = base + (8 * q + m) * s.bs + o0 + o4;
-            if (8 * q + m >= t.n) continue;
-            if (o0 + o4 + 4 <= last) {
-                was[q] = *reinterpret_cast<const f4*>(p);
-            } else {
-                for (int i = 0; i < 4; ++i)
-                    if (o0 + o4 + i < last) was[q][i] = p[i];
-            }
-        }
+        for (int k = 0; k < 2 * NR; ++k) w[k] = *reinterpret_cast<const uint4*>(row + min(16 * k, s.R - 16));
     };
-    int o0 = first + 32 * wave;
-    if (o0 < last) load(o0);
-    stage_h<NR>(a, s, t, 0, 32, s.rank[id], s.scale[id], h);
-    __syncthreads();
-    float unit = 1.0f, up = 1.0f;
-    if constexpr (TYPE == WV_ADAPTER_F16) {
-        float m = 0.0f;
-        for (int r = 8 * hi; r < s.R; r += 16)
+    auto load_base = [&](int o0, f4* x) {
+        const float* p = base + max(min(o0, whole - 32), first);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(h[n * LD + r + i]));
-        const int e = pair_exponent(m);
-        up = power(14 - e), unit = power(e - 14);
-    }
-    Terms<TYPE> hv[2 * NR];
-#pragma unroll
-    for (int k = 0; k < 2 * NR; ++k) {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = h[n * LD + 16 * k + 8 * hi + i] * up;
-        hv[k] = split8<TYPE>(v);
-    }
-    swap += wave * 32 * SW;
-    for (; o0 < last; o0 += 128) {
-        f16v acc;
+        for (int q = 0; q < 4; ++q) x[q] = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p + rb[q]));
+    };
+    auto outputs = [&](f16v& acc, const uint4* w) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-        f4 old[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) old[q] = was[q];
-        uint4 u[2 * NR];
-#pragma unroll
-        for (int k = 0; k < 2 * NR; ++k) u[k] = w[k];
-        if (o0 + 128 < last) load(o0 + 128);
 #pragma unroll
         for (int k = 0; k < 2 * NR; ++k) {
-            if (16 * k < s.R) acc = product<TYPE>(u[k], hv[k], acc);
+            Terms<TYPE> h;
+#pragma unroll
+            for (int c = 0; c < Terms<TYPE>::N; ++c) h.t[c] = l.h[k][c][lane];
+            acc = product<TYPE>(w[k], h, acc);
         }
+    };
+    float unit = 1.0f;
+    auto turn = [&](f16v acc) {  // into swap, in units of 1
         if constexpr (TYPE == WV_ADAPTER_F16) acc *= unit;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<g4*>(swap + n * SW + 8 * q + 4 * hi) = g4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+            *reinterpret_cast<g4*>(swap + n * kSwap + 8 * q + 4 * hi) = g4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
         wave_sync();
+    };
+    auto step = [&](int o0, f4* x, uint4* w) {
+        f16v acc;
+        outputs(acc, w);
+        __builtin_amdgcn_sched_barrier(0);
+        load_b(o0 + 128 * D, w);
+        __builtin_amdgcn_sched_barrier(0);
+        turn(acc);
+        f4 sum[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f4 x = old[q] + f4(*reinterpret_cast<const g4*>(swap + (8 * q + m) * SW + o4));
-            if (8 * q + m >= t.n) continue;
-            float* p = y + (8 * q + m) * s.ys + o0 + o4;
-            if (o0 + o4 + 4 <= last) {
-                *reinterpret_cast<f4*>(p) = x;
-            } else {
-                for (int i = 0; i < 4; ++i)
-                    if (o0 + o4 + i < last) p[i] = x[i];
-            }
-        }
+        for (int q = 0; q < 4; ++q) sum[q] = x[q] + f4(*reinterpret_cast<const g4*>(swap + rs[q]));
         wave_sync();
+        load_base(o0 + 256, x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) __builtin_nontemporal_store(sum[q], reinterpret_cast<f4*>(y + o0 + ry[q]));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int o0 = first + 32 * wave;
+    if (whole > first) load_base(o0, was[0]), load_base(o0 + 128, was[1]);
+    load_b(o0, w[0]);
+    if (D > 1) load_b(o0 + 128, w[D - 1]);
+    stage_operands<TYPE, NR>(a, s, t, rank, s.scale[id], l);
+    if constexpr (TYPE == WV_ADAPTER_F16) unit = power(exponent(l.most[n]) - 14);
+    // what was loaded so far is there (h came after it): the steps' waits need not allow for it
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    for (; o0 + 128 < whole; o0 += 256) {
+        step(o0, was[0], w[0]);
+        step(o0 + 128, was[1], w[D - 1]);
+    }
+    bool second = false;
+    if (o0 < whole) {
+        step(o0, was[0], w[0]);
+        o0 += 128, second = true;
+    }
+    if (o0 >= last || o0 != whole) return;
+    f16v acc;  // fewer than 32 outputs are left
+    second ? outputs(acc, w[D - 1]) : outputs(acc, w[0]);
+    turn(acc);
+    for (int i = lane; i < 32 * t.n; i += 64)
+        if (const int r = i >> 5, o = o0 + (i & 31); o < last) y[r * s.ys + o] = base[r * s.bs + o] + swap[r * kSwap + (i & 31)];
+}
+
+// Rows without an adapter: a wave a row, eight of them on their way.
+__device__ __forceinline__ void copy_rows(const SetArgs& s, int rows, int first, int last, const float* base, float* y) {
+    const int wave = threadIdx.x >> 6;
+    for (int o = first + 4 * int(threadIdx.x & 63); o < last; o += 256) {
+        if (o + 4 > last) {
+            for (int n = wave; n < rows; n += 4)
+                for (int i = o; i < last; ++i) y[n * s.ys + i] = base[n * s.bs + i];
+            continue;
+        }
+        f4 x[kTile / 4];
+#pragma unroll
+        for (int i = 0; i < kTile / 4; ++i)
+            if (wave + 4 * i < rows) x[i] = *reinterpret_cast<const f4*>(base + (wave + 4 * i) * s.bs + o);
+#pragma unroll
+        for (int i = 0; i < kTile / 4; ++i)
+            if (wave + 4 * i < rows) *reinterpret_cast<f4*>(y + (wave + 4 * i) * s.ys + o) = x[i];
     }
 }
 
+struct Nothing {};
 template <int TYPE, int NR, bool FEW>
 __global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) {
-    constexpr int LD = 32 * NR + 4;
-    __shared__ __align__(16) float h[(FEW ? kFew : 32) * LD];
-    __shared__ __align__(16) float swap[FEW ? 4 : 4 * 32 * 36];
+    __shared__ __align__(16) float h[kFew * (32 * NR + 4)];
+    __shared__ std::conditional_t<FEW, Nothing, UpLds<TYPE, NR>> lds;
     const SetArgs& s = a.set[blockIdx.z];
     const int first = blockIdx.x * 256 * turns;
     if (first >= s.rows) return;
     Tile t;
     if (!find_tile(a, tile0 + int(blockIdx.y), t)) return;
-    const int id = a.which[t.seq];
+    const int id = t.id;
     const int last = min(first + 256 * turns, s.rows);
     const float* base = s.base + t.t0 * s.bs;
     float* y = s.y + t.t0 * s.ys;
     const bool known = unsigned(id) < unsigned(s.n_adapters);
     if (known && (FEW || t.n <= kFew)) {
         up_few<TYPE, NR>(a, s, t, id, first, last, base, y, h);
-    } else if (!FEW && known && s.rank[id]) {
-        up_tile<TYPE, NR>(a, s, t, id, first, last, base, y, h, swap);
-    } else if (base != y) {
-        for (int n = 0; n < t.n; ++n)
-            for (int o = first + int(threadIdx.x); o < last; o += 256) y[n * s.ys + o] = base[n * s.bs + o];
+        return;
     }
+    if constexpr (!FEW) {
+        if (const int rank = known ? s.rank[id] : 0; rank) {
+            up_tile<TYPE, NR>(a, s, t, id, rank, first, last, base, y, lds);
+            return;
+        }
+    }
+    if (base != y) copy_rows(s, t.n, first, last, base, y);
 }
 
 // Tiles of a call, at most.
