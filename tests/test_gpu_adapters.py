@@ -126,6 +126,15 @@ def test_several_sets(new, which):
         c.check(c.run(True), True)
 
 
+@pytest.mark.parametrize("hint", [0, 1, 4, 5, 1000])
+def test_hints_only_steer(hint):
+    """Whatever the call is told of its longest sequence."""
+    c = Case(np.random.default_rng(hint), [300, 40], 600, [16, 40], [1, 70, 3, 0, 33], [0, 1, -1, 0, 0], pad=1)
+    c.batch = AdapterBatch(5, c.t, c.cu.data_ptr(), c.ids.data_ptr(), hint)
+    c.check(c.run())
+    c.check(c.run(True), True)
+
+
 @pytest.mark.parametrize("n", [1, 3, 40])
 def test_every_column_and_rank(n):
     """Tokens that are one column each: y is that column of A through B, within the roundings of one product chain."""

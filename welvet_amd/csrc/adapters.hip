@@ -65,6 +65,7 @@ struct SetArgs {
     float* h;  // [ranges][n_tokens][R]
     int64_t ys, bs;
     int rows, R, C, n_adapters;
+    int block0;  // of the blocks over all sets' outputs, its first
 };
 struct Args {
     SetArgs set[kMaxSets];
@@ -83,17 +84,19 @@ __device__ __forceinline__ float high(uint32_t w) {
     return TYPE == WV_ADAPTER_BF16 ? __uint_as_float(w & 0xffff0000) : float(__builtin_bit_cast(_Float16, uint16_t(w >> 16)));
 }
 
-// Up to 32 token rows of one sequence.
+// Token rows of one sequence, 32 at most.
 struct Tile {
     int t0, n, id;  // its adapter
 };
 // Tile `idx`: the first one of sequence idx, then all further ones in order of the sequences, found 64 sequences at a
-// time (a decode step has none, and its blocks no search). False: there is none.
+// time. False: there is none. FEW: a sequence is one tile, whatever its length.
+template <bool FEW>
 __device__ __forceinline__ bool find_tile(const Args& a, int idx, Tile& t) {
-    if (idx < a.n_seqs) {
+    if (FEW || idx < a.n_seqs) {
         t.id = a.which[idx];
         t.t0 = min(max(a.cu[idx], 0), a.n_tokens);
-        t.n = min(min(max(a.cu[idx + 1], t.t0), a.n_tokens) - t.t0, kTile);
+        t.n = min(max(a.cu[idx + 1], t.t0), a.n_tokens) - t.t0;
+        if (!FEW) t.n = min(t.n, kTile);
         return t.n > 0;
     }
     idx -= a.n_seqs;
@@ -369,12 +372,12 @@ template <int TYPE, int NR, bool FEW>
 __global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
     constexpr int ND = NR < 4 ? NR : 4;  // more would take all of a SIMD's registers for one wave
     __shared__ float lds[FEW ? 1 : 2 * 32 * (32 * ND + 4)];
-    const SetArgs& s = a.set[blockIdx.z];
+    const SetArgs& s = a.set[blockIdx.x / a.ranges];
     Tile t;
-    if (!find_tile(a, tile0 + int(blockIdx.y), t)) return;
+    if (!find_tile<FEW>(a, tile0 + int(blockIdx.y), t)) return;
     const int id = t.id;
     if (unsigned(id) >= unsigned(s.n_adapters)) return;
-    const int range = blockIdx.x, c0 = range * a.range;
+    const int range = blockIdx.x % a.ranges, c0 = range * a.range;
     float* h = s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R;
     if (FEW || t.n <= kFew)
         down_few<TYPE>(a, s, t, id, c0, min(c0 + a.range, a.cols), h);
@@ -638,11 +641,12 @@ template <int TYPE, int NR, bool FEW>
 __global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) {
     __shared__ __align__(16) float h[kFew * (32 * NR + 4)];
     __shared__ std::conditional_t<FEW, Nothing, UpLds<TYPE, NR>> lds;
-    const SetArgs& s = a.set[blockIdx.z];
-    const int first = blockIdx.x * 256 * turns;
-    if (first >= s.rows) return;
+    int set = 0;
+    while (set + 1 < kMaxSets && int(blockIdx.x) >= a.set[set + 1].block0) ++set;
+    const SetArgs& s = a.set[set];
+    const int first = (int(blockIdx.x) - s.block0) * 256 * turns;
     Tile t;
-    if (!find_tile(a, tile0 + int(blockIdx.y), t)) return;
+    if (!find_tile<FEW>(a, tile0 + int(blockIdx.y), t)) return;
     const int id = t.id;
     const int last = min(first + 256 * turns, s.rows);
     const float* base = s.base + t.t0 * s.bs;
@@ -658,7 +662,9 @@ __global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) 
             return;
         }
     }
-    if (base != y) copy_rows(s, t.n, first, last, base, y);
+    if (base != y)
+        for (int n0 = 0; n0 < t.n; n0 += kTile)
+            copy_rows(s, min(t.n - n0, kTile), first, last, base + n0 * s.bs, y + n0 * s.ys);
 }
 
 // Tiles of a call, at most.
@@ -675,22 +681,26 @@ int adapt_ranges(int cols, int n_seqs, int n_tokens, int n_sets, int& range) {
 }
 
 template <int TYPE, int NR, bool FEW>
-int launch_adapters(const Args& a, int n_sets, hipStream_t s) {
-    int rows = 0;
-    for (int i = 0; i < n_sets; ++i) rows = std::max(rows, a.set[i].rows);
-    const int64_t tiles = adapt_tiles(a.n_seqs, a.n_tokens), cols = (rows + 255) / 256;
-    const int turns = int(std::max<int64_t>(1, std::min<int64_t>(4, cols * tiles * n_sets / 2048)));
+int launch_adapters(Args& a, int n_sets, hipStream_t s) {
+    const int64_t tiles = FEW ? a.n_seqs : adapt_tiles(a.n_seqs, a.n_tokens);
+    int64_t units = 0, blocks = 0;
+    for (int i = 0; i < n_sets; ++i) units += (a.set[i].rows + 255) / 256;
+    const int turns = int(std::max<int64_t>(1, std::min<int64_t>(4, units * tiles / 2048)));
+    for (int i = 0; i < kMaxSets; ++i) {
+        a.set[i].block0 = i < n_sets ? int(blocks) : INT32_MAX;
+        if (i < n_sets) blocks += (a.set[i].rows + 256 * turns - 1) / (256 * turns);
+    }
     auto go = [&](auto kern, int64_t x, auto... more) {
         for (int64_t t0 = 0; t0 < tiles; t0 += 1 << 15) {
-            const dim3 grid{unsigned(x), unsigned(std::min<int64_t>(tiles - t0, 1 << 15)), unsigned(n_sets)};
+            const dim3 grid{unsigned(x), unsigned(std::min<int64_t>(tiles - t0, 1 << 15))};
             hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, int(t0), more...);
         }
     };
-    go(k_adapt_down<TYPE, NR, FEW>, a.ranges);
-    go(k_adapt_up<TYPE, NR, FEW>, (cols + turns - 1) / turns, turns);
+    go(k_adapt_down<TYPE, NR, FEW>, int64_t(a.ranges) * n_sets);
+    go(k_adapt_up<TYPE, NR, FEW>, blocks, turns);
     return int(hipGetLastError());
 }
-int launch_adapters(const Args& a, int n_sets, int type, bool few, hipStream_t s) {
+int launch_adapters(Args& a, int n_sets, int type, bool few, hipStream_t s) {
     int R = 0;
     for (int i = 0; i < n_sets; ++i) R = std::max(R, a.set[i].R);
     auto pick = [&](auto nr) {
