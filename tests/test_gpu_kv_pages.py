@@ -300,6 +300,26 @@ def test_slots_edges():
     assert s.cpu().numpy().tolist() == want
 
 
+@pytest.mark.parametrize("seqs", [4096, 4097, 20000])
+def test_slots_of_many_sequences(seqs):
+    rng = np.random.default_rng(seqs)
+    kv = KVCache(1, 1, 64, 32, 50)
+    new = rng.integers(0, 3, seqs)
+    ln = new + rng.integers(0, 60, seqs)
+    table = rng.integers(-1, 51, (seqs, 2)).astype(np.int32)
+    cu, dl, dt = ints(np.concatenate([[0], np.cumsum(new)])), ints(ln), ints(table)
+    n = int(new.sum()) + 3
+    s, p = ints(np.zeros(n), np.int64), ints(np.zeros(n))
+    kv.slots_dev(KVBatch(seqs, n, 2, cu.data_ptr(), dl.data_ptr(), dt.data_ptr()), s.data_ptr(), p.data_ptr())
+    wv.sync()
+    b = np.repeat(np.arange(seqs), new)
+    q = ln[b] - new[b] + np.concatenate([np.arange(k) for k in new])
+    page = table[b, np.minimum(q // 32, 1)].astype(np.int64)
+    want = np.where((page >= 0) & (page < 50), page * 32 + q % 32, -1)
+    assert np.array_equal(p.cpu().numpy(), np.concatenate([q, [0, 0, 0]]))
+    assert np.array_equal(s.cpu().numpy(), np.concatenate([want, [-1, -1, -1]]))
+
+
 @pytest.mark.parametrize("typ", ["f16", "q8"])
 def test_copy_pages(typ):
     kv = KVCache(3, 2, 128, 64, 9, typ)

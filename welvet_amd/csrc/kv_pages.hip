@@ -7,6 +7,7 @@
 
 #include "kv.h"
 #include "rt_internal.h"
+#include "wave_ops.h"
 
 namespace wv {
 namespace {
@@ -15,7 +16,7 @@ constexpr int kMaxSeqs = 16384;    // of a table: one column of it lies in LDS
 constexpr int kPlanThreads = 1024;
 constexpr int kCopyBlocks = 4096;  // of a copy, twice what runs at once
 
-typedef int32_t i4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int32_t i4 __attribute__((ext_vector_type(4)));
 
 struct Tables {
     int32_t *pages, *len, *refs;
@@ -41,166 +42,167 @@ Work work_of(int32_t* w, int n_seqs, int n_pages) {
     return k;
 }
 
-// Counts that atomics of this kernel have written: past the L1, which does not see those.
+// A count that other threads of this block may have changed by atomics: past the L1, which does not see those.
 __device__ __forceinline__ int32_t ld_now(const int32_t* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void add_to(int32_t* p, int32_t v) {
     __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// What the block's threads wrote before is there for the ones that read after.
-__device__ __forceinline__ void block_fence() {
-    __threadfence();
-    __syncthreads();
-    __threadfence();
-}
 
-// Sum of v over the threads before this one, and over all of them. `lds`: 17 values.
-template <class T>
-__device__ __forceinline__ T scan_before(T v, T* lds, T& all) {
+// Sum of v over the threads before this one, and over all of them. A wave's sums are held at 2^32 - 1, which no pool
+// has pages for. `lds`: 32 values, two turns' worth, so that one barrier does.
+__device__ __forceinline__ int64_t scan_before(uint32_t v, uint32_t* lds, int& turn, int64_t& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T o = __shfl_up(x, d, 64);
-        if (lane >= d) x += o;
-    }
-    if (lane == 63) lds[wave] = x;
+    uint32_t x = v;
+    auto add = [&](int o) { x = __builtin_elementwise_add_sat(x, uint32_t(o)); };
+    add(dpp_i<kDppRowShr1>(0, int(x)));
+    add(dpp_i<kDppRowShr2>(0, int(x)));
+    add(dpp_i<kDppRowShr4, 0xf, 0xe>(0, int(x)));
+    add(dpp_i<kDppRowShr8, 0xf, 0xc>(0, int(x)));
+    add(dpp_i<kDppRowBcast15, 0xa>(0, int(x)));
+    add(dpp_i<kDppRowBcast31, 0xc>(0, int(x)));
+    uint32_t* l = lds + 16 * (turn++ & 1);
+    if (lane == 63) l[wave] = x;
     __syncthreads();
-    T before = 0;
+    int64_t before = int64_t(x) - v;
     all = 0;
 #pragma unroll
     for (int w = 0; w < kPlanThreads / 64; ++w) {
-        if (w < wave) before += lds[w];
-        all += lds[w];
+        if (w < wave) before += l[w];
+        all += l[w];
     }
-    __syncthreads();
-    return before + x - v;
+    return before;
 }
 
 // Four counts from `at` on; those past the pool read as held.
 __device__ __forceinline__ i4 four_refs(const int32_t* refs, int at, int n) {
-    if (at + 4 <= n) return *reinterpret_cast<const i4*>(refs + at);
     i4 x = {1, 1, 1, 1};
+#pragma unroll
     for (int k = 0; k < 4; ++k)
-        if (at + k < n) x[k] = refs[at + k];
+        if (at + k < n) x[k] = ld_now(refs + at + k);
     return x;
 }
 
 __device__ __forceinline__ int pages_of(int len, int shift) { return (len + (1 << shift) - 1) >> shift; }
 
+// f(sequence's value, entry) for the entries 0 .. n - 1 of each lane's sequence: a few by the lane itself, the rest
+// by the whole wave, one sequence after the other.
+constexpr int kOwnEntries = 4;
+template <class F>
+__device__ __forceinline__ void for_entries(int n, int lane_value, F f) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int e = 0; e < kOwnEntries; ++e)
+        if (e < n) f(lane_value, e);
+    for (uint64_t m = __ballot(n > kOwnEntries); m; m &= m - 1) {
+        const int w = __builtin_ctzll(m);
+        const int k = __builtin_amdgcn_readlane(n, w), v = __builtin_amdgcn_readlane(lane_value, w);
+        for (int e = kOwnEntries + lane; e < k; e += 64) f(v, e);
+    }
+}
+
 // The whole of resize but the copies, by one block: its steps depend on each
-// other, and a table's entries and the pool's counts are a few 10 KB.
+// other, and a table's entries and the pool's counts are a few 10 KB. No other
+// block touches them, so a barrier orders them (its threads' stores and atomics
+// are in the L2 by then), and no step needs a fence for the whole device, which
+// costs some 3 us each. A thread takes a sequence. 8 sequences 9 us, 256
+// sequences of 65 pages in a pool of 17000 12 us: a chain of steps of 1 us.
 __global__ void __launch_bounds__(kPlanThreads) k_pages_resize(Tables t, Work w, const int32_t* __restrict__ to,
                                                                int32_t* __restrict__ ok) {
-    __shared__ int64_t lds[17];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, P = t.page_shift;
+    __shared__ uint32_t lds[32];
+    int turn = 0;
+    const int tid = threadIdx.x, P = t.page_shift;
     const int width = t.max_pages << P;  // below 2^31
-    auto length = [&](int b) { return min(max(t.len[b], 0), width); };
-    auto target = [&](int b) { return max(to[b], 0); };
-
-    // those that shrink, a wave each
-    for (int b = wave; b < t.n_seqs; b += kPlanThreads / 64) {
-        const int have = length(b), want = target(b);
-        if (want >= have) continue;
-        int32_t* row = t.pages + int64_t(b) * t.max_pages;
-        for (int e = pages_of(want, P) + lane; e < pages_of(have, P); e += 64) {
-            const int p = row[e];
-            if (unsigned(p) < unsigned(t.n_pages)) add_to(t.refs + p, -1);
-            row[e] = -1;
-        }
-    }
-    block_fence();
-    // The page that a growing sequence's next position lies in, if it has rows already: how many such sequences
-    // share it, and the last of them. (A sequence that shrank still has its old length here: it does not grow.)
-    auto last_page = [&](int b) {
-        const int have = length(b), want = target(b);
+    auto length = [&](int b) { return b < t.n_seqs ? min(max(t.len[b], 0), width) : 0; };
+    auto target = [&](int b) { return b < t.n_seqs ? max(to[b], 0) : 0; };
+    // The page that a growing sequence's next position lies in, if it has rows already.
+    auto last_page = [&](int b, int have, int want) {
         if (want <= have || want > width || !(have & ((1 << P) - 1))) return -1;
         const int p = t.pages[int64_t(b) * t.max_pages + (have >> P)];
         return unsigned(p) < unsigned(t.n_pages) ? p : -1;
     };
+
+    for (int b0 = 0; b0 < t.n_seqs; b0 += kPlanThreads) {
+        const int b = b0 + tid, have = length(b), want = target(b);
+        // those that shrink give their pages back
+        const int keep = pages_of(want, P);
+        for_entries(want < have ? pages_of(have, P) - keep : 0, b, [&](int s, int e) {
+            // the wave's other lanes know the sequence alone
+            int32_t* entry = t.pages + int64_t(s) * t.max_pages + pages_of(target(s), P) + e;
+            const int p = *entry;
+            if (unsigned(p) < unsigned(t.n_pages)) add_to(t.refs + p, -1);
+            *entry = -1;
+        });
+        if (const int p = last_page(b, have, want); p >= 0) w.a[p] = 0, w.b[p] = -1;
+    }
+    __syncthreads();
+    // how many sequences grow out of a page, and the last of them
     for (int b = tid; b < t.n_seqs; b += kPlanThreads)
-        if (const int p = last_page(b); p >= 0) w.a[p] = 0, w.b[p] = -1;
-    block_fence();
-    for (int b = tid; b < t.n_seqs; b += kPlanThreads)
-        if (const int p = last_page(b); p >= 0) {
+        if (const int p = last_page(b, length(b), target(b)); p >= 0) {
             add_to(w.a + p, 1);
             __hip_atomic_fetch_max(w.b + p, b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-    block_fence();
+    __syncthreads();
     // pages that each needs, and where in the list of free ones they begin
     int64_t total = 0;
     for (int b0 = 0; b0 < t.n_seqs; b0 += kPlanThreads) {
-        const int b = b0 + tid;
-        int64_t need = 0;
+        const int b = b0 + tid, have = length(b), want = target(b), p = last_page(b, have, want);
+        const bool grows = want > have && want <= width;
         int copy = -1;
-        bool grows = false;
-        if (b < t.n_seqs) {
-            const int have = length(b), want = target(b);
-            grows = want > have && want <= width;
-            if (grows) {
-                const int p = last_page(b);
-                if (p >= 0) {
-                    const int refs = ld_now(t.refs + p);
-                    if (refs > 1 && !(ld_now(w.a + p) == refs && ld_now(w.b + p) == b)) copy = p;
-                }
-                need = pages_of(want, P) - pages_of(have, P) + (copy >= 0);
-            }
+        if (p >= 0) {
+            const int refs = ld_now(t.refs + p), out = ld_now(w.a + p), last = ld_now(w.b + p);
+            if (refs > 1 && !(out == refs && last == b)) copy = p;
         }
         int64_t all;
-        const int64_t off = total + scan_before(need, lds, all);
+        const int64_t off =
+            total + scan_before(grows ? uint32_t(pages_of(want, P) - pages_of(have, P) + (copy >= 0)) : 0u, lds, turn, all);
         if (b < t.n_seqs) {
             w.src[b] = copy;
-            // past the pool's end no sequence is served any more, wherever it would begin
-            w.off[b] = grows ? int(min(off, int64_t(t.n_pages) + 1)) : -1;
+            w.off[b] = grows ? int(min(off, int64_t(t.n_pages) + 1)) : -1;  // past the pool none is served, wherever
         }
         total += all;
     }
-    block_fence();
     // the lowest free pages, as many as are needed
     const int most = int(min(total, int64_t(t.n_pages)));
     int found = 0;
+    __syncthreads();  // w.a counted
     for (int base = 0; base < t.n_pages && found < most; base += 4 * kPlanThreads) {
         const int at = base + 4 * tid;
         const i4 r = four_refs(t.refs, at, t.n_pages);
-        const int n = (r[0] <= 0) + (r[1] <= 0) + (r[2] <= 0) + (r[3] <= 0);
         int64_t all;
-        int64_t i = found + scan_before(int64_t(n), lds, all);
+        int64_t i = found + scan_before((r[0] <= 0) + (r[1] <= 0) + (r[2] <= 0) + (r[3] <= 0), lds, turn, all);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (r[k] <= 0 && i++ < most) w.a[i - 1] = at + k;
         found += int(all);
     }
     found = min(found, most);
-    block_fence();
-    // those that grow, a wave each
-    for (int b = wave; b < t.n_seqs; b += kPlanThreads / 64) {
-        const int have = length(b), want = target(b), off = w.off[b], old = w.src[b];
-        bool done = want <= width;
-        int from = -1, into = -1;
-        if (off >= 0) {
-            const int first = pages_of(have, P) - (old >= 0), n = pages_of(want, P) - first;
-            done = int64_t(off) + n <= found;
-            if (done) {
-                int32_t* row = t.pages + int64_t(b) * t.max_pages + first;
-                for (int e = lane; e < n; e += 64) {
-                    const int p = w.a[off + e];
-                    row[e] = p;
-                    t.refs[p] = 1;
-                }
-                if (old >= 0) from = old, into = w.a[off];
-            }
-        }
-        if (lane == 0) {
-            if (from >= 0) add_to(t.refs + from, -1);
-            w.src[b] = from;
+    __syncthreads();
+    // those that grow take them
+    for (int b0 = 0; b0 < t.n_seqs; b0 += kPlanThreads) {
+        const int b = b0 + tid, have = length(b), want = target(b);
+        const int off = b < t.n_seqs ? w.off[b] : -1, old = b < t.n_seqs ? w.src[b] : -1;
+        const int n = off >= 0 ? pages_of(want, P) - pages_of(have, P) + (old >= 0) : 0;
+        const bool serve = off >= 0 && int64_t(off) + n <= found;
+        for_entries(serve ? n : 0, b, [&](int s, int e) {
+            const int p = w.a[w.off[s] + e];
+            t.pages[int64_t(s) * t.max_pages + pages_of(length(s), P) - (w.src[s] >= 0) + e] = p;
+            t.refs[p] = 1;
+        });
+        const int into = serve && old >= 0 ? w.a[off] : -1;
+        // every lane's entries are written (the wave's lanes read its sequences' lengths and copies until here)
+        __builtin_amdgcn_wave_barrier();
+        if (b < t.n_seqs) {
+            if (into >= 0) add_to(t.refs + old, -1);
+            w.src[b] = into >= 0 ? old : -1;
             w.dst[b] = into;
             w.tail[b] = have & ((1 << P) - 1);
+            const bool done = serve || want <= have;
             if (done) t.len[b] = want;
             ok[b] = done;
         }
     }
-    if (tid == 0) w.n[0] = t.n_seqs;
 }
 
 // Copies pages of all layers: pair i from src[i] to dst[i], of its first
@@ -242,24 +244,26 @@ __global__ void __launch_bounds__(256) k_pages_copy(Copy c) {
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) copy_item(c, i);
 }
 
-// Rows of the table trade places, `cols` columns of all of them to a block,
+// Rows of the table trade places, 2^shift columns of all of them to a block,
 // through LDS, so that every row is read before any is written; the last block
 // does the same for the lengths. Entries that a sequence does not hold are -1
 // and count for nothing.
-__global__ void __launch_bounds__(256) k_pages_fork(Tables t, const int32_t* __restrict__ parent, int cols) {
+__global__ void __launch_bounds__(256) k_pages_fork(Tables t, const int32_t* __restrict__ parent, int shift) {
     extern __shared__ int32_t old[];
     const bool lens = blockIdx.x == gridDim.x - 1;
-    const int c0 = lens ? 0 : blockIdx.x * cols, n = lens ? 1 : min(cols, t.max_pages - c0);
+    if (lens) shift = 0;
+    const int c0 = lens ? 0 : blockIdx.x << shift, n = lens ? 1 : min(1 << shift, t.max_pages - c0);
     int32_t* rows = lens ? t.len : t.pages + c0;
     const int64_t stride = lens ? 1 : t.max_pages;
-    for (int i = threadIdx.x; i < t.n_seqs * n; i += 256) old[i] = rows[(i / n) * stride + i % n];
+    const int c = threadIdx.x & ((1 << shift) - 1), step = 256 >> shift;
+    for (int b = threadIdx.x >> shift; b < t.n_seqs; b += step) old[(b << shift) + c] = c < n ? rows[b * stride + c] : -1;
     __syncthreads();
-    for (int i = threadIdx.x; i < t.n_seqs * n; i += 256) {
-        const int b = i / n, p = parent[b];
+    for (int b = threadIdx.x >> shift; b < t.n_seqs; b += step) {
+        const int p = parent[b];
         if (p == b || p < -1 || p >= t.n_seqs) continue;
-        const int was = old[i], now = p < 0 ? (lens ? 0 : -1) : old[p * n + i % n];
-        if (was == now) continue;
-        rows[b * stride + i % n] = now;
+        const int was = old[(b << shift) + c], now = p < 0 ? (lens ? 0 : -1) : old[(p << shift) + c];
+        if (was == now || c >= n) continue;
+        rows[b * stride + c] = now;
         if (lens) continue;
         if (unsigned(now) < unsigned(t.n_pages)) add_to(t.refs + now, 1);
         if (unsigned(was) < unsigned(t.n_pages)) add_to(t.refs + was, -1);
@@ -270,45 +274,48 @@ __global__ void __launch_bounds__(256) k_pages_fork(Tables t, const int32_t* __r
 // moves to the i-th free one below U. One block; src and dst list the moves,
 // b the new place of the pages from U on.
 __global__ void __launch_bounds__(kPlanThreads) k_pages_plan(Tables t, Work w, int32_t* __restrict__ used) {
-    __shared__ int64_t lds[17];
+    __shared__ uint32_t lds[32];
+    int turn = 0;
     const int tid = threadIdx.x;
-    int64_t mine = 0, U;
+    uint32_t mine = 0;
     for (int at = 4 * tid; at < t.n_pages; at += 4 * kPlanThreads) {
         const i4 r = four_refs(t.refs, at, t.n_pages);
+#pragma unroll
         for (int k = 0; k < 4; ++k) mine += at + k < t.n_pages && r[k] > 0;
     }
-    scan_before(mine, lds, U);
+    int64_t U, all;
+    scan_before(mine, lds, turn, U);
     int64_t holes = 0, moves = 0;
     for (int base = 0; base < t.n_pages; base += 4 * kPlanThreads) {
         const int at = base + 4 * tid;
         const i4 r = four_refs(t.refs, at, t.n_pages);
-        int64_t n = 0;  // free pages below U, held ones from U on: no page is both
+        uint32_t n = 0;  // free pages below U in the upper half, held ones from U on in the lower: 4096 of them at most
+#pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int p = at + k;
-            if (p < t.n_pages) n += p < U ? int64_t(r[k] <= 0) << 32 : int64_t(r[k] > 0);
+            if (p < t.n_pages) n += p < U ? uint32_t(r[k] <= 0) << 16 : uint32_t(r[k] > 0);
         }
-        int64_t all;
-        const int64_t before = scan_before(n, lds, all);
-        int64_t h = holes + (before >> 32), m = moves + (before & 0xffffffff);
+        const int64_t before = scan_before(n, lds, turn, all);
+        int64_t h = holes + (before >> 16), m = moves + (before & 0xffff);
+#pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int p = at + k;
-            if (p >= t.n_pages) break;
+            if (p >= t.n_pages) continue;
             if (p < U) {
                 if (r[k] <= 0) w.dst[h++] = p;
-            } else if (r[k] > 0) {
-                w.src[m++] = p;
+            } else {
+                w.b[p] = p;
+                if (r[k] > 0) w.src[m++] = p;
             }
         }
-        holes += all >> 32;
-        moves += all & 0xffffffff;
+        holes += all >> 16;
+        moves += all & 0xffff;
     }
-    block_fence();
-    for (int64_t i = U + tid; i < t.n_pages; i += kPlanThreads) w.b[i] = int(i);
-    block_fence();
+    __syncthreads();
     for (int64_t i = tid; i < moves; i += kPlanThreads) {
         const int from = w.src[i], into = w.dst[i];
         w.b[from] = into;
-        t.refs[into] = t.refs[from];
+        t.refs[into] = ld_now(t.refs + from);
         t.refs[from] = 0;
     }
     if (tid == 0) {
@@ -327,17 +334,30 @@ __global__ void __launch_bounds__(256) k_pages_remap(Tables t, Work w) {
     }
 }
 
-// Slot and position of every new token of a batch.
+// Slot and position of every new token of a batch. A block has the sequences'
+// first rows in LDS (of more than 4096 every 2nd, 4th .. of them) and searches there.
+constexpr int kSlotSeqs = 4096;
 __global__ void __launch_bounds__(256) k_kv_slots(const int32_t* __restrict__ cu, const int32_t* __restrict__ kv_len,
                                                   const int32_t* __restrict__ pages, int n_seqs, int n_tokens,
-                                                  int max_pages, int page_shift, int n_pages,
+                                                  int max_pages, int page_shift, int n_pages, int step,
                                                   int64_t* __restrict__ slots, int32_t* __restrict__ pos) {
-    const int t = blockIdx.x * 256 + threadIdx.x;
+    __shared__ int32_t first[kSlotSeqs];
+    const int t = blockIdx.x * 256 + threadIdx.x, n = (n_seqs + (1 << step) - 1) >> step;
+    for (int i = threadIdx.x; i < n; i += 256) first[i] = cu[i << step];
+    __syncthreads();
     if (t >= n_tokens) return;
-    int lo = 0, hi = n_seqs;  // sequences whose rows begin at or before t
+    int lo = 0, hi = n;  // how many of them begin at or before t
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (cu[mid] <= t)
+        if (first[mid] <= t)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    lo = max(lo - 1, 0) << step, hi = min(lo + (1 << step), n_seqs);
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if ((step ? cu[mid] : first[mid]) <= t)
             lo = mid + 1;
         else
             hi = mid;
@@ -345,12 +365,16 @@ __global__ void __launch_bounds__(256) k_kv_slots(const int32_t* __restrict__ cu
     const int b = lo - 1;
     int64_t slot = -1;
     int p = 0;
-    if (b >= 0 && t < min(cu[b + 1], n_tokens)) {
-        const int64_t q = int64_t(max(kv_len[b], 0)) - min(cu[b + 1], n_tokens) + t;
-        p = int(q);
-        if (q >= 0 && q >> page_shift < max_pages) {
-            const int pg = pages[int64_t(b) * max_pages + (q >> page_shift)];
-            if (unsigned(pg) < unsigned(n_pages)) slot = (int64_t(pg) << page_shift) + (q & ((1 << page_shift) - 1));
+    if (b >= 0) {
+        const int end = min(cu[b + 1], n_tokens);
+        if (t < end) {
+            const int64_t q = int64_t(max(kv_len[b], 0)) - end + t;
+            p = int(q);
+            if (q >= 0 && q >> page_shift < max_pages) {
+                const int pg = pages[int64_t(b) * max_pages + (q >> page_shift)];
+                if (unsigned(pg) < unsigned(n_pages))
+                    slot = (int64_t(pg) << page_shift) + (q & ((1 << page_shift) - 1));
+            }
         }
     }
     slots[t] = slot;
@@ -413,11 +437,11 @@ int wv_kv_fork_dev(uint64_t cache, const wv_kv_tables* tables, const int32_t* d_
     if (rc || !k.n_seqs) return rc;
     if (!d_parent) return rt_fail(WV_E_ARG, "wv_kv_fork: nil parent");
     (void)hipSetDevice(c.device);
-    int cols = 64;
-    while (cols > 1 && cols * k.n_seqs > 4096) cols /= 2;
-    const unsigned blocks = unsigned((int64_t(k.max_pages) + cols - 1) / cols) + 1;
-    hipLaunchKernelGGL(k_pages_fork, dim3(blocks), dim3(256), unsigned(cols) * unsigned(k.n_seqs) * 4u,
-                       rt_stream(stream, c.device), k, d_parent, cols);
+    int shift = 6;  // up to four entries a thread, as long as 4 columns stay together
+    while (shift > 0 && (k.n_seqs << shift) > (shift > 2 ? 1024 : 4096)) --shift;
+    const unsigned blocks = unsigned((int64_t(k.max_pages) + (1 << shift) - 1) >> shift) + 1;
+    hipLaunchKernelGGL(k_pages_fork, dim3(blocks), dim3(256), unsigned(k.n_seqs) * 4u << shift,
+                       rt_stream(stream, c.device), k, d_parent, shift);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_kv_fork: kernel launch");
 }
@@ -479,9 +503,11 @@ int wv_kv_slots_dev(uint64_t cache, const wv_kv_batch* batch, int64_t* d_slots, 
     if (!d_slots || (b.n_seqs && (!b.d_cu_q || !b.d_kv_len || (b.max_pages && !b.d_pages))))
         return rt_fail(WV_E_ARG, "wv_kv_slots: nil slots/cu_q/kv_len/pages");
     (void)hipSetDevice(c.device);
+    int step = 0;
+    while ((int64_t(b.n_seqs) + (1 << step) - 1) >> step > kSlotSeqs) ++step;
     hipLaunchKernelGGL(k_kv_slots, dim3(unsigned((b.n_tokens + 255) / 256)), dim3(256), 0, rt_stream(stream, c.device),
                        b.d_cu_q, b.d_kv_len, b.d_pages, b.n_seqs, b.n_tokens, b.max_pages, c.layer(0).page_shift,
-                       c.c.n_pages, d_slots, d_pos);
+                       c.c.n_pages, step, d_slots, d_pos);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_kv_slots: kernel launch");
 }
