@@ -206,12 +206,16 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_resize(Tables t, Work w,
 }
 
 // Copies pages of all layers: pair i from src[i] to dst[i], of its first
-// tail[i] positions (NULL: all) the blocks of 32 that they lie in. A block
-// takes K or V (with its half of the scales) of one pair, layer and KV head.
+// tail[i] positions (NULL: all) what holds them: whole blocks of 32, of the
+// last one a unit's first keys (K) and the octets that they lie in (V, scales).
+// A block takes K or V (with its half of the scales) of one pair and KV head,
+// in one group of layers. 240 pages of 17 fp16 positions, 4 layers of 8 heads:
+// 17 us, 82 MB written; a resize without a copy 3 us.
 struct Copy {
     uint8_t* base;
     size_t layer_bytes, code_bytes;
     int n_layers, n_kv, block_bytes, page_shift, n_pages;
+    int groups;  // of the layers
     const int32_t *src, *dst, *tail, *count;
     int pairs;  // at most; count (if not NULL) holds how many there are
 };
@@ -220,27 +224,33 @@ __device__ __forceinline__ void copy_item(const Copy& c, int64_t item) {
     item >>= 1;
     const int head = int(item % c.n_kv);
     item /= c.n_kv;
-    const int layer = int(item % c.n_layers);
-    const int64_t i = item / c.n_layers;
+    const int group = int(item % c.groups);
+    const int64_t i = item / c.groups;
     const int from = c.src[i], into = c.dst[i], pb = c.page_shift - 5;
     if (unsigned(from) >= unsigned(c.n_pages) || unsigned(into) >= unsigned(c.n_pages) || from == into) return;
-    const int blocks = c.tail ? (c.tail[i] + 31) >> 5 : 1 << pb;
-    uint8_t* codes = c.base + size_t(layer) * c.layer_bytes + part * c.code_bytes;
+    const int keys = c.tail ? c.tail[i] : 1 << c.page_shift, whole = keys >> 5, rest = keys & 31;
     const int64_t b0 = (int64_t(from) * c.n_kv + head) << pb, b1 = (int64_t(into) * c.n_kv + head) << pb;
-    const uint4* p = reinterpret_cast<const uint4*>(codes + b0 * c.block_bytes);
-    uint4* q = reinterpret_cast<uint4*>(codes + b1 * c.block_bytes);
-    const int units = blocks * (c.block_bytes / 16);
-    for (int u = threadIdx.x; u < units; u += 256) q[u] = p[u];
-    // octets of a block's scales: [4][K 8, V 8]
-    float* scales = reinterpret_cast<float*>(c.base + size_t(layer) * c.layer_bytes + 2 * c.code_bytes);
-    for (int u = threadIdx.x; u < blocks * 32; u += 256) {
-        const int at = (u >> 5) * kKvScales + ((u >> 3) & 3) * 16 + 8 * part + (u & 7);
-        scales[b1 * kKvScales + at] = scales[b0 * kKvScales + at];
+    const int bu = c.block_bytes / 16, units = whole * bu;
+    for (int layer = group; layer < c.n_layers; layer += c.groups) {
+        uint8_t* codes = c.base + size_t(layer) * c.layer_bytes + part * c.code_bytes;
+        const uint4* p = reinterpret_cast<const uint4*>(codes + b0 * c.block_bytes);
+        uint4* q = reinterpret_cast<uint4*>(codes + b1 * c.block_bytes);
+        for (int u = threadIdx.x; u < units; u += 256) q[u] = p[u];
+        // octet o = 2a + b of a block holds no key before 16a + 4b
+        auto octet_used = [&](int o) { return 16 * (o >> 1) + 4 * (o & 1) < rest; };
+        if (rest)
+            for (int u = threadIdx.x; u < bu; u += 256)
+                if (part ? octet_used(4 * u / bu) : (u & 31) < rest) q[units + u] = p[units + u];
+        float* scales = reinterpret_cast<float*>(c.base + size_t(layer) * c.layer_bytes + 2 * c.code_bytes);
+        for (int u = threadIdx.x; u < (whole + (rest > 0)) * 32; u += 256) {
+            const int o = (u >> 3) & 3, at = (u >> 5) * kKvScales + o * 16 + 8 * part + (u & 7);
+            if ((u >> 5) < whole || octet_used(o)) scales[b1 * kKvScales + at] = scales[b0 * kKvScales + at];
+        }
     }
 }
 __global__ void __launch_bounds__(256) k_pages_copy(Copy c) {
     const int64_t pairs = c.count ? min(*c.count, c.pairs) : c.pairs;
-    const int64_t items = pairs * c.n_layers * c.n_kv * 2;
+    const int64_t items = pairs * c.groups * c.n_kv * 2;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) copy_item(c, i);
 }
 
@@ -388,8 +398,10 @@ int launch_copy(const KvCache& c, const int32_t* src, const int32_t* dst, const 
     k.n_layers = c.c.n_layers, k.n_kv = c.c.n_kv_heads, k.block_bytes = 32 * c.c.head_dim * kv_code_bytes(c.c.type);
     k.page_shift = c.layer(0).page_shift, k.n_pages = c.c.n_pages;
     k.src = src, k.dst = dst, k.tail = tail, k.count = count, k.pairs = pairs;
-    const int64_t pages = std::min<int64_t>(int64_t(pairs) * k.n_layers, kCopyBlocks);  // no overflow below
-    hipLaunchKernelGGL(k_pages_copy, dim3(unsigned(std::min<int64_t>(pages * k.n_kv * 2, kCopyBlocks))), dim3(256), 0, s, k);
+    // a layer to a block while there are few pairs, all layers where there are many
+    const int64_t items = int64_t(pairs) * k.n_kv * 2;
+    k.groups = int(std::max<int64_t>(1, std::min<int64_t>(k.n_layers, kCopyBlocks / items)));
+    hipLaunchKernelGGL(k_pages_copy, dim3(unsigned(std::min<int64_t>(items * k.groups, kCopyBlocks))), dim3(256), 0, s, k);
     return int(hipGetLastError());
 }
 
