@@ -71,7 +71,8 @@ def check(got, x, pos, f, layout, rot, gain, tol=TOL):
 @pytest.mark.parametrize("layout", ["half", "pairs"])
 @pytest.mark.parametrize("hd,rot,n,heads,kv", [(128, 128, 1, 32, 8), (64, 64, 5, 7, 1), (80, 20, 33, 3, 2), (2, 2, 3, 1, 1),
                                                (256, 128, 17, 4, 4), (6, 4, 40, 5, 0), (1024, 1022, 3, 2, 1),
-                                               (128, 64, 300, 8, 8), (66, 66, 9, 2, 3)])
+                                               (128, 64, 300, 8, 8), (66, 66, 9, 2, 3),
+                                               (80, 22, 30, 5, 2), (8, 2, 600, 300, 1), (64, 60, 5, 70, 3)])
 def test_layouts(layout, hd, rot, n, heads, kv):
     rng = np.random.default_rng(hd + rot + n)
     r = Rope(hd, rot, theta=1e4, layout=layout)
