@@ -567,12 +567,255 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
     attn_rows<HD, TYPE, ONCE, kWhole>(a, G, t, blockIdx.x, blockIdx.z);
 }
 
-// The same rows with their sequences in groups. MODE kLead: a tile's rows are of a group, over the keys it shares.
-template <int HD, int TYPE, bool ONCE, int MODE>
-__global__ void __launch_bounds__(256, 2) k_kv_attn_group_rows(KvAttn a, int G, int max_rows, int tile0) {
+// The keys that a group shares: 32 query rows of its sequences and one KV head
+// per block, each of its 4 waves over its own 32-key blocks, from the cache into
+// operands as in attn_rows, but on 32x32x16 products (S^T = K Q^T leaves a lane
+// with one row, l & 31, and the keys of octets h and 2 + h, h = l >> 5), so that
+// a key's codes are read and converted once for 32 rows. Meant for as many rows
+// as give the matrix unit work and are too few for the tiles of 128.
+template <int HD, int TYPE>
+__device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t, int kvh, int sp) {
+    constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
+    constexpr int S = HD / 16;                             // k steps of a score product
+    constexpr int NK = S / (TYPE == WV_KV_F16 ? 1 : 2);    // 16-byte K loads
+    constexpr int T = HD / 32;                             // dim tiles of the output
+    constexpr int NV = 2 * T / (TYPE == WV_KV_F16 ? 1 : 2);  // 16-byte V loads
+    constexpr int BB = 32 * HD * E;
+    constexpr int LD = HD + 4;
+    __shared__ float red[4][16][LD];
+    __shared__ float rm[4][32], rl[4][32];
+    __shared__ __align__(16) float scales[4][kKvScales];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int row = min(t.r0 + n, t.rows - 1);
+    int pos, p_first, p_last;
+    row_positions<kLead>(a, t, G, t.r0, 32, row, pos, p_first, p_last);
+    const Range rg = tile_range<kLead>(a, t, p_first, p_last, sp, 4);
+    const int first = a.window > 0 ? pos - a.window + 1 : 0;
+
+    const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
+    const int pb = a.c.page_shift - 5;
+    auto block_at = [&](int kb, bool& ok) {
+        const int pg = __builtin_amdgcn_readfirstlane(pages[kb >> pb]);
+        ok = unsigned(pg) < unsigned(a.c.n_pages);
+        return kv_block(a.c, ok ? pg : 0, kvh, (kb & ((1 << pb) - 1)) << 5);
+    };
+    u4 kr[NK], vr[NV];
+    float sc;  // scale `lane` of the block's 64
+    auto load_k = [&](int64_t b) {
+        const u4* p = reinterpret_cast<const u4*>(a.c.k + b * BB) + h * 32 + n;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) kr[i] = p[64 * i];
+        sc = a.c.s[b * kKvScales + lane];
+    };
+    auto load_v = [&](int64_t b) {
+        const u4* p = reinterpret_cast<const u4*>(a.c.v + b * BB) + h * (HD * E / 2) + n;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < NV / 2; ++i) vr[q * (NV / 2) + i] = p[q * HD * E + 32 * i];
+    };
+    int kb = rg.begin + wave;
+    bool ok = false;
+    int64_t blk = 0;
+    if (kb < rg.end) {
+        blk = block_at(kb, ok);
+        load_k(blk);
+    }
+
+    h8 qh[S], ql[S];
+    float qs;
+    {
+        const float* qp = a.q + int64_t(t.q0 + row / G) * a.qs + (kvh * G + row % G) * HD;
+        float x[S][8], m = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[s][j] = qp[TYPE == WV_KV_F16 ? 16 * s + 8 * h + j : 32 * (s / 2) + 16 * h + 8 * (s % 2) + j];
+                m = fmaxf(m, fabsf(x[s][j]));
+            }
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+        float inv;
+        qs = row_unit(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), a.scale, inv);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[s][j] *= inv;
+            split8(x[s], qh[s], ql[s]);
+        }
+    }
+    f16v o[T];
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[i][k] = 0.0f;
+    float mx = kNoMax, l = 0.0f;
+    int eo = -200;  // the lane's outputs are in units of 2^eo
+    float* ws = scales[wave];
+
+    while (kb < rg.end) {
+        const int next = kb + 4;
+        bool nok = false;
+        int64_t nblk = 0;
+        if (next < rg.end) nblk = block_at(next, nok);
+        load_v(blk);
+        {   // the V scales in place; a NaN one makes the K scale NaN, where the mask can drop it
+            const float v = __shfl_down(sc, 8, 64);  // of lanes that hold K scales: their key's V scale
+            ws[lane] = (lane & 8) ? fmaxf(sc, 0.0f) : v == v ? sc * kScore : v;
+        }
+        f16v s;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) s[k] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < S; ++c) {
+            h8 f;
+            if (TYPE == WV_KV_F16) {
+                f = as_half(kr[c]);
+            } else {
+                const u4 u = kr[c / 2];
+                f = c % 2 ? q8_half(u.z, u.w) : q8_half(u.x, u.y);
+            }
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[c], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[c], s, 0, 0, 0);
+        }
+        if (next < rg.end) load_k(nblk);
+        if (ok) {
+            f4 ks[4], vs[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f4* p = reinterpret_cast<const f4*>(&ws[(2 * (q >> 1) + h) * 16 + 4 * (q & 1)]);
+                ks[q] = p[0], vs[q] = p[2];
+            }
+            float top = 0.0f, m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= ks[i >> 2][i & 3];
+            // whole: every row of the block attends every key
+            const int k0 = kb << 5;
+            const bool whole = k0 + 31 <= rg.p_first && (a.window <= 0 || k0 > rg.p_last - a.window);
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = k0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (key > pos || key < first) s[i] = -INFINITY, vs[i >> 2][i & 3] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                m = fmaxf(m, s[i]);
+                top = fmaxf(top, vs[i >> 2][i & 3]);
+            }
+            auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+            m = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const int en = max(eo, int(max(r[0], r[1]) >> 23) - 126);  // top < 2^en
+            m = fmaxf(mx, ceilf(m * qs));
+            const float al = __builtin_amdgcn_exp2f(mx - m), f = al * ldexpf(1.0f, max(eo - en, -250));
+            eo = en;
+            mx = m;
+            const float unit = ldexpf(1.0f, -eo), up = 14.0f - m;
+            float p[16], add[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[i], qs, up));
+                add[i & 1] += e;
+                p[i] = e * (vs[i >> 2][i & 3] * unit);
+            }
+            l = fmaf(l, al, add[0] + add[1]);
+            h8 ph[2], pl[2];
+            split8(p, ph[0], pl[0]);
+            split8(p + 8, ph[1], pl[1]);
+            if (__ballot(f != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < T; ++i) o[i] *= f;
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < T; ++i) {
+                    h8 fv;
+                    if (TYPE == WV_KV_F16) {
+                        fv = as_half(vr[q * T + i]);
+                    } else {
+                        const u4 u = vr[q * (T / 2) + i / 2];
+                        fv = i % 2 ? q8_half(u.z, u.w) : q8_half(u.x, u.y);
+                    }
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv, pl[q], o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv, ph[q], o[i], 0, 0, 0);
+                }
+        }
+        kb = next;
+        ok = nok;
+        blk = nblk;
+    }
+
+    // as in attn_rows, 16 rows at a time
+    const auto lr = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(lr[0]) + __uint_as_float(lr[1]);
+    const float back = ldexpf(1.0f, max(eo, -126)), wl = l != 0.0f ? 1.0f / l : 0.0f;
+    if (h == 0) {
+        rm[wave][n] = mx;
+        rl[wave][n] = l;
+    }
+    const int c = threadIdx.x & 15;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        if (part) __syncthreads();
+        if ((n >> 4) == part) {
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int md = 8 * (k >> 2) + 4 * h + (k & 3);
+                    const int d = TYPE == WV_KV_F16 ? 32 * i + md : 64 * (i / 2) + 2 * md + i % 2;
+                    red[wave][n & 15][d] = o[i][k] * wl * back;
+                }
+        }
+        __syncthreads();
+        const int lrow = threadIdx.x >> 4, r = 16 * part + lrow, orow = t.r0 + r;
+        if (orow >= t.rows) continue;
+        float M = -INFINITY, w[4], L = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (rl[i][r] != 0.0f) M = fmaxf(M, rm[i][r]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = rl[i][r] != 0.0f ? __builtin_amdgcn_exp2f(rm[i][r] - M) * rl[i][r] : 0.0f;
+            L += w[i];
+        }
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        float* dst = a.part + ((int64_t(t.q0 + orow / G) * a.n_heads + kvh * G + orow % G) * a.splits + sp) * LD;
+#pragma unroll
+        for (int d = c; d < HD; d += 16) {
+            float x = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (w[i] != 0.0f) x += w[i] * inv * red[i][lrow][d];
+            dst[d] = x;
+        }
+        if (c == 0) {
+            dst[HD] = M;
+            dst[HD + 1] = L;
+        }
+    }
+}
+
+// A batch whose sequences are in groups, in one launch: the blocks of the
+// groups' rows over the shared keys, which take longest, then those of every
+// sequence's rows over its own. lead_tiles: 0 where the tiles of 128 rows took
+// the former.
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(256, 2) k_kv_attn_groups(KvAttn a, int G, int lead_tiles, int y0) {
     Tile t;
-    if (!find_group_tile<16, MODE>(a, G, tile0 + int(blockIdx.y), 1, max_rows, t)) return;
-    attn_rows<HD, TYPE, ONCE, MODE>(a, G, t, blockIdx.x, blockIdx.z);
+    int y = y0 + int(blockIdx.y);
+    if (y < lead_tiles * a.lead) {
+        if (find_group_tile<32, kLead>(a, G, y / a.lead, 1, INT32_MAX, t)) attn_lead<HD, TYPE>(a, G, t, blockIdx.x, y % a.lead);
+        return;
+    }
+    y -= lead_tiles * a.lead;
+    const int own = a.splits - a.lead;
+    if (find_group_tile<16, kOwn>(a, G, y / own, 1, INT32_MAX, t)) attn_rows<HD, TYPE, true, kOwn>(a, G, t, blockIdx.x, y % own);
 }
 
 // Many rows: 128 query rows of one sequence and KV head per block, 32 to a
@@ -1146,11 +1389,13 @@ int launch_kv_attn_groups(const KvAttn& a, const KvGroupPlan& p, hipStream_t s) 
     };
     auto pick = [&](auto hd, auto type) {
         constexpr int HD = decltype(hd)::value, TYPE = decltype(type)::value;
-        if (p.lead_many)
+        if (p.lead_many) {
             go(k_kv_attn_tile<HD, TYPE, kLead>, (rows + 127) / 128 + a.n_groups, p.lead, 1);
-        else
-            go(k_kv_attn_group_rows<HD, TYPE, false, kLead>, (rows + 15) / 16 + a.n_groups, p.lead, INT32_MAX);
-        go(k_kv_attn_group_rows<HD, TYPE, true, kOwn>, (rows + 15) / 16 + a.n_seqs, p.own, INT32_MAX);
+            go(k_kv_attn_groups<HD, TYPE>, ((rows + 15) / 16 + a.n_seqs) * p.own, 1, 0);
+        } else {
+            const int64_t lead = (rows + 31) / 32 + a.n_groups;
+            go(k_kv_attn_groups<HD, TYPE>, lead * p.lead + ((rows + 15) / 16 + a.n_seqs) * p.own, 1, int(lead));
+        }
         hipLaunchKernelGGL((k_kv_attn_join<HD, true>), dim3(unsigned(a.n_tokens), unsigned(a.n_heads)), dim3(256), 0, s, a);
     };
     std::integral_constant<int, 128> h128;
