@@ -24,18 +24,30 @@ def dev(x, dtype=None):
     return torch.from_numpy(np.ascontiguousarray(x if dtype is None else np.asarray(x, dtype))).cuda()
 
 
-class Batch:
-    """Groups of sequences in a cache: `groups` lists (members, shared), `before` and `after` count sequences of no
-    group; lens and new per sequence. Members hold the pages of the prefix that are full in common."""
+WIDE = 65536  # positions of a crowd's table
 
-    def __init__(self, rng, groups, lens, new, kv_heads, hd, page, typ, before=0, pad=0, layers=1, layer=0):
+
+class Batch:
+    """Groups of sequences in a cache: `groups` lists (members, shared), the first `before` sequences are of no group,
+    nor are those behind the last; lens and new per sequence. Members hold the pages of the prefix that are full in
+    common. crowd: 64 short sequences more, as a last group, and a table so wide that attention over whole sequences
+    would take longest: shared keys are read once for their group then, else where a call is large enough for that."""
+
+    def __init__(self, rng, groups, lens, new, kv_heads, hd, page, typ, before=0, pad=0, layers=1, layer=0,
+                 crowd=False):
+        if crowd:
+            at = before + sum(m for m, _ in groups)
+            groups = list(groups) + [(64, 64)]
+            lens = list(lens[:at]) + [65 + i % 5 for i in range(64)] + list(lens[at:])
+            new = list(new[:at]) + [1] * 64 + list(new[at:])
+        self.crowd = crowd
         self.rng, self.lens, self.new, self.typ, self.page, self.hd = rng, lens, new, typ, page, hd
         self.kv_heads, self.layer, self.pad, self.n_groups = kv_heads, layer, pad, len(groups)
         members = [m for m, _ in groups]
         self.group_cu = np.concatenate([[0], np.cumsum(members)]) + before
         self.shared = [s for _, s in groups]
         held = [-(-n // page) for n in lens]
-        width = max(max(held), 1)
+        width = WIDE // page if crowd else max(max(held), 1)
         pool = sum(held) + 3
         free = list(rng.permutation(pool))
         self.table = np.full((len(lens), width), -1, np.int32)
@@ -84,8 +96,11 @@ class Batch:
         b = KVBatch(len(self.new), self.out.shape[0], tb.shape[1], cu.data_ptr(), ln.data_ptr(), tb.data_ptr(), max_q)
         return b, KVGroups(self.n_groups, gc.data_ptr(), sh.data_ptr(), max_shared)
 
-    def attend(self, heads, window=0, max_q=0, max_shared=0, in_place=False, **kw):
+    def attend(self, heads, window=0, max_q=0, max_shared=0, in_place=False, grouped=None, **kw):
         self.arrays(heads)
+        b, g = self.structs(max_q, max_shared)
+        if self.crowd and max_shared == window == 0 and grouped is None or grouped:  # shared and own keys' partial rows
+            assert self.kv.attention_shared_scratch(b, g, heads, window) != self.kv.attention_scratch(b, heads, window)
         q = self.d[5]
         out = q if in_place else self.out
         self.kv.attention_shared_dev(self.layer, *self.structs(max_q, max_shared), q.data_ptr(), out.data_ptr(), heads,
@@ -115,22 +130,24 @@ class Batch:
             assert (out[at:] == 7.0).all(), "padding rows written"
 
 
+@pytest.mark.parametrize("crowd", [False, True])
 @pytest.mark.parametrize("typ", ["f16", "q8"])
 @pytest.mark.parametrize("shared", [0, 1, 31, 32, 33, 64, 95, 500])
 @pytest.mark.parametrize("heads,kv_heads,hd,page", [(8, 2, 128, 32), (3, 3, 64, 64), (16, 2, 64, 32)])
-def test_one_group(typ, shared, heads, kv_heads, hd, page):
+def test_one_group(typ, shared, heads, kv_heads, hd, page, crowd):
     rng = np.random.default_rng(shared + hd)
     new = [1, 1, 3, 0, 2]
     lens = [shared + n + x for n, x in zip(new, (0, 1, 40, 7, 130))]
-    b = Batch(rng, [(5, shared)], lens, new, kv_heads, hd, page, typ, pad=2)
+    b = Batch(rng, [(5, shared)], lens, new, kv_heads, hd, page, typ, pad=2, crowd=crowd)
     b.check(b.attend(heads))
     b.check(b.attend(heads, max_q=3, max_shared=shared))
 
 
+@pytest.mark.parametrize("crowd", [False, True])
 @pytest.mark.parametrize("typ", ["f16", "q8"])
 @pytest.mark.parametrize("window", [0, 1, 50, 400])
 @pytest.mark.parametrize("hint", [0, 1, 600, 100000])
-def test_several_groups(typ, window, hint):
+def test_several_groups(typ, window, hint, crowd):
     """Groups of several sizes, an empty one and one of one sequence, sequences before and behind them, windows;
     whatever the launch is told."""
     rng = np.random.default_rng(window + hint)
@@ -140,11 +157,11 @@ def test_several_groups(typ, window, hint):
     new = [int(x) for x in rng.integers(0, 5, len(lead))]
     new[3] = 20
     lens = [max(s + n + int(rng.integers(0, 200)), 1) for s, n in zip(lead, new)]
-    b = Batch(rng, groups, lens, new, 2, 128, 64, typ, before=before, pad=1, layers=2, layer=1)
+    b = Batch(rng, groups, lens, new, 2, 128, 64, typ, before=before, pad=1, layers=2, layer=1, crowd=crowd)
     b.check(b.attend(8, window, max_shared=hint, max_q=20 if hint else 0), window)
 
 
-@pytest.mark.parametrize("typ,hd", [("f16", 128), ("q8", 64)])
+@pytest.mark.parametrize("typ,hd", [("f16", 128), ("q8", 64), ("f16", 64), ("q8", 128)])
 def test_new_tokens_inside_the_shared_keys(typ, hd):
     """Sequences whose new tokens lie among the shared positions see no further than themselves; some end there, one
     has more new tokens than keys."""
@@ -152,13 +169,14 @@ def test_new_tokens_inside_the_shared_keys(typ, hd):
     shared = 320
     new = [60, 1, 5, 300, 33, 20]
     lens = [330, 320, 100, 320, 321, 9]
-    b = Batch(rng, [(6, shared)], lens, new, 2, hd, 32, typ)
+    b = Batch(rng, [(6, shared)], lens, new, 2, hd, 32, typ, crowd=True)
     out = b.attend(4)
     at = np.concatenate([[0], np.cumsum(new)])
     assert not out[at[5]:at[5] + 11].any()  # before position 0
     out9 = out[at[5] + 11:at[6]]
     b.new, keep = b.new[:5], b.q
     b.check(out[: at[5]])
+    keep = keep[: at[6]]
     ref, tol = attention(keep[at[5] + 11:], stored(b.k[5], typ), stored(b.v[5], typ), 9, np.float32(1 / math.sqrt(hd)))
     assert (np.abs(out9 - ref) <= tol).all()
 
@@ -166,26 +184,41 @@ def test_new_tokens_inside_the_shared_keys(typ, hd):
 @pytest.mark.parametrize("typ", ["f16", "q8"])
 @pytest.mark.parametrize("heads,kv_heads,hd,new,groups", [
     (8, 2, 128, 90, [(4, 700)]), (8, 2, 64, 90, [(4, 700), (2, 33), (5, 1500)]), (4, 4, 128, 300, [(5, 256)]),
-    (32, 4, 128, 1, [(200, 1000)]), (8, 1, 64, 2, [(70, 900), (75, 64)])])
+    (16, 4, 128, 1, [(100, 1000)]), (8, 1, 64, 2, [(70, 900), (75, 64)]), (8, 2, 64, 40, [(40, 4500)])])
 @pytest.mark.parametrize("window", [0, 300])
 def test_many_rows(typ, heads, kv_heads, hd, new, groups, window):
-    """Groups with rows enough for the tiles of 128, over more than 64 sequences."""
+    """Groups of many rows, over more than 64 sequences, and of many keys: ranges of several steps and of more than 64
+    blocks."""
     rng = np.random.default_rng(new + hd)
     lead = [s for m, s in groups for _ in range(m)]
     n = [int(x) for x in rng.integers(1, new + 1, len(lead))]
     lens = [s + k + int(rng.integers(0, 100)) for s, k in zip(lead, n)]
+    b = Batch(rng, groups, lens, n, kv_heads, hd, 32, typ, pad=3, crowd=True)
+    b.check(b.attend(heads, window, grouped=False), window)  # at times as many partial rows either way
     b = Batch(rng, groups, lens, n, kv_heads, hd, 32, typ, pad=3)
     b.check(b.attend(heads, window, max_q=new, max_shared=max(lead)), window)
 
 
-def test_many_groups():
+@pytest.mark.parametrize("typ,hd", [("f16", 64), ("q8", 128)])
+@pytest.mark.parametrize("window", [2500, 4000, 4700])
+def test_windows_inside_the_shared_keys(typ, hd, window):
+    """Windows that begin among the shared keys, before a range or within it, and among the own ones."""
+    rng = np.random.default_rng(window)
+    lens = [4800 + int(x) for x in rng.integers(1, 90, 20)] + [2000 + int(x) for x in rng.integers(1, 700, 20)] + [4400]
+    b = Batch(rng, [(20, 4800), (20, 2000)], lens, [1] * 40 + [3], 8, hd, 32, typ, crowd=True)
+    b.check(b.attend(8, window, grouped=True), window)
+
+
+@pytest.mark.parametrize("crowd", [False, True])
+def test_many_groups(crowd):
     """More than 64 groups."""
     rng = np.random.default_rng(1)
     groups = [(int(rng.integers(0, 4)), int(rng.integers(0, 100))) for _ in range(150)]
     lead = [s for m, s in groups for _ in range(m)] + [0, 0]
     n = [int(x) for x in rng.integers(0, 3, len(lead))]
     lens = [max(1, s + k + int(rng.integers(0, 50))) for s, k in zip(lead, n)]
-    b = Batch(rng, groups, lens, n, 1, 64, 32, "q8")
+    b = Batch(rng, groups, lens, n, 1, 64, 32, "q8", crowd=crowd)
+    b.check(b.attend(4))
     b.check(b.attend(4, max_shared=100))
 
 
@@ -193,7 +226,7 @@ def test_no_groups_and_in_place():
     rng = np.random.default_rng(2)
     b = Batch(rng, [], [70, 5, 200], [2, 1, 4], 2, 64, 32, "f16")
     b.check(b.attend(4))
-    b = Batch(rng, [(3, 150)], [151, 170, 300], [1, 2, 40], 2, 64, 32, "f16")
+    b = Batch(rng, [(3, 150)], [151, 170, 300], [1, 2, 40], 2, 64, 32, "f16", crowd=True)
     b.check(b.attend(4, in_place=True), padding=False)
 
 
@@ -201,14 +234,14 @@ def test_pages_and_rows_that_are_not_there():
     """A shared page outside the pool holds no keys; a NaN among the shared keys reaches who attends it alone."""
     rng = np.random.default_rng(3)
     new, lens, shared = [1, 2, 30], [200, 240, 190], 192
-    b = Batch(rng, [(3, shared)], lens, new, 1, 64, 32, "f16")
-    b.table[:, 2] = [99, -1, 1 << 30]
-    present = [np.ones(n, bool) for n in lens]
-    for p in present:
+    b = Batch(rng, [(3, shared)], lens, new, 1, 64, 32, "f16", crowd=True)
+    b.table[:3, 2] = [9999, -1, 1 << 30]
+    present = [np.ones(n, bool) for n in b.lens]
+    for p in present[:3]:
         p[64:96] = False
     b.check(b.attend(4), present=present)
-    b = Batch(rng, [(3, shared)], lens, new, 1, 64, 32, "q8")
-    for b_, k in enumerate(b.k):
+    b = Batch(rng, [(3, shared)], lens, new, 1, 64, 32, "q8", crowd=True)
+    for k in b.k[:3]:
         k[170, 0, 5] = np.nan  # the third sequence's first tokens stand before it
     b.fill()
     out = b.attend(4)
@@ -220,8 +253,8 @@ def test_large_scores_in_one_part():
     """Weights that all lie among the shared or all among the own keys."""
     rng = np.random.default_rng(4)
     for own in (0, 1):
-        b = Batch(rng, [(3, 64)], [90, 100, 200], [1, 1, 3], 1, 64, 32, "f16")
-        for k in b.k:
+        b = Batch(rng, [(3, 64)], [90, 100, 200], [1, 1, 3], 1, 64, 32, "f16", crowd=True)
+        for k in b.k[:3]:
             (k[64:] if own else k[:64])[:] *= 30
         for i in (1, 2):
             b.k[i][:64] = b.k[0][:64]
@@ -233,9 +266,10 @@ def test_captured():
     """Replays take new lengths, groups and tables; without scratch every sequence reads its keys itself."""
     rng = np.random.default_rng(6)
     heads, page = 8, 32
-    b = Batch(rng, [(3, 300), (2, 100)], [310, 340, 301, 180, 103, 40], [2, 1, 1, 3, 2, 1], 2, 64, page, "q8")
+    b = Batch(rng, [(3, 300), (2, 100)], [310, 340, 301, 180, 103, 40], [2, 1, 1, 3, 2, 1], 2, 64, page, "q8",
+              crowd=True)
     b.arrays(heads)
-    st = b.structs(3, 300)
+    st = b.structs()
     nb = b.kv.attention_shared_scratch(*st, heads)
     assert nb > 0
     sc = torch.full((nb // 4 + 4,), float("nan"), device="cuda")
@@ -253,9 +287,10 @@ def test_captured():
             b.lens = [n - 1 for n in b.lens]
             b.k, b.v = [x[:-1] for x in b.k], [x[:-1] for x in b.v]
             b.d[1].copy_(dev(b.lens, np.int32))
-            b.d[4].copy_(dev([200, 64], np.int32))
+            b.d[4].copy_(dev([200, 64, 63], np.int32))
         if step == 2:
-            b.d[3].copy_(dev([0, 3, 3], np.int32))
+            b.d[3].copy_(dev([0, 3, 3, 5], np.int32))
+            b.d[4].copy_(dev([200, 64, 60], np.int32))
         x = rng.standard_normal(b.q.shape).astype(np.float32)
         b.q = x
         q.copy_(dev(x))
@@ -265,29 +300,29 @@ def test_captured():
         assert torch.isnan(sc[nb // 4:]).all()
         b.check(b.out.cpu().numpy())
         b.check(other.cpu().numpy())
-        b.check(b.again(heads, 3, 300))  # the program's own call in between
+        b.check(b.again(heads, 0, 0))  # the program's own call in between
 
 
 def test_stream_and_repeats():
     rng = np.random.default_rng(7)
-    b = Batch(rng, [(9, 700)], [710 + 11 * i for i in range(9)], [1] * 9, 2, 128, 64, "f16")
-    first = b.attend(8, max_shared=700)
+    b = Batch(rng, [(9, 700)], [710 + 11 * i for i in range(9)], [1] * 9, 2, 128, 64, "f16", crowd=True)
+    first = b.attend(8)
     b.check(first)
     s = torch.cuda.Stream()
     q = b.d[5]
     for _ in range(3):
         out = torch.zeros_like(b.out)
         torch.cuda.synchronize()
-        b.kv.attention_shared_dev(0, *b.structs(0, 700), q.data_ptr(), out.data_ptr(), 8, 1 / math.sqrt(128),
+        b.kv.attention_shared_dev(0, *b.structs(), q.data_ptr(), out.data_ptr(), 8, 1 / math.sqrt(128),
                                   stream=s.cuda_stream)
         s.synchronize()
         assert np.array_equal(out.cpu().numpy(), first)
 
 
 def test_refusals():
-    b = Batch(np.random.default_rng(1), [(2, 40)], [50, 60], [1, 1], 2, 64, 32, "f16")
+    b = Batch(np.random.default_rng(1), [(2, 40)], [50, 60], [1, 1], 2, 64, 32, "f16", crowd=True)
     b.arrays(4)
-    bt, gr = b.structs(1, 40)
+    bt, gr = b.structs()
     q, p = b.d[5].data_ptr(), b.d[0].data_ptr()
 
     def call(batch=bt, groups=gr, layer=0, qp=q, heads=4, scale=0.125, **kw):

@@ -96,18 +96,19 @@ struct KvAttn {
 struct KvPlan {
     bool many, once;
     int splits;
+    double us;  // about what it takes
 };
 KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window);
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits);
 int launch_kv_attn(const KvAttn& a, hipStream_t s);
-// With groups: whether they are worth it, the shared keys' rows by the kernel of 128-row tiles, and into how many
-// ranges the shared and the own keys are cut.
+// With groups: whether that is faster than `whole`, attention over whole sequences, and into how many ranges the shared
+// and the own keys are cut.
 struct KvGroupPlan {
-    bool use, lead_many;
+    bool use;
     int lead, own;
 };
-KvGroupPlan kv_attn_group_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads,
-                               int window, int n_groups, int max_shared);
+KvGroupPlan kv_attn_group_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int n_heads, int window,
+                               int n_groups, int max_shared, const KvPlan& whole);
 int launch_kv_attn_groups(const KvAttn& a, const KvGroupPlan& p, hipStream_t s);
 
 }  // namespace wv

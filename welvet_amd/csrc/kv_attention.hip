@@ -120,17 +120,18 @@ constexpr int kWhole = 0, kOwn = 1, kLead = 2;
 __device__ __forceinline__ int group_keys(const KvAttn& a, int g) {
     return min(max(a.group_shared[g], 0), a.max_pages << a.c.page_shift) & ~31;
 }
-// The group of a sequence: 64 at a time. False: none.
-__device__ __forceinline__ bool find_group(const KvAttn& a, int seq, int& g) {
+// Keys that a sequence shares with its group, 64 groups at a time.
+__device__ __forceinline__ int shared_keys(const KvAttn& a, int seq) {
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < a.n_groups; base += 64) {
-        const int i = base + lane;
-        const uint64_t m = __ballot(i < a.n_groups && a.group_cu[i + 1] > seq);
+        const int i = min(base + lane, a.n_groups - 1);
+        const int first = a.group_cu[i], end = a.group_cu[i + 1], keys = group_keys(a, i);
+        const uint64_t m = __ballot(end > seq);
         if (!m) continue;
-        g = base + __builtin_ctzll(m);
-        return a.group_cu[g] <= seq;
+        const int w = __builtin_ctzll(m);
+        return __builtin_amdgcn_readlane(first, w) <= seq ? __builtin_amdgcn_readlane(keys, w) : 0;
     }
-    return false;
+    return 0;
 }
 
 // Tile `idx` of the batch's tiles of RT rows, over the sequences with at
@@ -175,17 +176,26 @@ __device__ __forceinline__ bool find_tile(const KvAttn& a, int G, int idx, int m
 // The same over the groups' rows (kLead), or over the sequences with the first key of their own (kOwn).
 template <int RT, int MODE>
 __device__ __forceinline__ bool find_group_tile(const KvAttn& a, int G, int idx, int min_rows, int max_rows, Tile& t) {
-    if constexpr (MODE == kOwn) {
-        if (!find_tile<RT>(a, G, idx, min_rows, max_rows, t)) return false;
-        int g;
-        if (find_group(a, t.seq, g)) t.from = group_keys(a, g);
+    if constexpr (MODE == kOwn) {  // a sequence's first tile, commonly its only one, is found without a search
+        if (idx < a.n_seqs) {
+            t.seq = idx;
+            t.q0 = min(max(a.cu[idx], 0), a.n_tokens);
+            t.n = min(max(a.cu[idx + 1], t.q0), a.n_tokens) - t.q0;
+            t.rows = t.n * G;
+            t.kv_len = max(a.kv_len[idx], 0);
+            t.from = shared_keys(a, idx);
+            return t.n > 0;
+        }
+        if (!find_tile<RT>(a, G, idx - a.n_seqs, min_rows, max_rows, t, 1)) return false;
+        t.from = shared_keys(a, t.seq);
         return true;
     }
     const int lane = threadIdx.x & 63;
     for (int base = 0; base < a.n_groups; base += 64) {
         const int g = base + lane;
-        int s0 = 0, s1 = 0, c0 = 0, n = 0, tiles = 0;
+        int s0 = 0, s1 = 0, c0 = 0, n = 0, tiles = 0, keys = 0;
         if (g < a.n_groups) {
+            keys = group_keys(a, g);
             s0 = min(max(a.group_cu[g], 0), a.n_seqs);
             s1 = min(max(a.group_cu[g + 1], s0), a.n_seqs);
             c0 = min(max(a.cu[s0], 0), a.n_tokens);
@@ -208,7 +218,7 @@ __device__ __forceinline__ bool find_group_tile(const KvAttn& a, int G, int idx,
             t.n = __builtin_amdgcn_readlane(n, w);
             t.rows = t.n * G;
             t.r0 = (idx - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(tiles, w))) * RT;
-            t.kv_len = group_keys(a, base + w);
+            t.kv_len = __builtin_amdgcn_readlane(keys, w);
             return true;
         }
         idx -= total;
@@ -589,15 +599,32 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int row = min(t.r0 + n, t.rows - 1);
+    float x[S][8];  // the query row, on its way while the rest is looked up
+    {
+        const float* qp = a.q + int64_t(t.q0 + row / G) * a.qs + (kvh * G + row % G) * HD;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[s][j] = qp[TYPE == WV_KV_F16 ? 16 * s + 8 * h + j : 32 * (s / 2) + 16 * h + 8 * (s % 2) + j];
+    }
     int pos, p_first, p_last;
     row_positions<kLead>(a, t, G, t.r0, 32, row, pos, p_first, p_last);
     const Range rg = tile_range<kLead>(a, t, p_first, p_last, sp, 4);
     const int first = a.window > 0 ? pos - a.window + 1 : 0;
 
+    // Lane l holds the page of the range's i'th block with i % 64 = l: no block waits for the table, which is read
+    // once in 64.
     const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
     const int pb = a.c.page_shift - 5;
+    int pg64 = 0, have = -1;
     auto block_at = [&](int kb, bool& ok) {
-        const int pg = __builtin_amdgcn_readfirstlane(pages[kb >> pb]);
+        const int i = kb - rg.begin;
+        if ((i >> 6) != have) {
+            have = i >> 6;
+            pg64 = pages[min(rg.begin + (i & ~63) + lane, rg.end - 1) >> pb];
+        }
+        const int pg = __builtin_amdgcn_readlane(pg64, i & 63);
         ok = unsigned(pg) < unsigned(a.c.n_pages);
         return kv_block(a.c, ok ? pg : 0, kvh, (kb & ((1 << pb) - 1)) << 5);
     };
@@ -627,15 +654,11 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
     h8 qh[S], ql[S];
     float qs;
     {
-        const float* qp = a.q + int64_t(t.q0 + row / G) * a.qs + (kvh * G + row % G) * HD;
-        float x[S][8], m = 0.0f;
+        float m = 0.0f;
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[s][j] = qp[TYPE == WV_KV_F16 ? 16 * s + 8 * h + j : 32 * (s / 2) + 16 * h + 8 * (s % 2) + j];
-                m = fmaxf(m, fabsf(x[s][j]));
-            }
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[s][j]));
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
         float inv;
         qs = row_unit(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])), a.scale, inv);
@@ -803,8 +826,7 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
 
 // A batch whose sequences are in groups, in one launch: the blocks of the
 // groups' rows over the shared keys, which take longest, then those of every
-// sequence's rows over its own. lead_tiles: 0 where the tiles of 128 rows took
-// the former.
+// sequence's rows over its own.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_groups(KvAttn a, int G, int lead_tiles, int y0) {
     Tile t;
@@ -842,7 +864,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_groups(KvAttn a, int G, int 
 // tile runs alone on its CU. Dropped, since they gained nothing: two groups of
 // four waves half a tile apart, or on halves of the keys; a barrier every second
 // step; steps of 64 keys.
-template <int HD, int TYPE, int MODE>
+template <int HD, int TYPE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int min_rows, int tile0) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
     constexpr int BB = 32 * HD * E;   // bytes of a block's codes
@@ -864,25 +886,19 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const bool once = gridDim.x * gridDim.y * gridDim.z <= 512;
     const int idx = tile0 + (once && y >= half ? y - half : int(gridDim.y) - 1 - y);
     Tile t;
-    if constexpr (MODE == kWhole) {
-        if (!find_tile<128>(a, G, idx, min_rows, INT32_MAX, t)) return;
-    } else {
-        if (!find_group_tile<128, MODE>(a, G, idx, min_rows, INT32_MAX, t)) return;
-    }
+    if (!find_tile<128>(a, G, idx, min_rows, INT32_MAX, t)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
 
     const int wr0 = t.r0 + 32 * wave;  // the wave's first row
     const bool busy = wr0 < t.rows;
     const int row = min(wr0 + n, t.rows - 1);
-    int pos, w_first, w_last, p_first, p_last;  // positions of the lane's row, of the wave's rows, of the tile's
-    row_positions<MODE>(a, t, G, t.r0, 128, row, pos, p_first, p_last);
-    if constexpr (MODE == kLead)
-        row_positions<MODE>(a, t, G, min(wr0, t.rows - 1), 32, row, pos, w_first, w_last);
-    else
-        w_first = t.kv_len - t.n + min(wr0, t.rows - 1) / G, w_last = t.kv_len - t.n + min(wr0 + 31, t.rows - 1) / G;
-    const Range rg = tile_range<MODE>(a, t, p_first, p_last, sp, 8);
+    int pos, p_first, p_last;
+    row_positions<kWhole>(a, t, G, t.r0, 128, row, pos, p_first, p_last);
+    const Range rg = tile_range<kWhole>(a, t, p_first, p_last, sp, 8);
     const int first = a.window > 0 ? pos - a.window + 1 : 0;
+    const int w_first = t.kv_len - t.n + min(wr0, t.rows - 1) / G;       // positions of the wave's first
+    const int w_last = t.kv_len - t.n + min(wr0 + 31, t.rows - 1) / G;   // and last row
 
     const int32_t* pages = a.pages + int64_t(t.seq) * a.max_pages;
     const int pb = a.c.page_shift - 5;
@@ -1181,8 +1197,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_tile(KvAttn a, int G, int mi
     const int head = kvh * G + row % G;
     const float back = ldexpf(1.0f, int(er));
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;  // back / l may be subnormal
-    float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp + (MODE == kOwn ? a.lead : 0)) * LD
-                        : a.out + orow * a.os + head * HD;
+    float* dst = a.part ? a.part + ((orow * a.n_heads + head) * a.splits + sp) * LD : a.out + orow * a.os + head * HD;
     const bool al = a.part || (!(reinterpret_cast<uintptr_t>(a.out) & 15) && !(a.os & 3));
 #pragma unroll
     for (int i = 0; i < T; ++i)
@@ -1271,7 +1286,7 @@ __global__ void __launch_bounds__(256) k_kv_attn_join(KvAttn a) {
 // a window of 512 96 / 54; head_dim 64, 1900 over 1900 76 / 91. Of a batch, the
 // tile kernel takes the sequences of more than kFewRows rows.
 KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads, int window) {
-    if (!n_seqs || !n_tokens) return {false, false, 1};
+    if (!n_seqs || !n_tokens) return {false, false, 1, 0.0};
     const int64_t G = n_heads / c.n_kv, rows = n_tokens * G;
     const int64_t most_q = max_q ? std::min(max_q, n_tokens) : (n_tokens + n_seqs - 1) / n_seqs;
     const int64_t width = int64_t(max_pages) << c.page_shift;
@@ -1297,7 +1312,7 @@ KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, in
         const double block_bytes = 64.0 * c.hd * kv_code_bytes(c.type);
         if (last(16) * block_bytes > 2e6)  // more than stays in an L2
             row = std::max(row, double(t16) * (last(16) - causal) * block_bytes / 11e6);
-        if (tile < row) return {true, false, int(s128)};
+        if (tile < row) return {true, false, int(s128), tile};
     }
     // Row kernel: ranges for two blocks a CU; more cost their join more than they gain (8192 keys, one token:
     // 8 / 16 / 64 ranges 18.7 / 15.1 / 21.6 us). Its waves take four key blocks at a time, in 1.1 to 1.6 us, or
@@ -1310,7 +1325,10 @@ KvPlan kv_attn_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, in
     };
     const int64_t best = int64_t(std::sqrt(1.6 * double(blocks)) + 0.5);
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>({768 / t16, best, blocks / 4, kMaxSplits}));
-    return {false, most_q * G <= 16, walk(1) <= walk(n) + 4.5 + 0.15 * double(n) ? 1 : int(n)};
+    const int64_t best_n = walk(1) <= walk(n) + 4.5 + 0.15 * double(n) ? 1 : n;
+    const double steps = double(t16 * blocks) / (c.hd == 128 ? 1150.0 : 2300.0);
+    return {false, most_q * G <= 16, int(best_n),
+            6.0 + std::max(steps, walk(best_n)) + (best_n > 1 ? 4.5 + 0.15 * double(best_n) : 0.0)};
 }
 
 size_t kv_attn_part_floats(const KvView& c, int n_tokens, int n_heads, int splits) {
@@ -1343,11 +1361,11 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
         const int64_t tiles = (rows + 127) / 128 + a.n_seqs;
         const int least = few ? kFewRows + 1 : 1;
         if (a.c.hd == 128)
-            f16 ? go(k_kv_attn_tile<128, WV_KV_F16, kWhole>, tiles, least)
-                : go(k_kv_attn_tile<128, WV_KV_Q8, kWhole>, tiles, least);
+            f16 ? go(k_kv_attn_tile<128, WV_KV_F16>, tiles, least)
+                : go(k_kv_attn_tile<128, WV_KV_Q8>, tiles, least);
         else
-            f16 ? go(k_kv_attn_tile<64, WV_KV_F16, kWhole>, tiles, least)
-                : go(k_kv_attn_tile<64, WV_KV_Q8, kWhole>, tiles, least);
+            f16 ? go(k_kv_attn_tile<64, WV_KV_F16>, tiles, least)
+                : go(k_kv_attn_tile<64, WV_KV_Q8>, tiles, least);
     }
     if (a.splits > 1) {
         const dim3 jg{unsigned(a.n_tokens), unsigned(a.n_heads)};
@@ -1359,21 +1377,46 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
     return int(hipGetLastError());
 }
 
-// The same for a batch whose sequences are in groups: the groups' rows over the shared keys, then every sequence's
-// rows over its own.
-KvGroupPlan kv_attn_group_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int max_q, int n_heads,
-                               int window, int n_groups, int max_shared) {
+// A batch whose sequences are in groups. A lead block (32 rows of a group over a range of its shared keys) takes some
+// 10 us to begin and to end, and 1.25 us a step of its four waves while it has a CU to itself, 2.2 beside another. So
+// one block a CU where the own keys' blocks are there to run beside it, two where those have little to do, and steps
+// enough to pay for itself, unless there are few blocks at all. 32 heads over 8 of 128, int8, ranges 1 / 2 / 4 / 8: 564
+// rows a KV head over 8192 shared keys 95 / 86 / 80 / 80 us, 1160 rows 150 / 135 / 134 / 154, 2252 rows 242 / 224 / 243
+// / 282; 1204 rows over 1024 keys 44 / 50 / 62 / 84; 256 rows over 8192, 1024 own keys each, 4 / 8 / 16: 52 / 59 / 70.
+// (The kernel of 128-row tiles in its place: 564 rows 104 us at best, 1160 167, 2252 252, 4244 over 1024 keys 135
+// against 117; ahead on 2400 rows over 32768 fp16 keys alone, 816 against 870.)
+// Own keys: as many ranges as the row kernel takes. Sequences of no group, which the host cannot see, may have as many
+// as the table is wide; a second range for them costs the others 1 us (7 sequences of 4000 keys beside 5 groups over
+// 4096: 55 to 45 us).
+// Groups are made use of where that is estimated to be faster than attention over whole sequences (grouped / whole as
+// measured): 64 sequences of one token behind 8192 int8 keys 55 / 138 us, behind 256 20 / 11; 8 behind 512 17 / 12; 2
+// behind 16384 24 / 21, 4 24 / 28; 12 of 50 tokens each behind 32768 fp16 keys 880 / 1115; 2 of 800 tokens behind 4096
+// 414 / 296 (there the tiles of 128 rows share the keys well enough); a window of 512 over 64 sequences 35 / 16.
+KvGroupPlan kv_attn_group_plan(const KvView& c, int n_seqs, int n_tokens, int max_pages, int n_heads, int window,
+                               int n_groups, int max_shared, const KvPlan& whole) {
     KvGroupPlan p{};
     const int64_t width = int64_t(max_pages) << c.page_shift;
     const int64_t shared = max_shared > 0 ? std::min<int64_t>(max_shared, width) : width;
     if (n_groups <= 0 || n_tokens <= 0 || n_seqs <= 1 || shared < 32) return p;
     const int64_t G = n_heads / c.n_kv, rows = n_tokens * G;
-    const int64_t t16 = (rows + 15) / 16 * c.n_kv, t128 = (rows + 127) / 128 * c.n_kv;
-    const int64_t blocks = shared / 32, own = std::max<int64_t>((width - shared + 31) / 32, 1);
-    p.use = true;
-    p.lead_many = rows / n_groups >= 1024;
-    p.lead = int(std::max<int64_t>(1, std::min<int64_t>({p.lead_many ? 512 / t128 : 1024 / t16, blocks / 4, 48})));
-    p.own = int(std::max<int64_t>(1, std::min<int64_t>({1024 / t16, own / 8, 16})));
+    const int64_t t32 = ((rows + 31) / 32 + n_groups / 2) * c.n_kv;
+    const int64_t t16 = std::max<int64_t>((rows + 15) / 16, std::min(n_seqs, n_tokens)) * c.n_kv;
+    const int64_t blocks = shared / 32, own = (width - shared + 31) / 32;
+    const int64_t fill = ((own >= 8 ? 256 : 512) + t32 - 1) / t32;
+    const int64_t worth = std::max(blocks / 32, std::min(blocks / 4, 128 / t32));
+    p.lead = int(std::max<int64_t>(1, std::min<int64_t>({fill, worth, 48})));
+    const int64_t n = std::min<int64_t>({768 / t16, int64_t(std::sqrt(1.6 * double(own))), own / 4, 16});
+    p.own = int(std::max<int64_t>({1, n, std::min<int64_t>(2, width / 2048)}));
+    // rounds of 512 lead blocks, the own keys' steps, the partial rows written and read, the join
+    const bool wide = c.hd == 128;
+    const int64_t seen = window > 0 ? std::min<int64_t>(blocks, window / 32 + 1) : blocks, all = t32 * p.lead;
+    const double steps = double(seen) / (4.0 * p.lead) * (wide ? 1.0 : 0.6);
+    const int64_t rest = all % 512;
+    double us = double(all / 512) * (11.0 + 2.2 * steps) + (rest > 256 ? 11.0 + 2.2 * steps : rest ? 11.0 + 1.25 * steps : 0.0);
+    const int64_t keys = window > 0 ? std::min<int64_t>(own, window / 32 + 1) : own;
+    us += double(t16 * keys) / (wide ? 1150.0 : 2300.0);
+    us += 5.0 + double(kv_attn_part_floats(c, n_tokens, n_heads, p.lead + p.own)) * 8.0 / 5.2e6;
+    p.use = us < whole.us;
     return p;
 }
 
@@ -1389,13 +1432,8 @@ int launch_kv_attn_groups(const KvAttn& a, const KvGroupPlan& p, hipStream_t s) 
     };
     auto pick = [&](auto hd, auto type) {
         constexpr int HD = decltype(hd)::value, TYPE = decltype(type)::value;
-        if (p.lead_many) {
-            go(k_kv_attn_tile<HD, TYPE, kLead>, (rows + 127) / 128 + a.n_groups, p.lead, 1);
-            go(k_kv_attn_groups<HD, TYPE>, ((rows + 15) / 16 + a.n_seqs) * p.own, 1, 0);
-        } else {
-            const int64_t lead = (rows + 31) / 32 + a.n_groups;
-            go(k_kv_attn_groups<HD, TYPE>, lead * p.lead + ((rows + 15) / 16 + a.n_seqs) * p.own, 1, int(lead));
-        }
+        const int64_t lead = (rows + 31) / 32 + a.n_groups;
+        go(k_kv_attn_groups<HD, TYPE>, lead * p.lead + ((rows + 15) / 16 + a.n_seqs) * p.own, 1, int(lead));
         hipLaunchKernelGGL((k_kv_attn_join<HD, true>), dim3(unsigned(a.n_tokens), unsigned(a.n_heads)), dim3(256), 0, s, a);
     };
     std::integral_constant<int, 128> h128;
@@ -1471,16 +1509,16 @@ int attention(const char* what, uint64_t cache, int32_t layer, const wv_kv_batch
     a.cu = batch->d_cu_q, a.kv_len = batch->d_kv_len, a.pages = batch->d_pages;
     a.n_seqs = batch->n_seqs, a.n_tokens = batch->n_tokens, a.max_pages = batch->max_pages;
     a.n_heads = n_heads, a.window = std::min(window, 1 << 30), a.scale = scale;
+    const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, batch->max_q, n_heads, a.window);
+    a.splits = plan.splits, a.many = plan.many, a.once = plan.once;
     KvGroupPlan gp{};
     if (groups && groups->n_groups) {
-        gp = kv_attn_group_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, batch->max_q, n_heads, a.window,
-                                groups->n_groups, groups->max_shared);
+        gp = kv_attn_group_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, n_heads, a.window, groups->n_groups,
+                                groups->max_shared, plan);
         a.group_cu = groups->d_cu_seq, a.group_shared = groups->d_shared, a.n_groups = groups->n_groups;
         // its ranges are joined in scratch: a captured call without any attends over whole sequences
         if (!d_scratch && rt_capturing(s)) gp.use = false;
     }
-    const KvPlan plan = kv_attn_plan(a.c, a.n_seqs, a.n_tokens, a.max_pages, batch->max_q, n_heads, a.window);
-    a.splits = plan.splits, a.many = plan.many, a.once = plan.once;
     if (gp.use) a.lead = gp.lead, a.splits = gp.lead + gp.own;
     const size_t floats = kv_attn_part_floats(a.c, a.n_tokens, n_heads, a.splits);
     RtScratch sc;
@@ -1533,8 +1571,10 @@ int wv_kv_attention_shared_scratch(uint64_t cache, const wv_kv_batch* batch, con
     if (rc) return rc;
     if (!bytes) return rt_fail(WV_E_ARG, "wv_kv_attention_shared_scratch: nil bytes");
     const KvView v = c.layer(0);
-    const KvGroupPlan gp = kv_attn_group_plan(v, batch->n_seqs, batch->n_tokens, batch->max_pages, batch->max_q, n_heads,
-                                              std::min(window, 1 << 30), groups->n_groups, groups->max_shared);
+    const int w = std::min(window, 1 << 30);
+    const KvPlan whole = kv_attn_plan(v, batch->n_seqs, batch->n_tokens, batch->max_pages, batch->max_q, n_heads, w);
+    const KvGroupPlan gp = kv_attn_group_plan(v, batch->n_seqs, batch->n_tokens, batch->max_pages, n_heads, w,
+                                              groups->n_groups, groups->max_shared, whole);
     if (!gp.use) return wv_kv_attention_scratch(cache, batch, n_heads, window, bytes);
     *bytes = kv_attn_part_floats(v, batch->n_tokens, n_heads, gp.lead + gp.own) * sizeof(float);
     return WV_OK;
