@@ -117,13 +117,27 @@ def test_sizes(typ, rows, cols, ranks, new, which, in_place):
 
 
 @pytest.mark.parametrize("new,which", [([1] * 5, [0, 1, 2, -1, 0]), ([40, 1, 90], [2, 0, 1])])
-def test_several_sets(new, which):
-    """Q, K and V: sets of unlike rows over the same input, and four at once."""
+@pytest.mark.parametrize("ranks", [[16, 8, 30], [16, 3, 1], [80, 70, 2]])
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+def test_several_sets(new, which, ranks, typ):
+    """Q, K and V: sets of unlike rows over the same input, and four at once; 48 to 320 ranks together."""
     rng = np.random.default_rng(3)
     for sets in ([512, 128, 128], [31, 700, 64, 5]):
-        c = Case(rng, sets, 768, [16, 8, 30], new, which, pad=1)
+        c = Case(rng, sets, 768, ranks, new, which, typ, pad=1)
         c.check(c.run())
         c.check(c.run(True), True)
+
+
+def test_sets_that_know_other_adapters():
+    """Sets of one call with more or fewer adapters, of other ranks, some of them unset."""
+    rng = np.random.default_rng(8)
+    for new in ([1, 2, 1, 1], [40, 33, 64, 5]):
+        a = Case(rng, [90, 200], 300, [16, 0, 7], new, [0, 1, 2, 0])
+        b = Case(rng, [60], 300, [40], new, [0, 1, 2, 0])
+        a.sets, a.w, a.rows, a.base = a.sets + b.sets, a.w + b.w, a.rows + b.rows, a.base + b.base
+        a.check(a.run())
+        a.sets, a.w, a.rows, a.base = a.sets[::-1], a.w[::-1], a.rows[::-1], a.base[::-1]
+        a.check(a.run(True), True)
 
 
 @pytest.mark.parametrize("hint", [0, 1, 4, 5, 1000])

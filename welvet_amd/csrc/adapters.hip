@@ -27,14 +27,17 @@ constexpr int kFew = 4;          // rows of a tile up to which they go one by on
 constexpr int kChunk = 512;      // columns that a wave takes at a time of such a row, 8 to a lane
 constexpr int kMaxRanges = 32;   // of the columns
 
+struct Known {
+    int32_t rank;
+    float scale;
+};
 struct Set {
     wv_adapters_config c{};
     int device = 0;
     int R = 0, C = 0;         // ranks and columns as stored: multiples of 16 and 64, zeros behind the adapter's own
     uint16_t* a = nullptr;    // [n_adapters][R][C]
     uint16_t* b = nullptr;    // [n_adapters][rows][R]
-    int32_t* rank = nullptr;  // [n_adapters], 0: unset
-    float* scale = nullptr;   // [n_adapters]
+    Known* known = nullptr;   // [n_adapters], rank 0: unset
 };
 std::mutex g_mu;
 std::unordered_map<uint64_t, Set> g_sets;
@@ -58,8 +61,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 // One set of a call as the kernels see it.
 struct SetArgs {
     const uint16_t *a, *b;
-    const int32_t* rank;
-    const float* scale;
+    const Known* known;
     const float* base;
     float* y;
     float* h;  // [ranges][n_tokens][R]
@@ -73,6 +75,7 @@ struct Args {
     const int32_t *cu, *which;
     int64_t xs;
     int cols, n_seqs, n_tokens, ranges, range;  // range: columns of one, a multiple of kChunk
+    int n_sets, ranks;                           // ranks: R of all sets
 };
 
 template <int TYPE>
@@ -223,7 +226,7 @@ __device__ __forceinline__ void down_few(const Args& a, const SetArgs& s, const 
             w[k] = cl + c < c1 ? *reinterpret_cast<const uint4*>(A + int64_t(r0 + k) * s.C + c) : uint4{};
     };
     load(a.x + int64_t(t.t0) * a.xs, 4 * wave, 0);
-    const int rank = s.rank[id];
+    const int rank = s.known[id].rank;
     for (int n = 0; n < t.n; ++n) {
         const float* x = a.x + int64_t(t.t0 + n) * a.xs;
         for (int r0 = 4 * wave; r0 < rank; r0 += 16) {
@@ -247,22 +250,31 @@ __device__ __forceinline__ void down_few(const Args& a, const SetArgs& s, const 
     }
 }
 
-// h of a tile of tokens, 32 NR ranks at a time, on products of 32 ranks x 32 tokens x 16 columns: a lane holds the
-// same 16 columns of its rank's row and of its token's (lanes from 32 on the 16 behind those), straight from memory.
-// The block's waves take every fourth 32 columns and meet in LDS.
+// h of a tile of tokens for all sets, whose ranks follow one another, 32 NR of them at a time, on products of 32 ranks
+// x 32 tokens x 16 columns: a lane holds the same 16 columns of its rank's row and of its token's (lanes from 32 on the
+// 16 behind those), straight from memory. The block's waves take every fourth 32 columns and meet in LDS.
 template <int TYPE, int NR>
-__device__ __forceinline__ void down_tile(const Args& a, const SetArgs& s, const Tile& t, const uint16_t* A, int rank,
-                                          int c0, int c1, float* h, float* lds) {
+__device__ __forceinline__ void down_tile(const Args& a, const Tile& t, int range, int c0, int c1, float* lds) {
     constexpr int LD = 32 * NR + 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hi = lane >> 5;
     const float* x = a.x + int64_t(t.t0 + min(n, t.n - 1)) * a.xs;
-    for (int r0 = 0; r0 < rank; r0 += 32 * NR) {
+    // rank r of all sets: its set, and the rank there
+    auto set_of = [&](int& r) {
+        int i = 0;
+        while (i + 1 < kMaxSets && r >= a.set[i].R) r -= a.set[i++].R;
+        return i;
+    };
+    for (int r0 = 0; r0 < a.ranks; r0 += 32 * NR) {
         f16v acc[NR];
         const uint16_t* row[NR];
 #pragma unroll
         for (int k = 0; k < NR; ++k) {
-            row[k] = A + int64_t(min(r0 + 32 * k + n, s.R - 1)) * s.C;
+            int r = min(r0 + 32 * k + n, a.ranks - 1);
+            const SetArgs& s = a.set[set_of(r)];
+            // of a set that does not know the adapter, anything: nobody reads it
+            const int id = unsigned(t.id) < unsigned(s.n_adapters) ? t.id : 0;
+            row[k] = s.a + (int64_t(id) * s.R + r) * s.C;
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[k][i] = 0.0f;
         }
@@ -355,14 +367,16 @@ __device__ __forceinline__ void down_tile(const Args& a, const SetArgs& s, const
             }
         }
         if (wave == 0 && n < t.n) {
-            float* d = h + int64_t(n) * s.R + r0 + 4 * hi;
 #pragma unroll
             for (int k = 0; k < NR; ++k)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (r0 + 32 * k + 8 * q < s.R)
-                        *reinterpret_cast<f4*>(d + 32 * k + 8 * q) =
-                            f4{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
+                for (int q = 0; q < 4; ++q) {
+                    int r = r0 + 32 * k + 8 * q + 4 * hi;
+                    if (r >= a.ranks) continue;
+                    const SetArgs& s = a.set[set_of(r)];  // the ranks of a set are a multiple of 16
+                    *reinterpret_cast<f4*>(s.h + (int64_t(range) * a.n_tokens + t.t0 + n) * s.R + r) =
+                        f4{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
+                }
         }
     }
 }
@@ -370,19 +384,21 @@ __device__ __forceinline__ void down_tile(const Args& a, const SetArgs& s, const
 // FEW: the caller says that no sequence has more than kFew rows (if one has, its rows go one by one all the same).
 template <int TYPE, int NR, bool FEW>
 __global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
-    constexpr int ND = NR < 4 ? NR : 4;  // more would take all of a SIMD's registers for one wave
-    __shared__ float lds[FEW ? 1 : 2 * 32 * (32 * ND + 4)];
-    const SetArgs& s = a.set[blockIdx.x / a.ranges];
+    __shared__ float lds[FEW ? 1 : 2 * 32 * (32 * NR + 4)];
     Tile t;
     if (!find_tile<FEW>(a, tile0 + int(blockIdx.y), t)) return;
-    const int id = t.id;
-    if (unsigned(id) >= unsigned(s.n_adapters)) return;
-    const int range = blockIdx.x % a.ranges, c0 = range * a.range;
-    float* h = s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R;
-    if (FEW || t.n <= kFew)
-        down_few<TYPE>(a, s, t, id, c0, min(c0 + a.range, a.cols), h);
-    else
-        down_tile<TYPE, ND>(a, s, t, s.a + int64_t(id) * s.R * s.C, s.rank[id], c0, min(c0 + a.range, s.C), h, lds);
+    const int range = FEW ? blockIdx.x % a.ranges : blockIdx.x, c0 = range * a.range;
+    auto few = [&](const SetArgs& s) {
+        if (unsigned(t.id) < unsigned(s.n_adapters))
+            down_few<TYPE>(a, s, t, t.id, c0, min(c0 + a.range, a.cols), s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R);
+    };
+    if constexpr (FEW) {
+        few(a.set[blockIdx.x / a.ranges]);
+    } else if (t.n <= kFew) {
+        for (int i = 0; i < a.n_sets; ++i) few(a.set[i]);
+    } else if (t.id >= 0) {
+        down_tile<TYPE, NR>(a, t, range, c0, min(c0 + a.range, a.set[0].C), lds);
+    }
 }
 
 // Rows of h into LDS (NR * 32 + 4 floats each), the ranges summed in their order, with the adapter's scale. What lies
@@ -420,8 +436,8 @@ __device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Ti
                                        const float* base, float* y, float* h) {
     constexpr int LD = 32 * NR + 4, NB = NR < 2 ? 4 : 8;  // 16-byte units of B that are loaded ahead
     const uint16_t* B = s.b + (int64_t(id) * s.rows + first) * s.R;
-    const int rank = s.rank[id];
-    const float scale = s.scale[id];
+    const int rank = s.known[id].rank;
+    const float scale = s.known[id].scale;
     for (int n0 = 0; n0 < t.n; n0 += kFew) {
         const int rows = min(t.n - n0, kFew);
         for (int o = threadIdx.x; o - int(threadIdx.x) < last - first; o += 256) {
@@ -525,7 +541,8 @@ __device__ __forceinline__ void stage_operands(const Args& a, const SetArgs& s, 
 
 // y of the block's outputs for a tile, on products of 32 outputs x 32 tokens x 16 ranks. A lane ends with 16 outputs
 // of one token; through LDS they become four times 4 side by side, 8 lanes a row, as base and y are read and written,
-// past the caches (a prompt's rows are more than they hold). The base of the next two steps is on its way meanwhile.
+// past the caches (a prompt's rows are more than they hold). B and base of the next step are on their way meanwhile; a
+// second step ahead takes the registers of a fourth block a CU and gained nothing.
 template <int TYPE, int NR>
 __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const Tile& t, int id, int rank, int first,
                                         int last, const float* base, float* y, UpLds<TYPE, NR>& l) {
@@ -544,20 +561,19 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
         const int r = min(8 * q + m, t.n - 1);
         rb[q] = r * s.bs + o4, ry[q] = r * s.ys + o4, rs[q] = r * kSwap + o4;
     }
-    constexpr int D = NR <= 2 ? 2 : 1;  // steps ahead that B is loaded, as registers allow
-    uint4 w[D][2 * NR];
-    f4 was[2][4];
-    auto load_b = [&](int o0, uint4* w) {
+    uint4 w[2 * NR];
+    f4 was[4];
+    auto load_b = [&](int o0) {
         const uint16_t* row = B + int64_t(min(o0 + n, last - 1)) * s.R;
 #pragma unroll
         for (int k = 0; k < 2 * NR; ++k) w[k] = *reinterpret_cast<const uint4*>(row + min(16 * k, s.R - 16));
     };
-    auto load_base = [&](int o0, f4* x) {
+    auto load_base = [&](int o0) {
         const float* p = base + max(min(o0, whole - 32), first);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) x[q] = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p + rb[q]));
+        for (int q = 0; q < 4; ++q) was[q] = __builtin_nontemporal_load(reinterpret_cast<const f4*>(p + rb[q]));
     };
-    auto outputs = [&](f16v& acc, const uint4* w) {
+    auto outputs = [&](f16v& acc) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
 #pragma unroll
@@ -576,42 +592,32 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
             *reinterpret_cast<g4*>(swap + n * kSwap + 8 * q + 4 * hi) = g4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
         wave_sync();
     };
-    auto step = [&](int o0, f4* x, uint4* w) {
+    int o0 = first + 32 * wave;
+    if (whole > first) load_base(o0);
+    load_b(o0);
+    stage_operands<TYPE, NR>(a, s, t, rank, s.known[id].scale, l);
+    if constexpr (TYPE == WV_ADAPTER_F16) unit = power(exponent(l.most[n]) - 14);
+    // what was loaded so far is there (h came after it): the steps' waits need not allow for it
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    for (; o0 < whole; o0 += 128) {
         f16v acc;
-        outputs(acc, w);
+        outputs(acc);
         __builtin_amdgcn_sched_barrier(0);
-        load_b(o0 + 128 * D, w);
+        load_b(o0 + 128);
         __builtin_amdgcn_sched_barrier(0);
         turn(acc);
         f4 sum[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sum[q] = x[q] + f4(*reinterpret_cast<const g4*>(swap + rs[q]));
+        for (int q = 0; q < 4; ++q) sum[q] = was[q] + f4(*reinterpret_cast<const g4*>(swap + rs[q]));
         wave_sync();
-        load_base(o0 + 256, x);
+        load_base(o0 + 128);
 #pragma unroll
         for (int q = 0; q < 4; ++q) __builtin_nontemporal_store(sum[q], reinterpret_cast<f4*>(y + o0 + ry[q]));
         __builtin_amdgcn_sched_barrier(0);
-    };
-    int o0 = first + 32 * wave;
-    if (whole > first) load_base(o0, was[0]), load_base(o0 + 128, was[1]);
-    load_b(o0, w[0]);
-    if (D > 1) load_b(o0 + 128, w[D - 1]);
-    stage_operands<TYPE, NR>(a, s, t, rank, s.scale[id], l);
-    if constexpr (TYPE == WV_ADAPTER_F16) unit = power(exponent(l.most[n]) - 14);
-    // what was loaded so far is there (h came after it): the steps' waits need not allow for it
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    for (; o0 + 128 < whole; o0 += 256) {
-        step(o0, was[0], w[0]);
-        step(o0 + 128, was[1], w[D - 1]);
-    }
-    bool second = false;
-    if (o0 < whole) {
-        step(o0, was[0], w[0]);
-        o0 += 128, second = true;
     }
     if (o0 >= last || o0 != whole) return;
     f16v acc;  // fewer than 32 outputs are left
-    second ? outputs(acc, w[D - 1]) : outputs(acc, w[0]);
+    outputs(acc);
     turn(acc);
     for (int i = lane; i < 32 * t.n; i += 64)
         if (const int r = i >> 5, o = o0 + (i & 31); o < last) y[r * s.ys + o] = base[r * s.bs + o] + swap[r * kSwap + (i & 31)];
@@ -657,38 +663,46 @@ __global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) 
         return;
     }
     if constexpr (!FEW) {
-        if (const int rank = known ? s.rank[id] : 0; rank) {
+        if (const int rank = known ? s.known[id].rank : 0; rank) {
             up_tile<TYPE, NR>(a, s, t, id, rank, first, last, base, y, lds);
             return;
         }
     }
-    if (base != y)
-        for (int n0 = 0; n0 < t.n; n0 += kTile)
-            copy_rows(s, min(t.n - n0, kTile), first, last, base + n0 * s.bs, y + n0 * s.ys);
+    if (base == y) return;
+    if constexpr (FEW) {
+        for (int n = 0; n < t.n; ++n)
+            for (int o = first + int(threadIdx.x); o < last; o += 256) y[n * s.ys + o] = base[n * s.bs + o];
+    } else {
+        copy_rows(s, t.n, first, last, base, y);
+    }
 }
 
 // Tiles of a call, at most.
 int64_t adapt_tiles(int n_seqs, int n_tokens) { return int64_t(n_seqs) + n_tokens / kTile; }
 
+// Whether the kernels of short sequences take a call.
+bool adapt_few(const wv_adapter_batch& b) { return b.max_q ? b.max_q <= kFew : b.n_tokens <= kFew; }
+
 // Into how many ranges the columns are cut: about eight blocks a CU, and ranges of whole chunks.
-int adapt_ranges(int cols, int n_seqs, int n_tokens, int n_sets, int& range) {
+int adapt_ranges(int cols, const wv_adapter_batch& b, int n_sets, int& range) {
     const int chunks = (cols + kChunk - 1) / kChunk;
-    const int64_t tiles = std::min<int64_t>(n_tokens, adapt_tiles(n_seqs, n_tokens)) * n_sets;
-    const int want = int(std::max<int64_t>(1, std::min<int64_t>({2048 / std::max<int64_t>(tiles, 1), chunks, kMaxRanges})));
+    const int64_t blocks = adapt_few(b) ? int64_t(std::min(b.n_seqs, b.n_tokens)) * n_sets : adapt_tiles(b.n_seqs, b.n_tokens);
+    const int want = int(std::max<int64_t>(1, std::min<int64_t>({2048 / std::max<int64_t>(blocks, 1), chunks, kMaxRanges})));
     const int each = (chunks + want - 1) / want;
     range = each * kChunk;
     return (chunks + each - 1) / each;
 }
 
-template <int TYPE, int NR, bool FEW>
-int launch_adapters(Args& a, int n_sets, hipStream_t s) {
-    const int64_t tiles = FEW ? a.n_seqs : adapt_tiles(a.n_seqs, a.n_tokens);
+template <int TYPE>
+int launch_adapters(Args& a, bool few, hipStream_t s) {
+    const int64_t tiles = few ? a.n_seqs : adapt_tiles(a.n_seqs, a.n_tokens);
     int64_t units = 0, blocks = 0;
-    for (int i = 0; i < n_sets; ++i) units += (a.set[i].rows + 255) / 256;
-    const int turns = int(std::max<int64_t>(1, std::min<int64_t>(4, units * tiles / 2048)));
+    int R = 0;
+    for (int i = 0; i < a.n_sets; ++i) units += (a.set[i].rows + 255) / 256, R = std::max(R, a.set[i].R);
+    const int turns = int(std::max<int64_t>(1, std::min<int64_t>(4, units * tiles / 1536)));
     for (int i = 0; i < kMaxSets; ++i) {
-        a.set[i].block0 = i < n_sets ? int(blocks) : INT32_MAX;
-        if (i < n_sets) blocks += (a.set[i].rows + 256 * turns - 1) / (256 * turns);
+        a.set[i].block0 = i < a.n_sets ? int(blocks) : INT32_MAX;
+        if (i < a.n_sets) blocks += (a.set[i].rows + 256 * turns - 1) / (256 * turns);
     }
     auto go = [&](auto kern, int64_t x, auto... more) {
         for (int64_t t0 = 0; t0 < tiles; t0 += 1 << 15) {
@@ -696,23 +710,24 @@ int launch_adapters(Args& a, int n_sets, hipStream_t s) {
             hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, int(t0), more...);
         }
     };
-    go(k_adapt_down<TYPE, NR, FEW>, int64_t(a.ranges) * n_sets);
-    go(k_adapt_up<TYPE, NR, FEW>, blocks, turns);
-    return int(hipGetLastError());
-}
-int launch_adapters(Args& a, int n_sets, int type, bool few, hipStream_t s) {
-    int R = 0;
-    for (int i = 0; i < n_sets; ++i) R = std::max(R, a.set[i].R);
-    auto pick = [&](auto nr) {
+    auto up = [&](auto nr) {
         constexpr int NR = decltype(nr)::value;
-        if (type == WV_ADAPTER_BF16)
-            return few ? launch_adapters<WV_ADAPTER_BF16, NR, true>(a, n_sets, s)
-                       : launch_adapters<WV_ADAPTER_BF16, NR, false>(a, n_sets, s);
-        return few ? launch_adapters<WV_ADAPTER_F16, NR, true>(a, n_sets, s)
-                   : launch_adapters<WV_ADAPTER_F16, NR, false>(a, n_sets, s);
+        few ? go(k_adapt_up<TYPE, NR, true>, blocks, turns) : go(k_adapt_up<TYPE, NR, false>, blocks, turns);
     };
-    return R <= 32 ? pick(std::integral_constant<int, 1>{}) : R <= 64 ? pick(std::integral_constant<int, 2>{})
-         : R <= 128 ? pick(std::integral_constant<int, 4>{}) : pick(std::integral_constant<int, 8>{});
+    std::integral_constant<int, 1> n1;
+    std::integral_constant<int, 2> n2;
+    std::integral_constant<int, 4> n4;
+    std::integral_constant<int, 8> n8;
+    if (few)
+        go(k_adapt_down<TYPE, 1, true>, int64_t(a.ranges) * a.n_sets);
+    else if (a.ranks <= 32)
+        go(k_adapt_down<TYPE, 1, false>, a.ranges);
+    else if (a.ranks <= 64)
+        go(k_adapt_down<TYPE, 2, false>, a.ranges);
+    else  // 128 at a time: more would take all of a SIMD's registers for one wave
+        go(k_adapt_down<TYPE, 4, false>, a.ranges);
+    R <= 32 ? up(n1) : R <= 64 ? up(n2) : R <= 128 ? up(n4) : up(n8);
+    return int(hipGetLastError());
 }
 
 }  // namespace
@@ -769,19 +784,18 @@ int wv_adapters_create(const wv_adapters_config* cfg, uint64_t* adapters) {
     s.R = (c.max_rank + 15) / 16 * 16;
     s.C = (c.cols + 63) / 64 * 64;
     const size_t n = size_t(c.n_adapters), na = n * s.R * s.C * 2, nb = n * c.rows * s.R * 2;
-    // one allocation: A, B (both multiples of 16 bytes), ranks, scales
+    // one allocation: A, B (both multiples of 16 bytes), ranks and scales
     uint8_t* p = nullptr;
-    hipError_t e = hipMalloc(reinterpret_cast<void**>(&p), na + nb + n * 8);
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&p), na + nb + n * sizeof(Known));
     if (e != hipSuccess) {
         (void)hipGetLastError();
         return rt_hip_fail(e, "wv_adapters_create: weights");
     }
     s.a = reinterpret_cast<uint16_t*>(p);
     s.b = reinterpret_cast<uint16_t*>(p + na);
-    s.rank = reinterpret_cast<int32_t*>(p + na + nb);
-    s.scale = reinterpret_cast<float*>(s.rank + n);
+    s.known = reinterpret_cast<Known*>(p + na + nb);
     hipStream_t st = rt_stream(nullptr, s.device);
-    e = hipMemsetAsync(s.rank, 0, n * 8, st);
+    e = hipMemsetAsync(s.known, 0, n * sizeof(Known), st);
     if (e == hipSuccess) e = hipStreamSynchronize(st);
     if (e != hipSuccess) {
         (void)hipFree(p);
@@ -817,8 +831,8 @@ int wv_adapters_set(uint64_t adapters, int32_t index, int32_t rank, float scale,
     hipError_t e = hipDeviceSynchronize();  // calls that still read the adapter
     if (e == hipSuccess && r) e = hipMemcpy(s.a + size_t(index) * R * C, ha.data(), ha.size() * 2, hipMemcpyHostToDevice);
     if (e == hipSuccess && r) e = hipMemcpy(s.b + size_t(index) * rows * R, hb.data(), hb.size() * 2, hipMemcpyHostToDevice);
-    if (e == hipSuccess) e = hipMemcpy(s.scale + index, &scale, 4, hipMemcpyHostToDevice);
-    if (e == hipSuccess) e = hipMemcpy(s.rank + index, &rank, 4, hipMemcpyHostToDevice);
+    const Known k{rank, scale};
+    if (e == hipSuccess) e = hipMemcpy(s.known + index, &k, sizeof k, hipMemcpyHostToDevice);
     return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_adapters_set");
 } catch (const std::bad_alloc&) {
     return rt_fail(WV_E_OOM, "wv_adapters_set: host memory exhausted");
@@ -845,7 +859,7 @@ int wv_adapters_scratch(const wv_adapter_batch* batch, const wv_adapter_rows* se
     if (rc) return rc;
     if (!bytes) return rt_fail(WV_E_ARG, "wv_adapters_scratch: nil bytes");
     int range;
-    *bytes = scratch_floats(s, n_sets, batch->n_tokens, adapt_ranges(s[0].c.cols, batch->n_seqs, batch->n_tokens, n_sets, range)) * 4;
+    *bytes = scratch_floats(s, n_sets, batch->n_tokens, adapt_ranges(s[0].c.cols, *batch, n_sets, range)) * 4;
     return WV_OK;
 }
 
@@ -873,15 +887,17 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
         if (k.y && k.base == k.y && k.bs != k.ys)  // rows written would be others' base still to be read
             return rt_fail(WV_E_SHAPE, "wv_adapters: base is y, at row strides of %lld and %lld", (long long)k.bs,
                            (long long)k.ys);
-        k.a = s[i].a, k.b = s[i].b, k.rank = s[i].rank, k.scale = s[i].scale;
+        k.a = s[i].a, k.b = s[i].b, k.known = s[i].known;
         k.rows = s[i].c.rows, k.R = s[i].R, k.C = s[i].C, k.n_adapters = s[i].c.n_adapters;
     }
     if (!a.n_seqs || !a.n_tokens) return WV_OK;
     if (!d_x || !batch->d_cu_q || !batch->d_adapter) return rt_fail(WV_E_ARG, "wv_adapters: nil x/cu_q/adapter");
     for (int i = 0; i < n_sets; ++i)
         if (!a.set[i].y) return rt_fail(WV_E_ARG, "wv_adapters: nil y");
+    a.n_sets = n_sets;
+    for (int i = 0; i < n_sets; ++i) a.ranks += s[i].R;
     a.x = d_x, a.xs = x_stride, a.cu = batch->d_cu_q, a.which = batch->d_adapter;
-    a.ranges = adapt_ranges(a.cols, a.n_seqs, a.n_tokens, n_sets, a.range);
+    a.ranges = adapt_ranges(a.cols, *batch, n_sets, a.range);
     (void)hipSetDevice(s[0].device);
     hipStream_t st = rt_stream(stream, s[0].device);
     const size_t floats = scratch_floats(s, n_sets, a.n_tokens, a.ranges);
@@ -901,8 +917,9 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
         a.set[i].h = h;
         h += size_t(a.ranges) * size_t(a.n_tokens) * size_t(a.set[i].R);
     }
-    const bool few = batch->max_q ? batch->max_q <= kFew : a.n_tokens <= kFew;
-    const int e = launch_adapters(a, n_sets, s[0].c.type, few, st);
+    const bool few = adapt_few(*batch);
+    const int e = s[0].c.type == WV_ADAPTER_BF16 ? launch_adapters<WV_ADAPTER_BF16>(a, few, st)
+                                                 : launch_adapters<WV_ADAPTER_F16>(a, few, st);
     return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_adapters: kernel launch");
 }
 
