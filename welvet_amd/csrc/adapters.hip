@@ -23,7 +23,7 @@ namespace {
 constexpr int kMaxSets = 4;      // of a call
 constexpr int kMaxRank = 256;
 constexpr int kTile = 32;        // token rows of a block
-constexpr int kFew = 4;          // rows of a tile up to which they go one by one
+constexpr int kFew = 4;          // rows of a tile up to which they go without matrix products
 constexpr int kChunk = 512;      // columns that a wave takes at a time of such a row, 8 to a lane
 constexpr int kMaxRanges = 32;   // of the columns
 
@@ -210,47 +210,98 @@ __device__ __forceinline__ int pair_exponent(float m) {
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 
-// h of a few tokens, one after the other: a wave takes every fourth group of four ranks, a lane 8 columns at a time.
-// The first loads do not wait for the adapter's rank (there are 16 rows in A at least).
-template <int TYPE>
-__device__ __forceinline__ void down_few(const Args& a, const SetArgs& s, const Tile& t, int id, int c0, int c1, float* h) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint16_t* A = s.a + int64_t(id) * s.R * s.C + c0 + 8 * lane;
-    const int cl = c0 + 8 * lane;
-    uint4 w[4];
-    float v[8];
-    auto load = [&](const float* x, int r0, int c) {
-        load8(x, cl + c, a.cols, v);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            w[k] = cl + c < c1 ? *reinterpret_cast<const uint4*>(A + int64_t(r0 + k) * s.C + c) : uint4{};
-    };
-    load(a.x + int64_t(t.t0) * a.xs, 4 * wave, 0);
-    const int rank = s.known[id].rank;
-    for (int n = 0; n < t.n; ++n) {
-        const float* x = a.x + int64_t(t.t0 + n) * a.xs;
-        for (int r0 = 4 * wave; r0 < rank; r0 += 16) {
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int c = 0; c < c1 - c0; c += kChunk) {
-                if (n || c || r0 >= 16) load(x, r0, c);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float f[8];
-                    wide8<TYPE>(w[k], f);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sum[k] = fmaf(f[i], v[i], sum[k]);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float y = wave_total(sum[k]);
-                if (lane == 0 && r0 + k < rank) h[int64_t(n) * s.R + r0 + k] = y;
-            }
-        }
-    }
+// a's lower half of lanes plus its upper one, and b's in the upper half; a's rows 0 and 2 plus its 1 and 3, and b's in
+// those; a row's total, in its last lane.
+__device__ __forceinline__ float fold_halves(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float fold_rows(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float row_total(float x) {
+    x += __int_as_float(dpp_i<kDppRowShr1>(0, __float_as_int(x)));
+    x += __int_as_float(dpp_i<kDppRowShr2>(0, __float_as_int(x)));
+    x += __int_as_float(dpp_i<kDppRowShr4, 0xf, 0xe>(0, __float_as_int(x)));
+    return x + __int_as_float(dpp_i<kDppRowShr8, 0xf, 0xc>(0, __float_as_int(x)));
 }
 
-// h of a tile of tokens for all sets, whose ranks follow one another, 32 NR of them at a time, on products of 32 ranks
+// h of NT of the tokens, those from `have` on the last one again: a wave takes every fourth group of four ranks, a lane 8
+// columns at a time, and meets the others at a group's end. The first loads do not wait for the adapter's rank (there are
+// 16 rows in A at least). Where the range is one chunk, the tokens' columns stay in registers and the next group of A is
+// on its way while one is summed (3 to 8% of a call); with more chunks there are blocks enough to wait for.
+template <int TYPE, int NT>
+__device__ __forceinline__ void down_rows(const Args& a, const SetArgs& s, int t0, int have, int id, int c0, int c1, float* h) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cl = c0 + 8 * lane;
+    const uint16_t* A = s.a + int64_t(id) * s.R * s.C;
+    uint4 w[4];
+    float v[NT][8], sum[4][NT];
+    auto load_x = [&](int c) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) load8(a.x + int64_t(t0 + min(n, have - 1)) * a.xs, cl + c, a.cols, v[n]);
+    };
+    auto load_w = [&](int r0, int c) {
+        const int at = min(cl + c, s.C - 8);  // where there is no such column, x is 0
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = *reinterpret_cast<const uint4*>(A + int64_t(r0 + k) * s.C + at);
+    };
+    auto clear = [&] {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sum[k][n] = 0.0f;
+    };
+    auto add = [&](const uint4 (&u)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float f[8];
+            wide8<TYPE>(u[k], f);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[k][n] = fmaf(f[i], v[n][i], sum[k][n]);
+        }
+    };
+    // the sums over the lanes: the four ranks' in a row of 16 lanes each, then in its last
+    auto store = [&](int r0, int rank) {
+        const int r = r0 + (lane >> 4);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float y = row_total(fold_rows(fold_halves(sum[0][n], sum[2][n]), fold_halves(sum[1][n], sum[3][n])));
+            if ((lane & 15) == 15 && r < rank && n < have) h[int64_t(n) * s.R + r] = y;
+        }
+    };
+    load_x(0);
+    load_w(4 * wave, 0);
+    const int rank = s.known[id].rank;
+    if (c1 - c0 <= kChunk) {
+        for (int r0 = 4 * wave; r0 < rank; r0 += 16) {
+            const uint4 u[4] = {w[0], w[1], w[2], w[3]};
+            load_w(r0 + 16 < rank ? r0 + 16 : r0, 0);
+            clear();
+            add(u);
+            store(r0, rank);
+        }
+        return;
+    }
+    for (int r0 = 4 * wave; r0 < rank; r0 += 16) {
+        clear();
+        for (int c = 0; c < c1 - c0; c += kChunk) {
+            if (c || r0 >= 16) load_x(c), load_w(r0, c);
+            add(w);
+        }
+        store(r0, rank);
+    }
+}
+// h of a short sequence, NT rows at a time.
+template <int TYPE, int NT>
+__device__ __forceinline__ void down_few(const Args& a, const SetArgs& s, const Tile& t, int id, int c0, int c1, float* h) {
+    for (int n = 0; n < t.n; n += NT, h += NT * s.R) down_rows<TYPE, NT>(a, s, t.t0 + n, min(t.n - n, NT), id, c0, c1, h);
+}
+
+// h of a tile of tokens for all sets, whose ranks follow one another, 32 NR of them to a block, on products of 32 ranks
 // x 32 tokens x 16 columns: a lane holds the same 16 columns of its rank's row and of its token's (lanes from 32 on the
 // 16 behind those), straight from memory. The block's waves take every fourth 32 columns and meet in LDS.
 template <int TYPE, int NR>
@@ -265,137 +316,137 @@ __device__ __forceinline__ void down_tile(const Args& a, const Tile& t, int rang
         while (i + 1 < kMaxSets && r >= a.set[i].R) r -= a.set[i++].R;
         return i;
     };
-    for (int r0 = 0; r0 < a.ranks; r0 += 32 * NR) {
-        f16v acc[NR];
-        const uint16_t* row[NR];
+    const int r0 = 32 * NR * blockIdx.z;
+    f16v acc[NR];
+    const uint16_t* row[NR];
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+        int r = min(r0 + 32 * k + n, a.ranks - 1);
+        const SetArgs& s = a.set[set_of(r)];
+        // of a set that does not know the adapter, anything: nobody reads it
+        const int id = unsigned(t.id) < unsigned(s.n_adapters) ? t.id : 0;
+        row[k] = s.a + (int64_t(id) * s.R + r) * s.C;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[k][i] = 0.0f;
+    }
+    float v[16];
+    uint4 w[NR][2];
+    auto load_a = [&](int c) {
 #pragma unroll
         for (int k = 0; k < NR; ++k) {
-            int r = min(r0 + 32 * k + n, a.ranks - 1);
-            const SetArgs& s = a.set[set_of(r)];
-            // of a set that does not know the adapter, anything: nobody reads it
-            const int id = unsigned(t.id) < unsigned(s.n_adapters) ? t.id : 0;
-            row[k] = s.a + (int64_t(id) * s.R + r) * s.C;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[k][i] = 0.0f;
+            w[k][0] = *reinterpret_cast<const uint4*>(row[k] + c);
+            w[k][1] = *reinterpret_cast<const uint4*>(row[k] + c + 8);
         }
-        float v[16];
-        uint4 w[NR][2];
-        auto load_a = [&](int c) {
+    };
+    auto load_x = [&](int c) {
 #pragma unroll
-            for (int k = 0; k < NR; ++k) {
-                w[k][0] = *reinterpret_cast<const uint4*>(row[k] + c);
-                w[k][1] = *reinterpret_cast<const uint4*>(row[k] + c + 8);
-            }
-        };
-        auto load_x = [&](int c) {
+        for (int q = 0; q < 4; ++q) {
+            const f4 y = *reinterpret_cast<const f4*>(x + c + 4 * q);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f4 y = *reinterpret_cast<const f4*>(x + c + 4 * q);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * q + i] = y[i];
-            }
-        };
-        int e = -113;  // fp16: the token's sums so far are in units of 2^(e - 14)
-        auto step = [&](auto next) {
-            if constexpr (TYPE == WV_ADAPTER_F16) {
-                float m = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
-                const int en = max(e, pair_exponent(m));
-                if (__ballot(en != e)) {
-                    const float f = ldexpf(1.0f, max(e - en, -200));
-#pragma unroll
-                    for (int k = 0; k < NR; ++k) acc[k] *= f;
-                }
-                e = en;
-                const float up = power(14 - e);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] *= up;
-            }
-            const Terms<TYPE> x0 = split8<TYPE>(v), x1 = split8<TYPE>(v + 8);
-            uint4 u[NR][2];
-#pragma unroll
-            for (int k = 0; k < NR; ++k) u[k][0] = w[k][0], u[k][1] = w[k][1];
-            next();
-#pragma unroll
-            for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][0], x0, acc[k]);
-#pragma unroll
-            for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][1], x1, acc[k]);
-        };
-        // whole steps without a branch (what would be loaded behind the last one is that one again), then what is left
-        // of a row, where A, padded with zeros to multiples of 64 columns, goes on
-        const int steps = (min(c1, a.cols) - c0) / 32, mine = (steps - wave + 3) / 4;
-        const int at = c0 + 32 * wave + 16 * hi;
-        if (mine > 0) {
-            load_x(at), load_a(at);
-            for (int i = 0; i < mine; ++i) {
-                const int c = at + 128 * min(i + 1, mine - 1);
-                step([&] { load_x(c), load_a(c); });
-            }
+            for (int i = 0; i < 4; ++i) v[4 * q + i] = y[i];
         }
-        if (const int c = c0 + 32 * steps + 16 * hi; c0 + 32 * steps < min(c1, a.cols) && (steps & 3) == wave) {
-            load8(x, c, a.cols, v);
-            load8(x, c + 8, a.cols, v + 8);
-            load_a(c);
-            step([] {});
-        }
+    };
+    int e = -113;  // fp16: the token's sums so far are in units of 2^(e - 14)
+    auto step = [&](auto next) {
         if constexpr (TYPE == WV_ADAPTER_F16) {
+            float m = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NR; ++k) acc[k] *= power(e - 14);
-        }
-        // waves 2 and 3 to 0 and 1, then 1 to 0
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+            const int en = max(e, pair_exponent(m));
+            if (__ballot(en != e)) {
+                const float f = ldexpf(1.0f, max(e - en, -200));
 #pragma unroll
-        for (int step = 2; step >= 1; step /= 2) {
-            float* mine = lds + ((wave & (step - 1)) * 32 + n) * LD + 4 * hi;
-            __syncthreads();
-            if (wave >= step && wave < 2 * step) {
-#pragma unroll
-                for (int k = 0; k < NR; ++k)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) mine[32 * k + 8 * q + i] = acc[k][4 * q + i];
+                for (int k = 0; k < NR; ++k) acc[k] *= f;
             }
-            __syncthreads();
-            if (wave < step) {
+            e = en;
+            const float up = power(14 - e);
 #pragma unroll
-                for (int k = 0; k < NR; ++k)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[k][4 * q + i] += mine[32 * k + 8 * q + i];
-            }
+            for (int i = 0; i < 16; ++i) v[i] *= up;
         }
-        if (wave == 0 && n < t.n) {
+        const Terms<TYPE> x0 = split8<TYPE>(v), x1 = split8<TYPE>(v + 8);
+        uint4 u[NR][2];
+#pragma unroll
+        for (int k = 0; k < NR; ++k) u[k][0] = w[k][0], u[k][1] = w[k][1];
+        next();
+#pragma unroll
+        for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][0], x0, acc[k]);
+#pragma unroll
+        for (int k = 0; k < NR; ++k) acc[k] = product<TYPE>(u[k][1], x1, acc[k]);
+    };
+    // whole steps without a branch (what would be loaded behind the last one is that one again), then what is left
+    // of a row, where A, padded with zeros to multiples of 64 columns, goes on
+    const int steps = (min(c1, a.cols) - c0) / 32, mine = (steps - wave + 3) / 4;
+    const int at = c0 + 32 * wave + 16 * hi;
+    if (mine > 0) {
+        load_x(at), load_a(at);
+        for (int i = 0; i < mine; ++i) {
+            const int c = at + 128 * min(i + 1, mine - 1);
+            step([&] { load_x(c), load_a(c); });
+        }
+    }
+    if (const int c = c0 + 32 * steps + 16 * hi; c0 + 32 * steps < min(c1, a.cols) && (steps & 3) == wave) {
+        load8(x, c, a.cols, v);
+        load8(x, c + 8, a.cols, v + 8);
+        load_a(c);
+        step([] {});
+    }
+    if constexpr (TYPE == WV_ADAPTER_F16) {
+#pragma unroll
+        for (int k = 0; k < NR; ++k) acc[k] *= power(e - 14);
+    }
+    // waves 2 and 3 to 0 and 1, then 1 to 0
+#pragma unroll
+    for (int step = 2; step >= 1; step /= 2) {
+        float* mine = lds + ((wave & (step - 1)) * 32 + n) * LD + 4 * hi;
+        __syncthreads();
+        if (wave >= step && wave < 2 * step) {
 #pragma unroll
             for (int k = 0; k < NR; ++k)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    int r = r0 + 32 * k + 8 * q + 4 * hi;
-                    if (r >= a.ranks) continue;
-                    const SetArgs& s = a.set[set_of(r)];  // the ranks of a set are a multiple of 16
-                    *reinterpret_cast<f4*>(s.h + (int64_t(range) * a.n_tokens + t.t0 + n) * s.R + r) =
-                        f4{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
-                }
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mine[32 * k + 8 * q + i] = acc[k][4 * q + i];
         }
+        __syncthreads();
+        if (wave < step) {
+#pragma unroll
+            for (int k = 0; k < NR; ++k)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[k][4 * q + i] += mine[32 * k + 8 * q + i];
+        }
+    }
+    if (wave == 0 && n < t.n) {
+#pragma unroll
+        for (int k = 0; k < NR; ++k)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                int r = r0 + 32 * k + 8 * q + 4 * hi;
+                if (r >= a.ranks) continue;
+                const SetArgs& s = a.set[set_of(r)];  // the ranks of a set are a multiple of 16
+                *reinterpret_cast<f4*>(s.h + (int64_t(range) * a.n_tokens + t.t0 + n) * s.R + r) =
+                    f4{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
+            }
     }
 }
 
-// FEW: the caller says that no sequence has more than kFew rows (if one has, its rows go one by one all the same).
-template <int TYPE, int NR, bool FEW>
+// FEW (1, kFew; 0: not so): the caller says that no sequence has more rows (if one has, they go FEW at a time).
+template <int TYPE, int NR, int FEW>
 __global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
     __shared__ float lds[FEW ? 1 : 2 * 32 * (32 * NR + 4)];
     Tile t;
-    if (!find_tile<FEW>(a, tile0 + int(blockIdx.y), t)) return;
+    if (!find_tile<(FEW > 0)>(a, tile0 + int(blockIdx.y), t)) return;
     const int range = FEW ? blockIdx.x % a.ranges : blockIdx.x, c0 = range * a.range;
     auto few = [&](const SetArgs& s) {
         if (unsigned(t.id) < unsigned(s.n_adapters))
-            down_few<TYPE>(a, s, t, t.id, c0, min(c0 + a.range, a.cols), s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R);
+            down_few<TYPE, FEW ? FEW : kFew>(a, s, t, t.id, c0, min(c0 + a.range, a.cols),
+                                             s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R);
     };
     if constexpr (FEW) {
         few(a.set[blockIdx.x / a.ranges]);
     } else if (t.n <= kFew) {
-        for (int i = 0; i < a.n_sets; ++i) few(a.set[i]);
+        for (int i = blockIdx.z; i < a.n_sets; i += gridDim.z) few(a.set[i]);
     } else if (t.id >= 0) {
         down_tile<TYPE, NR>(a, t, range, c0, min(c0 + a.range, a.set[0].C), lds);
     }
@@ -429,37 +480,37 @@ __device__ __forceinline__ void stage_h(const Args& a, const SetArgs& s, const T
     }
 }
 
-// y of the block's outputs for a few tokens, kFew at a time: a thread takes an output, and has its row of B on the
+// y of the block's outputs for a few tokens, NT at a time: a thread takes an output, and has its row of B on the
 // way before it looks at anything else.
-template <int TYPE, int NR>
+template <int TYPE, int NR, int NT>
 __device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Tile& t, int id, int first, int last,
                                        const float* base, float* y, float* h) {
     constexpr int LD = 32 * NR + 4, NB = NR < 2 ? 4 : 8;  // 16-byte units of B that are loaded ahead
     const uint16_t* B = s.b + (int64_t(id) * s.rows + first) * s.R;
     const int rank = s.known[id].rank;
     const float scale = s.known[id].scale;
-    for (int n0 = 0; n0 < t.n; n0 += kFew) {
-        const int rows = min(t.n - n0, kFew);
+    for (int n0 = 0; n0 < t.n; n0 += NT) {
+        const int rows = min(t.n - n0, NT);
         for (int o = threadIdx.x; o - int(threadIdx.x) < last - first; o += 256) {
             const bool in = o < last - first;
             const uint16_t* row = B + int64_t(in ? o : 0) * s.R;
             uint4 w[NB];
 #pragma unroll
             for (int k = 0; k < NB; ++k) w[k] = 8 * k < s.R ? *reinterpret_cast<const uint4*>(row + 8 * k) : uint4{};
-            float sum[kFew];
+            float sum[NT];
 #pragma unroll
-            for (int n = 0; n < kFew; ++n) sum[n] = in && n < rows ? base[(n0 + n) * s.bs + first + o] : 0.0f;
+            for (int n = 0; n < NT; ++n) sum[n] = in && n < rows ? base[(n0 + n) * s.bs + first + o] : 0.0f;
             if (o == int(threadIdx.x)) {
                 if (n0) __syncthreads();
                 stage_h<NR>(a, s, t, n0, rows, rank, scale, h);
                 __syncthreads();
             }
-            float add[kFew] = {};
+            float add[NT] = {};
             auto unit = [&](uint4 u, int r) {
                 float f[8];
                 wide8<TYPE>(u, f);
 #pragma unroll
-                for (int n = 0; n < kFew; ++n)
+                for (int n = 0; n < NT; ++n)
                     if (n < rows)
 #pragma unroll
                         for (int i = 0; i < 8; ++i) add[n] = fmaf(f[i], h[n * LD + r + i], add[n]);
@@ -469,7 +520,7 @@ __device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Ti
                 if (8 * k < rank) unit(w[k], 8 * k);
             for (int r = 8 * NB; r < rank; r += 8) unit(*reinterpret_cast<const uint4*>(row + r), r);
 #pragma unroll
-            for (int n = 0; n < kFew; ++n)
+            for (int n = 0; n < NT; ++n)
                 if (in && n < rows) y[(n0 + n) * s.ys + first + o] = sum[n] + add[n];
         }
     }
@@ -643,23 +694,23 @@ __device__ __forceinline__ void copy_rows(const SetArgs& s, int rows, int first,
 }
 
 struct Nothing {};
-template <int TYPE, int NR, bool FEW>
+template <int TYPE, int NR, int FEW>
 __global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) {
-    __shared__ __align__(16) float h[kFew * (32 * NR + 4)];
-    __shared__ std::conditional_t<FEW, Nothing, UpLds<TYPE, NR>> lds;
+    __shared__ __align__(16) float h[(FEW ? FEW : kFew) * (32 * NR + 4)];
+    __shared__ std::conditional_t<(FEW > 0), Nothing, UpLds<TYPE, NR>> lds;
     int set = 0;
     while (set + 1 < kMaxSets && int(blockIdx.x) >= a.set[set + 1].block0) ++set;
     const SetArgs& s = a.set[set];
     const int first = (int(blockIdx.x) - s.block0) * 256 * turns;
     Tile t;
-    if (!find_tile<FEW>(a, tile0 + int(blockIdx.y), t)) return;
+    if (!find_tile<(FEW > 0)>(a, tile0 + int(blockIdx.y), t)) return;
     const int id = t.id;
     const int last = min(first + 256 * turns, s.rows);
     const float* base = s.base + t.t0 * s.bs;
     float* y = s.y + t.t0 * s.ys;
     const bool known = unsigned(id) < unsigned(s.n_adapters);
     if (known && (FEW || t.n <= kFew)) {
-        up_few<TYPE, NR>(a, s, t, id, first, last, base, y, h);
+        up_few<TYPE, NR, FEW ? FEW : kFew>(a, s, t, id, first, last, base, y, h);
         return;
     }
     if constexpr (!FEW) {
@@ -680,8 +731,11 @@ __global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) 
 // Tiles of a call, at most.
 int64_t adapt_tiles(int n_seqs, int n_tokens) { return int64_t(n_seqs) + n_tokens / kTile; }
 
-// Whether the kernels of short sequences take a call.
-bool adapt_few(const wv_adapter_batch& b) { return b.max_q ? b.max_q <= kFew : b.n_tokens <= kFew; }
+// Whether the kernels of short sequences take a call: how many rows at a time, or 0.
+int adapt_few(const wv_adapter_batch& b) {
+    const int most = b.max_q ? b.max_q : b.n_tokens;
+    return most <= 1 ? 1 : most <= kFew ? kFew : 0;
+}
 
 // Into how many ranges the columns are cut: about eight blocks a CU, and ranges of whole chunks.
 int adapt_ranges(int cols, const wv_adapter_batch& b, int n_sets, int& range) {
@@ -694,7 +748,7 @@ int adapt_ranges(int cols, const wv_adapter_batch& b, int n_sets, int& range) {
 }
 
 template <int TYPE>
-int launch_adapters(Args& a, bool few, hipStream_t s) {
+int launch_adapters(Args& a, int few, hipStream_t s) {
     const int64_t tiles = few ? a.n_seqs : adapt_tiles(a.n_seqs, a.n_tokens);
     int64_t units = 0, blocks = 0;
     int R = 0;
@@ -704,28 +758,38 @@ int launch_adapters(Args& a, bool few, hipStream_t s) {
         a.set[i].block0 = i < a.n_sets ? int(blocks) : INT32_MAX;
         if (i < a.n_sets) blocks += (a.set[i].rows + 256 * turns - 1) / (256 * turns);
     }
-    auto go = [&](auto kern, int64_t x, auto... more) {
+    auto go = [&](auto kern, int64_t x, int z, auto... more) {
         for (int64_t t0 = 0; t0 < tiles; t0 += 1 << 15) {
-            const dim3 grid{unsigned(x), unsigned(std::min<int64_t>(tiles - t0, 1 << 15))};
+            const dim3 grid{unsigned(x), unsigned(std::min<int64_t>(tiles - t0, 1 << 15)), unsigned(z)};
             hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, a, int(t0), more...);
         }
     };
     auto up = [&](auto nr) {
         constexpr int NR = decltype(nr)::value;
-        few ? go(k_adapt_up<TYPE, NR, true>, blocks, turns) : go(k_adapt_up<TYPE, NR, false>, blocks, turns);
+        few == 1 ? go(k_adapt_up<TYPE, NR, 1>, blocks, 1, turns)
+        : few    ? go(k_adapt_up<TYPE, NR, kFew>, blocks, 1, turns)
+                 : go(k_adapt_up<TYPE, NR, 0>, blocks, 1, turns);
     };
     std::integral_constant<int, 1> n1;
     std::integral_constant<int, 2> n2;
     std::integral_constant<int, 4> n4;
     std::integral_constant<int, 8> n8;
-    if (few)
-        go(k_adapt_down<TYPE, 1, true>, int64_t(a.ranges) * a.n_sets);
-    else if (a.ranks <= 32)
-        go(k_adapt_down<TYPE, 1, false>, a.ranges);
-    else if (a.ranks <= 64)
-        go(k_adapt_down<TYPE, 2, false>, a.ranges);
-    else  // 128 at a time: more would take all of a SIMD's registers for one wave
-        go(k_adapt_down<TYPE, 4, false>, a.ranges);
+    if (few) {
+        go(few == 1 ? k_adapt_down<TYPE, 1, 1> : k_adapt_down<TYPE, 1, kFew>, int64_t(a.ranges) * a.n_sets, 1);
+    } else {
+        // Ranks of a block, 32 nr: all of them, as the terms of x are split once for them, unless a block a CU takes them
+        // in parts (all / in parts: 3 sets of rank 32 over 4096 columns, 8 sequences of 8 tokens, 14.3 / 9.9 us with the
+        // launch for B; 2 sets of rank 128, one of 10, 18.4 / 12.6; but 16 of 30 tokens, 384 blocks, 18.7 / 18.8, 64 of 8,
+        // 1536 blocks, 23.3 / 25.0).
+        auto parts = [&](int nr) { return (a.ranks + 32 * nr - 1) / (32 * nr); };
+        auto fits = [&](int nr) { return parts(nr) == 1 || a.ranges * tiles * parts(nr) <= 256; };
+        if (fits(1))
+            go(k_adapt_down<TYPE, 1, 0>, a.ranges, parts(1));
+        else if (fits(2))
+            go(k_adapt_down<TYPE, 2, 0>, a.ranges, parts(2));
+        else  // more than 128 at a time would take all of a SIMD's registers for one wave
+            go(k_adapt_down<TYPE, 4, 0>, a.ranges, parts(4));
+    }
     R <= 32 ? up(n1) : R <= 64 ? up(n2) : R <= 128 ? up(n4) : up(n8);
     return int(hipGetLastError());
 }
@@ -917,7 +981,7 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
         a.set[i].h = h;
         h += size_t(a.ranges) * size_t(a.n_tokens) * size_t(a.set[i].R);
     }
-    const bool few = adapt_few(*batch);
+    const int few = adapt_few(*batch);
     const int e = s[0].c.type == WV_ADAPTER_BF16 ? launch_adapters<WV_ADAPTER_BF16>(a, few, st)
                                                  : launch_adapters<WV_ADAPTER_F16>(a, few, st);
     return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_adapters: kernel launch");
