@@ -448,7 +448,7 @@ int wv_kv_read_dev(uint64_t cache, int32_t layer, const int64_t *d_slots, int32_
  * (the calls below keep it so; a new table is -1 everywhere, lengths and
  * counts 0). The calls on one table run one after the other: on one stream, or
  * ordered by the caller. They allocate nothing, need no host in between, and
- * can be captured. n_seqs is at most 16384. */
+ * can be captured. n_seqs is at most 16384; with none nothing is done. */
 typedef struct wv_kv_tables {
     int32_t n_seqs, max_pages;
     int32_t *d_pages;  /* [n_seqs][max_pages] */
@@ -539,7 +539,8 @@ int wv_kv_attention_scratch(uint64_t cache, const wv_kv_batch *batch, int32_t n_
  * times, one instruction before many requests). Group g is the sequences
  * d_cu_seq[g] .. d_cu_seq[g+1]-1 (ascending; sequences before the first and
  * behind the last group stand alone) and its positions 0 .. d_shared[g]-1: all
- * of its sequences hold the same rows there, in the same pages or in copies. */
+ * of its sequences hold the same rows there, in the same pages or in copies
+ * (the first one also where it has no row in the batch). */
 typedef struct wv_kv_groups {
     int32_t n_groups;
     int32_t max_shared; /* most shared positions of a group, 0: unknown. Steers the launch only. */
@@ -607,7 +608,8 @@ typedef struct wv_rope_rows {
     int64_t x_stride, y_stride;
     int32_t n_heads;
 } wv_rope_rows;
-/* Turns row t of q and of k (either may be NULL) to position d_pos[t], t < n.
+/* Turns row t of q and of k (either may be NULL) to position d_pos[t], t < n
+ * (at most 2^23).
  * A negative position turns back, which is also the gradient of the call at
  * the positive one. Angles are taken in f64 modulo a turn, sine, cosine and
  * products in f32: within 6e-7 gain of a pair's length (positions up to 2^24; at
@@ -663,7 +665,8 @@ typedef struct wv_adapter_rows {
  * products A x lie in f32 in d_scratch (wv_adapters_scratch bytes, 16-byte
  * aligned, held by the call until its work is done), or, with NULL, in the
  * library's own scratch, which a call under capture is refused. The sums have a
- * fixed order. Device pointers, enqueued on `stream`. */
+ * fixed order; a row whose x holds an infinity or a NaN may become NaN as a
+ * whole. Device pointers, enqueued on `stream`. */
 int wv_adapters_dev(const wv_adapter_batch *batch, const float *d_x, int64_t x_stride, const wv_adapter_rows *sets,
                     int32_t n_sets, void *d_scratch, size_t scratch_bytes, void *stream);
 /* Scratch bytes of such a call. Only the batch's sizes and the sets' handles are read. */

@@ -225,3 +225,22 @@ def test_refusals():
             call()
         assert e.value.code == code and text in str(e.value)
     assert not x.cpu().numpy().any()
+
+
+def test_rows_of_a_call():
+    """2^23 rows a call: more are refused, before anything is read."""
+    r = Rope(2, theta=1e4)
+    x = dev(np.ones((1, 1, 2), np.float32))
+    with pytest.raises(wv.WelvetError) as e:
+        r.apply_dev(x.data_ptr(), (1 << 23) + 1, x.data_ptr(), 1)
+    assert e.value.code == -2 and "at most 2^23" in str(e.value)
+    n = 1 << 23
+    pos = torch.arange(n, dtype=torch.int32, device="cuda") % 1000
+    y = torch.ones(n, 1, 2, device="cuda")
+    torch.cuda.synchronize()
+    r.apply_dev(pos.data_ptr(), n, y.data_ptr(), 1)
+    wv.sync()
+    y = y.cpu().numpy()
+    check(y[-5:], np.ones((5, 1, 2), np.float32), np.arange(n - 5, n) % 1000, freqs(2, 1e4), "half", 2, 1.0)
+    assert np.array_equal(y[:n // 8 // 1000 * 1000].reshape(-1, 1000, 2)[::97], np.broadcast_to(
+        y[:1000].reshape(1, 1000, 2), (len(range(0, n // 8 // 1000, 97)), 1000, 2)))

@@ -65,9 +65,8 @@ __device__ __forceinline__ void turn_of(const RopeArgs& a, double p, int d, floa
 typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // Eight values a thread: four pairs, or values that stay (of pairs side by side, where rot ends within the eight, both).
-// A thread keeps its four angles and turns them in every
-// head that is its; kAhead heads' values are on their way before the sines are taken. NT: rows of more than the
-// caches hold are written past them.
+// A thread keeps its four angles and turns them in every head that is its; kAhead heads' values are on their way before
+// the sines are taken. NT: rows of more than the caches hold are written past them.
 constexpr int kAhead = 3;
 template <bool PAIRS, bool NT>
 __global__ void __launch_bounds__(256) k_rope8(RopeArgs a, int units, int heads_a_pass) {
@@ -260,7 +259,7 @@ int wv_rope_dev(uint64_t rope, const int32_t* d_pos, int32_t n, const wv_rope_ro
                 void* stream) {
     Rope r;
     if (!rope_lookup(rope, r)) return rt_fail(WV_E_HANDLE, "wv_rope: unknown rope %llu", (unsigned long long)rope);
-    if (n < 0 || n > 1 << 28) return rt_fail(WV_E_SHAPE, "wv_rope: %d rows", n);
+    if (n < 0 || n > 1 << 23) return rt_fail(WV_E_SHAPE, "wv_rope: %d rows (at most 2^23)", n);  // 2^31 threads a launch
     RopeArgs a{};
     const wv_rope_rows* in[2] = {q, k};
     RopeRows* to[2] = {&a.q, &a.k};
