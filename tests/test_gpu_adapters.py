@@ -128,6 +128,27 @@ def test_several_sets(new, which, ranks, typ):
         c.check(c.run(True), True)
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("seqs,cols,hint", [(3, 700, 0), (300, 1100, 0), (300, 1100, 4), (5, 2500, 1)])
+def test_short_sequences(n, seqs, cols, hint):
+    """A few rows each, beside empty sequences: one range of the columns a block, or several."""
+    rng = np.random.default_rng(n)
+    c = Case(rng, [40, 9, 270], cols, [16, 40, 3], [0 if b % 7 == 3 else max(1, n - b % 3) for b in range(seqs)],
+             [b % 4 - 1 for b in range(seqs)], pad=1)
+    if hint:
+        c.batch = AdapterBatch(seqs, c.t, c.cu.data_ptr(), c.ids.data_ptr(), hint)
+    c.check(c.run())
+    c.check(c.run(True), True)
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [[10], [100] * 4, [300] * 4, [10, 2, 1, 4]])
+def test_many_ranks(new, typ):
+    """The sets' ranks by one block after another, by blocks of their own, or both."""
+    c = Case(np.random.default_rng(len(new)), [130, 90], 2048, [128, 100], new, [b % 2 for b in range(len(new))], typ)
+    c.check(c.run())
+
+
 def test_sets_that_know_other_adapters():
     """Sets of one call with more or fewer adapters, of other ranks, some of them unset."""
     rng = np.random.default_rng(8)

@@ -209,6 +209,29 @@ def test_fork_grow_write(typ, hd, kv_heads, page, layers):
         t.read()
 
 
+@pytest.mark.parametrize("seqs,width", [(1, 1), (1, 130), (3, 65), (8, 33), (9, 700), (33, 40), (64, 31), (257, 9),
+                                        (1025, 5), (4097, 3), (16384, 2)])
+def test_fork_sizes(seqs, width):
+    """Tables of all shapes: every row comes from where it should, and every page's holders are counted."""
+    rng = np.random.default_rng(seqs)
+    kv, pool = KVCache(1, 1, 64, 32, 2000, "f16"), 2000
+    held = rng.integers(0, width + 1, seqs)
+    t = np.where(np.arange(width) < held[:, None], rng.integers(0, pool, (seqs, width)), -1).astype(np.int32)
+    refs = np.bincount(t[t >= 0], minlength=pool).astype(np.int32)
+    dt, dn, dr = ints(t), ints(held * 32), ints(refs)
+    tables = KVTables(seqs, width, dt.data_ptr(), dn.data_ptr(), dr.data_ptr(), dt.data_ptr())
+    for _ in range(2):
+        parent = rng.integers(-2, seqs + 1, seqs).astype(np.int32)  # some are emptied, some outside the table
+        d = ints(parent)
+        kv.fork_dev(tables, d.data_ptr())
+        wv.sync()
+        stay = (parent < -1) | (parent >= seqs)
+        src = np.where(stay, np.arange(seqs), np.maximum(parent, 0))
+        t, held = np.where((parent == -1)[:, None], -1, t[src]), np.where(parent == -1, 0, held[src])
+        assert np.array_equal(dt.cpu().numpy(), t) and np.array_equal(dn.cpu().numpy(), held * 32)
+        assert np.array_equal(dr.cpu().numpy(), np.bincount(t[t >= 0], minlength=pool))
+
+
 @pytest.mark.parametrize("seqs,width,pool,page,seed", [(1, 4, 3, 32, 0), (7, 9, 41, 32, 1), (70, 5, 200, 64, 2),
                                                        (1500, 3, 2300, 32, 3), (33, 40, 9000, 32, 4)])
 def test_random_calls(seqs, width, pool, page, seed):

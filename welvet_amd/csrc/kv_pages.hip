@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kMaxSeqs = 16384;    // of a table: one column of it lies in LDS
 constexpr int kPlanThreads = 1024;
-constexpr int kCopyBlocks = 4096;  // of a copy, twice what runs at once
+constexpr int kCopyBlocks = 4096;  // of a copy, twice what runs at once (2048: up to 8% slower; 8192 the same)
 
 typedef int32_t i4 __attribute__((ext_vector_type(4)));
 
@@ -106,8 +106,8 @@ __device__ __forceinline__ void for_entries(int n, int lane_value, F f) {
 // other, and a table's entries and the pool's counts are a few 10 KB. No other
 // block touches them, so a barrier orders them (its threads' stores and atomics
 // are in the L2 by then), and no step needs a fence for the whole device, which
-// costs some 3 us each. A thread takes a sequence. 8 sequences 9 us, 256
-// sequences of 65 pages in a pool of 17000 12 us: a chain of steps of 1 us.
+// costs some 3 us each. A thread takes a sequence. 256 sequences of 65 pages in a
+// pool of 17000 6.6 us: a chain of steps, each a load's latency.
 __global__ void __launch_bounds__(kPlanThreads) k_pages_resize(Tables t, Work w, const int32_t* __restrict__ to,
                                                                int32_t* __restrict__ ok) {
     __shared__ uint32_t lds[32];
@@ -209,8 +209,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_resize(Tables t, Work w,
 // tail[i] positions (NULL: all) what holds them: whole blocks of 32, of the
 // last one a unit's first keys (K) and the octets that they lie in (V, scales).
 // A block takes K or V (with its half of the scales) of one pair and KV head,
-// in one group of layers. 240 pages of 17 fp16 positions, 4 layers of 8 heads:
-// 17 us, 82 MB written; a resize without a copy 3 us.
+// in one group of layers. Bound by the bytes: 64 whole pages of 64 fp16
+// positions, 4 layers of 8 heads of 128, 69 MB, 18.6 us, 512 214 us, 5.2 TB/s read
+// and written (a large copy: 5.1); none of 256 3.9 us.
 struct Copy {
     uint8_t* base;
     size_t layer_bytes, code_bytes;
@@ -257,15 +258,17 @@ __global__ void __launch_bounds__(256) k_pages_copy(Copy c) {
 // Rows of the table trade places, 2^shift columns of all of them to a block,
 // through LDS, so that every row is read before any is written; the last block
 // does the same for the lengths. Entries that a sequence does not hold are -1
-// and count for nothing.
-__global__ void __launch_bounds__(256) k_pages_fork(Tables t, const int32_t* __restrict__ parent, int shift) {
+// and count for nothing. Bound by the latency of its three loads in a row and
+// the counts' atomics: 8 sequences 2.3 us (a launch), 64 of 1024 pages 3.5, 1024
+// of 512 8.8 (blocks of 256 threads: 5.2 and 15.8).
+__global__ void __launch_bounds__(1024) k_pages_fork(Tables t, const int32_t* __restrict__ parent, int shift) {
     extern __shared__ int32_t old[];
     const bool lens = blockIdx.x == gridDim.x - 1;
     if (lens) shift = 0;
     const int c0 = lens ? 0 : blockIdx.x << shift, n = lens ? 1 : min(1 << shift, t.max_pages - c0);
     int32_t* rows = lens ? t.len : t.pages + c0;
     const int64_t stride = lens ? 1 : t.max_pages;
-    const int c = threadIdx.x & ((1 << shift) - 1), step = 256 >> shift;
+    const int c = threadIdx.x & ((1 << shift) - 1), step = int(blockDim.x) >> shift;
     for (int b = threadIdx.x >> shift; b < t.n_seqs; b += step) old[(b << shift) + c] = c < n ? rows[b * stride + c] : -1;
     __syncthreads();
     for (int b = threadIdx.x >> shift; b < t.n_seqs; b += step) {
@@ -398,7 +401,8 @@ int launch_copy(const KvCache& c, const int32_t* src, const int32_t* dst, const 
     k.n_layers = c.c.n_layers, k.n_kv = c.c.n_kv_heads, k.block_bytes = 32 * c.c.head_dim * kv_code_bytes(c.c.type);
     k.page_shift = c.layer(0).page_shift, k.n_pages = c.c.n_pages;
     k.src = src, k.dst = dst, k.tail = tail, k.count = count, k.pairs = pairs;
-    // a layer to a block while there are few pairs, all layers where there are many
+    // a layer to a block while there are few pairs, all layers where there are many (one page of 32 layers 4.4 / 28.8 us,
+    // 8 18.6 / 51, 64 221 / 220, 200 710 / 696)
     const int64_t items = int64_t(pairs) * k.n_kv * 2;
     k.groups = int(std::max<int64_t>(1, std::min<int64_t>(k.n_layers, kCopyBlocks / items)));
     hipLaunchKernelGGL(k_pages_copy, dim3(unsigned(std::min<int64_t>(items * k.groups, kCopyBlocks))), dim3(256), 0, s, k);
@@ -449,10 +453,13 @@ int wv_kv_fork_dev(uint64_t cache, const wv_kv_tables* tables, const int32_t* d_
     if (rc || !k.n_seqs) return rc;
     if (!d_parent) return rt_fail(WV_E_ARG, "wv_kv_fork: nil parent");
     (void)hipSetDevice(c.device);
-    int shift = 6;  // up to four entries a thread, as long as 4 columns stay together
+    // An entry a thread, but four before fewer than 4 columns stay together (of 1 / 2 / 4 / 8 / 16 columns: 64 sequences
+    // of 1024 pages 8.6 / 5.9 / 4.4 / 3.9 / 3.5 us, 256 9.0 / 6.1 / 5.0 / 4.8 / 5.8, 1024 of 512 12.3 / 9.1 / 8.8 / 10.1).
+    int shift = 5;
     while (shift > 0 && (k.n_seqs << shift) > (shift > 2 ? 1024 : 4096)) --shift;
     const unsigned blocks = unsigned((int64_t(k.max_pages) + (1 << shift) - 1) >> shift) + 1;
-    hipLaunchKernelGGL(k_pages_fork, dim3(blocks), dim3(256), unsigned(k.n_seqs) * 4u << shift,
+    const unsigned threads = unsigned(std::min(1024, ((k.n_seqs << shift) + 63) & ~63));
+    hipLaunchKernelGGL(k_pages_fork, dim3(blocks), dim3(threads), unsigned(k.n_seqs) * 4u << shift,
                        rt_stream(stream, c.device), k, d_parent, shift);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_kv_fork: kernel launch");
