@@ -4,6 +4,11 @@
 // Two launches: h = A x in ranges of the columns (so that one token's rows
 // still fill the GPU), whose sums meet when B h reads them, in order of the
 // ranges. A and B stay 16-bit, x, h and all sums are f32.
+// Of few rows bound by two launches and the weights' latency: one token, two sets
+// of rank 16 on 14336 x 4096, 2.8 + 3.2 us; 64 requests of one, three sets of rank
+// 32 on 1024 x 4096, 6.4 + 4.0 (50 MB of A and B from the caches). Of many by base
+// and y, and by x: 2000 rows, rank 64 on 14336 x 4096, 18.5 + 54 us (229 MB of base
+// and y at a large copy's 5.1 TB/s: 45).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -34,9 +39,10 @@ struct Known {
 struct Set {
     wv_adapters_config c{};
     int device = 0;
-    int R = 0, C = 0;         // ranks and columns as stored: multiples of 16 and 64, zeros behind the adapter's own
+    // Ranks, columns and rows as stored: multiples of 16, 64 and 32, zeros behind the adapter's own.
+    int R = 0, C = 0, O = 0;
     uint16_t* a = nullptr;    // [n_adapters][R][C]
-    uint16_t* b = nullptr;    // [n_adapters][rows][R]
+    uint16_t* b = nullptr;    // [n_adapters][O / 32][R / 8][32 rows][8 ranks]: 64 lanes' operands of a product lie together
     Known* known = nullptr;   // [n_adapters], rank 0: unset
 };
 std::mutex g_mu;
@@ -66,7 +72,7 @@ struct SetArgs {
     float* y;
     float* h;  // [ranges][n_tokens][R]
     int64_t ys, bs;
-    int rows, R, C, n_adapters;
+    int rows, R, C, O, n_adapters;
     int block0;  // of the blocks over all sets' outputs, its first
 };
 struct Args {
@@ -431,7 +437,9 @@ __device__ __forceinline__ void down_tile(const Args& a, const Tile& t, int rang
     }
 }
 
-// FEW (1, kFew; 0: not so): the caller says that no sequence has more rows (if one has, they go FEW at a time).
+// FEW (1, kFew; 0: not so): the caller says that no sequence has more rows (if one has, they go FEW at a time). Without,
+// the rows of a short one go singly: four at a time take registers that tiles want (18.5 us for 2000 rows of rank 64 over
+// 4096 columns, else 19.6).
 template <int TYPE, int NR, int FEW>
 __global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
     __shared__ float lds[FEW ? 1 : 2 * 32 * (32 * NR + 4)];
@@ -440,8 +448,8 @@ __global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
     const int range = FEW ? blockIdx.x % a.ranges : blockIdx.x, c0 = range * a.range;
     auto few = [&](const SetArgs& s) {
         if (unsigned(t.id) < unsigned(s.n_adapters))
-            down_few<TYPE, FEW ? FEW : kFew>(a, s, t, t.id, c0, min(c0 + a.range, a.cols),
-                                             s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R);
+            down_few<TYPE, FEW ? FEW : 1>(a, s, t, t.id, c0, min(c0 + a.range, a.cols),
+                                          s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R);
     };
     if constexpr (FEW) {
         few(a.set[blockIdx.x / a.ranges]);
@@ -486,17 +494,17 @@ template <int TYPE, int NR, int NT>
 __device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Tile& t, int id, int first, int last,
                                        const float* base, float* y, float* h) {
     constexpr int LD = 32 * NR + 4, NB = NR < 2 ? 4 : 8;  // 16-byte units of B that are loaded ahead
-    const uint16_t* B = s.b + (int64_t(id) * s.rows + first) * s.R;
+    const uint16_t* B = s.b + (int64_t(id) * s.O + first) * s.R;
     const int rank = s.known[id].rank;
     const float scale = s.known[id].scale;
     for (int n0 = 0; n0 < t.n; n0 += NT) {
         const int rows = min(t.n - n0, NT);
         for (int o = threadIdx.x; o - int(threadIdx.x) < last - first; o += 256) {
             const bool in = o < last - first;
-            const uint16_t* row = B + int64_t(in ? o : 0) * s.R;
+            const uint16_t* row = B + int64_t(in ? o & ~31 : 0) * s.R + 8 * (o & 31);
             uint4 w[NB];
 #pragma unroll
-            for (int k = 0; k < NB; ++k) w[k] = 8 * k < s.R ? *reinterpret_cast<const uint4*>(row + 8 * k) : uint4{};
+            for (int k = 0; k < NB; ++k) w[k] = 8 * k < s.R ? *reinterpret_cast<const uint4*>(row + 256 * k) : uint4{};
             float sum[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) sum[n] = in && n < rows ? base[(n0 + n) * s.bs + first + o] : 0.0f;
@@ -518,7 +526,7 @@ __device__ __forceinline__ void up_few(const Args& a, const SetArgs& s, const Ti
 #pragma unroll
             for (int k = 0; k < NB; ++k)
                 if (8 * k < rank) unit(w[k], 8 * k);
-            for (int r = 8 * NB; r < rank; r += 8) unit(*reinterpret_cast<const uint4*>(row + r), r);
+            for (int r = 8 * NB; r < rank; r += 8) unit(*reinterpret_cast<const uint4*>(row + 32 * r), r);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 if (in && n < rows) y[(n0 + n) * s.ys + first + o] = sum[n] + add[n];
@@ -599,7 +607,7 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
                                         int last, const float* base, float* y, UpLds<TYPE, NR>& l) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hi = lane >> 5, m = lane >> 3, o4 = 4 * (lane & 7);
-    const uint16_t* B = s.b + int64_t(id) * s.rows * s.R + 8 * hi;
+    const uint16_t* B = s.b + int64_t(id) * s.O * s.R + 8 * lane;
     float* swap = l.swap[wave];
     // Nothing in a step branches, so that loads stay on their way: rows behind the tile's last are that one again (to
     // the same place), ranks behind the stored ones the last ones (times h = 0), what would be loaded behind the last
@@ -615,9 +623,9 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
     uint4 w[2 * NR];
     f4 was[4];
     auto load_b = [&](int o0) {
-        const uint16_t* row = B + int64_t(min(o0 + n, last - 1)) * s.R;
+        const uint16_t* row = B + int64_t(min(o0, (last - 1) & ~31)) * s.R;
 #pragma unroll
-        for (int k = 0; k < 2 * NR; ++k) w[k] = *reinterpret_cast<const uint4*>(row + min(16 * k, s.R - 16));
+        for (int k = 0; k < 2 * NR; ++k) w[k] = *reinterpret_cast<const uint4*>(row + 32 * min(16 * k, s.R - 16));
     };
     auto load_base = [&](int o0) {
         const float* p = base + max(min(o0, whole - 32), first);
@@ -753,7 +761,9 @@ int launch_adapters(Args& a, int few, hipStream_t s) {
     int64_t units = 0, blocks = 0;
     int R = 0;
     for (int i = 0; i < a.n_sets; ++i) units += (a.set[i].rows + 255) / 256, R = std::max(R, a.set[i].R);
-    const int turns = int(std::max<int64_t>(1, std::min<int64_t>(4, units * tiles / 1536)));
+    // Outputs of a block: 256, or twice that where there are blocks enough (1 / 2 / 4 turns: 12 sequences of 350 tokens,
+    // 14336 outputs of rank 64, 158 / 143 / 148 us; 2 of 100 15.8 / 16.7 / 22.2).
+    const int turns = units * tiles >= 1 << 11 ? 2 : 1;
     for (int i = 0; i < kMaxSets; ++i) {
         a.set[i].block0 = i < a.n_sets ? int(blocks) : INT32_MAX;
         if (i < a.n_sets) blocks += (a.set[i].rows + 256 * turns - 1) / (256 * turns);
@@ -847,7 +857,8 @@ int wv_adapters_create(const wv_adapters_config* cfg, uint64_t* adapters) {
     s.device = rt_current_device();
     s.R = (c.max_rank + 15) / 16 * 16;
     s.C = (c.cols + 63) / 64 * 64;
-    const size_t n = size_t(c.n_adapters), na = n * s.R * s.C * 2, nb = n * c.rows * s.R * 2;
+    s.O = (c.rows + 31) / 32 * 32;
+    const size_t n = size_t(c.n_adapters), na = n * s.R * s.C * 2, nb = n * s.O * s.R * 2;
     // one allocation: A, B (both multiples of 16 bytes), ranks and scales
     uint8_t* p = nullptr;
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&p), na + nb + n * sizeof(Known));
@@ -887,14 +898,17 @@ int wv_adapters_set(uint64_t adapters, int32_t index, int32_t rank, float scale,
         return rt_fail(WV_E_SHAPE, "wv_adapters_set: rank %d of at most %d", rank, s.c.max_rank);
     if (!std::isfinite(scale)) return rt_fail(WV_E_ARG, "wv_adapters_set: scale %g", double(scale));
     if (rank && (!a || !b)) return rt_fail(WV_E_ARG, "wv_adapters_set: nil a/b");
-    const size_t R = size_t(s.R), C = size_t(s.C), rows = size_t(s.c.rows), cols = size_t(s.c.cols), r = size_t(rank);
-    std::vector<uint16_t> ha(rank ? R * C : 0), hb(rank ? rows * R : 0);
+    const size_t R = size_t(s.R), C = size_t(s.C), O = size_t(s.O), rows = size_t(s.c.rows), cols = size_t(s.c.cols);
+    const size_t r = size_t(rank);
+    std::vector<uint16_t> ha(rank ? R * C : 0), hb(rank ? O * R : 0);
     for (size_t i = 0; i < r; ++i) std::memcpy(&ha[i * C], a + i * cols, cols * 2);
-    for (size_t i = 0; i < rows && r; ++i) std::memcpy(&hb[i * R], b + i * r, r * 2);
+    for (size_t o = 0; o < rows; ++o)
+        for (size_t i = 0; i < r; i += 8)
+            std::memcpy(&hb[o / 32 * 32 * R + i / 8 * 256 + o % 32 * 8], b + o * r + i, std::min<size_t>(8, r - i) * 2);
     (void)hipSetDevice(s.device);
     hipError_t e = hipDeviceSynchronize();  // calls that still read the adapter
     if (e == hipSuccess && r) e = hipMemcpy(s.a + size_t(index) * R * C, ha.data(), ha.size() * 2, hipMemcpyHostToDevice);
-    if (e == hipSuccess && r) e = hipMemcpy(s.b + size_t(index) * rows * R, hb.data(), hb.size() * 2, hipMemcpyHostToDevice);
+    if (e == hipSuccess && r) e = hipMemcpy(s.b + size_t(index) * O * R, hb.data(), hb.size() * 2, hipMemcpyHostToDevice);
     const Known k{rank, scale};
     if (e == hipSuccess) e = hipMemcpy(s.known + index, &k, sizeof k, hipMemcpyHostToDevice);
     return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_adapters_set");
@@ -952,7 +966,7 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
             return rt_fail(WV_E_SHAPE, "wv_adapters: base is y, at row strides of %lld and %lld", (long long)k.bs,
                            (long long)k.ys);
         k.a = s[i].a, k.b = s[i].b, k.known = s[i].known;
-        k.rows = s[i].c.rows, k.R = s[i].R, k.C = s[i].C, k.n_adapters = s[i].c.n_adapters;
+        k.rows = s[i].c.rows, k.R = s[i].R, k.C = s[i].C, k.O = s[i].O, k.n_adapters = s[i].c.n_adapters;
     }
     if (!a.n_seqs || !a.n_tokens) return WV_OK;
     if (!d_x || !batch->d_cu_q || !batch->d_adapter) return rt_fail(WV_E_ARG, "wv_adapters: nil x/cu_q/adapter");
