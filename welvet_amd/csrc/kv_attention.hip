@@ -27,6 +27,7 @@ namespace {
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -324,7 +325,7 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
     constexpr int NV = T / (TYPE == WV_KV_F16 ? 1 : 2);   // 16-byte V loads
     constexpr int BB = 32 * HD * E;              // bytes of a block
     constexpr int LD = HD + 4;
-    __shared__ float red[4][16][LD];
+    __shared__ __align__(16) float red[4][16][LD];
     __shared__ float rm[4][16], rl[4][16];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -514,13 +515,17 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
     l = sum_over_quads(l);
     const float back = ldexpf(1.0f, max(eo, -126)), wl = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+    for (int i = 0; i < T; ++i) o[i] = o[i] * wl * back;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int md = 4 * g + k;
-            const int d = TYPE == WV_KV_F16 ? 16 * i + md : 32 * (i / 2) + 2 * md + i % 2;
-            red[wave][n][d] = o[i][k] * wl * back;
+    for (int i = 0; i < T; ++i) {
+        if (TYPE == WV_KV_F16) {
+            *reinterpret_cast<f4*>(&red[wave][n][16 * i + 4 * g]) = f4{o[i][0], o[i][1], o[i][2], o[i][3]};
+        } else if (i % 2) {  // two tiles' dims take turns
+            float* p = &red[wave][n][16 * (i - 1) + 8 * g];
+            *reinterpret_cast<f4*>(p) = f4{o[i - 1][0], o[i][0], o[i - 1][1], o[i][1]};
+            *reinterpret_cast<f4*>(p + 4) = f4{o[i - 1][2], o[i][2], o[i - 1][3], o[i][3]};
         }
+    }
     if (g == 0) {
         rm[wave][n] = mx;
         rl[wave][n] = l;
@@ -545,12 +550,14 @@ __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t,
     float* dst = a.part ? a.part + ((int64_t(tok) * a.n_heads + head) * a.splits + sp + (MODE == kOwn ? a.lead : 0)) * LD
                         : a.out + int64_t(tok) * a.os + head * HD;
 #pragma unroll
-    for (int d = c; d < HD; d += 16) {
-        float x = 0.0f;
+    for (int d = 4 * c; d < HD; d += 64) {
+        f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (w[i] != 0.0f) x += w[i] * red[i][r][d];
-        dst[d] = x;
+        for (int i = 0; i < 4; ++i) {
+            const f4 y = *reinterpret_cast<const f4*>(&red[i][r][d]);
+            if (w[i] != 0.0f) x += w[i] * y;
+        }
+        *reinterpret_cast<f4_at4*>(dst + d) = x;
     }
     if (a.part && c == 0) {
         dst[HD] = M;
@@ -582,7 +589,10 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // operands as in attn_rows, but on 32x32x16 products (S^T = K Q^T leaves a lane
 // with one row, l & 31, and the keys of octets h and 2 + h, h = l >> 5), so that
 // a key's codes are read and converted once for 32 rows. Meant for as many rows
-// as give the matrix unit work and are too few for the tiles of 128.
+// as give the matrix unit work and are too few for the tiles of 128. Bound by its
+// steps: 1024 cycles of matrix products each, 1500 of vector instructions, one
+// after the other in a wave. 2400 rows a KV head over 32768 fp16 keys 845 us, 8.2
+// TFLOP of products in halves at 760 TFLOP/s (a large product: 1153).
 template <int HD, int TYPE>
 __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t, int kvh, int sp) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
@@ -592,7 +602,7 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
     constexpr int NV = 2 * T / (TYPE == WV_KV_F16 ? 1 : 2);  // 16-byte V loads
     constexpr int BB = 32 * HD * E;
     constexpr int LD = HD + 4;
-    __shared__ float red[4][16][LD];
+    __shared__ __align__(16) float red[4][16][LD];
     __shared__ float rm[4][32], rl[4][32];
     __shared__ __align__(16) float scales[4][kKvScales];
 
@@ -786,13 +796,21 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
     for (int part = 0; part < 2; ++part) {
         if (part) __syncthreads();
         if ((n >> 4) == part) {
+            auto put = [&](int d, float x0, float x1, float x2, float x3) {
+                *reinterpret_cast<f4*>(&red[wave][n & 15][d]) = f4{x0 * wl * back, x1 * wl * back, x2 * wl * back, x3 * wl * back};
+            };
 #pragma unroll
             for (int i = 0; i < T; ++i)
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const int md = 8 * (k >> 2) + 4 * h + (k & 3);
-                    const int d = TYPE == WV_KV_F16 ? 32 * i + md : 64 * (i / 2) + 2 * md + i % 2;
-                    red[wave][n & 15][d] = o[i][k] * wl * back;
+                for (int k = 0; k < 16; k += 4) {
+                    const int md = 2 * k + 4 * h;  // of the tile's dims, 4 from here on
+                    if (TYPE == WV_KV_F16) {
+                        put(32 * i + md, o[i][k], o[i][k + 1], o[i][k + 2], o[i][k + 3]);
+                    } else if (i % 2) {  // two tiles' dims take turns
+                        const f16v &a0 = o[i - 1], &a1 = o[i];
+                        put(32 * (i - 1) + 2 * md, a0[k], a1[k], a0[k + 1], a1[k + 1]);
+                        put(32 * (i - 1) + 2 * md + 4, a0[k + 2], a1[k + 2], a0[k + 3], a1[k + 3]);
+                    }
                 }
         }
         __syncthreads();
@@ -810,12 +828,14 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
         float* dst = a.part + ((int64_t(t.q0 + orow / G) * a.n_heads + kvh * G + orow % G) * a.splits + sp) * LD;
 #pragma unroll
-        for (int d = c; d < HD; d += 16) {
-            float x = 0.0f;
+        for (int d = 4 * c; d < HD; d += 64) {
+            f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (w[i] != 0.0f) x += w[i] * inv * red[i][lrow][d];
-            dst[d] = x;
+            for (int i = 0; i < 4; ++i) {
+                const f4 y = *reinterpret_cast<const f4*>(&red[i][lrow][d]);
+                if (w[i] != 0.0f) x += w[i] * inv * y;
+            }
+            *reinterpret_cast<f4*>(dst + d) = x;
         }
         if (c == 0) {
             dst[HD] = M;
@@ -826,7 +846,9 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
 
 // A batch whose sequences are in groups, in one launch: the blocks of the
 // groups' rows over the shared keys, which take longest, then those of every
-// sequence's rows over its own.
+// sequence's rows over its own. 64 sequences of one token behind 8192 int8 keys
+// of 8 heads of 128 with up to 1024 of their own: 48 us (the shared keys alone 33,
+// the own alone 22, for the same issue slots), and the join 4.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_groups(KvAttn a, int G, int lead_tiles, int y0) {
     Tile t;
@@ -1378,7 +1400,7 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
 }
 
 // A batch whose sequences are in groups. A lead block (32 rows of a group over a range of its shared keys) takes some
-// 10 us to begin and to end, and 1.25 us a step of its four waves while it has a CU to itself, 2.2 beside another. So
+// 8 us to begin and to end, and 1.25 us a step of its four waves while it has a CU to itself, 2.2 beside another. So
 // one block a CU where the own keys' blocks are there to run beside it, two where those have little to do, and steps
 // enough to pay for itself, unless there are few blocks at all. 32 heads over 8 of 128, int8, ranges 1 / 2 / 4 / 8: 564
 // rows a KV head over 8192 shared keys 95 / 86 / 80 / 80 us, 1160 rows 150 / 135 / 134 / 154, 2252 rows 242 / 224 / 243
