@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // a key's codes are read and converted once for 32 rows. Meant for as many rows
 // as give the matrix unit work and are too few for the tiles of 128. Bound by its
 // steps: 1024 cycles of matrix products each, 1500 of vector instructions, one
-// after the other in a wave. 2400 rows a KV head over 32768 fp16 keys 845 us, 8.2
+// after the other in a wave. 2400 rows a KV head over 32768 fp16 keys 845 us, 0.64
 // TFLOP of products in halves at 760 TFLOP/s (a large product: 1153).
 template <int HD, int TYPE>
 __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t, int kvh, int sp) {
@@ -763,6 +763,9 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
 #pragma unroll
                 for (int i = 0; i < T; ++i) o[i] *= f;
             }
+            // Heads of 64: no wait for V before all of P is there (64 sequences behind 8192 fp16 keys 28 us, else 34). The
+            // longer steps of heads of 128 hide it, and lose 8% if the halves of P do not run beside the products.
+            if constexpr (HD == 64) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
