@@ -591,8 +591,8 @@ __global__ void __launch_bounds__(256, 2) k_kv_attn_rows(KvAttn a, int G, int ma
 // a key's codes are read and converted once for 32 rows. Meant for as many rows
 // as give the matrix unit work and are too few for the tiles of 128. Bound by its
 // steps: 1024 cycles of matrix products each, 1500 of vector instructions, one
-// after the other in a wave. 2400 rows a KV head over 32768 fp16 keys 845 us, 0.64
-// TFLOP of products in halves at 760 TFLOP/s (a large product: 1153).
+// after the other in a wave. 2800 rows a KV head over 32768 fp16 keys 845 us, 0.75
+// TFLOP of products in halves at 885 TFLOP/s (a large product: 1153).
 template <int HD, int TYPE>
 __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t, int kvh, int sp) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
@@ -1409,7 +1409,7 @@ int launch_kv_attn(const KvAttn& a, hipStream_t s) {
 // rows a KV head over 8192 shared keys 95 / 86 / 80 / 80 us, 1160 rows 150 / 135 / 134 / 154, 2252 rows 242 / 224 / 243
 // / 282; 1204 rows over 1024 keys 44 / 50 / 62 / 84; 256 rows over 8192, 1024 own keys each, 4 / 8 / 16: 52 / 59 / 70.
 // (The kernel of 128-row tiles in its place: 564 rows 104 us at best, 1160 167, 2252 252, 4244 over 1024 keys 135
-// against 117; ahead on 2400 rows over 32768 fp16 keys alone, 816 against 870.)
+// against 117; ahead on 2800 rows over 32768 fp16 keys alone, 816 against 870.)
 // Own keys: as many ranges as the row kernel takes. Sequences of no group, which the host cannot see, may have as many
 // as the table is wide; a second range for them costs the others 1 us (7 sequences of 4000 keys beside 5 groups over
 // 4096: 55 to 45 us).
