@@ -3,6 +3,7 @@ steps), slots and positions, Q, K and V projections with every request's adapter
 attention that reads shared prefixes once, and the output projection with its adapters. All of a step goes to one
 stream, or is replayed from a graph; afterwards each call's results are checked in float64 on what it was given."""
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -79,9 +80,11 @@ class Step:
                               device="cuda")
         torch.cuda.synchronize()
 
-    def enqueue(self, h):
+    def enqueue(self, h, mine=True):
+        """mine: with scratch of the step's own, else the library's."""
         p = lambda t: t.data_ptr()  # noqa: E731
-        own = dict(scratch_ptr=p(self.sd), scratch_bytes=self.sd.numel(), stream=h)
+        own = dict(scratch_ptr=p(self.sd), scratch_bytes=self.sd.numel(), stream=h) if mine else dict(stream=h)
+        att = dict(scratch_ptr=p(self.sa), scratch_bytes=self.sa.numel(), stream=h) if mine else dict(stream=h)
         self.kv.resize_dev(self.tables, p(self.to), p(self.ok), stream=h)
         self.kv.slots_dev(self.batch, p(self.slots), p(self.pos), stream=h)
         for i in range(3):
@@ -92,7 +95,7 @@ class Step:
                             k_out_ptr=p(self.k), stream=h)
         self.kv.write_dev(0, p(self.k), p(self.y[2]), p(self.slots), MOST, stream=h)
         self.kv.attention_shared_dev(0, self.batch, self.groups, p(self.q), p(self.att), HEADS, 1 / math.sqrt(HD),
-                                     scratch_ptr=p(self.sa), scratch_bytes=self.sa.numel(), stream=h)
+                                     **att)
         self.blobs[3].matvec_dev(p(self.att), p(self.base[3]), MOST, stream=h)
         apply_dev(self.sets[3:], self.ab, p(self.att), [p(self.y[3])], base_ptrs=[p(self.base[3])], **own)
 
@@ -207,3 +210,35 @@ def test_steps(typ, graph):
     new = [1] * 30 + [0] * 10 + [3] * 20 + [1] + [0] * 9
     new[7] = new[59] = 0
     step(new, [0, 15, 30, 60], [99, 100, 0])
+
+
+def test_threads():
+    """Steps of several batches at once, each from a host thread and on a stream of its own, in the library's scratch."""
+    steps = [Step("f16", seed) for seed in (5, 6, 7)]
+    new = [1] * 40 + [0] * 10 + [2] * 20
+    for s in steps:
+        s.inputs([100] + [0] * 39 + [60] + [0] * 29, [0] * SEQS, [0] * 4, [0] * 3)
+        s.enqueue(None)
+        wv.sync()
+        s.check()
+        s.fork([0 if b < 40 else 40 for b in range(SEQS)])
+        s.inputs(new, [(b % 4) - 1 for b in range(SEQS)], [0, 40, 70, 70], [100, 60, 0])
+    failed = []
+
+    def run(s):
+        try:
+            st = torch.cuda.Stream()
+            for _ in range(20):  # the same call, so the same results; the lengths are there after the first
+                s.enqueue(st.cuda_stream, False)
+            st.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(s,)) for s in steps]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for s in steps:
+        s.check()
