@@ -142,6 +142,50 @@ def test_short_sequences(n, seqs, cols, hint):
 
 
 @pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("seqs,sets,cols,ranks,most", [
+    (256, [300], 1500, [64, 40, 64], 1), (1000, [200, 33], 260, [16], 1), (1024, [70, 160, 40], 200, [16, 3, 0, 9], 2),
+    (257, [1030], 700, [80] * 60, 4), (300, [96, 64], 1000, [48, 20, 33, 5, 1], 3),
+])
+def test_many_requests(seqs, sets, cols, ranks, most, typ):
+    """Requests enough that those with one adapter are taken together: scattered, of no rows, without an adapter, of more
+    rows than one tile, of more than the call is told of."""
+    rng = np.random.default_rng(seqs)
+    new = [0 if b % 11 == 5 else 1 + b % most for b in range(seqs)]
+    which = list(rng.integers(-1, len(ranks) + 1, seqs))
+    which[3:3 + seqs // 3] = [0] * (seqs // 3)
+    if most > 2:
+        new[7], new[-1] = 45, 90
+    c = Case(rng, sets, cols, ranks, new, which, typ, pad=3)
+    c.batch = AdapterBatch(seqs, c.t, c.cu.data_ptr(), c.ids.data_ptr(), most)
+    got = c.run()
+    c.check(got)
+    assert all(np.array_equal(a, b) for a, b in zip(got, c.run()))
+    c.check(c.run(True), True)
+
+
+def test_many_requests_of_unlike_sets():
+    """Sets of one call with more or fewer adapters than the requests name, at strides of their own."""
+    rng = np.random.default_rng(12)
+    which = [b % 40 for b in range(400)]
+    a = Case(rng, [290], 500, [32] * 3, [1] * 400, which)
+    b = Case(rng, [110], 500, [48] * 37, [1] * 400, which)
+    x, base = dev(np.pad(a.x, ((0, 0), (0, 7)))), dev(rng.standard_normal((400, 600)).astype(np.float32))
+    y = torch.full((400, 500), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    c = AdapterBatch(400, 400, a.cu.data_ptr(), a.ids.data_ptr(), 1)
+    apply_dev([a.sets[0], b.sets[0]], c, x.data_ptr(), [y.data_ptr(), y.data_ptr() + 4 * 301],
+              base_ptrs=[base.data_ptr(), base.data_ptr() + 4 * 450], x_stride=507, y_strides=[500, 500],
+              base_strides=[600, 600])
+    wv.sync()
+    h, got = base.cpu().numpy(), y.cpu().numpy()
+    a.base, b.base, b.x = [h[:, :290]], [h[:, 450:560]], a.x
+    for case, part in ((a, got[:, :290]), (b, got[:, 301:411])):
+        want, tol = case.want(0)
+        assert (np.abs(part - want) <= tol).all()
+    assert (got[:, 290:301] == 7).all() and (got[:, 411:] == 7).all()
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
 @pytest.mark.parametrize("new", [[10], [100] * 4, [300] * 4, [10, 2, 1, 4]])
 def test_many_ranks(new, typ):
     """The sets' ranks by one block after another, by blocks of their own, or both."""

@@ -33,6 +33,9 @@ constexpr int kTile = 32;        // token rows of a block
 constexpr int kFew = 4;
 constexpr int kChunk = 512;      // columns that a wave takes at a time of such a row, 8 to a lane
 constexpr int kMaxRanges = 32;   // of the columns
+// How a call's rows are taken: FEW rows of a sequence at a time, tiles of a sequence, or tiles of an adapter.
+constexpr int kTiles = 0, kGrouped = -1;
+constexpr int kGroupIds = 256, kGroupSeqs = 1024;  // adapters and sequences of a grouped call, at most
 
 struct Known {
     int32_t rank;
@@ -84,6 +87,7 @@ struct Args {
     int64_t xs;
     int cols, n_seqs, n_tokens, ranges, range;  // range: columns of one, a multiple of kChunk
     int n_sets, ranks;                           // ranks: R of all sets
+    int ids;                                     // adapters of the set that has most
 };
 
 template <int TYPE>
@@ -95,18 +99,34 @@ __device__ __forceinline__ float high(uint32_t w) {
     return TYPE == WV_ADAPTER_BF16 ? __uint_as_float(w & 0xffff0000) : float(__builtin_bit_cast(_Float16, uint16_t(w >> 16)));
 }
 
-// Token rows of one sequence, 32 at most.
+// Token rows of one sequence, 32 at most, from t0 on, or of one adapter, as listed.
 struct Tile {
     int t0, n, id;  // its adapter
+    const int* list = nullptr;
+    __device__ __forceinline__ int row(int i) const { return list ? list[i] : t0 + i; }
+    __device__ __forceinline__ int from_first(int i) const { return list ? list[i] : i; }
 };
+// The rows of sequence s.
+__device__ __forceinline__ int rows_of(const Args& a, int s, int& first) {
+    first = min(max(a.cu[s], 0), a.n_tokens);
+    return min(max(a.cu[s + 1], first), a.n_tokens) - first;
+}
+// Sum over this lane and those before it.
+__device__ __forceinline__ int sum_so_far(int x) {
+    x += dpp_i<kDppRowShr1>(0, x);
+    x += dpp_i<kDppRowShr2>(0, x);
+    x += dpp_i<kDppRowShr4, 0xf, 0xe>(0, x);
+    x += dpp_i<kDppRowShr8, 0xf, 0xc>(0, x);
+    x += dpp_i<kDppRowBcast15, 0xa>(0, x);
+    return x + dpp_i<kDppRowBcast31, 0xc>(0, x);
+}
 // Tile `idx`: the first one of sequence idx, then all further ones in order of the sequences, found 64 sequences at a
 // time. False: there is none. FEW: a sequence is one tile, whatever its length.
 template <bool FEW>
 __device__ __forceinline__ bool find_tile(const Args& a, int idx, Tile& t) {
     if (FEW || idx < a.n_seqs) {
         t.id = a.which[idx];
-        t.t0 = min(max(a.cu[idx], 0), a.n_tokens);
-        t.n = min(max(a.cu[idx + 1], t.t0), a.n_tokens) - t.t0;
+        t.n = rows_of(a, idx, t.t0);
         if (!FEW) t.n = min(t.n, kTile);
         return t.n > 0;
     }
@@ -115,17 +135,8 @@ __device__ __forceinline__ bool find_tile(const Args& a, int idx, Tile& t) {
     for (int base = 0; base < a.n_seqs; base += 64) {
         const int s = base + lane;
         int c0 = 0, n = 0;
-        if (s < a.n_seqs) {
-            c0 = min(max(a.cu[s], 0), a.n_tokens);
-            n = min(max(a.cu[s + 1], c0), a.n_tokens) - c0;
-        }
-        const int tiles = max((n + kTile - 1) / kTile - 1, 0);
-        int incl = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(incl, d, 64);
-            if (lane >= d) incl += o;
-        }
+        if (s < a.n_seqs) n = rows_of(a, s, c0);
+        const int tiles = max((n + kTile - 1) / kTile - 1, 0), incl = sum_so_far(tiles);
         const int total = __builtin_amdgcn_readlane(incl, 63);
         if (idx < total) {
             const int w = __builtin_ctzll(__ballot(incl > idx));
@@ -138,6 +149,58 @@ __device__ __forceinline__ bool find_tile(const Args& a, int idx, Tile& t) {
         idx -= total;
     }
     return false;
+}
+
+// Tile `idx` of the rows in order of their adapters (those without one last): every block counts the adapters' rows,
+// finds its 32 of them and lists them in their order, so that blocks agree. 256 sequences at a time, a thread each.
+__device__ __forceinline__ bool find_group(const Args& a, int idx, Tile& t) {
+    __shared__ int count[kGroupIds + 1], list[kTile], sums[kGroupSeqs / 64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    int key = -1, c0 = 0, n = 0;
+    auto load = [&](int s) {
+        n = 0;
+        if (s < a.n_seqs) n = rows_of(a, s, c0), key = int(min(unsigned(a.which[s]), unsigned(a.ids)));
+    };
+    for (int i = tid; i <= a.ids; i += 256) count[i] = 0;
+    __syncthreads();
+    for (int base = 0; base < a.n_seqs; base += 256) {
+        load(base + tid);
+        if (n) atomicAdd(&count[key], n);
+    }
+    __syncthreads();
+    int id = -1, skip = 0;
+    for (int base = 0; base <= a.ids && id < 0; base += 64) {
+        const int tiles = base + lane <= a.ids ? (count[base + lane] + kTile - 1) / kTile : 0, incl = sum_so_far(tiles);
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        if (idx < total) {
+            const int w = __builtin_ctzll(__ballot(incl > idx));
+            id = base + w;
+            skip = kTile * (idx - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(tiles, w)));
+        }
+        idx -= total;
+    }
+    if (id < 0) return false;
+    int before = 0;
+    for (int base = 0; base < a.n_seqs; base += 256) {
+        if (a.n_seqs > 256) load(base + tid);
+        const int rows = key == id ? n : 0, incl = sum_so_far(rows);
+        int* l = sums + base / 64;
+        if (lane == 63) l[tid >> 6] = incl;
+        __syncthreads();
+        int first = before + incl - rows - skip;  // its rows' places in the list
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w < tid >> 6) first += l[w];
+            before += l[w];
+        }
+        for (int i = max(-first, 0); i < rows && first + i < kTile; ++i) list[first + i] = c0 + i;
+    }
+    __syncthreads();
+    t.t0 = 0;
+    t.n = min(count[id] - skip, kTile);
+    t.id = id < a.ids ? id : -1;
+    t.list = list;
+    return true;
 }
 
 // What this wave's lanes wrote to LDS is there for its other lanes.
@@ -317,7 +380,8 @@ __device__ __forceinline__ void down_tile(const Args& a, const Tile& t, int rang
     constexpr int LD = 32 * NR + 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hi = lane >> 5;
-    const float* x = a.x + int64_t(t.t0 + min(n, t.n - 1)) * a.xs;
+    const int row_n = t.row(min(n, t.n - 1));
+    const float* x = a.x + int64_t(row_n) * a.xs;
     // rank r of all sets: its set, and the rank there
     auto set_of = [&](int& r) {
         int i = 0;
@@ -433,29 +497,29 @@ __device__ __forceinline__ void down_tile(const Args& a, const Tile& t, int rang
                 int r = r0 + 32 * k + 8 * q + 4 * hi;
                 if (r >= a.ranks) continue;
                 const SetArgs& s = a.set[set_of(r)];  // the ranks of a set are a multiple of 16
-                *reinterpret_cast<f4*>(s.h + (int64_t(range) * a.n_tokens + t.t0 + n) * s.R + r) =
+                *reinterpret_cast<f4*>(s.h + (int64_t(range) * a.n_tokens + row_n) * s.R + r) =
                     f4{acc[k][4 * q], acc[k][4 * q + 1], acc[k][4 * q + 2], acc[k][4 * q + 3]};
             }
     }
 }
 
-// FEW (1, kFew; 0: not so): the caller says that no sequence has more rows (if one has, they go FEW at a time). Without,
+// FEW (1, kFew; kTiles and kGrouped: not so): the caller says that no sequence has more rows (if one has, they go FEW at a time). Without,
 // the rows of a short one go singly: four at a time take registers that tiles want (18.5 us for 2000 rows of rank 64 over
 // 4096 columns, else 19.6).
 template <int TYPE, int NR, int FEW>
 __global__ void __launch_bounds__(256) k_adapt_down(Args a, int tile0) {
-    __shared__ float lds[FEW ? 1 : 2 * 32 * (32 * NR + 4)];
+    __shared__ float lds[FEW > 0 ? 1 : 2 * 32 * (32 * NR + 4)];
     Tile t;
-    if (!find_tile<(FEW > 0)>(a, tile0 + int(blockIdx.y), t)) return;
-    const int range = FEW ? blockIdx.x % a.ranges : blockIdx.x, c0 = range * a.range;
+    if (!(FEW == kGrouped ? find_group(a, tile0 + int(blockIdx.y), t) : find_tile<(FEW > 0)>(a, tile0 + int(blockIdx.y), t))) return;
+    const int range = FEW > 0 ? blockIdx.x % a.ranges : blockIdx.x, c0 = range * a.range;
     auto few = [&](const SetArgs& s) {
         if (unsigned(t.id) < unsigned(s.n_adapters))
-            down_few<TYPE, FEW ? FEW : 1>(a, s, t, t.id, c0, min(c0 + a.range, a.cols),
+            down_few<TYPE, (FEW > 0 ? FEW : 1)>(a, s, t, t.id, c0, min(c0 + a.range, a.cols),
                                           s.h + (int64_t(range) * a.n_tokens + t.t0) * s.R);
     };
-    if constexpr (FEW) {
+    if constexpr (FEW > 0) {
         few(a.set[blockIdx.x / a.ranges]);
-    } else if (t.n <= kFew) {
+    } else if (FEW == kTiles && t.n <= kFew) {
         for (int i = blockIdx.z; i < a.n_sets; i += gridDim.z) few(a.set[i]);
     } else if (t.id >= 0) {
         down_tile<TYPE, NR>(a, t, range, c0, min(c0 + a.range, a.set[0].C), lds);
@@ -558,7 +622,7 @@ __device__ __forceinline__ void stage_operands(const Args& a, const SetArgs& s, 
         const int i = threadIdx.x + 256 * j, n = i / (8 * NR), r = 4 * (i % (8 * NR));
         x[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         if (r < s.R && n < t.n) {
-            const float* p = s.h + (int64_t(t.t0) + n) * s.R + r;
+            const float* p = s.h + int64_t(t.row(n)) * s.R + r;
             int k = 0;
             for (; k + 4 <= a.ranges; k += 4) {
                 f4 y[4];
@@ -620,7 +684,8 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int r = min(8 * q + m, t.n - 1);
-        rb[q] = r * s.bs + o4, ry[q] = r * s.ys + o4, rs[q] = r * kSwap + o4;
+        const int64_t at = t.from_first(r);
+        rb[q] = at * s.bs + o4, ry[q] = at * s.ys + o4, rs[q] = r * kSwap + o4;
     }
     uint4 w[2 * NR];
     f4 was[4];
@@ -681,77 +746,97 @@ __device__ __forceinline__ void up_tile(const Args& a, const SetArgs& s, const T
     outputs(acc);
     turn(acc);
     for (int i = lane; i < 32 * t.n; i += 64)
-        if (const int r = i >> 5, o = o0 + (i & 31); o < last) y[r * s.ys + o] = base[r * s.bs + o] + swap[r * kSwap + (i & 31)];
+        if (const int r = i >> 5, o = o0 + (i & 31); o < last) {
+            const int64_t at = t.from_first(r);
+            y[at * s.ys + o] = base[at * s.bs + o] + swap[r * kSwap + (i & 31)];
+        }
 }
 
 // Rows without an adapter: a wave a row, eight of them on their way.
-__device__ __forceinline__ void copy_rows(const SetArgs& s, int rows, int first, int last, const float* base, float* y) {
+__device__ __forceinline__ void copy_rows(const SetArgs& s, const Tile& t, int first, int last, const float* base, float* y) {
     const int wave = threadIdx.x >> 6;
     for (int o = first + 4 * int(threadIdx.x & 63); o < last; o += 256) {
         if (o + 4 > last) {
-            for (int n = wave; n < rows; n += 4)
-                for (int i = o; i < last; ++i) y[n * s.ys + i] = base[n * s.bs + i];
+            for (int n = wave; n < t.n; n += 4)
+                for (int i = o; i < last; ++i) y[t.from_first(n) * s.ys + i] = base[t.from_first(n) * s.bs + i];
             continue;
         }
         f4 x[kTile / 4];
 #pragma unroll
         for (int i = 0; i < kTile / 4; ++i)
-            if (wave + 4 * i < rows) x[i] = *reinterpret_cast<const f4*>(base + (wave + 4 * i) * s.bs + o);
+            if (const int n = wave + 4 * i; n < t.n) x[i] = *reinterpret_cast<const f4*>(base + t.from_first(n) * s.bs + o);
 #pragma unroll
         for (int i = 0; i < kTile / 4; ++i)
-            if (wave + 4 * i < rows) *reinterpret_cast<f4*>(y + (wave + 4 * i) * s.ys + o) = x[i];
+            if (const int n = wave + 4 * i; n < t.n) *reinterpret_cast<f4*>(y + t.from_first(n) * s.ys + o) = x[i];
     }
 }
 
 struct Nothing {};
 template <int TYPE, int NR, int FEW>
 __global__ void __launch_bounds__(256) k_adapt_up(Args a, int tile0, int turns) {
-    __shared__ __align__(16) float h[(FEW ? FEW : kFew) * (32 * NR + 4)];
+    __shared__ __align__(16) float h[(FEW > 0 ? FEW : kFew) * (32 * NR + 4)];
     __shared__ std::conditional_t<(FEW > 0), Nothing, UpLds<TYPE, NR>> lds;
     int set = 0;
     while (set + 1 < kMaxSets && int(blockIdx.x) >= a.set[set + 1].block0) ++set;
     const SetArgs& s = a.set[set];
     const int first = (int(blockIdx.x) - s.block0) * 256 * turns;
     Tile t;
-    if (!find_tile<(FEW > 0)>(a, tile0 + int(blockIdx.y), t)) return;
+    if (!(FEW == kGrouped ? find_group(a, tile0 + int(blockIdx.y), t) : find_tile<(FEW > 0)>(a, tile0 + int(blockIdx.y), t))) return;
     const int id = t.id;
     const int last = min(first + 256 * turns, s.rows);
     const float* base = s.base + t.t0 * s.bs;
     float* y = s.y + t.t0 * s.ys;
     const bool known = unsigned(id) < unsigned(s.n_adapters);
-    if (known && (FEW || t.n <= kFew)) {
-        up_few<TYPE, NR, FEW ? FEW : kFew>(a, s, t, id, first, last, base, y, h);
-        return;
+    if constexpr (FEW != kGrouped) {
+        if (known && (FEW > 0 || t.n <= kFew)) {
+            up_few<TYPE, NR, (FEW > 0 ? FEW : kFew)>(a, s, t, id, first, last, base, y, h);
+            return;
+        }
     }
-    if constexpr (!FEW) {
+    if constexpr (FEW <= 0) {
         if (const int rank = known ? s.known[id].rank : 0; rank) {
             up_tile<TYPE, NR>(a, s, t, id, rank, first, last, base, y, lds);
             return;
         }
     }
     if (base == y) return;
-    if constexpr (FEW) {
+    if constexpr (FEW > 0) {
         for (int n = 0; n < t.n; ++n)
             for (int o = first + int(threadIdx.x); o < last; o += 256) y[n * s.ys + o] = base[n * s.bs + o];
     } else {
-        copy_rows(s, t.n, first, last, base, y);
+        copy_rows(s, t, first, last, base, y);
     }
 }
 
-// Tiles of a call, at most.
-int64_t adapt_tiles(int n_seqs, int n_tokens) { return int64_t(n_seqs) + n_tokens / kTile; }
-
-// Whether the kernels of short sequences take a call: how many rows at a time, or 0.
-int adapt_few(const wv_adapter_batch& b) {
-    const int most = b.max_q ? b.max_q : b.n_tokens;
-    return most <= 1 ? 1 : most <= kFew ? kFew : 0;
+int most_ids(const Set* s, int n_sets) {
+    int n = 0;
+    for (int i = 0; i < n_sets; ++i) n = std::max(n, s[i].c.n_adapters);
+    return n;
+}
+// How a call's rows are taken. Short sequences' by adapter where that saves more of A's and B's traffic than finding
+// them costs, some 4 us a call: the more, the more sequences there are (by sequence / by adapter, 8 adapters, rank 64 on
+// 4096 x 4096: 64 sequences 9.7 / 11.9 us, 128 13.1 / 12.7, 256 21.5 / 16.7, 600 45 / 29; rank 16: 256 12.6 / 12.4; rank
+// 128 on 4096 x 14336: 64 28 / 26, 256 74 / 36), and not where an adapter has fewer than four (256 sequences: 32 adapters
+// 25 / 24, 64 32 / 36, three sets 63 / 50; of 128, two sets of rank 128, as many adapters 106 / 158).
+int adapt_mode(const Set* s, int n_sets, const wv_adapter_batch& b) {
+    const int most = b.max_q ? b.max_q : b.n_tokens, ids = most_ids(s, n_sets);
+    if (most > kFew) return kTiles;
+    double bytes = 0.0;
+    for (int i = 0; i < n_sets; ++i) bytes += 2.0 * s[i].R * (double(s[i].C) + s[i].O);
+    const double n = std::min(b.n_seqs, b.n_tokens);
+    if (ids <= kGroupIds && b.n_seqs <= kGroupSeqs && b.n_tokens >= 4 * ids && n * n * bytes >= 15e9) return kGrouped;
+    return most <= 1 ? 1 : kFew;
+}
+int64_t adapt_tiles(const wv_adapter_batch& b, int mode, int ids) {  // at most
+    if (mode > 0) return b.n_seqs;
+    return (mode == kGrouped ? std::min(b.n_seqs, ids + 1) : b.n_seqs) + b.n_tokens / kTile;
 }
 
 // Into how many ranges the columns are cut: about eight blocks a CU (two: 11.5 us for 64 rows of three sets of rank 32,
 // four or more 11.0), and ranges of whole chunks (of 128 columns, 32 ranges: 8 rows over 4096 columns 9.5 us, else 8.7).
-int adapt_ranges(int cols, const wv_adapter_batch& b, int n_sets, int& range) {
-    const int chunks = (cols + kChunk - 1) / kChunk;
-    const int64_t blocks = adapt_few(b) ? int64_t(std::min(b.n_seqs, b.n_tokens)) * n_sets : adapt_tiles(b.n_seqs, b.n_tokens);
+int adapt_ranges(const Set* s, int n_sets, const wv_adapter_batch& b, int& range) {
+    const int chunks = (s[0].c.cols + kChunk - 1) / kChunk, mode = adapt_mode(s, n_sets, b);
+    const int64_t blocks = mode > 0 ? int64_t(std::min(b.n_seqs, b.n_tokens)) * n_sets : adapt_tiles(b, mode, most_ids(s, n_sets));
     const int want = int(std::max<int64_t>(1, std::min<int64_t>({2048 / std::max<int64_t>(blocks, 1), chunks, kMaxRanges})));
     const int each = (chunks + want - 1) / want;
     range = each * kChunk;
@@ -759,8 +844,7 @@ int adapt_ranges(int cols, const wv_adapter_batch& b, int n_sets, int& range) {
 }
 
 template <int TYPE>
-int launch_adapters(Args& a, int few, hipStream_t s) {
-    const int64_t tiles = few ? a.n_seqs : adapt_tiles(a.n_seqs, a.n_tokens);
+int launch_adapters(Args& a, int mode, int64_t tiles, hipStream_t s) {
     int64_t units = 0, blocks = 0;
     int R = 0;
     for (int i = 0; i < a.n_sets; ++i) units += (a.set[i].rows + 255) / 256, R = std::max(R, a.set[i].R);
@@ -779,16 +863,17 @@ int launch_adapters(Args& a, int few, hipStream_t s) {
     };
     auto up = [&](auto nr) {
         constexpr int NR = decltype(nr)::value;
-        few == 1 ? go(k_adapt_up<TYPE, NR, 1>, blocks, 1, turns)
-        : few    ? go(k_adapt_up<TYPE, NR, kFew>, blocks, 1, turns)
-                 : go(k_adapt_up<TYPE, NR, 0>, blocks, 1, turns);
+        mode == 1          ? go(k_adapt_up<TYPE, NR, 1>, blocks, 1, turns)
+        : mode == kFew     ? go(k_adapt_up<TYPE, NR, kFew>, blocks, 1, turns)
+        : mode == kGrouped ? go(k_adapt_up<TYPE, NR, kGrouped>, blocks, 1, turns)
+                           : go(k_adapt_up<TYPE, NR, kTiles>, blocks, 1, turns);
     };
     std::integral_constant<int, 1> n1;
     std::integral_constant<int, 2> n2;
     std::integral_constant<int, 4> n4;
     std::integral_constant<int, 8> n8;
-    if (few) {
-        go(few == 1 ? k_adapt_down<TYPE, 1, 1> : k_adapt_down<TYPE, 1, kFew>, int64_t(a.ranges) * a.n_sets, 1);
+    if (mode > 0) {
+        go(mode == 1 ? k_adapt_down<TYPE, 1, 1> : k_adapt_down<TYPE, 1, kFew>, int64_t(a.ranges) * a.n_sets, 1);
     } else {
         // Ranks of a block, 32 nr: all of them, as the terms of x are split once for them, unless a block a CU takes them
         // in parts (all / in parts: 3 sets of rank 32 over 4096 columns, 8 sequences of 8 tokens, 14.3 / 9.9 us with the
@@ -796,12 +881,11 @@ int launch_adapters(Args& a, int few, hipStream_t s) {
         // 1536 blocks, 23.3 / 25.0).
         auto parts = [&](int nr) { return (a.ranks + 32 * nr - 1) / (32 * nr); };
         auto fits = [&](int nr) { return parts(nr) == 1 || a.ranges * tiles * parts(nr) <= 256; };
-        if (fits(1))
-            go(k_adapt_down<TYPE, 1, 0>, a.ranges, parts(1));
-        else if (fits(2))
-            go(k_adapt_down<TYPE, 2, 0>, a.ranges, parts(2));
-        else  // more than 128 at a time would take all of a SIMD's registers for one wave
-            go(k_adapt_down<TYPE, 4, 0>, a.ranges, parts(4));
+        auto down = [&](auto nr) {
+            constexpr int NR = decltype(nr)::value;
+            go(mode == kGrouped ? k_adapt_down<TYPE, NR, kGrouped> : k_adapt_down<TYPE, NR, kTiles>, a.ranges, parts(NR));
+        };
+        fits(1) ? down(n1) : fits(2) ? down(n2) : down(n4);  // more than 128 would take all of a SIMD's registers for one wave
     }
     R <= 32 ? up(n1) : R <= 64 ? up(n2) : R <= 128 ? up(n4) : up(n8);
     return int(hipGetLastError());
@@ -940,7 +1024,7 @@ int wv_adapters_scratch(const wv_adapter_batch* batch, const wv_adapter_rows* se
     if (rc) return rc;
     if (!bytes) return rt_fail(WV_E_ARG, "wv_adapters_scratch: nil bytes");
     int range;
-    *bytes = scratch_floats(s, n_sets, batch->n_tokens, adapt_ranges(s[0].c.cols, *batch, n_sets, range)) * 4;
+    *bytes = scratch_floats(s, n_sets, batch->n_tokens, adapt_ranges(s, n_sets, *batch, range)) * 4;
     return WV_OK;
 }
 
@@ -978,7 +1062,8 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
     a.n_sets = n_sets;
     for (int i = 0; i < n_sets; ++i) a.ranks += s[i].R;
     a.x = d_x, a.xs = x_stride, a.cu = batch->d_cu_q, a.which = batch->d_adapter;
-    a.ranges = adapt_ranges(a.cols, *batch, n_sets, a.range);
+    a.ids = most_ids(s, n_sets);
+    a.ranges = adapt_ranges(s, n_sets, *batch, a.range);
     (void)hipSetDevice(s[0].device);
     hipStream_t st = rt_stream(stream, s[0].device);
     const size_t floats = scratch_floats(s, n_sets, a.n_tokens, a.ranges);
@@ -998,9 +1083,10 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
         a.set[i].h = h;
         h += size_t(a.ranges) * size_t(a.n_tokens) * size_t(a.set[i].R);
     }
-    const int few = adapt_few(*batch);
-    const int e = s[0].c.type == WV_ADAPTER_BF16 ? launch_adapters<WV_ADAPTER_BF16>(a, few, st)
-                                                 : launch_adapters<WV_ADAPTER_F16>(a, few, st);
+    const int mode = adapt_mode(s, n_sets, *batch);
+    const int64_t tiles = adapt_tiles(*batch, mode, a.ids);
+    const int e = s[0].c.type == WV_ADAPTER_BF16 ? launch_adapters<WV_ADAPTER_BF16>(a, mode, tiles, st)
+                                                 : launch_adapters<WV_ADAPTER_F16>(a, mode, tiles, st);
     return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_adapters: kernel launch");
 }
 
