@@ -474,7 +474,8 @@ int wv_kv_fork_dev(uint64_t cache, const wv_kv_tables *tables, const int32_t *d_
  *   keeps it), and the new pages.
  * The first sequence that does not find enough, and all growing ones behind it,
  * stay as they are, as does one that the table has no room for: d_ok[b] is 0
- * there, else 1. */
+ * there, else 1 (wv_kv_slots_served_dev keeps such a sequence's new rows from
+ * being written). */
 int wv_kv_resize_dev(uint64_t cache, const wv_kv_tables *tables, const int32_t *d_len, int32_t *d_ok, void *stream);
 
 /* Moves pages so that the U pages that are held come first in the pool: the
@@ -506,8 +507,16 @@ typedef struct wv_kv_batch {
 /* Slot and position of every row of a batch (whose kv_len counts its new
  * tokens), as wv_kv_write_dev and wv_rope_dev take them: d_slots[t] and d_pos[t]
  * (may be NULL), n_tokens each. Padding rows get slot -1 and position 0, rows
- * whose page is outside the pool or past the table slot -1. */
+ * whose page is outside the pool or past the table slot -1. Every sequence has
+ * to hold its new positions: the rows of one that wv_kv_resize_dev refused
+ * would get slots of positions that it has, and maybe shares, already. */
 int wv_kv_slots_dev(uint64_t cache, const wv_kv_batch *batch, int64_t *d_slots, int32_t *d_pos, void *stream);
+/* The same after a resize that may have refused some: d_ok[b], as it wrote it,
+ * is 0 for a sequence whose rows all get slot -1 and position 0, as padding
+ * does. Nothing is written for them then and what the sequence holds stays;
+ * what attention makes of them is of no use. */
+int wv_kv_slots_served_dev(uint64_t cache, const wv_kv_batch *batch, const int32_t *d_ok, int64_t *d_slots,
+                           int32_t *d_pos, void *stream);
 
 /* Causal grouped-query attention of a batch's new tokens over the cache
  * (layers/mha/attn.go:40-118 with its causal and sliding-window masks). Token

@@ -47,7 +47,7 @@ EXPORTS = (
     "wv_decoder_use_graph", "wv_decoder_generate", "wv_decoder_prefill", "wv_decoder_free",
     "wv_kv_create", "wv_kv_info", "wv_kv_free", "wv_kv_write_dev", "wv_kv_read_dev", "wv_kv_attention_dev",
     "wv_kv_attention_scratch", "wv_kv_attention_shared_dev", "wv_kv_attention_shared_scratch", "wv_kv_tables_work", "wv_kv_fork_dev", "wv_kv_resize_dev", "wv_kv_compact_dev",
-    "wv_kv_copy_pages_dev", "wv_kv_slots_dev", "wv_rope_create", "wv_rope_free", "wv_rope_dev",
+    "wv_kv_copy_pages_dev", "wv_kv_slots_dev", "wv_kv_slots_served_dev", "wv_rope_create", "wv_rope_free", "wv_rope_dev",
     "wv_adapters_create", "wv_adapters_set", "wv_adapters_free", "wv_adapters_dev", "wv_adapters_scratch",
     "wv_sample_dev",
     "wv_decoder_generate_sampled", "wv_decoder_forward_paged",
@@ -133,6 +133,7 @@ def lib():
     L.wv_kv_compact_dev.argtypes = [ctypes.c_uint64, _P, _P, _P]
     L.wv_kv_copy_pages_dev.argtypes = [ctypes.c_uint64, _P, _P, ctypes.c_int32, _P]
     L.wv_kv_slots_dev.argtypes = [ctypes.c_uint64, _P, _P, _P, _P]
+    L.wv_kv_slots_served_dev.argtypes = [ctypes.c_uint64, _P, _P, _P, _P, _P]
     L.wv_rope_create.argtypes = [_P, _P]
     L.wv_rope_free.argtypes = [ctypes.c_uint64]
     L.wv_rope_dev.argtypes = [ctypes.c_uint64, _P, ctypes.c_int32, _P, _P, _P]

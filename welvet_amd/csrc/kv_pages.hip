@@ -348,12 +348,14 @@ __global__ void __launch_bounds__(256) k_pages_remap(Tables t, Work w) {
 }
 
 // Slot and position of every new token of a batch. A block has the sequences'
-// first rows in LDS (of more than 4096 every 2nd, 4th .. of them) and searches there.
+// first rows in LDS (of more than 4096 every 2nd, 4th .. of them) and searches there. ok (may be null): a sequence
+// with a 0 was refused its new positions. Its rows would fall on the last ones that it holds, and maybe others too.
 constexpr int kSlotSeqs = 4096;
 __global__ void __launch_bounds__(256) k_kv_slots(const int32_t* __restrict__ cu, const int32_t* __restrict__ kv_len,
                                                   const int32_t* __restrict__ pages, int n_seqs, int n_tokens,
                                                   int max_pages, int page_shift, int n_pages, int step,
-                                                  int64_t* __restrict__ slots, int32_t* __restrict__ pos) {
+                                                  const int32_t* __restrict__ ok, int64_t* __restrict__ slots,
+                                                  int32_t* __restrict__ pos) {
     __shared__ int32_t first[kSlotSeqs];
     const int t = blockIdx.x * 256 + threadIdx.x, n = (n_seqs + (1 << step) - 1) >> step;
     for (int i = threadIdx.x; i < n; i += 256) first[i] = cu[i << step];
@@ -380,7 +382,7 @@ __global__ void __launch_bounds__(256) k_kv_slots(const int32_t* __restrict__ cu
     int p = 0;
     if (b >= 0) {
         const int end = min(cu[b + 1], n_tokens);
-        if (t < end) {
+        if (t < end && (!ok || ok[b])) {
             const int64_t q = int64_t(max(kv_len[b], 0)) - end + t;
             p = int(q);
             if (q >= 0 && q >> page_shift < max_pages) {
@@ -424,6 +426,31 @@ int check_tables(const char* what, uint64_t cache, const wv_kv_tables* t, KvCach
     k = {t->d_pages, t->d_kv_len, t->d_refs, t->n_seqs, t->max_pages, c.c.n_pages, c.layer(0).page_shift};
     w = work_of(t->d_work, t->n_seqs, c.c.n_pages);
     return WV_OK;
+}
+
+// wv_kv_slots_dev, and with ok wv_kv_slots_served_dev.
+int slots_of(const char* what, uint64_t cache, const wv_kv_batch* batch, const int32_t* ok, int64_t* d_slots,
+             int32_t* d_pos, void* stream) {
+    KvCache c;
+    if (!kv_lookup(cache, c)) return rt_fail(WV_E_HANDLE, "%s: unknown cache %llu", what, (unsigned long long)cache);
+    if (!batch) return rt_fail(WV_E_ARG, "%s: nil batch", what);
+    const wv_kv_batch& b = *batch;
+    if (b.n_seqs < 0 || b.n_tokens < 0 || b.max_pages < 0 || b.n_tokens > 1 << 28 || b.n_seqs > 1 << 24)
+        return rt_fail(WV_E_SHAPE, "%s: %d sequences, %d tokens, %d pages", what, b.n_seqs, b.n_tokens, b.max_pages);
+    if (int64_t(b.max_pages) * c.c.page_size >= int64_t(1) << 31)
+        return rt_fail(WV_E_SHAPE, "%s: a table of %d pages of %d positions (2^31 and more)", what, b.max_pages,
+                       c.c.page_size);
+    if (!b.n_tokens) return WV_OK;
+    if (!d_slots || (b.n_seqs && (!b.d_cu_q || !b.d_kv_len || (b.max_pages && !b.d_pages))))
+        return rt_fail(WV_E_ARG, "%s: nil slots/cu_q/kv_len/pages", what);
+    (void)hipSetDevice(c.device);
+    int step = 0;
+    while ((int64_t(b.n_seqs) + (1 << step) - 1) >> step > kSlotSeqs) ++step;
+    hipLaunchKernelGGL(k_kv_slots, dim3(unsigned((b.n_tokens + 255) / 256)), dim3(256), 0, rt_stream(stream, c.device),
+                       b.d_cu_q, b.d_kv_len, b.d_pages, b.n_seqs, b.n_tokens, b.max_pages, c.layer(0).page_shift,
+                       c.c.n_pages, step, ok, d_slots, d_pos);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? WV_OK : rt_hip_fail(e, what);
 }
 
 }  // namespace
@@ -509,26 +536,14 @@ int wv_kv_copy_pages_dev(uint64_t cache, const int32_t* d_src, const int32_t* d_
 }
 
 int wv_kv_slots_dev(uint64_t cache, const wv_kv_batch* batch, int64_t* d_slots, int32_t* d_pos, void* stream) {
-    KvCache c;
-    if (!kv_lookup(cache, c)) return rt_fail(WV_E_HANDLE, "wv_kv_slots: unknown cache %llu", (unsigned long long)cache);
-    if (!batch) return rt_fail(WV_E_ARG, "wv_kv_slots: nil batch");
-    const wv_kv_batch& b = *batch;
-    if (b.n_seqs < 0 || b.n_tokens < 0 || b.max_pages < 0 || b.n_tokens > 1 << 28 || b.n_seqs > 1 << 24)
-        return rt_fail(WV_E_SHAPE, "wv_kv_slots: %d sequences, %d tokens, %d pages", b.n_seqs, b.n_tokens, b.max_pages);
-    if (int64_t(b.max_pages) * c.c.page_size >= int64_t(1) << 31)
-        return rt_fail(WV_E_SHAPE, "wv_kv_slots: a table of %d pages of %d positions (2^31 and more)", b.max_pages,
-                       c.c.page_size);
-    if (!b.n_tokens) return WV_OK;
-    if (!d_slots || (b.n_seqs && (!b.d_cu_q || !b.d_kv_len || (b.max_pages && !b.d_pages))))
-        return rt_fail(WV_E_ARG, "wv_kv_slots: nil slots/cu_q/kv_len/pages");
-    (void)hipSetDevice(c.device);
-    int step = 0;
-    while ((int64_t(b.n_seqs) + (1 << step) - 1) >> step > kSlotSeqs) ++step;
-    hipLaunchKernelGGL(k_kv_slots, dim3(unsigned((b.n_tokens + 255) / 256)), dim3(256), 0, rt_stream(stream, c.device),
-                       b.d_cu_q, b.d_kv_len, b.d_pages, b.n_seqs, b.n_tokens, b.max_pages, c.layer(0).page_shift,
-                       c.c.n_pages, step, d_slots, d_pos);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? WV_OK : rt_hip_fail(e, "wv_kv_slots: kernel launch");
+    return slots_of("wv_kv_slots", cache, batch, nullptr, d_slots, d_pos, stream);
+}
+
+int wv_kv_slots_served_dev(uint64_t cache, const wv_kv_batch* batch, const int32_t* d_ok, int64_t* d_slots,
+                           int32_t* d_pos, void* stream) {
+    if (batch && batch->n_seqs > 0 && batch->n_tokens > 0 && !d_ok)
+        return rt_fail(WV_E_ARG, "wv_kv_slots_served: nil ok");
+    return slots_of("wv_kv_slots_served", cache, batch, d_ok, d_slots, d_pos, stream);
 }
 
 }  // extern "C"

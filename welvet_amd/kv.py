@@ -116,7 +116,8 @@ class KVCache:
 
     def resize_dev(self, tables: KVTables, len_ptr: int, ok_ptr: int, stream: int | None = None) -> None:
         """Sequence b to len[b] positions (int32): pages given back, or the lowest free ones taken and a shared last
-        page copied. ok[b] (int32) is 0 where the pool or the table had no room and b stayed as it was."""
+        page copied. ok[b] (int32) is 0 where the pool or the table had no room and b stayed as it was (slots_dev takes
+        it, so that b's new rows are not written)."""
         check(lib().wv_kv_resize_dev(self.handle, ctypes.byref(tables), len_ptr, ok_ptr, stream))
 
     def compact_dev(self, tables: KVTables, used_ptr: int | None = None, stream: int | None = None) -> None:
@@ -127,9 +128,14 @@ class KVCache:
         """n pages copied in all layers, src to dst (int32)."""
         check(lib().wv_kv_copy_pages_dev(self.handle, src_ptr, dst_ptr, n, stream))
 
-    def slots_dev(self, batch: KVBatch, slots_ptr: int, pos_ptr: int | None = None, stream: int | None = None) -> None:
-        """Slot (int64) and position (int32) of every row of a batch."""
-        check(lib().wv_kv_slots_dev(self.handle, ctypes.byref(batch), slots_ptr, pos_ptr, stream))
+    def slots_dev(self, batch: KVBatch, slots_ptr: int, pos_ptr: int | None = None, stream: int | None = None,
+                  ok_ptr: int | None = None) -> None:
+        """Slot (int64) and position (int32) of every row of a batch. ok (resize_dev's): rows of a sequence that was
+        refused get slot -1 and position 0; without it every sequence has to hold its new positions."""
+        if ok_ptr is None:
+            check(lib().wv_kv_slots_dev(self.handle, ctypes.byref(batch), slots_ptr, pos_ptr, stream))
+        else:
+            check(lib().wv_kv_slots_served_dev(self.handle, ctypes.byref(batch), ok_ptr, slots_ptr, pos_ptr, stream))
 
     def free(self) -> None:
         if self.handle:
