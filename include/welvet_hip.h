@@ -586,7 +586,7 @@ int wv_kv_attention_shared_scratch(uint64_t cache, const wv_kv_batch *batch, con
  *   WV_ROPE_RAMP_DIMS   the same with r falling from 1 to 0 between the pairs
  *                       i0 and i1: r = 1 - (i - i0) / max(i1 - i0, 0.001) within
  *                       [0, 1], i0 the floor of the i at which n_i = high, i1
- *                       the ceiling of that for low, both within 0 .. rot_dim/2 - 1 */
+ *                       the ceiling of that for low, both within 0 .. rot_dim - 1 */
 #define WV_ROPE_HALF 0  /* pair i at (i, i + rot_dim / 2) */
 #define WV_ROPE_PAIRS 1 /* pair i at (2i, 2i + 1) */
 #define WV_ROPE_NONE 0

@@ -170,8 +170,9 @@ std::vector<double> rope_turns(const wv_rope_config& c) {
     double i0 = 0.0, i1 = 0.0;
     if (c.scaling == WV_ROPE_RAMP_DIMS) {
         const auto at = [&](double n) { return c.rot_dim * std::log(c.trained / (two_pi * n)) / (2.0 * std::log(theta)); };
-        i0 = std::fmin(std::fmax(std::floor(at(c.high)), 0.0), half - 1.0);
-        i1 = std::fmin(std::fmax(std::ceil(at(c.low)), 0.0), half - 1.0);
+        // as published the range ends at rot - 1, behind the last pair: of long trained lengths that pair is not all scaled
+        i0 = std::fmin(std::fmax(std::floor(at(c.high)), 0.0), c.rot_dim - 1.0);
+        i1 = std::fmin(std::fmax(std::ceil(at(c.low)), 0.0), c.rot_dim - 1.0);
     }
     for (int i = 0; i < half; ++i) {
         double w = std::pow(theta, -2.0 * i / c.rot_dim);
