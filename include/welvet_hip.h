@@ -602,7 +602,7 @@ typedef struct wv_rope_config {
     double theta;      /* > 1 */
     double factor;     /* every scaling: > 0, that of the context's length */
     double low, high;  /* ramps: turns, 0 < low < high */
-    double gain;       /* > 0; 1: none */
+    double gain;       /* > 0, as f32; 1: none */
 } wv_rope_config;
 int wv_rope_create(const wv_rope_config *cfg, uint64_t *rope);
 /* Releases a rotation once its work is done (waits for the device). */

@@ -205,7 +205,7 @@ int wv_rope_create(const wv_rope_config* cfg, uint64_t* rope) try {
         return rt_fail(WV_E_ARG, "wv_rope_create: layout %d", c.layout);
     if (c.scaling < WV_ROPE_NONE || c.scaling > WV_ROPE_RAMP_TURNS)
         return rt_fail(WV_E_ARG, "wv_rope_create: scaling %d", c.scaling);
-    if (!(c.theta > 1.0) || !std::isfinite(c.theta) || !(c.gain > 0.0) || !std::isfinite(c.gain))
+    if (!(c.theta > 1.0) || !std::isfinite(c.theta) || !(float(c.gain) > 0.0f) || !std::isfinite(float(c.gain)))
         return rt_fail(WV_E_ARG, "wv_rope_create: theta %g, gain %g", c.theta, c.gain);
     if (c.scaling != WV_ROPE_NONE && (!(c.factor > 0.0) || !std::isfinite(c.factor)))
         return rt_fail(WV_E_ARG, "wv_rope_create: factor %g", c.factor);
@@ -216,6 +216,9 @@ int wv_rope_create(const wv_rope_config* cfg, uint64_t* rope) try {
     Rope r;
     r.c = c;
     const std::vector<double> turns = rope_turns(c);
+    // a factor next to 0 has no frequencies, and a gain that f32 does not hold would make NaN of zeros
+    for (const double t : turns)
+        if (!std::isfinite(t)) return rt_fail(WV_E_ARG, "wv_rope_create: frequencies past f64 at factor %g", c.factor);
     int rc = rt_ensure_init();
     if (rc) return rc;
     r.device = rt_current_device();
