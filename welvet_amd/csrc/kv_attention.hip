@@ -1496,11 +1496,11 @@ int check_batch(const char* what, uint64_t cache, const wv_kv_batch* b, int32_t 
     return WV_OK;
 }
 
+// Sizes alone: scratch is sized before there are arrays.
 int check_groups(const char* what, const wv_kv_groups* g) {
     if (!g) return rt_fail(WV_E_ARG, "%s: nil groups", what);
     if (g->n_groups < 0 || g->n_groups > 1 << 24 || g->max_shared < 0)
         return rt_fail(WV_E_SHAPE, "%s: %d groups, max_shared %d", what, g->n_groups, g->max_shared);
-    if (g->n_groups && (!g->d_cu_seq || !g->d_shared)) return rt_fail(WV_E_ARG, "%s: nil cu_seq/shared", what);
     return WV_OK;
 }
 
@@ -1610,6 +1610,8 @@ int wv_kv_attention_shared_dev(uint64_t cache, int32_t layer, const wv_kv_batch*
                                float* d_out, int64_t out_stride, void* d_scratch, size_t scratch_bytes, void* stream) {
     const int rc = check_groups("wv_kv_attention_shared", groups);
     if (rc) return rc;
+    if (groups->n_groups && (!groups->d_cu_seq || !groups->d_shared))
+        return rt_fail(WV_E_ARG, "wv_kv_attention_shared: nil cu_seq/shared");
     return attention("wv_kv_attention_shared", cache, layer, batch, groups, d_q, q_stride, n_heads, scale, window, d_out,
                      out_stride, d_scratch, scratch_bytes, stream);
 }
