@@ -1557,11 +1557,11 @@ int attention(const char* what, uint64_t cache, int32_t layer, const wv_kv_batch
     } else if (floats && rt_capturing(s)) {
         a.splits = 1;  // what a replay writes must not lie in a slot that other calls take
     } else if (floats) {
-        if ((rc = sc.get(floats, s, "wv_kv_attention: scratch"))) return rc;
+        if ((rc = sc.get(floats, s, what))) return rc;
         a.part = sc.f();
     }
     const int e = gp.use ? launch_kv_attn_groups(a, gp, s) : launch_kv_attn(a, s);
-    return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), "wv_kv_attention: kernel launch");
+    return e == hipSuccess ? WV_OK : rt_hip_fail(hipError_t(e), what);
 }
 
 }  // namespace
