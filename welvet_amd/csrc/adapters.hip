@@ -272,9 +272,11 @@ __device__ __forceinline__ f16v product(uint4 w, const Terms<TYPE>& x, f16v acc)
     }
     return acc;
 }
-// Exponent e of a magnitude's bits (it is below 2^(e + 1)), within what a power of two in f32 can bring to 2^14 and
-// back; of the larger of this lane's and lane ^ 32's.
-__device__ __forceinline__ int exponent(uint32_t bits) { return min(max(int(bits >> 23) - 127, -113), 127); }
+// Exponent e of a magnitude's bits (it is below 2^(e + 1)), within what a normal power of two in f32 brings to 2^14
+// (2^(14 - e)) and back (2^(e - 14): from kLeast on; one less has no bits, and took whole rows with it); of the larger
+// of this lane's and lane ^ 32's. What lies under 2^kLeast comes to less than 2^14, and to no less than fp16 holds.
+constexpr int kLeast = -112;
+__device__ __forceinline__ int exponent(uint32_t bits) { return min(max(int(bits >> 23) - 127, kLeast), 127); }
 __device__ __forceinline__ int pair_exponent(float m) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
     return exponent(max(r[0], r[1]));
@@ -418,7 +420,7 @@ __device__ __forceinline__ void down_tile(const Args& a, const Tile& t, int rang
             for (int i = 0; i < 4; ++i) v[4 * q + i] = y[i];
         }
     };
-    int e = -113;  // fp16: the token's sums so far are in units of 2^(e - 14)
+    int e = kLeast;  // fp16: the token's sums so far are in units of 2^(e - 14)
     auto step = [&](auto next) {
         if constexpr (TYPE == WV_ADAPTER_F16) {
             float m = 0.0f;
