@@ -676,8 +676,8 @@ typedef struct wv_adapter_rows {
  * library's own scratch, which a call under capture is refused. The sums have a
  * fixed order; a row whose x, or whose adapter, holds an infinity or a NaN may
  * become NaN as a whole. Of WV_ADAPTER_F16 sets x and A x may be taken to 22
- * bits, and to 2^-39 of the row's largest. Device pointers, enqueued on
- * `stream`. */
+ * bits, and to 2^-39 of the row's largest; of WV_ADAPTER_BF16 sets to 2^-133.
+ * Device pointers, enqueued on `stream`. */
 int wv_adapters_dev(const wv_adapter_batch *batch, const float *d_x, int64_t x_stride, const wv_adapter_rows *sets,
                     int32_t n_sets, void *d_scratch, size_t scratch_bytes, void *stream);
 /* Scratch bytes of such a call. Only the batch's sizes and the sets' handles are read. */

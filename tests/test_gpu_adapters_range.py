@@ -9,7 +9,7 @@ from test_gpu_adapters import U, Case, dev, held
 from welvet_amd.adapters import AdapterBatch, apply_dev
 
 pytestmark = pytest.mark.gpu
-TYPES = ["f16"]
+TYPES = ["f16", "bf16"]
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -23,19 +23,23 @@ def bound(x, A, B, scale, typ):
     """y without base, and what it may be off by. f32 products: chains of a quarter of the columns (or 16), joined by
     at most 40 sums, as in test_gpu_adapters. fp16 sets hold a tile's x and h as two fp16 terms under a power of two
     that brings the row's largest to 2^14: a value is off by 2^-22 of itself, or, where the second term is subnormal, by
-    half of 2^-24 of those units, 2^-39 of the row's largest. Sums below the normal f32 numbers are off by 2^-149."""
+    half of 2^-24 of those units, 2^-39 of the row's largest. bf16 sets hold them as three terms, exact but for what lies
+    under the smallest subnormal: off by 2^-133. Sums below the normal f32 numbers are off by 2^-149."""
     x = x.astype(np.float64)
     top = np.abs(x).max(1, keepdims=True)
     h, hs = x @ A.T, np.abs(x) @ np.abs(A).T
     dh = (x.shape[1] / 4 + 64) * U * hs
     two = typ == "f16"
-    if two:
-        dh += 2.0 ** -22 * hs + 2.0 ** -39 * top * np.abs(A).sum(1)
+    dh += (2.0 ** -22 * hs + 2.0 ** -39 * top * np.abs(A).sum(1)) if two else 2.0 ** -133 * np.abs(A).sum(1)
     dh += 2.0 ** -148
     y, dy = scale * (h @ B.T), dh @ np.abs(B).T + (A.shape[0] + 4) * U * (np.abs(h) @ np.abs(B).T)
+    dy *= abs(scale)
     if two:
-        dy += 2.0 ** -22 * (np.abs(h) @ np.abs(B).T) + 2.0 ** -39 * (np.abs(h) + dh).max(1, keepdims=True) * np.abs(B).sum(1)
-    return y, abs(scale) * dy + 2.0 ** -148 + 2 * U * np.abs(y)
+        dy += abs(scale) * (2.0 ** -22 * (np.abs(h) @ np.abs(B).T)
+                            + 2.0 ** -39 * (np.abs(h) + dh).max(1, keepdims=True) * np.abs(B).sum(1))
+    else:
+        dy += 2.0 ** -133 * np.abs(B).sum(1)  # h has its scale by then
+    return y, dy + 2.0 ** -148 + 2 * U * np.abs(y)
 
 
 def run(typ, x, new, scale, cols, rows=70, rank=20):
@@ -95,7 +99,7 @@ def test_columns_of_unlike_magnitudes(typ, up):
 @pytest.mark.parametrize("n", [3, 40])
 def test_single_columns(typ, n):
     """Tokens that are one column each: y is that column of A through B, within the roundings of one product chain and,
-    by tiles of fp16 sets, of x and h to 22 bits."""
+    by tiles, of x and h as `bound` has them."""
     rng = np.random.default_rng(n)
     cols, rank, rows = 700, 24, 50
     for size in (1.0, 2.0 ** -112, 1e-36, 1e30):
@@ -111,8 +115,11 @@ def test_single_columns(typ, n):
             y = c.run()[0].astype(np.float64)
             h = c.x[np.arange(n), at].astype(np.float64)[:, None] * A[:, at].T
             s = np.abs(h) @ np.abs(B).T
-            two = 2.0 ** -21 * s + 2.0 ** -38 * np.abs(h).max(1, keepdims=True) * np.abs(B).sum(1) if typ == "f16" else 0
-            tol = scale * ((rank + 6) * U * s + two) + 2.0 ** -148
+            tol = scale * (rank + 6) * U * s + 2.0 ** -148
+            if typ == "f16":
+                tol += scale * (2.0 ** -21 * s + 2.0 ** -38 * np.abs(h).max(1, keepdims=True) * np.abs(B).sum(1))
+            else:
+                tol += 2.0 ** -133 * (scale * np.abs(A[:, at].T) + 1) @ np.abs(B).T
             assert (np.abs(y - scale * (h @ B.T)) <= tol).all(), f"{typ}, {size}, column {first} on"
 
 
