@@ -660,7 +660,7 @@ typedef struct wv_adapter_batch {
 } wv_adapter_batch;
 /* What one set adds to: row t of y at t * y_stride floats (0: rows), of base at
  * t * base_stride. d_base NULL: y itself. Otherwise y may be base at the same
- * stride, but overlap neither it nor x in another way. */
+ * stride, but overlap neither it nor x, nor another set's rows, in another way. */
 typedef struct wv_adapter_rows {
     uint64_t adapters;
     float *d_y;

@@ -1063,6 +1063,12 @@ int wv_adapters_dev(const wv_adapter_batch* batch, const float* d_x, int64_t x_s
     if (!d_x || !batch->d_cu_q || !batch->d_adapter) return rt_fail(WV_E_ARG, "wv_adapters: nil x/cu_q/adapter");
     for (int i = 0; i < n_sets; ++i)
         if (!a.set[i].y) return rt_fail(WV_E_ARG, "wv_adapters: nil y");
+    for (int i = 0; i < n_sets; ++i) {  // blocks of one set would write what others' read or write
+        if (a.set[i].y == d_x) return rt_fail(WV_E_ARG, "wv_adapters: the rows of set %d are x", i);
+        for (int j = 0; j < n_sets; ++j)
+            if (i != j && (a.set[i].y == a.set[j].y || a.set[i].y == a.set[j].base))
+                return rt_fail(WV_E_ARG, "wv_adapters: the rows of set %d are those of set %d", i, j);
+    }
     a.n_sets = n_sets;
     for (int i = 0; i < n_sets; ++i) a.ranks += s[i].R;
     a.x = d_x, a.xs = x_stride, a.cu = batch->d_cu_q, a.which = batch->d_adapter;
