@@ -610,7 +610,7 @@ int wv_rope_free(uint64_t rope);
 
 /* Rows of n_heads heads, row t at t * stride floats (0: n_heads * head_dim).
  * d_y NULL: in place; d_y may also be d_x at x_stride, but not overlap it
- * otherwise. */
+ * otherwise, nor the other rows of the call. */
 typedef struct wv_rope_rows {
     const float *d_x;
     float *d_y;

@@ -5,6 +5,7 @@ import torch
 
 import welvet_amd as wv
 from welvet_amd.adapters import AdapterBatch, Adapters, apply_dev
+from welvet_amd.rope import Rope
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +39,24 @@ def test_adapters():
     wv.sync()
     add = 64 * 0.5 * 4 * 0.25  # sums of whole numbers: exact
     assert (y == 2.0 + add).all() and (z == 3.0 + add).all()
+
+
+def test_rope():
+    """q and k that are the same rows, or one's output the other's input; one input for two outputs is fine."""
+    r = Rope(8, theta=100.0)
+    x, y, z = (torch.full((3, 2, 8), v, device="cuda") for v in (1.0, 2.0, 3.0))
+    pos = torch.zeros(3, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    p, px, py, pz = (t.data_ptr() for t in (pos, x, y, z))
+    for kw in (dict(k_ptr=px), dict(k_ptr=py, k_out_ptr=px), dict(k_ptr=py, q_out_ptr=py),
+               dict(k_ptr=px, q_out_ptr=pz, k_out_ptr=pz), dict(k_ptr=px, q_out_ptr=py)):
+        with pytest.raises(wv.WelvetError) as e:
+            r.apply_dev(p, 3, px, 2, n_kv_heads=2, **kw)
+        assert e.value.code == -1 and "are those of k" in str(e.value)
+    wv.sync()
+    assert all((t == v).all() for t, v in ((x, 1.0), (y, 2.0), (z, 3.0)))
+    r.apply_dev(p, 3, px, 2, px, 1, q_out_ptr=py, k_out_ptr=pz, k_stride=16, k_out_stride=16)
+    wv.sync()
+    assert (y == 1.0).all() and (z[:, 0] == 1.0).all() and (z[:, 1] == 3.0).all()
+    r.apply_dev(p, 3, px, 2, px, 0)  # no heads of k
+    wv.sync()

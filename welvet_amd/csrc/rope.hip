@@ -285,6 +285,8 @@ int wv_rope_dev(uint64_t rope, const int32_t* d_pos, int32_t n, const wv_rope_ro
     }
     if (!n || !(a.q.heads + a.k.heads)) return WV_OK;
     if (!d_pos) return rt_fail(WV_E_ARG, "wv_rope: nil pos");
+    if (a.q.heads && a.k.heads && (a.q.y == a.k.y || a.q.y == a.k.x || a.k.y == a.q.x))  // turned once, twice or half
+        return rt_fail(WV_E_ARG, "wv_rope: the rows of q are those of k");
     a.turns = r.turns, a.pos = d_pos, a.n = n, a.hd = r.c.head_dim, a.rot = r.c.rot_dim, a.gain = float(r.c.gain);
     (void)hipSetDevice(r.device);
     hipStream_t s = rt_stream(stream, r.device);
