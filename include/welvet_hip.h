@@ -635,14 +635,16 @@ int wv_rope_dev(uint64_t rope, const int32_t *d_pos, int32_t n, const wv_rope_ro
 typedef struct wv_adapters_config {
     int32_t rows, cols;  /* at most 2^24 */
     int32_t max_rank;    /* 1 to 256 */
-    int32_t n_adapters;  /* at most 2^20 */
+    int32_t n_adapters;  /* at most 2^20. Steers the launch too: rows of many short sequences are taken by
+                            adapter only where a call has four for each, and sets of at most 256. */
     int32_t type;        /* WV_ADAPTER_* */
 } wv_adapters_config;
 /* Allocates on the current device; every adapter is unset (rank 0). */
 int wv_adapters_create(const wv_adapters_config *cfg, uint64_t *adapters);
 /* Adapter `index`: host arrays a [rank][cols] and b [rows][rank] of the set's
  * type (copied), its scale; rank 0 unsets it. Waits for the device's work, so
- * that calls before it see the old adapter and those after it the new one. */
+ * that calls before it see the old adapter and those after it the new one; not
+ * while a stream is under capture, which that wait may end. */
 int wv_adapters_set(uint64_t adapters, int32_t index, int32_t rank, float scale, const uint16_t *a,
                     const uint16_t *b);
 /* Releases a set once its work is done (waits for the device). */

@@ -5,10 +5,12 @@
 // still fill the GPU), whose sums meet when B h reads them, in order of the
 // ranges. A and B stay 16-bit, x, h and all sums are f32.
 // Of few rows bound by two launches and the weights' latency: one token, two sets
-// of rank 16 on 14336 x 4096, 2.8 + 3.2 us; 64 requests of one, three sets of rank
-// 32 on 1024 x 4096, 6.4 + 4.0 (50 MB of A and B from the caches). Of many by base
-// and y, and by x: 2000 rows, rank 64 on 14336 x 4096, 18.5 + 54 us (229 MB of base
-// and y at a large copy's 5.1 TB/s: 45).
+// of rank 16 on 14336 x 4096, 3.3 + 3.8 us; 64 requests of one, three sets of rank
+// 32 on 1024 x 4096, 7.2 + 5.9 (50 MB of A and B from the caches). Of many by base
+// and y, and by x: 2184 rows of 12 requests, rank 64 on 14336 x 4096, 14.8 + 56.7 us
+// (250 MB of base and y at a large copy's 5.1 TB/s: 49), fp16 13.9 + 42.3. Rows by
+// adapter: 256 requests, 8 adapters of rank 64, three sets on 1024 x 4096, 15.6 + 8.9;
+// of rank 128 on 4096 x 14336 21.0 + 18.3.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -821,7 +823,8 @@ int most_ids(const Set* s, int n_sets) {
 // them costs, some 4 us a call: the more, the more sequences there are (by sequence / by adapter, 8 adapters, rank 64 on
 // 4096 x 4096: 64 sequences 9.7 / 11.9 us, 128 13.1 / 12.7, 256 21.5 / 16.7, 600 45 / 29; rank 16: 256 12.6 / 12.4; rank
 // 128 on 4096 x 14336: 64 28 / 26, 256 74 / 36), and not where an adapter has fewer than four (256 sequences: 32 adapters
-// 25 / 24, 64 32 / 36, three sets 63 / 50; of 128, two sets of rank 128, as many adapters 106 / 158).
+// 25 / 24, 64 32 / 36, three sets 63 / 50; of 128, two sets of rank 128, as many adapters 106 / 158). How many adapters
+// are in use the host does not see: it goes by how many the sets have room for.
 int adapt_mode(const Set* s, int n_sets, const wv_adapter_batch& b) {
     const int most = b.max_q ? b.max_q : b.n_tokens, ids = most_ids(s, n_sets);
     if (most > kFew) return kTiles;

@@ -313,9 +313,10 @@ __device__ __forceinline__ float row_unit(float amax, float scale, float& inv) {
 // over 8 of 128, 134 us, 5.2 TB/s; one of 131071 fp16 keys 106 us, 5.2 TB/s. A
 // short one by a wave's chain from score to second product, 1.1 to 1.5 us a key
 // block, and by the join's launch: 2048 int8 keys 8 + 3 us.
-// ONCE: no other block reads a sequence's keys, and they are loaded past the
-// caches (131071 fp16 keys 106 us, else 112); not where several tiles read them
-// (64 tokens of 32 heads over 8000 fp16 keys 56 us so, else 43).
+// ONCE: keys are loaded past the caches, where no other block reads them (131071
+// fp16 keys 106 us, else 112); not where several tiles do (64 tokens of 32 heads
+// over 8000 fp16 keys 56 us so, else 43). Of sequences in groups the own keys
+// always are, also where a sequence has rows for several tiles.
 template <int HD, int TYPE, bool ONCE, int MODE>
 __device__ __forceinline__ void attn_rows(const KvAttn& a, int G, const Tile& t, int kvh, int sp) {
     constexpr int E = TYPE == WV_KV_F16 ? 2 : 1;
@@ -851,7 +852,8 @@ __device__ __forceinline__ void attn_lead(const KvAttn& a, int G, const Tile& t,
 // groups' rows over the shared keys, which take longest, then those of every
 // sequence's rows over its own. 64 sequences of one token behind 8192 int8 keys
 // of 8 heads of 128 with up to 1024 of their own: 48 us (the shared keys alone 33,
-// the own alone 22, for the same issue slots), and the join 4.
+// the own alone 22), and the join 4: 1.3 waves a SIMD on average, which wait for
+// data 36 % of their time. Registers and 70 KB of LDS leave room for two blocks a CU.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(256, 2) k_kv_attn_groups(KvAttn a, int G, int lead_tiles, int y0) {
     Tile t;
